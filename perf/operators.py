@@ -168,8 +168,7 @@ def _plain_scan(st):
     if st["kind"] == "scan":
         return out
     # c_t = dh_t + a_{t+1} c_{t+1}, from the end of every sequence
-    dh = st["dh"].float()
-    dh.index_put_((batch, last), torch.where(some[:, None], st["dstate"], 0.0), accumulate=True)
+    dh = st["dh"].float().index_put((batch, last), torch.where(some[:, None], st["dstate"], 0.0), accumulate=True)
     nxt = torch.zeros_like(a)
     nxt[:, :-1] = keep[:, 1:]
     c = _scan(nxt.flip(1), dh.flip(1)).flip(1)
