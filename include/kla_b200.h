@@ -556,6 +556,51 @@ int kla_b200_mobius_scan_bwd(const kla_b200_rawscan_args *args, void *stream);
 int kla_b200_affine_scan_fwd(const kla_b200_rawscan_args *args, void *stream);
 int kla_b200_affine_scan_bwd(const kla_b200_rawscan_args *args, void *stream);
 
+/*
+ * The gated recurrence, beside the raw affine scan above: the coefficients are formed from gates on the way, activations are
+ * float32 or bfloat16 with any strides, sequences start from a state and leave one.
+ *
+ *   h_t = a_t h_{t-1} + (1 - a_t) x_t,  a_t = sigmoid(gate_t),  h_{-1} = state (zeros when NULL)
+ *
+ * x, gate, h and their gradients are [B, L, D]; states float32 [sequences, D] contiguous. Without cu_seqlens the batch entries
+ * are the sequences (sequences == B). With cu_seqlens B is 1 and sequence n is the rows cu_seqlens[n] to cu_seqlens[n + 1] (not
+ * decreasing, of any length; clamped to [0, L]); rows that belong to none get h, dx and dgate of zero. The state a sequence
+ * leaves is that behind its last step, the one it started from where it has no steps. The recurrence runs in float32.
+ * ckpt: kla_b200_gated_ckpt_bytes of scratch that the forward fills for the backward, NULL in inference.
+ * The backward reads x, gate, dh, ckpt, dstate_out (NULL: zeros) and writes dx, dgate, dstate (NULL: not wanted).
+ */
+typedef struct kla_b200_gated_args {
+    int64_t B, L, D, sequences;
+    int32_t dtype;
+    const int32_t *cu_seqlens; /* device, [sequences + 1], or NULL */
+    kla_b200_tensor3 x, gate;
+    const float *state;        /* in  [sequences, D] or NULL */
+    kla_b200_tensor3 h;        /* out (forward) */
+    float *state_out;          /* out (forward) */
+    float *ckpt;
+    kla_b200_tensor3 dh;       /* in  (backward) */
+    const float *dstate_out;   /* in  (backward) */
+    kla_b200_tensor3 dx, dgate;
+    float *dstate;
+} kla_b200_gated_args;
+
+size_t kla_b200_gated_ckpt_bytes(int64_t sequences, int64_t L, int64_t D, int packed);
+int kla_b200_gated_scan_fwd(const kla_b200_gated_args *args, void *stream);
+int kla_b200_gated_scan_bwd(const kla_b200_gated_args *args, void *stream);
+
+/* One token of it: x, gate [B, D] with row strides, h [B, D] contiguous, state and state_out float32 [B, D] (may be one buffer). */
+typedef struct kla_b200_gated_step_args {
+    int64_t B, D;
+    int32_t dtype;
+    const void *x, *gate;
+    int64_t x_stride_b, gate_stride_b;
+    const float *state;
+    float *state_out;
+    void *h;
+} kla_b200_gated_step_args;
+
+int kla_b200_gated_step(const kla_b200_gated_step_args *args, void *stream);
+
 /* Human-readable text for a return code; for KLA_B200_ECUDA it includes the
  * CUDA error string of the failing call on this thread. */
 const char *kla_b200_strerror(int code);

@@ -42,6 +42,10 @@ SYMBOLS = (
     "kla_b200_mobius_scan_bwd",
     "kla_b200_affine_scan_fwd",
     "kla_b200_affine_scan_bwd",
+    "kla_b200_gated_ckpt_bytes",
+    "kla_b200_gated_scan_fwd",
+    "kla_b200_gated_scan_bwd",
+    "kla_b200_gated_step",
     "kla_b200_strerror",
     "kla_b200_version",
     "kla_b200_launch_count",
@@ -135,6 +139,21 @@ class RawScanArgs(Structure):
         ("B", c_int64), ("L", c_int64), ("N", c_int64),
         ("inp", c_void_p * 6), ("out", c_void_p * 4),
         ("state0", c_void_p), ("dstate0", c_void_p),
+    ]
+
+
+class GatedArgs(Structure):
+    _fields_ = [
+        ("B", c_int64), ("L", c_int64), ("D", c_int64), ("sequences", c_int64), ("dtype", c_int32), ("cu_seqlens", c_void_p),
+        ("x", Tensor3), ("gate", Tensor3), ("state", c_void_p), ("h", Tensor3), ("state_out", c_void_p), ("ckpt", c_void_p),
+        ("dh", Tensor3), ("dstate_out", c_void_p), ("dx", Tensor3), ("dgate", Tensor3), ("dstate", c_void_p),
+    ]
+
+
+class GatedStepArgs(Structure):
+    _fields_ = [
+        ("B", c_int64), ("D", c_int64), ("dtype", c_int32), ("x", c_void_p), ("gate", c_void_p),
+        ("x_stride_b", c_int64), ("gate_stride_b", c_int64), ("state", c_void_p), ("state_out", c_void_p), ("h", c_void_p),
     ]
 
 
@@ -256,6 +275,14 @@ def load() -> ctypes.CDLL:
         fn = getattr(lib, "kla_b200_" + name)
         fn.restype = c_int
         fn.argtypes = [POINTER(RawScanArgs), c_void_p]
+    lib.kla_b200_gated_ckpt_bytes.restype = c_size_t
+    lib.kla_b200_gated_ckpt_bytes.argtypes = [c_int64, c_int64, c_int64, c_int]
+    lib.kla_b200_gated_scan_fwd.restype = c_int
+    lib.kla_b200_gated_scan_fwd.argtypes = [POINTER(GatedArgs), c_void_p]
+    lib.kla_b200_gated_scan_bwd.restype = c_int
+    lib.kla_b200_gated_scan_bwd.argtypes = [POINTER(GatedArgs), c_void_p]
+    lib.kla_b200_gated_step.restype = c_int
+    lib.kla_b200_gated_step.argtypes = [POINTER(GatedStepArgs), c_void_p]
     lib.kla_b200_conv_step.restype = c_int
     lib.kla_b200_conv_step.argtypes = [POINTER(ConvStepArgs), c_void_p]
     lib.kla_b200_conv_seq.restype = c_int
@@ -294,7 +321,7 @@ _host = None
 _HOST_ENTRIES = (
     "scan_fwd", "scan_bwd", "slab_aggregate", "chunk_fold", "epilogue_bwd", "step", "conv_step", "step_layer",
     "linear", "token_work_bytes", "token", "add_norm", "swiglu", "argmax", "qk_norm", "conv_seq", "conv_seq_bwd", "mobius_scan_fwd", "mobius_scan_bwd", "affine_scan_fwd", "affine_scan_bwd",
-    "ckpt_bytes", "segment_scratch_bytes", "strerror",
+    "gated_ckpt_bytes", "gated_scan_fwd", "gated_scan_bwd", "gated_step", "ckpt_bytes", "segment_scratch_bytes", "strerror",
 )
 
 

@@ -39,6 +39,8 @@ NVCC_FLAGS = [
 
 _SCAN_DEPS = ["kla_common.cuh", "kla_fwd.cuh", "kla_bwd.cuh", "kla_agg.cuh", "kla_launch.cuh", "kla_scan_inst.cu"]
 
+_HEADER = os.path.join(INCLUDE, "kla_b200.h")
+
 
 def _units():
     """(object name, source, extra flags, files it depends on)."""
@@ -49,6 +51,7 @@ def _units():
                 flags = [f"-DKLA_INST_KIND={kind}", f"-DKLA_INST_DT={dt}", f"-DKLA_INST_LPCS={lp}"]
                 units.append((f"scan_{kname}_{dname}_{lname}", "kla_scan_inst.cu", flags, _SCAN_DEPS))
     units.append(("scan_agg", "kla_scan_inst.cu", ["-DKLA_INST_KIND=2"], _SCAN_DEPS))
+    units.append(("gated", "kla_gated.cu", [], [*_SCAN_DEPS, "kla_entry.h", "kla_gated.cuh", "kla_gated.cu", _HEADER]))
     return units
 
 
@@ -61,7 +64,7 @@ def _nvcc() -> str:
 
 def _sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cuh"))
-                  + glob.glob(os.path.join(INCLUDE, "*.h")))
+                  + glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(INCLUDE, "*.h")))
 
 
 def _newer(target: str, deps) -> bool:

@@ -10,6 +10,7 @@
 #include "kla_block.cuh"
 #include "kla_conv_bwd.cuh"
 #include "kla_decode.cuh"
+#include "kla_entry.h"
 #include "kla_epilogue.cuh"
 #include "kla_launch.cuh"
 #include "kla_linear.cuh"
@@ -66,9 +67,7 @@ int vec2_ok(const kla_b200_tensor3 &t) {
 
 // cuTensorMapEncodeTiled is fetched from the driver at run time, so the library
 // links against the CUDA runtime only.
-using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+using entry::EncodeTiledFn;
 EncodeTiledFn encode_tiled_fn() {
     static EncodeTiledFn fn = [] {
         void *p = nullptr;
@@ -1203,6 +1202,17 @@ int kla_b200_step_layer(const kla_b200_step_layer_args *a, void *stream) {
     while (lpc * 4 < a->S) lpc *= 2;
     return dispatch_step_layer(a->in_dtype, a->out_dtype, a->decode_from_prior != 0, lpc, prm, static_cast<cudaStream_t>(stream));
 }
+
+}  // extern "C"
+
+namespace kla::entry {
+int cuda_fail(cudaError_t e) { return ::cuda_fail(e); }
+void count_launch() { g_launches.fetch_add(1); }
+int wait_ctl(WaitCtl *w) { return ::wait_ctl(w); }
+EncodeTiledFn encode_tiled_fn() { return ::encode_tiled_fn(); }
+}  // namespace kla::entry
+
+extern "C" {
 
 const char *kla_b200_strerror(int code) {
     switch (code) {

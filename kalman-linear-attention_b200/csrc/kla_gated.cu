@@ -1,0 +1,137 @@
+// Entry points of the gated recurrence (kla_gated.cuh): argument checks, kernel and cluster choice, launches.
+#include "../../include/kla_b200.h"
+#include "kla_entry.h"
+#include "kla_gated.cuh"
+#include "kla_launch.cuh"
+
+namespace {
+
+using namespace kla;
+
+bool aligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+int check_rows(const kla_b200_tensor3 &t, size_t esz) {
+    if (t.ptr == nullptr || t.stride_b < 0 || t.stride_t < 0) return KLA_B200_EINVAL;
+    return aligned(t.ptr, esz) ? KLA_B200_OK : KLA_B200_EALIGN;
+}
+bool pairs(const kla_b200_tensor3 &t, size_t esz) { return aligned(t.ptr, 2 * esz) && t.stride_b % 2 == 0 && t.stride_t % 2 == 0; }
+Tensor3 t3(const kla_b200_tensor3 &t) { return Tensor3{t.ptr, t.stride_b, t.stride_t}; }
+
+// Sequences of this many steps in tiles of `tile`: how many CTAs of a cluster share one.
+int pick_ranks(int64_t cells, int64_t steps, int tile) {
+    const int64_t slots = 2 * device_sms(), tiles = (steps + tile - 1) / tile;
+    int best = 1;
+    double least = 0.0;
+    for (int r = 1; r <= kGatedMaxCluster && (r == 1 || r <= tiles); r *= 2) {
+        const double t = (double)((cells * r + slots - 1) / slots) * (double)((tiles + r - 1) / r) * (r == 1 ? 1.0 : 1.15);
+        if (r == 1 || t < least) { best = r; least = t; }
+    }
+    return best;
+}
+
+template <typename K>
+int launch(K kern, GatedParams &prm, int64_t sequences, int ranks, cudaStream_t st) {
+    const int64_t grid = sequences * prm.blocks * ranks;
+    if (grid == 0) return KLA_B200_OK;
+    if (grid > 0x7fffffffll) return KLA_B200_EUNSUPPORTED;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ranks;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kGatedWarps * 32);
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = ranks > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, prm);
+    if (e != cudaSuccess) return entry::cuda_fail(e);
+    entry::count_launch();
+    return KLA_B200_OK;
+}
+
+template <typename T, bool PAIR>
+int run(GatedParams &prm, bool backward, int64_t sequences, int ranks, cudaStream_t st) {
+    constexpr int TS = sizeof(T) == 2 ? 16 : 8;
+    if (backward)
+        return ranks > 1 ? launch(kla_gated_bwd_kernel<T, PAIR, true>, prm, sequences, ranks, st)
+                         : launch(kla_gated_bwd_kernel<T, PAIR, false>, prm, sequences, ranks, st);
+    return ranks > 1 ? launch(kla_gated_fwd_kernel<T, PAIR, true, TS>, prm, sequences, ranks, st)
+                     : launch(kla_gated_fwd_kernel<T, PAIR, false, TS>, prm, sequences, ranks, st);
+}
+
+int gated(const kla_b200_gated_args *a, void *stream, bool backward) {
+    if (a == nullptr || a->B < 0 || a->L < 0 || a->D < 0 || a->sequences < 0) return KLA_B200_EINVAL;
+    if (a->dtype != KLA_B200_F32 && a->dtype != KLA_B200_BF16) return KLA_B200_EUNSUPPORTED;
+    if (a->B > (1 << 30) || a->L > (1 << 30) || a->D > (1 << 30) || a->sequences > (1 << 30)) return KLA_B200_EUNSUPPORTED;
+    const bool packed = a->cu_seqlens != nullptr;
+    if (packed ? a->B != 1 : a->sequences != a->B) return KLA_B200_EINVAL;
+    const int64_t N = a->sequences;
+    if (a->D == 0 || (N == 0 && (!packed || a->L == 0))) return KLA_B200_OK;
+    const size_t esz = a->dtype == KLA_B200_BF16 ? 2 : 4;
+    const kla_b200_tensor3 *in[5] = {&a->x, &a->gate, backward ? &a->dh : &a->h, &a->dx, &a->dgate};
+    bool vec = a->D % 2 == 0;
+    if (a->L > 0)
+        for (int i = 0; i < (backward ? 5 : 3); ++i) {
+            if (const int rc = check_rows(*in[i], esz)) return rc;
+            vec = vec && pairs(*in[i], esz);
+        }
+    if (!backward && N > 0 && a->state_out == nullptr) return KLA_B200_EINVAL;
+    if (backward && N > 0 && a->L > 0 && a->ckpt == nullptr) return KLA_B200_EINVAL;
+    for (const void *p : {(const void *)a->cu_seqlens, (const void *)a->state, (const void *)a->state_out, (const void *)a->ckpt,
+                          (const void *)a->dstate_out, (const void *)a->dstate})
+        if (!aligned(p, 4)) return KLA_B200_EALIGN;
+    GatedParams prm{};
+    prm.N = (int)N; prm.L = (int)a->L; prm.D = (int)a->D;
+    prm.blocks = (int)((a->D + kGatedChannels - 1) / kGatedChannels);
+    prm.x = t3(a->x); prm.g = t3(a->gate); prm.h = t3(a->h);
+    prm.cu = a->cu_seqlens; prm.h0 = a->state; prm.end = a->state_out; prm.ckpt = a->ckpt;
+    prm.dh = t3(a->dh); prm.dx = t3(a->dx); prm.dg = t3(a->dgate);
+    prm.dend = a->dstate_out; prm.dh0 = a->dstate;
+    const int64_t sequences = N + packed;
+    const int tile = backward ? kGatedUnit : kGatedWarps * (esz == 2 ? 16 : 8);
+    const int ranks = pick_ranks(N * prm.blocks, packed && N > 0 ? (a->L + N - 1) / N : a->L, tile);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (esz == 2) return vec ? run<__nv_bfloat16, true>(prm, backward, sequences, ranks, st) : run<__nv_bfloat16, false>(prm, backward, sequences, ranks, st);
+    return vec ? run<float, true>(prm, backward, sequences, ranks, st) : run<float, false>(prm, backward, sequences, ranks, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t kla_b200_gated_ckpt_bytes(int64_t sequences, int64_t L, int64_t D, int packed) {
+    if (sequences <= 0 || L < 0 || D <= 0) return 0;
+    const size_t per = (size_t)((L + kGatedUnit - 1) / kGatedUnit);
+    size_t units = packed ? (size_t)(L / kGatedUnit) + (size_t)sequences + 1 : per;
+    for (const size_t f : {packed ? (size_t)1 : (size_t)sequences, (size_t)D, sizeof(float)}) {
+        if (f != 0 && units > SIZE_MAX / f) return SIZE_MAX;
+        units *= f;
+    }
+    return units;
+}
+
+int kla_b200_gated_scan_fwd(const kla_b200_gated_args *args, void *stream) { return gated(args, stream, false); }
+int kla_b200_gated_scan_bwd(const kla_b200_gated_args *args, void *stream) { return gated(args, stream, true); }
+
+int kla_b200_gated_step(const kla_b200_gated_step_args *a, void *stream) {
+    if (a == nullptr || a->B < 0 || a->D < 0 || a->x_stride_b < 0 || a->gate_stride_b < 0) return KLA_B200_EINVAL;
+    if (a->dtype != KLA_B200_F32 && a->dtype != KLA_B200_BF16) return KLA_B200_EUNSUPPORTED;
+    if (a->B > (1 << 30) || a->D > (1 << 30)) return KLA_B200_EUNSUPPORTED;
+    if (a->B == 0 || a->D == 0) return KLA_B200_OK;
+    if (!a->x || !a->gate || !a->state || !a->state_out || !a->h) return KLA_B200_EINVAL;
+    const size_t esz = a->dtype == KLA_B200_BF16 ? 2 : 4;
+    if (!aligned(a->x, esz) || !aligned(a->gate, esz) || !aligned(a->h, esz) || !aligned(a->state, 4) || !aligned(a->state_out, 4)) return KLA_B200_EALIGN;
+    GatedStepParams prm{a->B * a->D, (int)a->D, a->x, a->gate, a->x_stride_b, a->gate_stride_b, a->state, a->state_out, a->h};
+    const int64_t grid = (prm.n + 255) / 256;
+    if (grid > 0x7fffffffll) return KLA_B200_EUNSUPPORTED;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (esz == 2) kla_gated_step_kernel<__nv_bfloat16><<<(unsigned)grid, 256, 0, st>>>(prm);
+    else kla_gated_step_kernel<float><<<(unsigned)grid, 256, 0, st>>>(prm);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return entry::cuda_fail(e);
+    entry::count_launch();
+    return KLA_B200_OK;
+}
+
+}  // extern "C"

@@ -8,6 +8,7 @@
 // and unit last strides checked); canonical() and step() do that check themselves and answer "not this route" otherwise,
 // which sends the wrapper to its general path with its error messages.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
@@ -47,6 +48,10 @@ struct Entry {
     int (*argmax)(int64_t, int64_t, int32_t, const void *, int64_t, int64_t *, void *) = nullptr;
     int (*conv_seq)(const kla_b200_conv_seq_args *, void *) = nullptr;
     int (*conv_seq_bwd)(const kla_b200_conv_seq_bwd_args *, void *) = nullptr;
+    size_t (*gated_ckpt_bytes)(int64_t, int64_t, int64_t, int) = nullptr;
+    int (*gated_fwd)(const kla_b200_gated_args *, void *) = nullptr;
+    int (*gated_bwd)(const kla_b200_gated_args *, void *) = nullptr;
+    int (*gated_step)(const kla_b200_gated_step_args *, void *) = nullptr;
     int (*rawscan[4])(const kla_b200_rawscan_args *, void *) = {};  // Moebius forward, backward, affine forward, backward
     size_t (*ckpt_bytes)(int64_t, int64_t, int64_t, int64_t) = nullptr;
     size_t (*segment_scratch_bytes)(int64_t, int64_t, int64_t) = nullptr;
@@ -80,6 +85,10 @@ void bind(const py::dict &d) {
     take(lib.rawscan[1], d, "kla_b200_mobius_scan_bwd");
     take(lib.rawscan[2], d, "kla_b200_affine_scan_fwd");
     take(lib.rawscan[3], d, "kla_b200_affine_scan_bwd");
+    take(lib.gated_ckpt_bytes, d, "kla_b200_gated_ckpt_bytes");
+    take(lib.gated_fwd, d, "kla_b200_gated_scan_fwd");
+    take(lib.gated_bwd, d, "kla_b200_gated_scan_bwd");
+    take(lib.gated_step, d, "kla_b200_gated_step");
     take(lib.ckpt_bytes, d, "kla_b200_ckpt_bytes");
     take(lib.segment_scratch_bytes, d, "kla_b200_segment_scratch_bytes");
     take(lib.strerror, d, "kla_b200_strerror");
@@ -625,6 +634,103 @@ Tensor swiglu_step(const Tensor &x, const Tensor &norm_w_, double eps, const Ten
     return project(h, w3, b3, {}, 0.0, x);
 }
 
+// ---------------------------------------------------------------------------------------------- the gated recurrence
+
+void unsupported(const std::string &what) {
+    PyErr_SetString(PyExc_NotImplementedError, what.c_str());
+    throw py::error_already_set();
+}
+// x and gate of the gated recurrence: one shape, type and device the kernels take.
+void check_gated(const Tensor &x, const Tensor &gate, int64_t dims) {
+    if (!x.is_cuda() || !gate.is_cuda()) unsupported("The b200 gated recurrence needs CUDA tensors; x is on " + x.device().str() + ", gate on " + gate.device().str() + ".");
+    require_type(x);
+    require(gate.scalar_type() == x.scalar_type(), "gate and x have different types");
+    require(x.dim() == dims, dims == 3 ? "x is [B, L, D]" : "x is [B, D]");
+    require(gate.sizes() == x.sizes(), "gate and x have different shapes");
+    require(gate.device() == x.device(), "gate and x are on different devices");
+    if (!sm100(x.device())) unsupported("The b200 kernels need an sm_100 device.");
+}
+void check_state(const OptTensor &s, const Tensor &x, int64_t n, int64_t D, const char *what) {
+    if (s) require(s->device() == x.device() && s->scalar_type() == at::kFloat && s->dim() == 2 && s->size(0) == n && s->size(1) == D, what);
+}
+Tensor rows(const Tensor &t) { return rows_ok(t) ? t : t.contiguous(); }
+
+kla_b200_gated_args gated_args(const Tensor &x, const Tensor &gate, const OptTensor &cu) {
+    kla_b200_gated_args a{};
+    a.B = x.size(0); a.L = x.size(1); a.D = x.size(2);
+    a.sequences = cu ? cu->size(0) - 1 : a.B;
+    a.dtype = dt(x.scalar_type());
+    a.cu_seqlens = cu ? cu->data_ptr<int32_t>() : nullptr;
+    a.x = t3(x); a.gate = t3(gate);
+    return a;
+}
+
+// kla_b200_gated_scan_fwd -> h, the states sequences leave, what the backward takes: x and gate as they were read, cu_seqlens, ckpt
+std::tuple<Tensor, Tensor, Tensor, Tensor, OptTensor, OptTensor> gated_fwd(const Tensor &x_, const Tensor &gate_, const OptTensor &state_,
+                                                                           const OptTensor &cu_, bool need_ckpt) {
+    check_gated(x_, gate_, 3);
+    const c10::cuda::CUDAGuard guard(x_.device());
+    OptTensor cu;
+    if (cu_) {
+        require(cu_->device() == x_.device() && cu_->dim() == 1 && cu_->size(0) >= 1, "cu_seqlens is a vector of at least one bound on x's device");
+        require(cu_->scalar_type() == at::kInt || cu_->scalar_type() == at::kLong, "cu_seqlens holds int32 or int64");
+        require(x_.size(0) == 1, "packed sequences are one batch entry: x is [1, L, D]");
+        cu = cu_->to(at::kInt).contiguous();
+    }
+    const Tensor x = rows(x_), gate = rows(gate_);
+    kla_b200_gated_args a = gated_args(x, gate, cu);
+    check_state(state_, x, a.sequences, a.D, "initial_state is float32 [sequences, D] on x's device");
+    const OptTensor state = state_ ? OptTensor(state_->contiguous()) : state_;
+    Tensor h = fresh(x, x.sizes()), end = f32(x, {a.sequences, a.D});
+    OptTensor ckpt;
+    if (need_ckpt) ckpt = f32(x, {(int64_t)(lib.gated_ckpt_bytes(a.sequences, a.L, a.D, cu.has_value()) / sizeof(float))});
+    a.h = t3(h); a.state = fp(state); a.state_out = fp(end); a.ckpt = fp(ckpt);
+    check(lib.gated_fwd(&a, stream_of(x)));
+    return {h, end, x, gate, cu, ckpt};
+}
+
+// kla_b200_gated_scan_bwd -> dx, dgate, and (where wanted) the gradient of the states sequences start from
+std::tuple<Tensor, Tensor, OptTensor> gated_bwd(const Tensor &x, const Tensor &gate, const OptTensor &cu, const Tensor &ckpt, const Tensor &dh_,
+                                                const OptTensor &dend_, bool want_state) {
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor dh = rows(dh_.scalar_type() == x.scalar_type() ? dh_ : dh_.to(x.scalar_type()));
+    kla_b200_gated_args a = gated_args(x, gate, cu);
+    const OptTensor dend = dend_ ? OptTensor(dend_->to(at::kFloat).contiguous()) : dend_;
+    Tensor dx = fresh(x, x.sizes()), dgate = fresh(x, x.sizes());
+    OptTensor dstate;
+    if (want_state) dstate = f32(x, {a.sequences, a.D});
+    a.dh = t3(dh); a.dx = t3(dx); a.dgate = t3(dgate); a.ckpt = fp(ckpt);
+    a.dstate_out = fp(dend); a.dstate = fp(dstate);
+    check(lib.gated_bwd(&a, stream_of(x)));
+    return {dx, dgate, dstate};
+}
+
+// kla_b200_gated_step -> h, the new state (state_out where given)
+std::tuple<Tensor, Tensor> gated_step(const Tensor &x_, const Tensor &gate_, const Tensor &state_, const OptTensor &out) {
+    check_gated(x_, gate_, 2);
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const Tensor x = rows(x_), gate = rows(gate_);
+    const int64_t B = x.size(0), D = x.size(1);
+    check_state(state_, x, B, D, "state is float32 [B, D] on x's device");
+    check_state(out, x, B, D, "state_out is float32 [B, D] on x's device");
+    require(!out || out->is_contiguous(), "state_out is contiguous");
+    // state_out may be state itself; any other overlap would be read after it is written
+    if (out && out->numel() > 0) {
+        if (!(state_.is_contiguous() && state_.data_ptr() == out->data_ptr())) at::assert_no_overlap(*out, state_);
+        at::assert_no_overlap(*out, x_);
+        at::assert_no_overlap(*out, gate_);
+    }
+    if (wants_grad({&x_, &gate_, &state_})) unsupported("gated_step_b200 has no backward: use gated_scan_b200, or call it under torch.no_grad().");
+    const Tensor state = state_.contiguous();
+    Tensor h = fresh(x, {B, D}), next = out ? *out : f32(x, {B, D});
+    kla_b200_gated_step_args a{};
+    a.B = B; a.D = D; a.dtype = dt(x.scalar_type());
+    a.x = x.data_ptr(); a.gate = gate.data_ptr(); a.x_stride_b = x.stride(0); a.gate_stride_b = gate.stride(0);
+    a.state = fp(state); a.state_out = fp(next); a.h = h.data_ptr();
+    check(lib.gated_step(&a, stream_of(x)));
+    return {h, next};
+}
+
 // ------------------------------------------------------------------------------------------ a token as one kernel
 
 py::object entry(const py::dict &d, const char *name) {
@@ -987,6 +1093,9 @@ PYBIND11_MODULE(_kla_host, m) {
     m.def("conv_seq", &conv_seq);
     m.def("conv_seq_bwd", &conv_seq_bwd);
     m.def("rawscan", &rawscan);
+    m.def("gated_fwd", &gated_fwd);
+    m.def("gated_bwd", &gated_bwd);
+    m.def("gated_step", &gated_step);
     m.def("step", &step);
     m.def("layer_step", &layer_step);
     m.def("model_token", &model_token);

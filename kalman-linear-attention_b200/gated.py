@@ -1,0 +1,59 @@
+"""The gated recurrence on the B200 kernels, beside the raw affine scan (``affine_scan_b200``):
+
+    h_t = a_t h_{t-1} + (1 - a_t) x_t,   a_t = sigmoid(gate_t),   h_{-1} = initial_state (zeros when None)
+
+channel by channel. Where ``affine_scan_b200`` takes materialised float32 coefficients and starts from zero, this forms them
+from gates on the way, in float32 whatever the activations' type, takes a batch of sequences or packed sequences of different
+lengths, starts from states and returns the states it ends in, and spreads few or long sequences over the GPU. Differentiable
+with respect to ``x``, ``gate`` and ``initial_state``. ``gated_step_b200`` is one token of it. There is no CPU or eager path:
+what the kernels do not take raises ``NotImplementedError``.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+
+class _GatedScanB200(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, initial_state, cu_seqlens):
+        h, end, x, gate, cu, ckpt = _lib.host().gated_fwd(x, gate, initial_state, cu_seqlens, True)
+        ctx.set_materialize_grads(False)
+        ctx.packed, ctx.carried = cu is not None, initial_state is not None
+        ctx.save_for_backward(x, gate, ckpt, *((cu,) if cu is not None else ()))
+        return h, end
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, dend):
+        x, gate, ckpt, *rest = ctx.saved_tensors
+        if dh is None:
+            if dend is None:
+                return None, None, None, None
+            dh = torch.zeros((), device=x.device, dtype=x.dtype).expand(x.shape)
+        want_state = ctx.carried and ctx.needs_input_grad[2]
+        dx, dgate, dstate = _lib.host().gated_bwd(x, gate, rest[0] if ctx.packed else None, ckpt, dh, dend, want_state)
+        return dx, dgate, dstate, None
+
+
+def gated_scan_b200(x: torch.Tensor, gate: torch.Tensor, initial_state: torch.Tensor | None = None,
+                    cu_seqlens: torch.Tensor | None = None):
+    """``(h, state)``: ``h`` like ``x``, ``state`` float32 ``[sequences, D]``, the value behind every sequence's last step.
+
+    ``x``, ``gate``: ``[B, L, D]`` float32 or bfloat16, any strides with adjacent channels (others are copied), such as the
+    halves of one projection. ``initial_state``: float32 ``[sequences, D]``. ``cu_seqlens``: bounds of packed sequences,
+    ``[sequences + 1]`` int32 (int64 is converted) on the device, ``x`` being ``[1, L, D]``: sequence ``n`` is the rows
+    ``cu_seqlens[n]`` to ``cu_seqlens[n + 1]``; the bounds must not decrease, which is not checked (values outside ``[0, L]``
+    are clamped). A sequence without rows leaves the state it started from; rows that belong to no sequence get zeros, in
+    ``h`` and in the gradients. Once a state is infinite the values after it are NaN."""
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (initial_state is not None and initial_state.requires_grad)):
+        return _GatedScanB200.apply(x, gate, initial_state, cu_seqlens)
+    return _lib.host().gated_fwd(x, gate, initial_state, cu_seqlens, False)[:2]
+
+
+def gated_step_b200(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, state_out: torch.Tensor | None = None):
+    """One token: ``(h, new_state)`` for ``x``, ``gate`` ``[B, D]`` and ``state`` float32 ``[B, D]``. ``state_out`` receives the
+    new state where it is given, and may be ``state`` itself (a captured token then advances it with every replay). No backward."""
+    return _lib.host().gated_step(x, gate, state, state_out)
