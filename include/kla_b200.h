@@ -601,6 +601,36 @@ typedef struct kla_b200_gated_step_args {
 
 int kla_b200_gated_step(const kla_b200_gated_step_args *args, void *stream);
 
+/*
+ * The gated feed-forward block, forward and backward, beside the swiglu pieces of the decode calls above: bfloat16 with float32
+ * accumulation.
+ *
+ *   g = x Wg^T + bg,  u = x Wu^T + bu,  h = act(g) u,  y = h w3^T + b3 (+ residual)      w12 = [Wg; Wu]
+ *
+ * Matrices are row-major with unit stride along a row. x, w12, w3, h, gu, dy, dgu: 16-byte aligned, row strides a multiple of 8
+ * (elements) that is at least the width; y, residual and dx: any stride; gradients of weights and biases contiguous, the
+ * weights' 16-byte aligned.
+ * h is an output of the forward and an input of the backward; so is gu (rows [g, u], gu_stride a multiple of 16, u half a row
+ * behind g), which is NULL in inference. dgu is scratch like gu, work scratch of kla_b200_mlp_work_bytes. In the backward every
+ * gradient may be NULL: not wanted. Sums over rows are added in a fixed order: results do not change from run to run.
+ */
+typedef struct kla_b200_mlp_args {
+    int64_t rows, d, H, out;   /* x [rows, d], w12 [2 H, d], w3 [out, H], y [rows, out] */
+    int32_t activation;
+    const void *x, *w12, *w3, *b12, *b3, *residual; /* b12 [2 H], b3 [out], residual [rows, out] or NULL */
+    int64_t x_stride, w12_stride, w3_stride, residual_stride;
+    void *h, *gu, *y;          /* [rows, H], [rows, 2, H], [rows, out] */
+    int64_t h_stride, gu_stride, y_stride;
+    const void *dy;
+    int64_t dy_stride;
+    void *dgu, *dx, *dw12, *dw3, *db12, *db3, *work;
+    int64_t dx_stride;
+} kla_b200_mlp_args;
+
+size_t kla_b200_mlp_work_bytes(const kla_b200_mlp_args *args);
+int kla_b200_mlp_fwd(const kla_b200_mlp_args *args, void *stream);
+int kla_b200_mlp_bwd(const kla_b200_mlp_args *args, void *stream);
+
 /* Human-readable text for a return code; for KLA_B200_ECUDA it includes the
  * CUDA error string of the failing call on this thread. */
 const char *kla_b200_strerror(int code);

@@ -16,6 +16,7 @@ from . import seqshard  # noqa: F401
 from .seqshard import kla_scan_seq_sharded  # noqa: F401
 from .rawscan import affine_scan_b200, mobius_scan_b200  # noqa: F401
 from .gated import gated_scan_b200, gated_step_b200  # noqa: F401
+from .mlp import gated_mlp_b200  # noqa: F401
 from .decode import LayerDecoder, ModelDecoder  # noqa: F401
 from . import layer  # noqa: F401
 from .layer import fused_forward  # noqa: F401

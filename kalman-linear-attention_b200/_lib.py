@@ -46,6 +46,9 @@ SYMBOLS = (
     "kla_b200_gated_scan_fwd",
     "kla_b200_gated_scan_bwd",
     "kla_b200_gated_step",
+    "kla_b200_mlp_work_bytes",
+    "kla_b200_mlp_fwd",
+    "kla_b200_mlp_bwd",
     "kla_b200_strerror",
     "kla_b200_version",
     "kla_b200_launch_count",
@@ -154,6 +157,17 @@ class GatedStepArgs(Structure):
     _fields_ = [
         ("B", c_int64), ("D", c_int64), ("dtype", c_int32), ("x", c_void_p), ("gate", c_void_p),
         ("x_stride_b", c_int64), ("gate_stride_b", c_int64), ("state", c_void_p), ("state_out", c_void_p), ("h", c_void_p),
+    ]
+
+
+class MlpArgs(Structure):
+    _fields_ = [
+        ("rows", c_int64), ("d", c_int64), ("H", c_int64), ("out", c_int64), ("activation", c_int32),
+        *((n, c_void_p) for n in ("x", "w12", "w3", "b12", "b3", "residual")),
+        *((n, c_int64) for n in ("x_stride", "w12_stride", "w3_stride", "residual_stride")),
+        ("h", c_void_p), ("gu", c_void_p), ("y", c_void_p), ("h_stride", c_int64), ("gu_stride", c_int64), ("y_stride", c_int64),
+        ("dy", c_void_p), ("dy_stride", c_int64), *((n, c_void_p) for n in ("dgu", "dx", "dw12", "dw3", "db12", "db3", "work")),
+        ("dx_stride", c_int64),
     ]
 
 
@@ -283,6 +297,12 @@ def load() -> ctypes.CDLL:
     lib.kla_b200_gated_scan_bwd.argtypes = [POINTER(GatedArgs), c_void_p]
     lib.kla_b200_gated_step.restype = c_int
     lib.kla_b200_gated_step.argtypes = [POINTER(GatedStepArgs), c_void_p]
+    lib.kla_b200_mlp_work_bytes.restype = c_size_t
+    lib.kla_b200_mlp_work_bytes.argtypes = [POINTER(MlpArgs)]
+    for name in ("mlp_fwd", "mlp_bwd"):
+        fn = getattr(lib, "kla_b200_" + name)
+        fn.restype = c_int
+        fn.argtypes = [POINTER(MlpArgs), c_void_p]
     lib.kla_b200_conv_step.restype = c_int
     lib.kla_b200_conv_step.argtypes = [POINTER(ConvStepArgs), c_void_p]
     lib.kla_b200_conv_seq.restype = c_int
@@ -321,7 +341,7 @@ _host = None
 _HOST_ENTRIES = (
     "scan_fwd", "scan_bwd", "slab_aggregate", "chunk_fold", "epilogue_bwd", "step", "conv_step", "step_layer",
     "linear", "token_work_bytes", "token", "add_norm", "swiglu", "argmax", "qk_norm", "conv_seq", "conv_seq_bwd", "mobius_scan_fwd", "mobius_scan_bwd", "affine_scan_fwd", "affine_scan_bwd",
-    "gated_ckpt_bytes", "gated_scan_fwd", "gated_scan_bwd", "gated_step", "ckpt_bytes", "segment_scratch_bytes", "strerror",
+    "mlp_work_bytes", "mlp_fwd", "mlp_bwd", "gated_ckpt_bytes", "gated_scan_fwd", "gated_scan_bwd", "gated_step", "ckpt_bytes", "segment_scratch_bytes", "strerror",
 )
 
 

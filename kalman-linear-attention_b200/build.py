@@ -52,6 +52,7 @@ def _units():
                 units.append((f"scan_{kname}_{dname}_{lname}", "kla_scan_inst.cu", flags, _SCAN_DEPS))
     units.append(("scan_agg", "kla_scan_inst.cu", ["-DKLA_INST_KIND=2"], _SCAN_DEPS))
     units.append(("gated", "kla_gated.cu", [], [*_SCAN_DEPS, "kla_entry.h", "kla_gated.cuh", "kla_gated.cu", _HEADER]))
+    units.append(("mlp", "kla_mlp.cu", [], [*_SCAN_DEPS, "kla_entry.h", "kla_mlp.cuh", "kla_mlp.cu", _HEADER]))
     return units
 
 

@@ -52,6 +52,9 @@ struct Entry {
     int (*gated_fwd)(const kla_b200_gated_args *, void *) = nullptr;
     int (*gated_bwd)(const kla_b200_gated_args *, void *) = nullptr;
     int (*gated_step)(const kla_b200_gated_step_args *, void *) = nullptr;
+    size_t (*mlp_work_bytes)(const kla_b200_mlp_args *) = nullptr;
+    int (*mlp_fwd)(const kla_b200_mlp_args *, void *) = nullptr;
+    int (*mlp_bwd)(const kla_b200_mlp_args *, void *) = nullptr;
     int (*rawscan[4])(const kla_b200_rawscan_args *, void *) = {};  // Moebius forward, backward, affine forward, backward
     size_t (*ckpt_bytes)(int64_t, int64_t, int64_t, int64_t) = nullptr;
     size_t (*segment_scratch_bytes)(int64_t, int64_t, int64_t) = nullptr;
@@ -89,6 +92,9 @@ void bind(const py::dict &d) {
     take(lib.gated_fwd, d, "kla_b200_gated_scan_fwd");
     take(lib.gated_bwd, d, "kla_b200_gated_scan_bwd");
     take(lib.gated_step, d, "kla_b200_gated_step");
+    take(lib.mlp_work_bytes, d, "kla_b200_mlp_work_bytes");
+    take(lib.mlp_fwd, d, "kla_b200_mlp_fwd");
+    take(lib.mlp_bwd, d, "kla_b200_mlp_bwd");
     take(lib.ckpt_bytes, d, "kla_b200_ckpt_bytes");
     take(lib.segment_scratch_bytes, d, "kla_b200_segment_scratch_bytes");
     take(lib.strerror, d, "kla_b200_strerror");
@@ -731,6 +737,102 @@ std::tuple<Tensor, Tensor> gated_step(const Tensor &x_, const Tensor &gate_, con
     return {h, next};
 }
 
+// ---------------------------------------------------------------------------------- the gated feed-forward block
+
+int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
+// A matrix whose rows the tensor cores' loads can take: 16-byte aligned and apart. Others are copied into such rows.
+Tensor tile_rows(const Tensor &t) {
+    const int64_t n = t.size(1);
+    if ((n <= 1 || t.stride(1) == 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+        (t.size(0) <= 1 ? n % 8 == 0 : t.stride(0) % 8 == 0 && t.stride(0) >= n))
+        return t;
+    return fresh(t, {t.size(0), up8(n)}).narrow(1, 0, n).copy_(t);
+}
+int64_t row_stride(const Tensor &t) { return t.size(0) <= 1 ? up8(t.size(1)) : t.stride(0); }
+
+kla_b200_mlp_args mlp_args(const Tensor &x, const Tensor &w12, const Tensor &w3, int act) {
+    kla_b200_mlp_args a{};
+    a.rows = x.size(0); a.d = x.size(1); a.H = w3.size(1); a.out = w3.size(0);
+    a.activation = act;
+    a.x = x.data_ptr(); a.w12 = w12.data_ptr(); a.w3 = w3.data_ptr();
+    a.x_stride = row_stride(x); a.w12_stride = row_stride(w12); a.w3_stride = row_stride(w3);
+    return a;
+}
+
+// x [rows, d] -> y [rows, out]; with `train` also what the backward takes: x, w12 and w3 as they were read, h, gate and up
+std::tuple<Tensor, OptTensor, OptTensor, OptTensor, OptTensor, OptTensor> mlp_fwd(
+    const Tensor &x_, const Tensor &w12_, const Tensor &w3_, const OptTensor &b12_, const OptTensor &b3_, const OptTensor &residual_,
+    const py::object &activation, bool train) {
+    if (!x_.is_cuda()) unsupported("The b200 gated feed-forward block needs CUDA tensors; x is on " + x_.device().str() + ".");
+    int act = 0;
+    try {
+        act = act_code(activation);
+    } catch (const std::exception &) {
+        throw py::value_error("kla_b200: activation is 'silu', 'gelu', 'relu' or None");
+    }
+    require(x_.dim() == 2 && w12_.dim() == 2 && w3_.dim() == 2, "w12 and w3 are matrices, x has rows");
+    const int64_t rows_n = x_.size(0), d = x_.size(1), H = w3_.size(1), out = w3_.size(0);
+    require(w12_.size(0) == 2 * H && w12_.size(1) == d, "w12 is [2 H, d] for x [..., d] and w3 [out, H]");
+    require(d > 0 && H > 0 && out > 0, "widths are positive");
+    require(!b12_ || (b12_->dim() == 1 && b12_->size(0) == 2 * H), "b12 is [2 H]");
+    require(!b3_ || (b3_->dim() == 1 && b3_->size(0) == out), "b3 is [out]");
+    require(!residual_ || (residual_->dim() == 2 && residual_->size(0) == rows_n && residual_->size(1) == out), "residual has the output's shape");
+    for (const Tensor *t : {&x_, &w12_, &w3_, b12_ ? &*b12_ : &x_, b3_ ? &*b3_ : &x_, residual_ ? &*residual_ : &x_}) {
+        require(t->device() == x_.device(), "all tensors are on x's device");
+        if (t->scalar_type() != at::kBFloat16)
+            unsupported(std::string("The b200 gated feed-forward block runs in bfloat16, not ") + c10::toString(t->scalar_type()) + "; convert, or use it under autocast.");
+    }
+    if (!sm100(x_.device())) unsupported("The b200 kernels need an sm_100 device.");
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const OptTensor b12 = b12_ ? OptTensor(b12_->contiguous()) : b12_, b3 = b3_ ? OptTensor(b3_->contiguous()) : b3_;
+    const OptTensor residual = residual_ ? OptTensor(rows(*residual_)) : residual_;
+    if (!train && act == KLA_B200_ACT_SILU && few_rows(x_, w12_, b12, {}) && kernel_pays(rows_n, 2 * H, d) && out < kWidePlain && kernel_pays(rows_n, out, H) && H % 8 == 0) {
+        // a token: the projections of the decode kernels, which read the weights once with all SMs
+        const OptTensor none;
+        Extra e{none};
+        e.swiglu = true;
+        const Tensor h = linear_rows(x_, w12_, b12, e, false);
+        if (few_rows(h, w3_, b3, {})) return {linear_rows(h, w3_, b3, Extra{none, 0.0, residual}, false), {}, {}, {}, {}, {}};
+    }
+    const Tensor x = tile_rows(x_), w12 = tile_rows(w12_), w3 = tile_rows(w3_);
+    kla_b200_mlp_args a = mlp_args(x, w12, w3, act);
+    const int64_t Hp = up8(H);
+    Tensor y = fresh(x, {rows_n, out}), h = fresh(x, {rows_n, Hp});
+    OptTensor gu;
+    if (train) gu = fresh(x, {rows_n, 2 * Hp});
+    a.b12 = b12 ? b12->data_ptr() : nullptr; a.b3 = b3 ? b3->data_ptr() : nullptr;
+    if (residual) { a.residual = residual->data_ptr(); a.residual_stride = rows_n <= 1 ? out : residual->stride(0); }
+    a.h = h.data_ptr(); a.h_stride = Hp;
+    if (gu) { a.gu = gu->data_ptr(); a.gu_stride = 2 * Hp; }
+    a.y = y.data_ptr(); a.y_stride = out;
+    check(lib.mlp_fwd(&a, stream_of(x)));
+    if (!train) return {y, {}, {}, {}, {}, {}};
+    return {y, x, w12, w3, h, gu};
+}
+
+// -> dx, dw12, dw3, db12, db3, each where wanted
+std::tuple<OptTensor, OptTensor, OptTensor, OptTensor, OptTensor> mlp_bwd(
+    const Tensor &dy_, const Tensor &x, const Tensor &w12, const Tensor &w3, const Tensor &h, const Tensor &gu, int64_t d, const py::object &activation,
+    const std::vector<bool> &want) {
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor dy = tile_rows(dy_.scalar_type() == at::kBFloat16 ? dy_ : dy_.to(at::kBFloat16));
+    kla_b200_mlp_args a = mlp_args(x, w12, w3, act_code(activation));
+    a.dy = dy.data_ptr(); a.dy_stride = row_stride(dy);
+    a.h = h.data_ptr(); a.h_stride = h.size(1);
+    a.gu = gu.data_ptr(); a.gu_stride = gu.size(1);
+    auto make = [&](bool on, at::IntArrayRef sizes) { return on ? OptTensor(fresh(x, sizes)) : OptTensor(); };
+    OptTensor dx = make(want[0], {a.rows, d}), dw12 = make(want[1], {2 * a.H, d}), dw3 = make(want[2], {a.out, a.H}),
+              db12 = make(want[3], {2 * a.H}), db3 = make(want[4], {a.out});
+    auto ptr = [](const OptTensor &t) { return t ? t->data_ptr() : nullptr; };
+    a.dx = ptr(dx); a.dx_stride = d; a.dw12 = ptr(dw12); a.dw3 = ptr(dw3); a.db12 = ptr(db12); a.db3 = ptr(db3);
+    const Tensor dgu = fresh(x, {want[0] || want[1] || want[3] ? a.rows : 0, gu.size(1)});
+    const Tensor work = fresh(x, {want[1] || want[2] || want[3] || want[4] ? (int64_t)lib.mlp_work_bytes(&a) : 0}, at::kByte);
+    a.dgu = dgu.data_ptr();
+    a.work = work.data_ptr();
+    check(lib.mlp_bwd(&a, stream_of(x)));
+    return {dx, dw12, dw3, db12, db3};
+}
+
 // ------------------------------------------------------------------------------------------ a token as one kernel
 
 py::object entry(const py::dict &d, const char *name) {
@@ -1093,6 +1195,8 @@ PYBIND11_MODULE(_kla_host, m) {
     m.def("conv_seq", &conv_seq);
     m.def("conv_seq_bwd", &conv_seq_bwd);
     m.def("rawscan", &rawscan);
+    m.def("mlp_fwd", &mlp_fwd);
+    m.def("mlp_bwd", &mlp_bwd);
     m.def("gated_fwd", &gated_fwd);
     m.def("gated_bwd", &gated_bwd);
     m.def("gated_step", &gated_step);

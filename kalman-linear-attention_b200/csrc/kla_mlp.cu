@@ -1,0 +1,260 @@
+// Entry points of the gated feed-forward block (kla_mlp.cuh): argument checks, tensor maps, tile choice, launches.
+#include <cstring>
+
+#include "../../include/kla_b200.h"
+#include "kla_entry.h"
+#include "kla_launch.cuh"
+#include "kla_mlp.cuh"
+
+namespace {
+
+using namespace kla;
+
+bool aligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+bool rows_of_16(const void *p, int64_t stride) { return aligned(p, 16) && stride % 8 == 0; }
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
+
+// A [halves][outer][inner] bfloat16 tensor of boxes box_inner x box_outer in the 128-byte swizzle.
+int make_map(CUtensorMap *tm, const void *p, int64_t inner, int64_t outer, int64_t stride, int64_t halves, int64_t half_stride, int box_outer) {
+    entry::EncodeTiledFn enc = entry::encode_tiled_fn();
+    if (enc == nullptr) return KLA_B200_EUNSUPPORTED;
+    const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)halves};
+    const cuuint64_t strides[2] = {(cuuint64_t)stride * 2, (cuuint64_t)(halves > 1 ? half_stride : stride * outer) * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_outer, 1}, ones[3] = {1, 1, 1};
+    const CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? KLA_B200_OK : KLA_B200_EINVAL;
+}
+
+// An operand in memory: `rows` of the product by the summed axis. adjacent_rows: the rows are the adjacent axis.
+struct Operand {
+    const void *p;
+    int64_t stride, half_stride;
+    bool adjacent_rows;
+    int halves;
+};
+struct Product {
+    Operand a, b;
+    int64_t M, N, K;  // N, K of one half where halves are
+    int mode;
+    bool gated() const { return b.halves == kHalvesBoth; }
+};
+struct Plan {
+    int BN, tiles_m, tiles_n, splits;
+};
+
+// Columns of a tile and shares of the summed axis: the least time of the busiest CTA, counted in blocks of 128 x 256 x 64. A block of
+// fewer columns costs more than its share, A being read all the same.
+Plan plan(const Product &p, bool may_split, int sms) {
+    const int64_t tm = up(p.M, kMlpBM) * (p.a.halves == kHalvesRows ? 2 : 1);
+    const int64_t blocks = up(p.K, kMlpBK) * (p.a.halves == kHalvesSummed ? 2 : 1);
+    Plan best{};
+    double least = 0.0;
+    for (const int bn : {256, 192, 128, 64}) {
+        if (p.gated() && bn % 128) continue;
+        const double cost = bn == 256 ? 1.0 : bn == 192 ? 0.8 : bn == 128 ? 0.62 : 0.5;
+        const int64_t tn = up(p.N, p.gated() ? bn / 2 : bn), tiles = tm * tn;
+        for (int s = 1; s <= (may_split ? 32 : 1) && s <= blocks; ++s) {
+            // a tile's end (the last epilogue, filling the ring) is about 3 blocks; partial sums are written and read again
+            const double t = (double)up(tiles * s, sms) * (up(blocks, s) * cost + (may_split ? 1.0 : 0.0)) + 3.0 + (s > 1 ? 4.0 + 0.3 * s * tiles / sms : 0.0);
+            if (best.BN == 0 || t < least) { best = Plan{bn, (int)tm, (int)tn, s}; least = t; }
+        }
+    }
+    return best;
+}
+
+int fill(MlpParams *prm, const Product &p, const Plan &pl) {
+    *prm = MlpParams{};
+    const int64_t mh = p.a.halves == kHalvesNone ? 1 : 2, nh = p.b.halves == kHalvesNone ? 1 : 2;
+    int rc = p.a.adjacent_rows ? make_map(&prm->map_a, p.a.p, p.M, p.K, p.a.stride, mh, p.a.half_stride, kMlpBK)
+                               : make_map(&prm->map_a, p.a.p, p.K, p.M, p.a.stride, mh, p.a.half_stride, kMlpBM);
+    if (rc) return rc;
+    rc = p.b.adjacent_rows ? make_map(&prm->map_b, p.b.p, p.N, p.K, p.b.stride, nh, p.b.half_stride, kMlpBK)
+                           : make_map(&prm->map_b, p.b.p, p.K, p.N, p.b.stride, nh, p.b.half_stride, p.gated() ? pl.BN / 2 : pl.BN);
+    if (rc) return rc;
+    prm->a = MlpOperand{p.a.adjacent_rows, p.a.halves};
+    prm->b = MlpOperand{p.b.adjacent_rows, p.b.halves};
+    prm->M = (int)p.M; prm->N = (int)p.N; prm->K = (int)p.K;
+    prm->BN = pl.BN; prm->tiles_m = pl.tiles_m; prm->tiles_n = pl.tiles_n; prm->splits = pl.splits;
+    prm->blocks_stretch = (int)up(p.K, kMlpBK);
+    prm->blocks_k = prm->blocks_stretch * (p.a.halves == kHalvesSummed ? 2 : 1);
+    return entry::wait_ctl(&prm->wait);
+}
+
+template <int MODE>
+int launch(const MlpParams &prm, cudaStream_t st) {
+    const cudaError_t set = cudaFuncSetAttribute(kla_mlp_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMlpSmem);
+    if (set != cudaSuccess) return entry::cuda_fail(set);
+    const int64_t tiles = (int64_t)prm.tiles_m * prm.tiles_n * prm.splits;
+    if (tiles > 0x3fffffffll) return KLA_B200_EUNSUPPORTED;
+    const int grid = (int)(tiles < device_sms() ? tiles : device_sms());
+    kla_mlp_kernel<MODE><<<grid, kMlpThreads, kMlpSmem, st>>>(prm);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return entry::cuda_fail(e);
+    entry::count_launch();
+    return KLA_B200_OK;
+}
+
+Product product(const Operand &a, const Operand &b, int64_t M, int64_t N, int64_t K, int mode) { return Product{a, b, M, N, K, mode}; }
+Operand plain(const void *p, int64_t stride, bool adjacent_rows = false) { return Operand{p, stride, 0, adjacent_rows, kHalvesNone}; }
+
+Product product_gate_up(const kla_b200_mlp_args &a) {
+    return product(plain(a.x, a.x_stride), Operand{a.w12, a.w12_stride, a.w12_stride * a.H, false, kHalvesBoth}, a.rows, a.H, a.d, kMlpGated);
+}
+Product product_down(const kla_b200_mlp_args &a) { return product(plain(a.h, a.h_stride), plain(a.w3, a.w3_stride), a.rows, a.out, a.H, kMlpPlain); }
+Product product_dgu(const kla_b200_mlp_args &a) { return product(plain(a.dy, a.dy_stride), plain(a.w3, a.w3_stride, true), a.rows, a.H, a.out, kMlpGrad); }
+Product product_dx(const kla_b200_mlp_args &a) {
+    return product(Operand{a.dgu, a.gu_stride, a.gu_stride / 2, false, kHalvesSummed},
+                   Operand{a.w12, a.w12_stride, a.w12_stride * a.H, true, kHalvesSummed}, a.rows, a.d, a.H, kMlpPlain);
+}
+Product product_dw3(const kla_b200_mlp_args &a) { return product(plain(a.dy, a.dy_stride, true), plain(a.h, a.h_stride, true), a.out, a.H, a.rows, kMlpPartial); }
+Product product_dw12(const kla_b200_mlp_args &a) {
+    return product(Operand{a.dgu, a.gu_stride, a.gu_stride / 2, true, kHalvesRows}, plain(a.x, a.x_stride, true), a.H, a.d, a.rows, kMlpPartial);
+}
+
+int64_t weight_rows(const Product &p) { return p.M * (p.a.halves == kHalvesRows ? 2 : 1); }
+size_t partial_bytes(const Product &p, int sms) { return (size_t)plan(p, true, sms).splits * weight_rows(p) * up(p.N, 4) * 4 * sizeof(float); }
+size_t sum_bytes(int64_t rows, int64_t cols) { return (size_t)up(rows, kMlpSumRows) * cols * sizeof(float); }
+
+// The gradient of a weight: partial sums of shares of the rows, then their sum.
+int weight_gradient(const Product &p, void *out, float *work, cudaStream_t st) {
+    const Plan pl = plan(p, true, device_sms());
+    MlpParams prm;
+    if (const int rc = fill(&prm, p, pl)) return rc;
+    prm.partial = work;
+    prm.partial_stride = up(p.N, 4) * 4;
+    prm.partial_rows = weight_rows(p);
+    if (const int rc = launch<kMlpPartial>(prm, st)) return rc;
+    MlpReduceParams r{work, prm.partial_rows * prm.partial_stride, prm.partial_stride, pl.splits, (int)prm.partial_rows, (int)p.N,
+                      static_cast<__nv_bfloat16 *>(out)};
+    const int64_t grid = up(prm.partial_rows * up(p.N, 4), 256);
+    kla_mlp_reduce_kernel<<<(unsigned)grid, 256, 0, st>>>(r);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return entry::cuda_fail(e);
+    entry::count_launch();
+    return KLA_B200_OK;
+}
+
+int row_sums(const void *x, int64_t stride, int64_t rows, int64_t cols, float *work, void *out, cudaStream_t st) {
+    const int64_t stretches = up(rows, kMlpSumRows);
+    MlpSumParams s{static_cast<const __nv_bfloat16 *>(x), stride, (int)rows, (int)cols, work};
+    kla_mlp_rowsum_kernel<<<dim3((unsigned)up(cols, 64), (unsigned)stretches), 256, 0, st>>>(s);
+    MlpSumEndParams e{work, (int)stretches, (int)cols, static_cast<__nv_bfloat16 *>(out)};
+    kla_mlp_rowsum_end_kernel<<<(unsigned)up(cols, 256), 256, 0, st>>>(e);
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return entry::cuda_fail(err);
+    entry::count_launch();
+    entry::count_launch();
+    return KLA_B200_OK;
+}
+
+int check_sizes(const kla_b200_mlp_args *a) {
+    if (a == nullptr || a->rows < 0 || a->d <= 0 || a->H <= 0 || a->out <= 0) return KLA_B200_EINVAL;
+    if (a->activation < KLA_B200_ACT_SILU || a->activation > KLA_B200_ACT_NONE) return KLA_B200_EINVAL;
+    // row sums walk stretches of kMlpSumRows rows as a grid's second axis; coordinates of tensor maps are 32 bits
+    if (a->rows > 65535ll * kMlpSumRows || a->d > (1 << 24) || a->H > (1 << 24) || a->out > (1 << 24)) return KLA_B200_EUNSUPPORTED;
+    return KLA_B200_OK;
+}
+// an operand of the tensor cores: rows of `width` elements, 16 bytes at a time
+int check_operand(const void *p, int64_t stride, int64_t width) {
+    if (p == nullptr || stride < width) return KLA_B200_EINVAL;
+    return rows_of_16(p, stride) ? KLA_B200_OK : KLA_B200_EALIGN;
+}
+int check_plain(const void *p, int64_t stride, int64_t width) {
+    if (p == nullptr || stride < width) return KLA_B200_EINVAL;
+    return aligned(p, 2) ? KLA_B200_OK : KLA_B200_EALIGN;
+}
+
+}  // namespace
+
+extern "C" {
+
+int kla_b200_mlp_fwd(const kla_b200_mlp_args *a, void *stream) {
+    int rc = check_sizes(a);
+    if (rc) return rc;
+    if (a->rows == 0) return KLA_B200_OK;
+    if ((rc = check_operand(a->x, a->x_stride, a->d)) || (rc = check_operand(a->w12, a->w12_stride, a->d)) || (rc = check_operand(a->w3, a->w3_stride, a->H)) ||
+        (rc = check_operand(a->h, a->h_stride, a->H)) || (rc = check_plain(a->y, a->y_stride, a->out)))
+        return rc;
+    if (a->gu != nullptr && (a->gu_stride % 16 || (rc = check_operand(a->gu, a->gu_stride, 2 * a->H)))) return rc ? rc : KLA_B200_EALIGN;
+    if (a->residual != nullptr && (rc = check_plain(a->residual, a->residual_stride, a->out))) return rc;
+    if (!aligned(a->b12, 2) || !aligned(a->b3, 2)) return KLA_B200_EALIGN;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int sms = device_sms();
+    MlpParams prm;
+    const Product first = product_gate_up(*a), second = product_down(*a);
+    if ((rc = fill(&prm, first, plan(first, false, sms)))) return rc;
+    prm.act = a->activation;
+    prm.bias = static_cast<const __nv_bfloat16 *>(a->b12);
+    prm.out = static_cast<__nv_bfloat16 *>(a->h); prm.out_stride = a->h_stride; prm.out_vec = 1;
+    prm.gu = static_cast<__nv_bfloat16 *>(a->gu); prm.gu_stride = a->gu_stride; prm.gu_half = a->gu_stride / 2;
+    if ((rc = launch<kMlpGated>(prm, st))) return rc;
+    if ((rc = fill(&prm, second, plan(second, false, sms)))) return rc;
+    prm.bias = static_cast<const __nv_bfloat16 *>(a->b3);
+    prm.out = static_cast<__nv_bfloat16 *>(a->y); prm.out_stride = a->y_stride; prm.out_vec = rows_of_16(a->y, a->y_stride);
+    prm.side = static_cast<const __nv_bfloat16 *>(a->residual); prm.side_stride = a->residual_stride;
+    prm.side_vec = rows_of_16(a->residual, a->residual_stride);
+    return launch<kMlpPlain>(prm, st);
+}
+
+size_t kla_b200_mlp_work_bytes(const kla_b200_mlp_args *a) {
+    if (check_sizes(a) || a->rows == 0) return 0;
+    const int sms = device_sms();
+    size_t n = partial_bytes(product_dw3(*a), sms);
+    for (const size_t m : {partial_bytes(product_dw12(*a), sms), sum_bytes(a->rows, 2 * a->H), sum_bytes(a->rows, a->out)}) n = m > n ? m : n;
+    return n;
+}
+
+int kla_b200_mlp_bwd(const kla_b200_mlp_args *a, void *stream) {
+    int rc = check_sizes(a);
+    if (rc) return rc;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (!aligned(a->dw12, 16) || !aligned(a->dw3, 16) || !aligned(a->db12, 2) || !aligned(a->db3, 2) || !aligned(a->work, 16)) return KLA_B200_EALIGN;
+    if (a->rows == 0) {
+        const struct { void *p; int64_t n; } sums[4] = {{a->dw12, 2 * a->H * a->d}, {a->dw3, a->out * a->H}, {a->db12, 2 * a->H}, {a->db3, a->out}};
+        for (const auto &s : sums)
+            if (s.p != nullptr) {
+                const cudaError_t e = cudaMemsetAsync(s.p, 0, (size_t)s.n * 2, st);
+                if (e != cudaSuccess) return entry::cuda_fail(e);
+            }
+        return KLA_B200_OK;
+    }
+    const bool inner = a->dx != nullptr || a->dw12 != nullptr || a->db12 != nullptr;
+    if ((rc = check_operand(a->dy, a->dy_stride, a->out))) return rc;
+    if (inner) {
+        if ((rc = check_operand(a->w3, a->w3_stride, a->H)) || (rc = check_operand(a->gu, a->gu_stride, 2 * a->H)) || (rc = check_operand(a->dgu, a->gu_stride, 2 * a->H)))
+            return rc;
+        if (a->gu_stride % 16) return KLA_B200_EALIGN;
+    }
+    if (a->dx != nullptr && ((rc = check_operand(a->w12, a->w12_stride, a->d)) || (rc = check_plain(a->dx, a->dx_stride, a->d)))) return rc;
+    if (a->dw12 != nullptr && (rc = check_operand(a->x, a->x_stride, a->d))) return rc;
+    if (a->dw3 != nullptr && (rc = check_operand(a->h, a->h_stride, a->H))) return rc;
+    if ((a->dw12 || a->dw3 || a->db12 || a->db3) && a->work == nullptr) return KLA_B200_EINVAL;
+    const int sms = device_sms();
+    float *work = static_cast<float *>(a->work);
+    MlpParams prm;
+    if (a->dw3 != nullptr && (rc = weight_gradient(product_dw3(*a), a->dw3, work, st))) return rc;
+    if (a->db3 != nullptr && (rc = row_sums(a->dy, a->dy_stride, a->rows, a->out, work, a->db3, st))) return rc;
+    if (!inner) return KLA_B200_OK;
+    const Product dgu = product_dgu(*a);
+    if ((rc = fill(&prm, dgu, plan(dgu, false, sms)))) return rc;
+    prm.act = a->activation;
+    prm.side = static_cast<const __nv_bfloat16 *>(a->gu); prm.side_stride = a->gu_stride; prm.side_half = a->gu_stride / 2; prm.side_vec = 1;
+    prm.out = static_cast<__nv_bfloat16 *>(a->dgu); prm.out_stride = a->gu_stride; prm.out_half = a->gu_stride / 2; prm.out_vec = 1;
+    if ((rc = launch<kMlpGrad>(prm, st))) return rc;
+    if (a->dx != nullptr) {
+        const Product dx = product_dx(*a);
+        if ((rc = fill(&prm, dx, plan(dx, false, sms)))) return rc;
+        prm.out = static_cast<__nv_bfloat16 *>(a->dx); prm.out_stride = a->dx_stride; prm.out_vec = rows_of_16(a->dx, a->dx_stride);
+        if ((rc = launch<kMlpPlain>(prm, st))) return rc;
+    }
+    if (a->dw12 != nullptr && (rc = weight_gradient(product_dw12(*a), a->dw12, work, st))) return rc;
+    if (a->db12 != nullptr) {
+        __nv_bfloat16 *g = static_cast<__nv_bfloat16 *>(a->dgu), *out = static_cast<__nv_bfloat16 *>(a->db12);
+        if ((rc = row_sums(g, a->gu_stride, a->rows, a->H, work, out, st))) return rc;
+        if ((rc = row_sums(g + a->gu_stride / 2, a->gu_stride, a->rows, a->H, work, out + a->H, st))) return rc;
+    }
+    return KLA_B200_OK;
+}
+
+}  // extern "C"

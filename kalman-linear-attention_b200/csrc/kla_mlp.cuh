@@ -1,0 +1,532 @@
+// The gated feed-forward block on the tensor cores, forward and backward, bfloat16 with float32 accumulation:
+//
+//   g = x Wg^T + bg,  u = x Wu^T + bu,  h = act(g) u,  y = h W3^T + b3 (+ residual)
+//   dh = dy W3,  dg = dh u act'(g),  du = dh act(g);   dx = [dg du] W12,  dW12 = [dg du]^T x,  dW3 = dy^T h
+//
+// One kernel takes all six products; what differs is how its operands lie in memory and what its epilogue does:
+//   * x Wg^T and x Wu^T are one product whose B tile is rows of Wg beside the same rows of Wu, so that the accumulator holds
+//     gate and up of the same columns: the epilogue adds the biases and writes act(g) u (in training g and u, too);
+//   * dy W3 turns into dg and du in its epilogue, from the stored g and u;
+//   * sums over the rows (the weights' gradients) have few output tiles and a long axis: it is split over CTAs, whose float32
+//     partial sums a second kernel adds in a fixed order.
+// An operand whose summed axis is not the adjacent one in memory (W3, W12, and both of a weight's gradient) is read as it is, as
+// an MN-major operand of the tensor core; nothing is transposed in memory.
+//
+// A CTA per SM walks output tiles of 128 x BN. One warp issues TMA loads of 64-wide blocks of the summed axis into a ring of
+// kMlpStages, one thread issues tcgen05.mma from them into one of two accumulators in tensor memory, eight warps empty the
+// other accumulator meanwhile, through a stage of shared memory that turns a thread's row into coalesced 64-byte pieces.
+// Rows and columns past the ends are zeros of the TMA loads; widths that are no multiple of a tile cost only the padding.
+#pragma once
+
+#include "kla_common.cuh"
+
+namespace kla {
+
+constexpr int kMlpBM = 128, kMlpBK = 64, kMlpMaxBN = 256;
+constexpr int kMlpStages = 4;
+constexpr int kMlpEpiWarps = 8;
+constexpr int kMlpThreads = (4 + kMlpEpiWarps) * 32;
+constexpr int kMlpStageBytes = (kMlpBM + kMlpMaxBN) * kMlpBK * 2;
+constexpr int kMlpPitch = 80;  // bytes of a row of a warp's stage: 64 and 16 more, so that rows start in different banks
+constexpr int kMlpEpiBytes = kMlpEpiWarps * 32 * kMlpPitch;
+constexpr size_t kMlpSmem = 1024 + (size_t)kMlpStages * kMlpStageBytes + kMlpEpiBytes + 256;
+
+// wait sites of the status word
+constexpr int kMlpSiteEmpty = 0x40, kMlpSiteFull = 0x41, kMlpSiteAccEmpty = 0x42, kMlpSiteAccFull = 0x43, kMlpSiteDrain = 0x44;
+
+enum MlpMode {
+    kMlpPlain = 0,   // out = acc (+ bias) (+ residual)
+    kMlpGated = 1,   // out = act(gate) up; optionally gate and up themselves
+    kMlpGrad = 2,    // out = gradients of gate and up
+    kMlpPartial = 3  // float32 sums of a share of the summed axis
+};
+
+// How an operand's tile is fetched: rows are the product's m or n.
+enum MlpHalves {
+    kHalvesNone = 0,
+    kHalvesSummed = 1,  // the summed axis is two stretches of `stretch` (third coordinate of the tensor map)
+    kHalvesRows = 2,    // the rows are: tiles do not cross
+    kHalvesBoth = 3     // a tile is rows of the first beside the same rows of the second (gate and up)
+};
+struct MlpOperand {
+    int mn_major;  // rows are adjacent in memory, not the summed axis
+    int halves;
+};
+
+struct MlpParams {
+    CUtensorMap map_a, map_b;
+    MlpOperand a, b;
+    int M, N, K;       // rows, columns (of one half where halves are rows), summed length (of one stretch)
+    int BN;            // columns of a tile (gated: of gate and up together)
+    int tiles_m, tiles_n, splits;
+    int blocks_k;      // 64-wide blocks of the summed axis, all stretches
+    int blocks_stretch;
+    int act;
+    __nv_bfloat16 *out;
+    long long out_stride, out_half;  // elements; out_half: to the rows or columns of the second half
+    int out_vec;                     // rows can be written 16 bytes at a time
+    const __nv_bfloat16 *bias;       // [N], gated [2][N]
+    const __nv_bfloat16 *side;       // residual [M, N], grad: gate and up
+    long long side_stride, side_half;
+    int side_vec;
+    __nv_bfloat16 *gu;               // gated, training: gate and up, rows of gu_stride, up gu_half behind
+    long long gu_stride, gu_half;
+    float *partial;                  // [splits][M (both halves)][partial_stride]
+    long long partial_stride, partial_rows;
+    WaitCtl wait;
+};
+
+__device__ __forceinline__ uint64_t global_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+// A bounded wait without sleeps (mbarrier.try_wait suspends the thread by itself); gives up like mbar_wait.
+__device__ __forceinline__ bool mlp_wait(const WaitCtl &w, uint64_t *bar, uint32_t parity, int site) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t begin = global_ns();
+    do {
+        for (int i = 0; i < 32; ++i)
+            if (mbar_try_wait(bar, parity)) return true;
+    } while (global_ns() - begin < w.limit_ns);
+    atomicCAS(w.status, 0, kStatusWait | site);
+    return false;
+}
+
+// Shared memory descriptor of an operand tile in the 128-byte swizzle: 8 rows of 128 bytes make an atom of 1024.
+//   summed axis adjacent: a row of 64 summed elements per m or n; atoms of 8 rows follow one another (stride offset)
+//   rows adjacent: a line of 64 m or n per summed element; atoms of 8 summed elements follow one another (stride offset), the
+//   next 64 rows lie a whole box of 64 x 64 further (leading offset)
+__device__ __forceinline__ uint64_t mlp_desc(uint32_t addr, bool mn_major) {
+    uint64_t d = (uint64_t)((addr & 0x3ffffu) >> 4);
+    d |= (uint64_t)(mn_major ? kMlpBK * 128 / 16 : 1) << 16;
+    d |= (uint64_t)(1024 / 16) << 32;
+    d |= 1ull << 46;  // sm_100
+    d |= 2ull << 61;  // 128-byte swizzle
+    return d;
+}
+
+__device__ __forceinline__ void mlp_mma(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(acc), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+}
+__device__ __forceinline__ void mlp_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_load32(float (&v)[32], uint32_t addr) {
+    uint32_t *r = reinterpret_cast<uint32_t *>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tcgen05_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tcgen05_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// A warp's stage: 32 rows of 64 bytes. Rows go in and out a row per lane; memory is walked four lanes to a row.
+struct MlpStage {
+    char *base;
+    int lane;
+    __device__ __forceinline__ void put_row(const uint4 (&v)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(base + lane * kMlpPitch + 16 * i) = v[i];
+        __syncwarp();
+    }
+    __device__ __forceinline__ void get_row(uint4 (&v)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4 *>(base + lane * kMlpPitch + 16 * i);
+        __syncwarp();
+    }
+    // E: element type; rows x cols of them are there
+    template <typename E>
+    __device__ __forceinline__ void store(E *p, long long stride, int rows, int cols, bool vec) const {
+        constexpr int per = 16 / sizeof(E);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + lane / 4, c = lane % 4 * per;
+            const char *from = base + r * kMlpPitch + lane % 4 * 16;
+            if (r < rows) {
+                E *to = p + r * stride + c;
+                if (vec && c + per <= cols) {
+                    *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(from);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < per; ++e)
+                        if (c + e < cols) to[e] = reinterpret_cast<const E *>(from)[e];
+                }
+            }
+        }
+        __syncwarp();
+    }
+    // zeros where there are none
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p, long long stride, int rows, int cols, bool vec) const {
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + lane / 4, c = lane % 4 * 8;
+            v[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (r < rows) {
+                const __nv_bfloat16 *from = p + r * stride + c;
+                if (vec && c + 8 <= cols) {
+                    v[i] = __ldg(reinterpret_cast<const uint4 *>(from));
+                } else {
+                    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (c + e < cols) w[e / 2] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(from) + e) << (e % 2 * 16);
+                    v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(base + (i * 8 + lane / 4) * kMlpPitch + lane % 4 * 16) = v[i];
+        __syncwarp();
+    }
+};
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ void pack_row(uint4 (&v)[4], const float (&x)[32]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v[i] = make_uint4(pack2(x[8 * i], x[8 * i + 1]), pack2(x[8 * i + 2], x[8 * i + 3]), pack2(x[8 * i + 4], x[8 * i + 5]), pack2(x[8 * i + 6], x[8 * i + 7]));
+}
+__device__ __forceinline__ float row_at(const uint4 (&v)[4], int j) {  // j a constant after unrolling
+    const uint32_t w = j / 2 % 4 == 0 ? v[j / 8].x : j / 2 % 4 == 1 ? v[j / 8].y : j / 2 % 4 == 2 ? v[j / 8].z : v[j / 8].w;
+    return j % 2 ? __uint_as_float(w & 0xffff0000u) : __uint_as_float(w << 16);
+}
+
+// The activation and its derivative.
+template <bool SLOPE>
+__device__ __forceinline__ void mlp_act(float g, int act, float &f, float &df) {
+    if (act == 0) {  // silu
+        const float s = rcp_approx(1.0f + exp2f(-g * 1.4426950408889634f));
+        f = g * s;
+        if (SLOPE) df = fmaf(f, 1.0f - s, s);
+    } else if (act == 1) {  // gelu
+        const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+        f = g * cdf;
+        if (SLOPE) df = fmaf(g * 0.3989422804014327f, exp2f(-0.72134752044448170f * g * g), cdf);
+    } else if (act == 2) {  // relu; NaN stays
+        f = g < 0.0f ? 0.0f : g;
+        if (SLOPE) df = g > 0.0f ? 1.0f : 0.0f;
+    } else {
+        f = g;
+        if (SLOPE) df = 1.0f;
+    }
+}
+
+struct MlpTile {
+    int m, n, split;    // first row (of its half), first column (gated: of gate), share of the summed axis
+    int m_half;
+    int k0, k1;         // blocks
+};
+__device__ __forceinline__ MlpTile mlp_tile(const MlpParams &p, int t) {
+    MlpTile r;
+    const int per = p.tiles_m * p.tiles_n;
+    r.split = t / per;
+    t -= r.split * per;
+    const int tm = t / p.tiles_n, tn = t - tm * p.tiles_n;
+    const int per_half = p.a.halves == kHalvesRows ? p.tiles_m / 2 : p.tiles_m;
+    r.m_half = tm / per_half;
+    r.m = (tm - r.m_half * per_half) * kMlpBM;
+    r.n = tn * (p.b.halves == kHalvesBoth ? p.BN / 2 : p.BN);
+    r.k0 = (int)((long long)p.blocks_k * r.split / p.splits);
+    r.k1 = (int)((long long)p.blocks_k * (r.split + 1) / p.splits);
+    return r;
+}
+
+__device__ __forceinline__ void mlp_fetch(void *dst, const CUtensorMap *map, const MlpOperand &op, int row, int rows, int k, int half, uint64_t *bar) {
+    char *at = static_cast<char *>(dst);
+    if (op.mn_major) {
+        for (int r = 0; r < rows; r += 64) tma_load_3d(at + r * 128, map, row + r, k, half, bar);
+    } else if (op.halves == kHalvesBoth) {
+        tma_load_3d(at, map, k, row, 0, bar);
+        tma_load_3d(at + rows / 2 * 128, map, k, row, 1, bar);
+    } else {
+        tma_load_3d(at, map, k, row, half, bar);
+    }
+}
+
+template <int MODE>
+__global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_constant__ MlpParams prm) {
+    extern __shared__ char raw[];
+    char *smem = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    char *epi = smem + kMlpStages * kMlpStageBytes;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(epi + kMlpEpiBytes);
+    uint64_t *full = bars, *empty = bars + kMlpStages, *acc_full = empty + kMlpStages, *acc_empty = acc_full + 2, *drain = acc_empty + 2;
+    uint32_t *tmem_at = reinterpret_cast<uint32_t *>(drain + 1);
+    int *failed = reinterpret_cast<int *>(tmem_at + 1);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kMlpStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], kMlpEpiWarps); }
+        mbar_init(drain, 1);
+        *failed = 0;
+        mbar_fence_init();
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_at)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tcgen05_before_sync();
+    __syncthreads();
+    tcgen05_after_sync();
+    const uint32_t tmem = *tmem_at;
+    const int tiles = prm.tiles_m * prm.tiles_n * prm.splits;
+    int issued = 0;  // producer: blocks whose loads were issued
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const uint32_t bytes = (kMlpBM + prm.BN) * kMlpBK * 2;
+            int block = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+                const MlpTile tl = mlp_tile(prm, t);
+                for (int kb = tl.k0; kb < tl.k1; ++kb, ++block) {
+                    const int s = block % kMlpStages;
+                    if (block >= kMlpStages && !mlp_wait(prm.wait, &empty[s], (block / kMlpStages + 1) & 1, kMlpSiteEmpty)) { ok = false; break; }
+                    if (block == prm.wait.skip_tile) { ok = false; break; }  // the tests' incomplete hand-over: nothing more is issued
+                    char *at = smem + s * kMlpStageBytes;
+                    const int stretch = kb / prm.blocks_stretch, k = (kb - stretch * prm.blocks_stretch) * kMlpBK;
+                    mbar_arrive_expect_tx(&full[s], bytes);
+                    mlp_fetch(at, &prm.map_a, prm.a, tl.m, kMlpBM, k, prm.a.halves == kHalvesRows ? tl.m_half : stretch, &full[s]);
+                    mlp_fetch(at + kMlpBM * kMlpBK * 2, &prm.map_b, prm.b, tl.n, prm.BN, k, stretch, &full[s]);
+                    issued = block + 1;
+                }
+            }
+            if (!ok) *failed = 1;
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // float32 accumulators of bfloat16 operands; majors; N / 8; M / 16
+            const uint32_t idesc = 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(prm.a.mn_major != 0) << 15 | (uint32_t)(prm.b.mn_major != 0) << 16 |
+                                   (uint32_t)(prm.BN / 8) << 17 | (uint32_t)(kMlpBM / 16) << 24;
+            const uint64_t step_a = (prm.a.mn_major ? 2048 : 32) / 16, step_b = (prm.b.mn_major ? 2048 : 32) / 16;
+            int block = 0, acc = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x, ++acc) {
+                const MlpTile tl = mlp_tile(prm, t);
+                if (acc >= 2 && !mlp_wait(prm.wait, &acc_empty[acc % 2], (acc / 2 + 1) & 1, kMlpSiteAccEmpty)) { ok = false; break; }
+                tcgen05_after_sync();
+                const uint32_t d = tmem + acc % 2 * kMlpMaxBN;
+                for (int kb = tl.k0; kb < tl.k1; ++kb, ++block) {
+                    const int s = block % kMlpStages;
+                    if (!mlp_wait(prm.wait, &full[s], (block / kMlpStages) & 1, kMlpSiteFull)) { ok = false; break; }
+                    tcgen05_after_sync();
+                    const uint32_t at = smem_u32(smem + s * kMlpStageBytes);
+                    const uint64_t da = mlp_desc(at, prm.a.mn_major), db = mlp_desc(at + kMlpBM * kMlpBK * 2, prm.b.mn_major);
+#pragma unroll
+                    for (int i = 0; i < kMlpBK / 16; ++i) mlp_mma(d, da + i * step_a, db + i * step_b, idesc, kb > tl.k0 || i > 0);
+                    mlp_commit(&empty[s]);
+                }
+                if (ok) mlp_commit(&acc_full[acc % 2]);
+            }
+            if (!ok) *failed = 1;
+        }
+    } else if (warp >= 4) {
+        const int quad = warp % 4, part = (warp - 4) / 4;
+        const MlpStage st{epi + (warp - 4) * 32 * kMlpPitch, lane};
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        int acc = 0;
+        for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++acc) {
+            const MlpTile tl = mlp_tile(prm, t);
+            bool ok = true;
+            if (lane == 0) ok = mlp_wait(prm.wait, &acc_full[acc % 2], (acc / 2) & 1, kMlpSiteAccFull);
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (!ok) {
+                if (lane == 0) *failed = 1;
+                break;
+            }
+            tcgen05_after_sync();
+            const uint32_t d = tmem + acc % 2 * kMlpMaxBN + lanes;
+            const int m = tl.m + quad * 32, rows = prm.M - m;
+            const int width = MODE == kMlpGated ? prm.BN / 2 : prm.BN;
+            for (int c = part * (width / 2); c < (part + 1) * (width / 2); c += 32) {
+                const int n = tl.n + c, cols = prm.N - n;
+                const bool last = c + 32 >= (part + 1) * (width / 2);
+                float v[32], w[32];
+                tmem_load32(v, d + c);
+                if (MODE == kMlpGated) tmem_load32(w, d + width + c);
+                tmem_load_wait();
+                if (last) {
+                    tcgen05_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&acc_empty[acc % 2]);
+                }
+                if (cols <= 0) continue;
+                uint4 r[4];
+                if (MODE == kMlpPartial) {
+                    float *p = prm.partial + (long long)tl.split * prm.partial_rows * prm.partial_stride +
+                               ((long long)tl.m_half * prm.M + m) * prm.partial_stride + n;
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            r[i] = make_uint4(__float_as_uint(v[16 * q + 4 * i]), __float_as_uint(v[16 * q + 4 * i + 1]),
+                                              __float_as_uint(v[16 * q + 4 * i + 2]), __float_as_uint(v[16 * q + 4 * i + 3]));
+                        st.put_row(r);
+                        st.store(p + 16 * q, prm.partial_stride, rows, cols - 16 * q, true);
+                    }
+                    continue;
+                }
+                __nv_bfloat16 *out = prm.out + tl.m_half * prm.out_half + (long long)m * prm.out_stride + n;
+                if (MODE == kMlpPlain) {
+                    if (prm.bias != nullptr) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] += j < cols ? __bfloat162float(prm.bias[n + j]) : 0.0f;
+                    }
+                    if (prm.side != nullptr) {
+                        st.load(prm.side + (long long)m * prm.side_stride + n, prm.side_stride, rows, cols, prm.side_vec);
+                        st.get_row(r);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] += row_at(r, j);
+                    }
+                    pack_row(r, v);
+                    st.put_row(r);
+                    st.store(out, prm.out_stride, rows, cols, prm.out_vec);
+                } else if (MODE == kMlpGated) {
+                    if (prm.bias != nullptr) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (j < cols) {
+                                v[j] += __bfloat162float(prm.bias[n + j]);
+                                w[j] += __bfloat162float(prm.bias[prm.N + n + j]);
+                            }
+                    }
+                    if (prm.gu != nullptr) {
+                        __nv_bfloat16 *gu = prm.gu + (long long)m * prm.gu_stride + n;
+                        pack_row(r, v);
+                        st.put_row(r);
+                        st.store(gu, prm.gu_stride, rows, cols, true);
+                        pack_row(r, w);
+                        st.put_row(r);
+                        st.store(gu + prm.gu_half, prm.gu_stride, rows, cols, true);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        float f, df;
+                        mlp_act<false>(v[j], prm.act, f, df);
+                        v[j] = f * w[j];
+                    }
+                    pack_row(r, v);
+                    st.put_row(r);
+                    st.store(out, prm.out_stride, rows, cols, prm.out_vec);
+                } else {
+                    const __nv_bfloat16 *side = prm.side + (long long)m * prm.side_stride + n;
+                    uint4 up[4];
+                    st.load(side, prm.side_stride, rows, cols, true);
+                    st.get_row(r);
+                    st.load(side + prm.side_half, prm.side_stride, rows, cols, true);
+                    st.get_row(up);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        float f, df;
+                        mlp_act<true>(row_at(r, j), prm.act, f, df);
+                        w[j] = v[j] * f;                       // of up
+                        v[j] = v[j] * row_at(up, j) * df;      // of gate
+                    }
+                    pack_row(r, v);
+                    st.put_row(r);
+                    st.store(out, prm.out_stride, rows, cols, true);
+                    pack_row(r, w);
+                    st.put_row(r);
+                    st.store(out + prm.out_half, prm.out_stride, rows, cols, true);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    __syncthreads();
+    if (*failed) {  // a wait ran out: copies and products still under way end before the memory they use is given back
+        if (warp == 0 && lane == 0)
+            for (int b = max(0, issued - kMlpStages); b < issued; ++b) mlp_wait(prm.wait, &full[b % kMlpStages], (b / kMlpStages) & 1, kMlpSiteDrain);
+        if (warp == 1 && lane == 0) {
+            mlp_commit(drain);
+            mlp_wait(prm.wait, drain, 0, kMlpSiteDrain);
+        }
+        __syncwarp();
+    }
+    tcgen05_before_sync();
+    __syncthreads();
+    if (warp == 2) {
+        tcgen05_after_sync();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+// out[r][c] = sum over splits, in their order, of partial[split][r][c]; four columns a thread.
+struct MlpReduceParams {
+    const float *partial;
+    long long split_stride, stride;  // elements; stride a multiple of 4
+    int splits, rows, cols;
+    __nv_bfloat16 *out;              // [rows, cols] contiguous
+};
+__global__ void __launch_bounds__(256) kla_mlp_reduce_kernel(const MlpReduceParams prm) {
+    const int quads = (prm.cols + 3) / 4;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (long long)prm.rows * quads) return;
+    const long long r = i / quads;
+    const int c = (int)(i - r * quads) * 4;
+    const float *p = prm.partial + r * prm.stride + c;
+    float4 s = *reinterpret_cast<const float4 *>(p);
+    for (int k = 1; k < prm.splits; ++k) {
+        const float4 v = *reinterpret_cast<const float4 *>(p + k * prm.split_stride);
+        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    __nv_bfloat16 *out = prm.out + r * prm.cols + c;
+    const float v[4] = {s.x, s.y, s.z, s.w};
+    if (prm.cols % 4 == 0) {
+        *reinterpret_cast<uint2 *>(out) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < prm.cols) out[e] = __float2bfloat16_rn(v[e]);
+    }
+}
+
+// Sums over rows of a bfloat16 matrix (a bias's gradient): a block adds 64 columns of a stretch of rows, the sums of the
+// stretches are added by the same kernel's second launch in their order, as float32 [stretches][cols].
+constexpr int kMlpSumRows = 256;
+struct MlpSumParams {
+    const __nv_bfloat16 *x;
+    long long stride;
+    int rows, cols;
+    float *partial;
+};
+__global__ void __launch_bounds__(256) kla_mlp_rowsum_kernel(const MlpSumParams prm) {
+    __shared__ float part[4][64];
+    const int c = blockIdx.x * 64 + threadIdx.x % 64, g = threadIdx.x / 64;
+    const int r0 = blockIdx.y * kMlpSumRows, r1 = min(prm.rows, r0 + kMlpSumRows);
+    float s = 0.0f;
+    if (c < prm.cols)
+        for (int r = r0 + g; r < r1; r += 4) s += __bfloat162float(prm.x[(long long)r * prm.stride + c]);
+    part[g][threadIdx.x % 64] = s;
+    __syncthreads();
+    if (g == 0 && c < prm.cols)
+        prm.partial[(long long)blockIdx.y * prm.cols + c] = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
+}
+struct MlpSumEndParams {
+    const float *partial;
+    int stretches, cols;
+    __nv_bfloat16 *out;
+};
+__global__ void __launch_bounds__(256) kla_mlp_rowsum_end_kernel(const MlpSumEndParams prm) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= prm.cols) return;
+    float s = 0.0f;
+    for (int k = 0; k < prm.stretches; ++k) s += prm.partial[(long long)k * prm.cols + c];
+    prm.out[c] = __float2bfloat16_rn(s);
+}
+
+}  // namespace kla

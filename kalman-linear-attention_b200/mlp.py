@@ -1,0 +1,60 @@
+"""The gated feed-forward block on the B200 kernels:
+
+    y = (act(x Wg^T + bg) * (x Wu^T + bu)) W3^T + b3 (+ residual),    w12 = [Wg; Wu]
+
+which is the swiglu MLP of a block of the reference's ``SequenceModel`` (src/kla/layers/common.py:99-122) for ``act = silu``,
+differentiable with respect to everything it is given. Both first projections, their biases, the activation and the product are
+one kernel on the tensor cores; so are the second projection, its bias and the residual sum. The backward has no elementwise pass of
+its own either: the gradients of gate and up are formed where the gradient of their product is. bfloat16, accumulated in float32.
+For the few rows of decoded tokens in inference the projections are the decode kernels (``kla_b200_linear``). There is no CPU or
+eager path: what the kernels do not take raises ``NotImplementedError``.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+
+class _GatedMlpB200(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w12, w3, b12, b3, residual, activation):
+        y, *kept = _lib.host().mlp_fwd(x, w12, w3, b12, b3, residual, activation, True)
+        ctx.save_for_backward(*kept)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w12, w3, h, gu = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        grads = (None,) * 5
+        if any(need[:5]):
+            grads = _lib.host().mlp_bwd(dy, x, w12, w3, h, gu, x.shape[1], ctx.activation, list(need[:5]))
+        return (*grads, dy if need[5] else None, None)
+
+
+def gated_mlp_b200(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, b12: torch.Tensor | None = None, b3: torch.Tensor | None = None,
+                   residual: torch.Tensor | None = None, activation: str | None = "silu") -> torch.Tensor:
+    """``x`` ``[..., d]``, ``w12`` ``[2 H, d]`` (gate's rows, then up's), ``w3`` ``[out, H]``, ``b12`` ``[2 H]``, ``b3`` ``[out]``,
+    ``residual`` ``[..., out]`` added to the result in float32 before it is rounded. ``activation``: ``"silu"``, ``"gelu"`` (the exact
+    one), ``"relu"`` or None. Any sizes and strides: rows that are not 16-byte aligned (a width that is no multiple of 8) are copied
+    first. Under a bfloat16 autocast other floating types of ``x``, weights and biases are converted as ``F.linear`` does."""
+    if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:
+        x, w12, w3, b12, b3 = (t.to(torch.bfloat16) if t is not None and t.is_cuda else t for t in (x, w12, w3, b12, b3))
+    if x.dim() == 0:
+        raise ValueError("kla_b200: x is [..., d]")
+    lead = x.shape[:-1]
+    if residual is not None:
+        if residual.dim() == 0 or residual.shape[:-1] != lead:
+            raise ValueError("kla_b200: residual has the output's shape")
+        residual = residual.reshape(lead.numel(), residual.shape[-1])
+    rows = x.reshape(lead.numel(), x.shape[-1])
+    given = (rows, w12, w3, b12, b3, residual)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given):
+        y = _GatedMlpB200.apply(*given, activation)
+    else:
+        y = _lib.host().mlp_fwd(*given, activation, False)[0]
+    return y.view(*lead, y.shape[-1])
