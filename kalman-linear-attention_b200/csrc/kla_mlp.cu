@@ -65,6 +65,12 @@ Plan plan(const Product &p, bool may_split, int sms) {
 
 int fill(MlpParams *prm, const Product &p, const Plan &pl) {
     *prm = MlpParams{};
+    // tensor maps are made by the driver for the thread's context, which a new thread (autograd's, or a caller's) has only
+    // once the runtime has bound it
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaSetDevice(dev);
+    if (e != cudaSuccess) return entry::cuda_fail(e);
     const int64_t mh = p.a.halves == kHalvesNone ? 1 : 2, nh = p.b.halves == kHalvesNone ? 1 : 2;
     int rc = p.a.adjacent_rows ? make_map(&prm->map_a, p.a.p, p.M, p.K, p.a.stride, mh, p.a.half_stride, kMlpBK)
                                : make_map(&prm->map_a, p.a.p, p.K, p.M, p.a.stride, mh, p.a.half_stride, kMlpBM);

@@ -9,6 +9,7 @@ exponential and reciprocal by 2^-20. Errors go through products by their absolut
 
 import ctypes
 import importlib
+import threading
 
 import pytest
 import torch
@@ -252,6 +253,21 @@ def test_captured_on_another_stream_and_the_same_every_time():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_a_new_threads_first_call():
+    """Its memory comes from the allocator's cache, so nothing before the call has bound the device's context to the thread."""
+    t, _ = inputs(300, 64, 96, 64)
+    y0 = kla_b200.gated_mlp_b200(**t)
+    del_me = kla_b200.gated_mlp_b200(**t)
+    torch.cuda.synchronize()
+    del del_me  # what the thread's call takes
+    got = []
+    thread = threading.Thread(target=lambda: got.append(kla_b200.gated_mlp_b200(**t)))
+    thread.start()
+    thread.join()
+    assert len(got) == 1 and torch.equal(got[0], y0)
 
 
 @pytest.mark.gpu
