@@ -1,5 +1,5 @@
 // Entry points of the gated feed-forward block (kla_mlp.cuh): argument checks, tensor maps, tile choice, launches.
-#include <cstring>
+#include <mutex>
 
 #include "../../include/kla_b200.h"
 #include "kla_entry.h"
@@ -40,26 +40,27 @@ struct Product {
     bool gated() const { return b.halves == kHalvesBoth; }
 };
 struct Plan {
-    int BN, tiles_m, tiles_n, splits;
+    int BN, CG, tiles_m, tiles_n, splits;
 };
 
-// Columns of a tile and shares of the summed axis: the least time of the busiest CTA, counted in blocks of 128 x 256 x 64. A block of
-// fewer columns costs more than its share, A being read all the same.
+// Columns of a tile, CTAs sharing it and shares of the summed axis: the least time of the busiest CTA, counted in blocks of 128 x 256 x
+// 64 a CTA. A block of fewer columns costs more than its share, A being read all the same, and a CTA alone reads twice as much of B.
 Plan plan(const Product &p, bool may_split, int sms) {
-    const int64_t tm = up(p.M, kMlpBM) * (p.a.halves == kHalvesRows ? 2 : 1);
     const int64_t blocks = up(p.K, kMlpBK) * (p.a.halves == kHalvesSummed ? 2 : 1);
     Plan best{};
     double least = 0.0;
-    for (const int bn : {256, 192, 128, 64}) {
-        if (p.gated() && bn % 128) continue;
-        const double cost = bn == 256 ? 1.0 : bn == 192 ? 0.8 : bn == 128 ? 0.62 : 0.5;
-        const int64_t tn = up(p.N, p.gated() ? bn / 2 : bn), tiles = tm * tn;
-        for (int s = 1; s <= (may_split ? 32 : 1) && s <= blocks; ++s) {
-            // a tile's end (the last epilogue, filling the ring) is about 3 blocks; partial sums are written and read again
-            const double t = (double)up(tiles * s, sms) * (up(blocks, s) * cost + (may_split ? 1.0 : 0.0)) + 3.0 + (s > 1 ? 4.0 + 0.3 * s * tiles / sms : 0.0);
-            if (best.BN == 0 || t < least) { best = Plan{bn, (int)tm, (int)tn, s}; least = t; }
+    for (const int cg : {2, 1})
+        for (const int bn : {256, 192, 128, 64}) {
+            if (p.gated() && bn % 128) continue;
+            const double cost = (bn == 256 ? 1.0 : bn == 192 ? 0.8 : bn == 128 ? 0.62 : 0.5) * (cg == 1 ? 1.6 : 1.0);
+            const int64_t tm = up(p.M, kMlpBM * cg) * (p.a.halves == kHalvesRows ? 2 : 1);
+            const int64_t tn = up(p.N, p.gated() ? bn / 2 : bn), tiles = tm * tn;
+            for (int s = 1; s <= (may_split ? 32 : 1) && s <= blocks; ++s) {
+                // a tile's end (the last epilogue, filling the ring) is about 4 blocks; partial sums are written and read again
+                const double t = (double)up(tiles * s, sms / cg) * (up(blocks, s) * cost + (s > 1 ? 1.0 : 0.0)) + 4.0 + (s > 1 ? 5.0 + 0.3 * s * tiles * cg / sms : 0.0);
+                if (best.BN == 0 || t < least) { best = Plan{bn, cg, (int)tm, (int)tn, s}; least = t; }
+            }
         }
-    }
     return best;
 }
 
@@ -76,7 +77,7 @@ int fill(MlpParams *prm, const Product &p, const Plan &pl) {
                                : make_map(&prm->map_a, p.a.p, p.K, p.M, p.a.stride, mh, p.a.half_stride, kMlpBM);
     if (rc) return rc;
     rc = p.b.adjacent_rows ? make_map(&prm->map_b, p.b.p, p.N, p.K, p.b.stride, nh, p.b.half_stride, kMlpBK)
-                           : make_map(&prm->map_b, p.b.p, p.K, p.N, p.b.stride, nh, p.b.half_stride, p.gated() ? pl.BN / 2 : pl.BN);
+                           : make_map(&prm->map_b, p.b.p, p.K, p.N, p.b.stride, nh, p.b.half_stride, p.gated() ? pl.BN / 2 : pl.BN / pl.CG);
     if (rc) return rc;
     prm->a = MlpOperand{p.a.adjacent_rows, p.a.halves};
     prm->b = MlpOperand{p.b.adjacent_rows, p.b.halves};
@@ -87,18 +88,62 @@ int fill(MlpParams *prm, const Product &p, const Plan &pl) {
     return entry::wait_ctl(&prm->wait);
 }
 
-template <int MODE>
-int launch(const MlpParams &prm, cudaStream_t st) {
-    const cudaError_t set = cudaFuncSetAttribute(kla_mlp_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMlpSmem);
-    if (set != cudaSuccess) return entry::cuda_fail(set);
+// CTA pairs that can be resident at once: SMs without a partner in their cluster of SMs take none.
+int resident_pairs() {
+    static std::mutex mu;
+    static int pairs[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return device_sms() / 2;
+    std::lock_guard<std::mutex> lock(mu);
+    if (pairs[dev] == 0) {
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 2;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)device_sms() / 2 * 2);
+        cfg.blockDim = dim3(kMlpThreads);
+        cfg.dynamicSmemBytes = MlpRing<2>::kSmem;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, kla_mlp_kernel<kMlpPlain, 2>, &cfg) != cudaSuccess || n < 1) {
+            cudaGetLastError();
+            return device_sms() / 2;
+        }
+        pairs[dev] = n;
+    }
+    return pairs[dev];
+}
+
+template <int MODE, int CG>
+int launch_as(const MlpParams &prm, cudaStream_t st) {
+    cudaError_t e = cudaFuncSetAttribute(kla_mlp_kernel<MODE, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MlpRing<CG>::kSmem);
+    if (e == cudaSuccess && CG == 2)
+        e = cudaFuncSetAttribute(kla_mlp_kernel<kMlpPlain, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MlpRing<2>::kSmem);
+    if (e != cudaSuccess) return entry::cuda_fail(e);
     const int64_t tiles = (int64_t)prm.tiles_m * prm.tiles_n * prm.splits;
     if (tiles > 0x3fffffffll) return KLA_B200_EUNSUPPORTED;
-    const int grid = (int)(tiles < device_sms() ? tiles : device_sms());
-    kla_mlp_kernel<MODE><<<grid, kMlpThreads, kMlpSmem, st>>>(prm);
-    const cudaError_t e = cudaGetLastError();
+    const int64_t most = CG == 2 ? resident_pairs() : device_sms();
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = CG;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(tiles < most ? tiles : most) * CG);
+    cfg.blockDim = dim3(kMlpThreads);
+    cfg.dynamicSmemBytes = MlpRing<CG>::kSmem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = CG == 2 ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, kla_mlp_kernel<MODE, CG>, prm);
     if (e != cudaSuccess) return entry::cuda_fail(e);
     entry::count_launch();
     return KLA_B200_OK;
+}
+template <int MODE>
+int launch(const MlpParams &prm, const Plan &pl, cudaStream_t st) {
+    return pl.CG == 2 ? launch_as<MODE, 2>(prm, st) : launch_as<MODE, 1>(prm, st);
 }
 
 Product product(const Operand &a, const Operand &b, int64_t M, int64_t N, int64_t K, int mode) { return Product{a, b, M, N, K, mode}; }
@@ -119,18 +164,28 @@ Product product_dw12(const kla_b200_mlp_args &a) {
 }
 
 int64_t weight_rows(const Product &p) { return p.M * (p.a.halves == kHalvesRows ? 2 : 1); }
-size_t partial_bytes(const Product &p, int sms) { return (size_t)plan(p, true, sms).splits * weight_rows(p) * up(p.N, 4) * 4 * sizeof(float); }
+size_t partial_bytes(const Product &p, int sms) {
+    const int splits = plan(p, true, sms).splits;
+    return splits > 1 ? (size_t)splits * weight_rows(p) * up(p.N, 4) * 4 * sizeof(float) : 0;
+}
 size_t sum_bytes(int64_t rows, int64_t cols) { return (size_t)up(rows, kMlpSumRows) * cols * sizeof(float); }
 
-// The gradient of a weight: partial sums of shares of the rows, then their sum.
+// The gradient of a weight: in one go, or partial sums of shares of the rows and then their sum.
 int weight_gradient(const Product &p, void *out, float *work, cudaStream_t st) {
     const Plan pl = plan(p, true, device_sms());
     MlpParams prm;
     if (const int rc = fill(&prm, p, pl)) return rc;
+    if (pl.splits == 1) {
+        prm.out = static_cast<__nv_bfloat16 *>(out);
+        prm.out_stride = p.N;
+        prm.out_half = p.M * p.N;
+        prm.out_vec = rows_of_16(out, p.N);
+        return launch<kMlpPlain>(prm, pl, st);
+    }
     prm.partial = work;
     prm.partial_stride = up(p.N, 4) * 4;
     prm.partial_rows = weight_rows(p);
-    if (const int rc = launch<kMlpPartial>(prm, st)) return rc;
+    if (const int rc = launch<kMlpPartial>(prm, pl, st)) return rc;
     MlpReduceParams r{work, prm.partial_rows * prm.partial_stride, prm.partial_stride, pl.splits, (int)prm.partial_rows, (int)p.N,
                       static_cast<__nv_bfloat16 *>(out)};
     const int64_t grid = up(prm.partial_rows * up(p.N, 4), 256);
@@ -189,18 +244,20 @@ int kla_b200_mlp_fwd(const kla_b200_mlp_args *a, void *stream) {
     const int sms = device_sms();
     MlpParams prm;
     const Product first = product_gate_up(*a), second = product_down(*a);
-    if ((rc = fill(&prm, first, plan(first, false, sms)))) return rc;
+    Plan pl = plan(first, false, sms);
+    if ((rc = fill(&prm, first, pl))) return rc;
     prm.act = a->activation;
     prm.bias = static_cast<const __nv_bfloat16 *>(a->b12);
     prm.out = static_cast<__nv_bfloat16 *>(a->h); prm.out_stride = a->h_stride; prm.out_vec = 1;
     prm.gu = static_cast<__nv_bfloat16 *>(a->gu); prm.gu_stride = a->gu_stride; prm.gu_half = a->gu_stride / 2;
-    if ((rc = launch<kMlpGated>(prm, st))) return rc;
-    if ((rc = fill(&prm, second, plan(second, false, sms)))) return rc;
+    if ((rc = launch<kMlpGated>(prm, pl, st))) return rc;
+    pl = plan(second, false, sms);
+    if ((rc = fill(&prm, second, pl))) return rc;
     prm.bias = static_cast<const __nv_bfloat16 *>(a->b3);
     prm.out = static_cast<__nv_bfloat16 *>(a->y); prm.out_stride = a->y_stride; prm.out_vec = rows_of_16(a->y, a->y_stride);
     prm.side = static_cast<const __nv_bfloat16 *>(a->residual); prm.side_stride = a->residual_stride;
     prm.side_vec = rows_of_16(a->residual, a->residual_stride);
-    return launch<kMlpPlain>(prm, st);
+    return launch<kMlpPlain>(prm, pl, st);
 }
 
 size_t kla_b200_mlp_work_bytes(const kla_b200_mlp_args *a) {
@@ -243,16 +300,18 @@ int kla_b200_mlp_bwd(const kla_b200_mlp_args *a, void *stream) {
     if (a->db3 != nullptr && (rc = row_sums(a->dy, a->dy_stride, a->rows, a->out, work, a->db3, st))) return rc;
     if (!inner) return KLA_B200_OK;
     const Product dgu = product_dgu(*a);
-    if ((rc = fill(&prm, dgu, plan(dgu, false, sms)))) return rc;
+    Plan pl = plan(dgu, false, sms);
+    if ((rc = fill(&prm, dgu, pl))) return rc;
     prm.act = a->activation;
     prm.side = static_cast<const __nv_bfloat16 *>(a->gu); prm.side_stride = a->gu_stride; prm.side_half = a->gu_stride / 2; prm.side_vec = 1;
     prm.out = static_cast<__nv_bfloat16 *>(a->dgu); prm.out_stride = a->gu_stride; prm.out_half = a->gu_stride / 2; prm.out_vec = 1;
-    if ((rc = launch<kMlpGrad>(prm, st))) return rc;
+    if ((rc = launch<kMlpGrad>(prm, pl, st))) return rc;
     if (a->dx != nullptr) {
         const Product dx = product_dx(*a);
-        if ((rc = fill(&prm, dx, plan(dx, false, sms)))) return rc;
+        pl = plan(dx, false, sms);
+        if ((rc = fill(&prm, dx, pl))) return rc;
         prm.out = static_cast<__nv_bfloat16 *>(a->dx); prm.out_stride = a->dx_stride; prm.out_vec = rows_of_16(a->dx, a->dx_stride);
-        if ((rc = launch<kMlpPlain>(prm, st))) return rc;
+        if ((rc = launch<kMlpPlain>(prm, pl, st))) return rc;
     }
     if (a->dw12 != nullptr && (rc = weight_gradient(product_dw12(*a), a->dw12, work, st))) return rc;
     if (a->db12 != nullptr) {

@@ -13,7 +13,7 @@
 // an MN-major operand of the tensor core; nothing is transposed in memory.
 //
 // A CTA per SM walks output tiles of 128 x BN. One warp issues TMA loads of 64-wide blocks of the summed axis into a ring of
-// kMlpStages, one thread issues tcgen05.mma from them into one of two accumulators in tensor memory, eight warps empty the
+// MlpRing::kStages, one thread issues tcgen05.mma from them into one of two accumulators in tensor memory, eight warps empty the
 // other accumulator meanwhile, through a stage of shared memory that turns a thread's row into coalesced 64-byte pieces.
 // Rows and columns past the ends are zeros of the TMA loads; widths that are no multiple of a tile cost only the padding.
 #pragma once
@@ -22,14 +22,18 @@
 
 namespace kla {
 
-constexpr int kMlpBM = 128, kMlpBK = 64, kMlpMaxBN = 256;
-constexpr int kMlpStages = 4;
+constexpr int kMlpBM = 128, kMlpBK = 64, kMlpMaxBN = 256;  // rows of a CTA, summed length of a block, columns of a tile
 constexpr int kMlpEpiWarps = 8;
 constexpr int kMlpThreads = (4 + kMlpEpiWarps) * 32;
-constexpr int kMlpStageBytes = (kMlpBM + kMlpMaxBN) * kMlpBK * 2;
 constexpr int kMlpPitch = 80;  // bytes of a row of a warp's stage: 64 and 16 more, so that rows start in different banks
-constexpr int kMlpEpiBytes = kMlpEpiWarps * 32 * kMlpPitch;
-constexpr size_t kMlpSmem = 1024 + (size_t)kMlpStages * kMlpStageBytes + kMlpEpiBytes + 256;
+constexpr int kMlpEpiBytes = kMlpEpiWarps * 2 * 32 * kMlpPitch;  // two stages a warp
+// CG CTAs share a tile of CG x 128 rows: each holds its rows of A and its share of the columns of B
+template <int CG>
+struct MlpRing {
+    static constexpr int kBytes = (kMlpBM + kMlpMaxBN / CG) * kMlpBK * 2;
+    static constexpr int kStages = CG == 2 ? 5 : 3;
+    static constexpr size_t kSmem = 1024 + (size_t)kStages * kBytes + kMlpEpiBytes + 256;
+};
 
 // wait sites of the status word
 constexpr int kMlpSiteEmpty = 0x40, kMlpSiteFull = 0x41, kMlpSiteAccEmpty = 0x42, kMlpSiteAccFull = 0x43, kMlpSiteDrain = 0x44;
@@ -106,14 +110,50 @@ __device__ __forceinline__ uint64_t mlp_desc(uint32_t addr, bool mn_major) {
     return d;
 }
 
+template <int CG>
 __device__ __forceinline__ void mlp_mma(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(acc), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
-        : "memory");
+    if constexpr (CG == 2)
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(acc), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+            : "memory");
+    else
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(acc), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+            : "memory");
 }
+// an arrival at the barrier, in a pair at both CTAs', when the products issued so far are done
+template <int CG>
 __device__ __forceinline__ void mlp_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    if constexpr (CG == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// the address that `p` has in the pair's first CTA
+__device__ __forceinline__ uint32_t in_leader(const void *p) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+    return r;
+}
+template <int CG>
+__device__ __forceinline__ void mlp_arrive_leader(uint64_t *bar) {
+    if constexpr (CG == 2) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_leader(bar)) : "memory");
+    else mbar_arrive(bar);
+}
+template <int CG>
+__device__ __forceinline__ void mlp_load(void *dst, const CUtensorMap *tm, int x, int y, int z, uint64_t *bar, uint32_t leader_bar) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z), "r"(leader_bar)
+            : "memory");
+    else
+        tma_load_3d(dst, tm, x, y, z, bar);
+}
+__device__ __forceinline__ void mlp_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_load32(float (&v)[32], uint32_t addr) {
     uint32_t *r = reinterpret_cast<uint32_t *>(v);
@@ -131,64 +171,67 @@ __device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::l
 __device__ __forceinline__ void tcgen05_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tcgen05_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// A warp's stage: 32 rows of 64 bytes. Rows go in and out a row per lane; memory is walked four lanes to a row.
+// A warp's stage: 32 rows of 64 bytes. Rows go in and out a row per lane; memory is walked four lanes to a row. The caller puts
+// __syncwarp() between the two.
 struct MlpStage {
     char *base;
     int lane;
     __device__ __forceinline__ void put_row(const uint4 (&v)[4]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(base + lane * kMlpPitch + 16 * i) = v[i];
-        __syncwarp();
     }
     __device__ __forceinline__ void get_row(uint4 (&v)[4]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4 *>(base + lane * kMlpPitch + 16 * i);
-        __syncwarp();
     }
     // E: element type; rows x cols of them are there
     template <typename E>
     __device__ __forceinline__ void store(E *p, long long stride, int rows, int cols, bool vec) const {
         constexpr int per = 16 / sizeof(E);
+        const int r0 = lane / 4, c = lane % 4 * per;
+        const char *from = base + r0 * kMlpPitch + lane % 4 * 16;
+        E *to = p + r0 * stride + c;
+        if (vec && cols >= 4 * per) {
+            uint4 v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + lane / 4, c = lane % 4 * per;
-            const char *from = base + r * kMlpPitch + lane % 4 * 16;
-            if (r < rows) {
-                E *to = p + r * stride + c;
-                if (vec && c + per <= cols) {
-                    *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(from);
-                } else {
+            for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4 *>(from + i * 8 * kMlpPitch);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (r0 + 8 * i < rows) *reinterpret_cast<uint4 *>(to + i * 8 * stride) = v[i];
+        } else {
+            for (int i = 0; i < 4; ++i)
+                if (r0 + 8 * i < rows) {
 #pragma unroll
                     for (int e = 0; e < per; ++e)
-                        if (c + e < cols) to[e] = reinterpret_cast<const E *>(from)[e];
+                        if (c + e < cols) to[i * 8 * stride + e] = reinterpret_cast<const E *>(from + i * 8 * kMlpPitch)[e];
                 }
-            }
         }
-        __syncwarp();
     }
-    // zeros where there are none
-    __device__ __forceinline__ void load(const __nv_bfloat16 *p, long long stride, int rows, int cols, bool vec) const {
-        uint4 v[4];
+    // what store would write, from memory into registers; zeros where there is nothing
+    __device__ __forceinline__ void fetch(uint4 (&v)[4], const __nv_bfloat16 *p, long long stride, int rows, int cols, bool vec) const {
+        const int r0 = lane / 4, c = lane % 4 * 8;
+        const __nv_bfloat16 *from = p + r0 * stride + c;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + lane / 4, c = lane % 4 * 8;
-            v[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (r < rows) {
-                const __nv_bfloat16 *from = p + r * stride + c;
-                if (vec && c + 8 <= cols) {
-                    v[i] = __ldg(reinterpret_cast<const uint4 *>(from));
-                } else {
+        for (int i = 0; i < 4; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (vec && cols >= 32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (r0 + 8 * i < rows) v[i] = __ldg(reinterpret_cast<const uint4 *>(from + i * 8 * stride));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (r0 + 8 * i < rows) {
                     uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        if (c + e < cols) w[e / 2] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(from) + e) << (e % 2 * 16);
+                        if (c + e < cols) w[e / 2] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(from + i * 8 * stride) + e) << (e % 2 * 16);
                     v[i] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
-            }
         }
+    }
+    __device__ __forceinline__ void put_fetched(const uint4 (&v)[4]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(base + (i * 8 + lane / 4) * kMlpPitch + lane % 4 * 16) = v[i];
-        __syncwarp();
     }
 };
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -200,22 +243,46 @@ __device__ __forceinline__ void pack_row(uint4 (&v)[4], const float (&x)[32]) {
     for (int i = 0; i < 4; ++i)
         v[i] = make_uint4(pack2(x[8 * i], x[8 * i + 1]), pack2(x[8 * i + 2], x[8 * i + 3]), pack2(x[8 * i + 4], x[8 * i + 5]), pack2(x[8 * i + 6], x[8 * i + 7]));
 }
-__device__ __forceinline__ float row_at(const uint4 (&v)[4], int j) {  // j a constant after unrolling
-    const uint32_t w = j / 2 % 4 == 0 ? v[j / 8].x : j / 2 % 4 == 1 ? v[j / 8].y : j / 2 % 4 == 2 ? v[j / 8].z : v[j / 8].w;
-    return j % 2 ? __uint_as_float(w & 0xffff0000u) : __uint_as_float(w << 16);
+
+// Gate and up as the backward finds them: 16 bits with a sign, six of exponent and nine of mantissa. Rounded to bfloat16 their
+// two roundings would be half of the error of a gradient (0.0030 of dx and dW12 in the 2-norm, against 0.0017 of rounding
+// the result alone); nine bits leave the rounding of the gradients that go into the products (0.0025). 2^-31 to 2^33 at full
+// accuracy, steps of 2^-40 below; what is larger, infinite or NaN comes back as NaN.
+constexpr uint32_t kKeptTop = 0x7fffu << 14;
+__device__ __forceinline__ uint32_t keep2(float lo, float hi) {
+    const uint32_t a = __float_as_uint(lo * 0x1p-96f), b = __float_as_uint(hi * 0x1p-96f);
+    const uint32_t ma = min((a & 0x7fffffffu) + 0x2000u, kKeptTop), mb = min((b & 0x7fffffffu) + 0x2000u, kKeptTop);
+    return (ma >> 14 | (a >> 16 & 0x8000u)) | ((mb << 2 & 0x7fff0000u) | (b & 0x80000000u));
+}
+__device__ __forceinline__ float kept(uint32_t w, bool high) {  // one half of a word
+    const uint32_t m = high ? (w >> 2 & kKeptTop) : (w << 14 & kKeptTop), sign = high ? w & 0x80000000u : w << 16 & 0x80000000u;
+    return m == kKeptTop ? __uint_as_float(0x7fffffffu) : __uint_as_float(m | sign) * 0x1p96f;
+}
+__device__ __forceinline__ uint32_t word_at(const uint4 (&v)[4], int j) {  // j a constant after unrolling
+    return j / 2 % 4 == 0 ? v[j / 8].x : j / 2 % 4 == 1 ? v[j / 8].y : j / 2 % 4 == 2 ? v[j / 8].z : v[j / 8].w;
+}
+__device__ __forceinline__ void keep_row(uint4 (&v)[4], const float (&x)[32]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v[i] = make_uint4(keep2(x[8 * i], x[8 * i + 1]), keep2(x[8 * i + 2], x[8 * i + 3]), keep2(x[8 * i + 4], x[8 * i + 5]), keep2(x[8 * i + 6], x[8 * i + 7]));
 }
 
+__device__ __forceinline__ float mlp_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // The activation and its derivative.
 template <bool SLOPE>
 __device__ __forceinline__ void mlp_act(float g, int act, float &f, float &df) {
     if (act == 0) {  // silu
-        const float s = rcp_approx(1.0f + exp2f(-g * 1.4426950408889634f));
+        const float s = rcp_approx(1.0f + mlp_ex2(-1.4426950408889634f * g));
         f = g * s;
         if (SLOPE) df = fmaf(f, 1.0f - s, s);
     } else if (act == 1) {  // gelu
         const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
         f = g * cdf;
-        if (SLOPE) df = fmaf(g * 0.3989422804014327f, exp2f(-0.72134752044448170f * g * g), cdf);
+        if (SLOPE) df = fmaf(g * 0.3989422804014327f, mlp_ex2(-0.72134752044448170f * g * g), cdf);
     } else if (act == 2) {  // relu; NaN stays
         f = g < 0.0f ? 0.0f : g;
         if (SLOPE) df = g > 0.0f ? 1.0f : 0.0f;
@@ -230,6 +297,7 @@ struct MlpTile {
     int m_half;
     int k0, k1;         // blocks
 };
+template <int CG>
 __device__ __forceinline__ MlpTile mlp_tile(const MlpParams &p, int t) {
     MlpTile r;
     const int per = p.tiles_m * p.tiles_n;
@@ -238,49 +306,58 @@ __device__ __forceinline__ MlpTile mlp_tile(const MlpParams &p, int t) {
     const int tm = t / p.tiles_n, tn = t - tm * p.tiles_n;
     const int per_half = p.a.halves == kHalvesRows ? p.tiles_m / 2 : p.tiles_m;
     r.m_half = tm / per_half;
-    r.m = (tm - r.m_half * per_half) * kMlpBM;
+    r.m = (tm - r.m_half * per_half) * kMlpBM * CG;
     r.n = tn * (p.b.halves == kHalvesBoth ? p.BN / 2 : p.BN);
     r.k0 = (int)((long long)p.blocks_k * r.split / p.splits);
     r.k1 = (int)((long long)p.blocks_k * (r.split + 1) / p.splits);
     return r;
 }
 
-__device__ __forceinline__ void mlp_fetch(void *dst, const CUtensorMap *map, const MlpOperand &op, int row, int rows, int k, int half, uint64_t *bar) {
-    char *at = static_cast<char *>(dst);
-    if (op.mn_major) {
-        for (int r = 0; r < rows; r += 64) tma_load_3d(at + r * 128, map, row + r, k, half, bar);
-    } else if (op.halves == kHalvesBoth) {
-        tma_load_3d(at, map, k, row, 0, bar);
-        tma_load_3d(at + rows / 2 * 128, map, k, row, 1, bar);
+// `rows` rows of an operand from `row` on, a block of the summed axis from k on
+template <int CG>
+__device__ __forceinline__ void mlp_fetch(void *dst, const CUtensorMap *map, bool mn_major, int row, int rows, int k, int half, uint64_t *bar, uint32_t leader_bar) {
+    if (mn_major) {
+        for (int r = 0; r < rows; r += 64) mlp_load<CG>(static_cast<char *>(dst) + r * 128, map, row + r, k, half, bar, leader_bar);
     } else {
-        tma_load_3d(at, map, k, row, half, bar);
+        mlp_load<CG>(dst, map, k, row, half, bar, leader_bar);
     }
 }
 
-template <int MODE>
+template <int MODE, int CG>
 __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_constant__ MlpParams prm) {
+    using Ring = MlpRing<CG>;
+    constexpr int S = Ring::kStages;
     extern __shared__ char raw[];
     char *smem = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    char *epi = smem + kMlpStages * kMlpStageBytes;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(epi + kMlpEpiBytes);
-    uint64_t *full = bars, *empty = bars + kMlpStages, *acc_full = empty + kMlpStages, *acc_empty = acc_full + 2, *drain = acc_empty + 2;
+    char *epi = smem + S * Ring::kBytes;
+    // full, acc_empty: of the leader (the pair's first CTA); empty, acc_full: of each CTA
+    uint64_t *full = reinterpret_cast<uint64_t *>(epi + kMlpEpiBytes), *empty = full + S, *acc_full = empty + S, *acc_empty = acc_full + 2, *drain = acc_empty + 2;
     uint32_t *tmem_at = reinterpret_cast<uint32_t *>(drain + 1);
     int *failed = reinterpret_cast<int *>(tmem_at + 1);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    uint32_t rank = 0;
+    if (CG == 2) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const int first = blockIdx.x / CG, step = gridDim.x / CG;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kMlpStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], kMlpEpiWarps); }
+        for (int s = 0; s < S; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], kMlpEpiWarps * CG); }
         mbar_init(drain, 1);
         *failed = 0;
         mbar_fence_init();
     }
     if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_at)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (CG == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_at)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_at)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     tcgen05_before_sync();
-    __syncthreads();
+    if constexpr (CG == 2) mlp_cluster_sync();
+    else __syncthreads();
     tcgen05_after_sync();
     const uint32_t tmem = *tmem_at;
     const int tiles = prm.tiles_m * prm.tiles_n * prm.splits;
@@ -288,59 +365,83 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
 
     if (warp == 0) {
         if (lane == 0) {
-            const uint32_t bytes = (kMlpBM + prm.BN) * kMlpBK * 2;
+            // B's rows of this CTA; a gated pair's first CTA has gate's, its second up's
+            const bool both = prm.b.halves == kHalvesBoth;
+            const int b_rows = prm.BN / CG, b_first = both ? 0 : (int)rank * b_rows;
+            const uint32_t bytes = (kMlpBM + (prm.b.mn_major ? (b_rows + 63) / 64 * 64 : b_rows)) * kMlpBK * 2;
             int block = 0;
             bool ok = true;
-            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-                const MlpTile tl = mlp_tile(prm, t);
+            for (int t = first; ok && t < tiles; t += step) {
+                const MlpTile tl = mlp_tile<CG>(prm, t);
                 for (int kb = tl.k0; kb < tl.k1; ++kb, ++block) {
-                    const int s = block % kMlpStages;
-                    if (block >= kMlpStages && !mlp_wait(prm.wait, &empty[s], (block / kMlpStages + 1) & 1, kMlpSiteEmpty)) { ok = false; break; }
+                    const int s = block % S;
+                    if (block >= S && !mlp_wait(prm.wait, &empty[s], (block / S + 1) & 1, kMlpSiteEmpty)) { ok = false; break; }
                     if (block == prm.wait.skip_tile) { ok = false; break; }  // the tests' incomplete hand-over: nothing more is issued
-                    char *at = smem + s * kMlpStageBytes;
+                    char *at = smem + s * Ring::kBytes, *at_b = at + kMlpBM * kMlpBK * 2;
                     const int stretch = kb / prm.blocks_stretch, k = (kb - stretch * prm.blocks_stretch) * kMlpBK;
-                    mbar_arrive_expect_tx(&full[s], bytes);
-                    mlp_fetch(at, &prm.map_a, prm.a, tl.m, kMlpBM, k, prm.a.halves == kHalvesRows ? tl.m_half : stretch, &full[s]);
-                    mlp_fetch(at + kMlpBM * kMlpBK * 2, &prm.map_b, prm.b, tl.n, prm.BN, k, stretch, &full[s]);
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes * CG);
+                    const uint32_t bar = CG == 2 ? in_leader(&full[s]) : 0u;
+                    mlp_fetch<CG>(at, &prm.map_a, prm.a.mn_major, tl.m + (int)rank * kMlpBM, kMlpBM, k, prm.a.halves == kHalvesRows ? tl.m_half : stretch, &full[s], bar);
+                    if (both && CG == 1) {
+                        mlp_fetch<CG>(at_b, &prm.map_b, false, tl.n, b_rows / 2, k, 0, &full[s], bar);
+                        mlp_fetch<CG>(at_b + b_rows / 2 * 128, &prm.map_b, false, tl.n, b_rows / 2, k, 1, &full[s], bar);
+                    } else {
+                        mlp_fetch<CG>(at_b, &prm.map_b, prm.b.mn_major, tl.n + b_first, b_rows, k, both ? (int)rank : stretch, &full[s], bar);
+                    }
                     issued = block + 1;
                 }
             }
             if (!ok) *failed = 1;
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (lane == 0 && rank == 0) {
             // float32 accumulators of bfloat16 operands; majors; N / 8; M / 16
             const uint32_t idesc = 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(prm.a.mn_major != 0) << 15 | (uint32_t)(prm.b.mn_major != 0) << 16 |
-                                   (uint32_t)(prm.BN / 8) << 17 | (uint32_t)(kMlpBM / 16) << 24;
+                                   (uint32_t)(prm.BN / 8) << 17 | (uint32_t)(kMlpBM * CG / 16) << 24;
             const uint64_t step_a = (prm.a.mn_major ? 2048 : 32) / 16, step_b = (prm.b.mn_major ? 2048 : 32) / 16;
             int block = 0, acc = 0;
             bool ok = true;
-            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x, ++acc) {
-                const MlpTile tl = mlp_tile(prm, t);
+            for (int t = first; ok && t < tiles; t += step, ++acc) {
+                const MlpTile tl = mlp_tile<CG>(prm, t);
                 if (acc >= 2 && !mlp_wait(prm.wait, &acc_empty[acc % 2], (acc / 2 + 1) & 1, kMlpSiteAccEmpty)) { ok = false; break; }
                 tcgen05_after_sync();
                 const uint32_t d = tmem + acc % 2 * kMlpMaxBN;
                 for (int kb = tl.k0; kb < tl.k1; ++kb, ++block) {
-                    const int s = block % kMlpStages;
-                    if (!mlp_wait(prm.wait, &full[s], (block / kMlpStages) & 1, kMlpSiteFull)) { ok = false; break; }
+                    const int s = block % S;
+                    if (!mlp_wait(prm.wait, &full[s], (block / S) & 1, kMlpSiteFull)) { ok = false; break; }
                     tcgen05_after_sync();
-                    const uint32_t at = smem_u32(smem + s * kMlpStageBytes);
+                    const uint32_t at = smem_u32(smem + s * Ring::kBytes);
                     const uint64_t da = mlp_desc(at, prm.a.mn_major), db = mlp_desc(at + kMlpBM * kMlpBK * 2, prm.b.mn_major);
 #pragma unroll
-                    for (int i = 0; i < kMlpBK / 16; ++i) mlp_mma(d, da + i * step_a, db + i * step_b, idesc, kb > tl.k0 || i > 0);
-                    mlp_commit(&empty[s]);
+                    for (int i = 0; i < kMlpBK / 16; ++i) mlp_mma<CG>(d, da + i * step_a, db + i * step_b, idesc, kb > tl.k0 || i > 0);
+                    mlp_commit<CG>(&empty[s]);
                 }
-                if (ok) mlp_commit(&acc_full[acc % 2]);
+                if (ok) mlp_commit<CG>(&acc_full[acc % 2]);
             }
             if (!ok) *failed = 1;
         }
     } else if (warp >= 4) {
         const int quad = warp % 4, part = (warp - 4) / 4;
-        const MlpStage st{epi + (warp - 4) * 32 * kMlpPitch, lane};
+        const MlpStage st{epi + (warp - 4) * 2 * 32 * kMlpPitch, lane}, st2{st.base + 32 * kMlpPitch, lane};
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        const int width = MODE == kMlpGated ? prm.BN / 2 : prm.BN, c0 = part * (width / 2), c1 = c0 + width / 2;
+        const int row0 = (int)rank * kMlpBM + quad * 32;
+        // what the epilogue reads besides the accumulator is fetched a chunk of 32 columns ahead, the next tile's first during the
+        // wait for its accumulator
+        uint4 f1[4], f2[4];
+        auto fetch = [&](int m, int n) {
+            if (MODE == kMlpPlain && prm.side != nullptr) st.fetch(f1, prm.side + (long long)m * prm.side_stride + n, prm.side_stride, prm.M - m, prm.N - n, prm.side_vec);
+            if (MODE == kMlpGrad) {
+                const __nv_bfloat16 *p = prm.side + (long long)m * prm.side_stride + n;
+                st.fetch(f1, p, prm.side_stride, prm.M - m, prm.N - n, true);
+                st.fetch(f2, p + prm.side_half, prm.side_stride, prm.M - m, prm.N - n, true);
+            }
+        };
         int acc = 0;
-        for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++acc) {
-            const MlpTile tl = mlp_tile(prm, t);
+        for (int t = first; t < tiles; t += step, ++acc) {
+            const MlpTile tl = mlp_tile<CG>(prm, t);
+            const int m = tl.m + row0, rows = prm.M - m;
+            fetch(m, tl.n + c0);
             bool ok = true;
             if (lane == 0) ok = mlp_wait(prm.wait, &acc_full[acc % 2], (acc / 2) & 1, kMlpSiteAccFull);
             ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -350,34 +451,44 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
             }
             tcgen05_after_sync();
             const uint32_t d = tmem + acc % 2 * kMlpMaxBN + lanes;
-            const int m = tl.m + quad * 32, rows = prm.M - m;
-            const int width = MODE == kMlpGated ? prm.BN / 2 : prm.BN;
-            for (int c = part * (width / 2); c < (part + 1) * (width / 2); c += 32) {
+            for (int c = c0; c < c1; c += 32) {
                 const int n = tl.n + c, cols = prm.N - n;
-                const bool last = c + 32 >= (part + 1) * (width / 2);
                 float v[32], w[32];
+                uint4 r[4], q[4];
                 tmem_load32(v, d + c);
                 if (MODE == kMlpGated) tmem_load32(w, d + width + c);
+                const bool side = (MODE == kMlpPlain && prm.side != nullptr) || MODE == kMlpGrad;
+                if (side) {
+                    st.put_fetched(f1);
+                    if (MODE == kMlpGrad) st2.put_fetched(f2);
+                    __syncwarp();
+                    st.get_row(r);
+                    if (MODE == kMlpGrad) st2.get_row(q);
+                    __syncwarp();
+                    if (c + 32 < c1) fetch(m, n + 32);
+                }
                 tmem_load_wait();
-                if (last) {
+                if (c + 32 >= c1) {
                     tcgen05_before_sync();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&acc_empty[acc % 2]);
+                    if (lane == 0) mlp_arrive_leader<CG>(&acc_empty[acc % 2]);
                 }
                 if (cols <= 0) continue;
-                uint4 r[4];
                 if (MODE == kMlpPartial) {
                     float *p = prm.partial + (long long)tl.split * prm.partial_rows * prm.partial_stride +
                                ((long long)tl.m_half * prm.M + m) * prm.partial_stride + n;
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
+                    for (int h = 0; h < 2; ++h) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            r[i] = make_uint4(__float_as_uint(v[16 * q + 4 * i]), __float_as_uint(v[16 * q + 4 * i + 1]),
-                                              __float_as_uint(v[16 * q + 4 * i + 2]), __float_as_uint(v[16 * q + 4 * i + 3]));
-                        st.put_row(r);
-                        st.store(p + 16 * q, prm.partial_stride, rows, cols - 16 * q, true);
+                            r[i] = make_uint4(__float_as_uint(v[16 * h + 4 * i]), __float_as_uint(v[16 * h + 4 * i + 1]),
+                                              __float_as_uint(v[16 * h + 4 * i + 2]), __float_as_uint(v[16 * h + 4 * i + 3]));
+                        (h ? st2 : st).put_row(r);
                     }
+                    __syncwarp();
+                    st.store(p, prm.partial_stride, rows, cols, true);
+                    st2.store(p + 16, prm.partial_stride, rows, cols - 16, true);
+                    __syncwarp();
                     continue;
                 }
                 __nv_bfloat16 *out = prm.out + tl.m_half * prm.out_half + (long long)m * prm.out_stride + n;
@@ -386,14 +497,16 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] += j < cols ? __bfloat162float(prm.bias[n + j]) : 0.0f;
                     }
-                    if (prm.side != nullptr) {
-                        st.load(prm.side + (long long)m * prm.side_stride + n, prm.side_stride, rows, cols, prm.side_vec);
-                        st.get_row(r);
+                    if (side) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] += row_at(r, j);
+                        for (int j = 0; j < 32; ++j) {
+                            const uint32_t x = word_at(r, j);
+                            v[j] += __uint_as_float(j % 2 ? x & 0xffff0000u : x << 16);
+                        }
                     }
                     pack_row(r, v);
                     st.put_row(r);
+                    __syncwarp();
                     st.store(out, prm.out_stride, rows, cols, prm.out_vec);
                 } else if (MODE == kMlpGated) {
                     if (prm.bias != nullptr) {
@@ -405,13 +518,15 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
                             }
                     }
                     if (prm.gu != nullptr) {
+                        keep_row(r, v);
+                        st.put_row(r);
+                        keep_row(r, w);
+                        st2.put_row(r);
+                        __syncwarp();
                         __nv_bfloat16 *gu = prm.gu + (long long)m * prm.gu_stride + n;
-                        pack_row(r, v);
-                        st.put_row(r);
                         st.store(gu, prm.gu_stride, rows, cols, true);
-                        pack_row(r, w);
-                        st.put_row(r);
-                        st.store(gu + prm.gu_half, prm.gu_stride, rows, cols, true);
+                        st2.store(gu + prm.gu_half, prm.gu_stride, rows, cols, true);
+                        __syncwarp();
                     }
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
@@ -421,47 +536,55 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
                     }
                     pack_row(r, v);
                     st.put_row(r);
+                    __syncwarp();
                     st.store(out, prm.out_stride, rows, cols, prm.out_vec);
                 } else {
-                    const __nv_bfloat16 *side = prm.side + (long long)m * prm.side_stride + n;
-                    uint4 up[4];
-                    st.load(side, prm.side_stride, rows, cols, true);
-                    st.get_row(r);
-                    st.load(side + prm.side_half, prm.side_stride, rows, cols, true);
-                    st.get_row(up);
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
                         float f, df;
-                        mlp_act<true>(row_at(r, j), prm.act, f, df);
-                        w[j] = v[j] * f;                       // of up
-                        v[j] = v[j] * row_at(up, j) * df;      // of gate
+                        mlp_act<true>(kept(word_at(r, j), j % 2), prm.act, f, df);
+                        w[j] = v[j] * f;                                      // of up
+                        v[j] = v[j] * kept(word_at(q, j), j % 2) * df;        // of gate
                     }
                     pack_row(r, v);
                     st.put_row(r);
-                    st.store(out, prm.out_stride, rows, cols, true);
                     pack_row(r, w);
-                    st.put_row(r);
-                    st.store(out + prm.out_half, prm.out_stride, rows, cols, true);
+                    st2.put_row(r);
+                    __syncwarp();
+                    st.store(out, prm.out_stride, rows, cols, true);
+                    st2.store(out + prm.out_half, prm.out_stride, rows, cols, true);
                 }
+                __syncwarp();
             }
         }
     }
     __syncwarp();
-    __syncthreads();
-    if (*failed) {  // a wait ran out: copies and products still under way end before the memory they use is given back
-        if (warp == 0 && lane == 0)
-            for (int b = max(0, issued - kMlpStages); b < issued; ++b) mlp_wait(prm.wait, &full[b % kMlpStages], (b / kMlpStages) & 1, kMlpSiteDrain);
-        if (warp == 1 && lane == 0) {
-            mlp_commit(drain);
+    if constexpr (CG == 2) mlp_cluster_sync();
+    else __syncthreads();
+    int bad = *failed;
+    if constexpr (CG == 2) {
+        uint32_t there;
+        int other;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_u32(failed)), "r"(rank ^ 1u));
+        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(other) : "r"(there) : "memory");
+        bad |= other;
+    }
+    if (bad) {  // a wait ran out: copies and products still under way end, or get as long again, before their memory is given back
+        if (warp == 0 && lane == 0 && rank == 0)
+            for (int b = max(0, issued - S); b < issued; ++b) mlp_wait(prm.wait, &full[b % S], (b / S) & 1, kMlpSiteDrain);
+        if (warp == 1 && lane == 0 && rank == 0) {
+            mlp_commit<CG>(drain);
             mlp_wait(prm.wait, drain, 0, kMlpSiteDrain);
         }
         __syncwarp();
     }
     tcgen05_before_sync();
-    __syncthreads();
+    if constexpr (CG == 2) mlp_cluster_sync();
+    else __syncthreads();
     if (warp == 2) {
         tcgen05_after_sync();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+        if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
 }
 

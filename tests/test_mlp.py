@@ -2,7 +2,8 @@
 
 Tolerances are counted, not chosen: ``oracle`` carries a bound beside every value. A product of n terms accumulated in float32
 is off by at most (n + 2) 2^-23 of the sum of its terms' absolute values (an addition of the tensor core may truncate: a whole
-step of 2^-23); what is rounded to bfloat16 on the way (h, and for the backward g, u, dg, du) by 2^-8 of itself; the activation's
+step of 2^-23); what is rounded to bfloat16 on the way (h, and in the backward dg, du) by 2^-8 of itself; g and u, kept for the
+backward with nine bits of mantissa, by 2^-10 of themselves and 2^-41; the activation's
 exponential and reciprocal by 2^-20. Errors go through products by their absolute values. Slopes: |silu'| and |gelu'| are below
 1.13, |silu''| and |gelu''| below 0.8; relu's slope is undetermined where g is within its own error of zero.
 """
@@ -45,6 +46,9 @@ class V:
     def rounded(self):
         return V(self.x, self.e + HALF * (self.x.abs() + self.e))
 
+    def kept(self):
+        return V(self.x, self.e + 2.0 ** -10 * (self.x.abs() + self.e) + 2.0 ** -41)
+
 
 def oracle(x, w12, w3, b12, b3, residual, act, dy):
     d64 = lambda t: None if t is None else V(t.detach().double().cuda())  # noqa: E731
@@ -75,7 +79,7 @@ def oracle(x, w12, w3, b12, b3, residual, act, dy):
     out = {"y": y.rounded()}
     if dy is None:
         return out
-    gs, us = g.rounded(), u.rounded()
+    gs, us = g.kept(), u.kept()
     dh = dy @ w3
     dg, du = (dh * us * f(gs, True)).rounded(), (dh * f(gs, False)).rounded()
     dgu = V(torch.cat((dg.x, du.x), 1), torch.cat((dg.e, du.e), 1))
@@ -225,6 +229,27 @@ def test_nan_and_infinity_stay_in_their_rows():
     y = kla_b200.gated_mlp_b200(**t)
     bad = ~torch.isfinite(y).all(1)
     assert bad[[7, 200]].all() and bad.sum() == 2 and torch.equal(y[~bad], y0[~bad])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [2.0 ** -30, 2.0 ** -12, 2.0 ** 12])
+def test_scales_of_gate_and_up(scale):
+    """The kept gate and up hold their accuracy over the range that is documented."""
+    t, dy = inputs(140, 64, 72, 64)
+    t["x"] *= scale
+    check(t, dy, act=None)
+
+
+@pytest.mark.gpu
+def test_gate_and_up_beyond_the_kept_range_have_nan_gradients():
+    t, dy = inputs(140, 64, 72, 64)
+    t["x"][3] *= 2.0 ** 40
+    given = {**t, "x": t["x"].detach().requires_grad_()}
+    y = kla_b200.gated_mlp_b200(**given, activation=None)
+    dx, = torch.autograd.grad(y, given["x"], dy)
+    assert torch.isfinite(y).all() and torch.isnan(dx[3]).any()
+    keep = torch.arange(140) != 3
+    assert torch.isfinite(dx[keep]).all()
 
 
 @pytest.mark.gpu
