@@ -1,4 +1,5 @@
 // Entry points of the gated feed-forward block (kla_mlp.cuh): argument checks, tensor maps, tile choice, launches.
+#include <algorithm>
 #include <mutex>
 
 #include "../../include/kla_b200.h"
@@ -83,6 +84,7 @@ int fill(MlpParams *prm, const Product &p, const Plan &pl) {
     prm->b = MlpOperand{p.b.adjacent_rows, p.b.halves};
     prm->M = (int)p.M; prm->N = (int)p.N; prm->K = (int)p.K;
     prm->BN = pl.BN; prm->tiles_m = pl.tiles_m; prm->tiles_n = pl.tiles_n; prm->splits = pl.splits;
+    prm->stages = std::min(kMlpMaxStages, kMlpRingBytes / mlp_block_bytes(pl.BN, pl.CG, p.b.adjacent_rows));
     prm->blocks_stretch = (int)up(p.K, kMlpBK);
     prm->blocks_k = prm->blocks_stretch * (p.a.halves == kHalvesSummed ? 2 : 1);
     return entry::wait_ctl(&prm->wait);
@@ -103,7 +105,7 @@ int resident_pairs() {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)device_sms() / 2 * 2);
         cfg.blockDim = dim3(kMlpThreads);
-        cfg.dynamicSmemBytes = MlpRing<2>::kSmem;
+        cfg.dynamicSmemBytes = kMlpSmem;
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
         int n = 0;
@@ -118,9 +120,9 @@ int resident_pairs() {
 
 template <int MODE, int CG>
 int launch_as(const MlpParams &prm, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(kla_mlp_kernel<MODE, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MlpRing<CG>::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(kla_mlp_kernel<MODE, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMlpSmem);
     if (e == cudaSuccess && CG == 2)
-        e = cudaFuncSetAttribute(kla_mlp_kernel<kMlpPlain, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MlpRing<2>::kSmem);
+        e = cudaFuncSetAttribute(kla_mlp_kernel<kMlpPlain, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMlpSmem);
     if (e != cudaSuccess) return entry::cuda_fail(e);
     const int64_t tiles = (int64_t)prm.tiles_m * prm.tiles_n * prm.splits;
     if (tiles > 0x3fffffffll) return KLA_B200_EUNSUPPORTED;
@@ -132,7 +134,7 @@ int launch_as(const MlpParams &prm, cudaStream_t st) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(tiles < most ? tiles : most) * CG);
     cfg.blockDim = dim3(kMlpThreads);
-    cfg.dynamicSmemBytes = MlpRing<CG>::kSmem;
+    cfg.dynamicSmemBytes = kMlpSmem;
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = CG == 2 ? 1 : 0;

@@ -13,7 +13,7 @@
 // an MN-major operand of the tensor core; nothing is transposed in memory.
 //
 // A CTA per SM walks output tiles of 128 x BN. One warp issues TMA loads of 64-wide blocks of the summed axis into a ring of
-// MlpRing::kStages, one thread issues tcgen05.mma from them into one of two accumulators in tensor memory, eight warps empty the
+// blocks, one thread issues tcgen05.mma from them into one of two accumulators in tensor memory, eight warps empty the
 // other accumulator meanwhile, through a stage of shared memory that turns a thread's row into coalesced 64-byte pieces.
 // Rows and columns past the ends are zeros of the TMA loads; widths that are no multiple of a tile cost only the padding.
 #pragma once
@@ -25,15 +25,13 @@ namespace kla {
 constexpr int kMlpBM = 128, kMlpBK = 64, kMlpMaxBN = 256;  // rows of a CTA, summed length of a block, columns of a tile
 constexpr int kMlpEpiWarps = 8;
 constexpr int kMlpThreads = (4 + kMlpEpiWarps) * 32;
-constexpr int kMlpPitch = 80;  // bytes of a row of a warp's stage: 64 and 16 more, so that rows start in different banks
-constexpr int kMlpEpiBytes = kMlpEpiWarps * 2 * 32 * kMlpPitch;  // two stages a warp
-// CG CTAs share a tile of CG x 128 rows: each holds its rows of A and its share of the columns of B
-template <int CG>
-struct MlpRing {
-    static constexpr int kBytes = (kMlpBM + kMlpMaxBN / CG) * kMlpBK * 2;
-    static constexpr int kStages = CG == 2 ? 5 : 3;
-    static constexpr size_t kSmem = 1024 + (size_t)kStages * kBytes + kMlpEpiBytes + 256;
-};
+constexpr int kMlpEpiBytes = kMlpEpiWarps * 2 * 32 * 64;  // two stages of 32 rows of 64 bytes a warp
+constexpr int kMlpRingBytes = 192 * 1024, kMlpMaxStages = 8;
+constexpr size_t kMlpSmem = 1024 + kMlpRingBytes + kMlpEpiBytes + 256;
+// A block of the ring: A's rows of a CTA and its share of B's, which in a pair of CTAs is half of them. What is in flight is what
+// bounds the loads (a tile's block takes about 1 us from L2): with 5 blocks of 32 KB in place of 6 K=4096 N=1024 ran at 1213 TFLOP/s
+inline __host__ __device__ int mlp_b_rows(int BN, int cg, bool mn_major) { return mn_major ? (BN / cg + 63) / 64 * 64 : BN / cg; }
+inline __host__ __device__ int mlp_block_bytes(int BN, int cg, bool mn_major) { return (kMlpBM + mlp_b_rows(BN, cg, mn_major)) * kMlpBK * 2; }
 
 // wait sites of the status word
 constexpr int kMlpSiteEmpty = 0x40, kMlpSiteFull = 0x41, kMlpSiteAccEmpty = 0x42, kMlpSiteAccFull = 0x43, kMlpSiteDrain = 0x44;
@@ -63,6 +61,7 @@ struct MlpParams {
     int M, N, K;       // rows, columns (of one half where halves are rows), summed length (of one stretch)
     int BN;            // columns of a tile (gated: of gate and up together)
     int tiles_m, tiles_n, splits;
+    int stages;        // blocks of the ring
     int blocks_k;      // 64-wide blocks of the summed axis, all stretches
     int blocks_stretch;
     int act;
@@ -80,21 +79,29 @@ struct MlpParams {
     WaitCtl wait;
 };
 
-__device__ __forceinline__ uint64_t global_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
+// A bounded wait without sleeps (mbarrier.try_wait suspends the thread by itself), counted in cycles of at most 2 GHz; gives up like
+// mbar_wait. Barriers are addressed by their shared memory address: the ring's two threads run through this once a block, one
+// instruction after the other, and are what bounds a block's time as soon as they take more than its products (0.3 us).
+__device__ __forceinline__ bool mlp_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
-// A bounded wait without sleeps (mbarrier.try_wait suspends the thread by itself); gives up like mbar_wait.
-__device__ __forceinline__ bool mlp_wait(const WaitCtl &w, uint64_t *bar, uint32_t parity, int site) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t begin = global_ns();
+__device__ __noinline__ bool mlp_wait_long(const WaitCtl &w, uint32_t bar, uint32_t parity, int site) {
+    const long long begin = clock64(), limit = 2ll * w.limit_ns;
     do {
         for (int i = 0; i < 32; ++i)
-            if (mbar_try_wait(bar, parity)) return true;
-    } while (global_ns() - begin < w.limit_ns);
+            if (mlp_try(bar, parity)) return true;
+    } while (clock64() - begin < limit);
     atomicCAS(w.status, 0, kStatusWait | site);
     return false;
+}
+__device__ __forceinline__ bool mlp_wait(const WaitCtl &w, uint32_t bar, uint32_t parity, int site) {
+    return mlp_try(bar, parity) || mlp_wait_long(w, bar, parity, site);
 }
 
 // Shared memory descriptor of an operand tile in the 128-byte swizzle: 8 rows of 128 bytes make an atom of 1024.
@@ -125,32 +132,38 @@ __device__ __forceinline__ void mlp_mma(uint32_t acc, uint64_t a, uint64_t b, ui
 }
 // an arrival at the barrier, in a pair at both CTAs', when the products issued so far are done
 template <int CG>
-__device__ __forceinline__ void mlp_commit(uint64_t *bar) {
+__device__ __forceinline__ void mlp_commit(uint32_t bar) {
     if constexpr (CG == 2)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
     else
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-// the address that `p` has in the pair's first CTA
-__device__ __forceinline__ uint32_t in_leader(const void *p) {
+// the address that `addr` has in the pair's first CTA
+__device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
     uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
     return r;
 }
 template <int CG>
-__device__ __forceinline__ void mlp_arrive_leader(uint64_t *bar) {
+__device__ __forceinline__ void mlp_arrive_leader(uint32_t bar) {
     if constexpr (CG == 2) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_leader(bar)) : "memory");
-    else mbar_arrive(bar);
+    else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mlp_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 template <int CG>
-__device__ __forceinline__ void mlp_load(void *dst, const CUtensorMap *tm, int x, int y, int z, uint64_t *bar, uint32_t leader_bar) {
+__device__ __forceinline__ void mlp_load(uint32_t dst, uint64_t tm, int x, int y, int z, uint32_t bar) {  // bar: the leader's
     if constexpr (CG == 2)
         asm volatile(
             "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-            " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z), "r"(leader_bar)
+            " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(tm), "r"(x), "r"(y), "r"(z), "r"(bar)
             : "memory");
     else
-        tma_load_3d(dst, tm, x, y, z, bar);
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(tm), "r"(x), "r"(y), "r"(z), "r"(bar)
+            : "memory");
 }
 __device__ __forceinline__ void mlp_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -171,30 +184,32 @@ __device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::l
 __device__ __forceinline__ void tcgen05_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tcgen05_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// A warp's stage: 32 rows of 64 bytes. Rows go in and out a row per lane; memory is walked four lanes to a row. The caller puts
-// __syncwarp() between the two.
+// A warp's stage: 32 rows of 64 bytes. Rows go in and out a row per lane; memory is walked four lanes to a row. The 16-byte pieces
+// of a row change places with the row's number, which keeps both ways free of bank conflicts. The caller puts __syncwarp() between
+// the two.
 struct MlpStage {
     char *base;
     int lane;
+    __device__ __forceinline__ char *piece(int row, int i) const { return base + row * 64 + (i ^ (row >> 1 & 3)) * 16; }
     __device__ __forceinline__ void put_row(const uint4 (&v)[4]) const {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(base + lane * kMlpPitch + 16 * i) = v[i];
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(piece(lane, i)) = v[i];
     }
     __device__ __forceinline__ void get_row(uint4 (&v)[4]) const {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4 *>(base + lane * kMlpPitch + 16 * i);
+        for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4 *>(piece(lane, i));
     }
     // E: element type; rows x cols of them are there
     template <typename E>
     __device__ __forceinline__ void store(E *p, long long stride, int rows, int cols, bool vec) const {
         constexpr int per = 16 / sizeof(E);
         const int r0 = lane / 4, c = lane % 4 * per;
-        const char *from = base + r0 * kMlpPitch + lane % 4 * 16;
+        const char *from = piece(r0, lane % 4);  // rows 8 apart hold a piece at the same place
         E *to = p + r0 * stride + c;
         if (vec && cols >= 4 * per) {
             uint4 v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4 *>(from + i * 8 * kMlpPitch);
+            for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4 *>(from + i * 8 * 64);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (r0 + 8 * i < rows) *reinterpret_cast<uint4 *>(to + i * 8 * stride) = v[i];
@@ -203,7 +218,7 @@ struct MlpStage {
                 if (r0 + 8 * i < rows) {
 #pragma unroll
                     for (int e = 0; e < per; ++e)
-                        if (c + e < cols) to[i * 8 * stride + e] = reinterpret_cast<const E *>(from + i * 8 * kMlpPitch)[e];
+                        if (c + e < cols) to[i * 8 * stride + e] = reinterpret_cast<const E *>(from + i * 8 * 64)[e];
                 }
         }
     }
@@ -231,7 +246,7 @@ struct MlpStage {
     }
     __device__ __forceinline__ void put_fetched(const uint4 (&v)[4]) const {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(base + (i * 8 + lane / 4) * kMlpPitch + lane % 4 * 16) = v[i];
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(piece(i * 8 + lane / 4, lane % 4)) = v[i];
     }
 };
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -313,25 +328,14 @@ __device__ __forceinline__ MlpTile mlp_tile(const MlpParams &p, int t) {
     return r;
 }
 
-// `rows` rows of an operand from `row` on, a block of the summed axis from k on
-template <int CG>
-__device__ __forceinline__ void mlp_fetch(void *dst, const CUtensorMap *map, bool mn_major, int row, int rows, int k, int half, uint64_t *bar, uint32_t leader_bar) {
-    if (mn_major) {
-        for (int r = 0; r < rows; r += 64) mlp_load<CG>(static_cast<char *>(dst) + r * 128, map, row + r, k, half, bar, leader_bar);
-    } else {
-        mlp_load<CG>(dst, map, k, row, half, bar, leader_bar);
-    }
-}
-
 template <int MODE, int CG>
 __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_constant__ MlpParams prm) {
-    using Ring = MlpRing<CG>;
-    constexpr int S = Ring::kStages;
     extern __shared__ char raw[];
     char *smem = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    char *epi = smem + S * Ring::kBytes;
+    char *epi = smem + kMlpRingBytes;
+    const int S = prm.stages, block_bytes = mlp_block_bytes(prm.BN, CG, prm.b.mn_major);
     // full, acc_empty: of the leader (the pair's first CTA); empty, acc_full: of each CTA
-    uint64_t *full = reinterpret_cast<uint64_t *>(epi + kMlpEpiBytes), *empty = full + S, *acc_full = empty + S, *acc_empty = acc_full + 2, *drain = acc_empty + 2;
+    uint64_t *full = reinterpret_cast<uint64_t *>(epi + kMlpEpiBytes), *empty = full + kMlpMaxStages, *acc_full = empty + kMlpMaxStages, *acc_empty = acc_full + 2, *drain = acc_empty + 2;
     uint32_t *tmem_at = reinterpret_cast<uint32_t *>(drain + 1);
     int *failed = reinterpret_cast<int *>(tmem_at + 1);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -363,66 +367,89 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
     const int tiles = prm.tiles_m * prm.tiles_n * prm.splits;
     int issued = 0;  // producer: blocks whose loads were issued
 
+    const uint32_t smem_at = smem_u32(smem), full_at = smem_u32(full), empty_at = smem_u32(empty), acc_full_at = smem_u32(acc_full), acc_empty_at = smem_u32(acc_empty);
+
     if (warp == 0) {
         if (lane == 0) {
-            // B's rows of this CTA; a gated pair's first CTA has gate's, its second up's
-            const bool both = prm.b.halves == kHalvesBoth;
-            const int b_rows = prm.BN / CG, b_first = both ? 0 : (int)rank * b_rows;
-            const uint32_t bytes = (kMlpBM + (prm.b.mn_major ? (b_rows + 63) / 64 * 64 : b_rows)) * kMlpBK * 2;
-            int block = 0;
+            const WaitCtl wait = prm.wait;
+            const uint64_t map_a = reinterpret_cast<uint64_t>(&prm.map_a), map_b = reinterpret_cast<uint64_t>(&prm.map_b);
+            const bool a_lines = prm.a.mn_major != 0, b_lines = prm.b.mn_major != 0;
+            // B's rows of this CTA; a gated pair's first CTA has gate's, its second up's, a CTA alone both, one behind the other
+            const bool both = prm.b.halves == kHalvesBoth, a_rows_half = prm.a.halves == kHalvesRows;
+            const int b_rows = prm.BN / CG / (both && CG == 1 ? 2 : 1), b_first = both ? 0 : (int)rank * b_rows, stretch_blocks = prm.blocks_stretch;
+            const uint32_t bytes = CG * block_bytes;
+            const uint32_t leader_full = CG == 2 ? in_leader(full_at) : full_at;
+            int s = 0;
+            uint32_t phase = 1;  // the ring begins empty: a wait for the phase before the first passes
             bool ok = true;
             for (int t = first; ok && t < tiles; t += step) {
                 const MlpTile tl = mlp_tile<CG>(prm, t);
-                for (int kb = tl.k0; kb < tl.k1; ++kb, ++block) {
-                    const int s = block % S;
-                    if (block >= S && !mlp_wait(prm.wait, &empty[s], (block / S + 1) & 1, kMlpSiteEmpty)) { ok = false; break; }
-                    if (block == prm.wait.skip_tile) { ok = false; break; }  // the tests' incomplete hand-over: nothing more is issued
-                    char *at = smem + s * Ring::kBytes, *at_b = at + kMlpBM * kMlpBK * 2;
-                    const int stretch = kb / prm.blocks_stretch, k = (kb - stretch * prm.blocks_stretch) * kMlpBK;
-                    if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes * CG);
-                    const uint32_t bar = CG == 2 ? in_leader(&full[s]) : 0u;
-                    mlp_fetch<CG>(at, &prm.map_a, prm.a.mn_major, tl.m + (int)rank * kMlpBM, kMlpBM, k, prm.a.halves == kHalvesRows ? tl.m_half : stretch, &full[s], bar);
-                    if (both && CG == 1) {
-                        mlp_fetch<CG>(at_b, &prm.map_b, false, tl.n, b_rows / 2, k, 0, &full[s], bar);
-                        mlp_fetch<CG>(at_b + b_rows / 2 * 128, &prm.map_b, false, tl.n, b_rows / 2, k, 1, &full[s], bar);
-                    } else {
-                        mlp_fetch<CG>(at_b, &prm.map_b, prm.b.mn_major, tl.n + b_first, b_rows, k, both ? (int)rank : stretch, &full[s], bar);
+                int stretch = tl.k0 / stretch_blocks, kb = tl.k0 - stretch * stretch_blocks;
+                const int m = tl.m + (int)rank * kMlpBM, n = tl.n + b_first;
+                for (int left = tl.k1 - tl.k0; left > 0; --left) {
+                    if (!mlp_wait(wait, empty_at + 8 * s, phase, kMlpSiteEmpty) || issued == wait.skip_tile) {  // skip_tile: the tests'
+                        ok = false;                                                                            // incomplete hand-over
+                        break;
                     }
-                    issued = block + 1;
+                    const uint32_t at_a = smem_at + s * block_bytes, at_b = at_a + kMlpBM * kMlpBK * 2, bar = leader_full + 8 * s;
+                    const int k = kb * kMlpBK, za = a_rows_half ? tl.m_half : stretch, zb = both ? (int)rank : stretch;
+                    if (rank == 0) mlp_expect(full_at + 8 * s, bytes);
+                    if (a_lines) {
+                        mlp_load<CG>(at_a, map_a, m, k, za, bar);
+                        mlp_load<CG>(at_a + 64 * 128, map_a, m + 64, k, za, bar);
+                    } else {
+                        mlp_load<CG>(at_a, map_a, k, m, za, bar);
+                    }
+                    if (b_lines) {
+                        for (int r = 0; r < b_rows; r += 64) mlp_load<CG>(at_b + r * 128, map_b, n + r, k, zb, bar);
+                    } else {
+                        mlp_load<CG>(at_b, map_b, k, n, zb, bar);
+                        if (both && CG == 1) mlp_load<CG>(at_b + b_rows * 128, map_b, k, n, 1, bar);
+                    }
+                    ++issued;
+                    if (++s == S) { s = 0; phase ^= 1; }
+                    if (++kb == stretch_blocks) { kb = 0; ++stretch; }
                 }
             }
             if (!ok) *failed = 1;
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
+            const WaitCtl wait = prm.wait;
             // float32 accumulators of bfloat16 operands; majors; N / 8; M / 16
             const uint32_t idesc = 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(prm.a.mn_major != 0) << 15 | (uint32_t)(prm.b.mn_major != 0) << 16 |
                                    (uint32_t)(prm.BN / 8) << 17 | (uint32_t)(kMlpBM * CG / 16) << 24;
             const uint64_t step_a = (prm.a.mn_major ? 2048 : 32) / 16, step_b = (prm.b.mn_major ? 2048 : 32) / 16;
-            int block = 0, acc = 0;
+            const uint64_t desc_a = mlp_desc(smem_at, prm.a.mn_major), desc_b = mlp_desc(smem_at + kMlpBM * kMlpBK * 2, prm.b.mn_major);
+            int s = 0;
+            uint32_t phase = 0, acc = 0, acc_phase = 1;
             bool ok = true;
-            for (int t = first; ok && t < tiles; t += step, ++acc) {
+            for (int t = first; ok && t < tiles; t += step) {
                 const MlpTile tl = mlp_tile<CG>(prm, t);
-                if (acc >= 2 && !mlp_wait(prm.wait, &acc_empty[acc % 2], (acc / 2 + 1) & 1, kMlpSiteAccEmpty)) { ok = false; break; }
+                if (!mlp_wait(wait, acc_empty_at + 8 * acc, acc_phase, kMlpSiteAccEmpty)) { ok = false; break; }
                 tcgen05_after_sync();
-                const uint32_t d = tmem + acc % 2 * kMlpMaxBN;
-                for (int kb = tl.k0; kb < tl.k1; ++kb, ++block) {
-                    const int s = block % S;
-                    if (!mlp_wait(prm.wait, &full[s], (block / S) & 1, kMlpSiteFull)) { ok = false; break; }
+                const uint32_t d = tmem + acc * kMlpMaxBN;
+                bool add = false;
+                for (int left = tl.k1 - tl.k0; left > 0; --left) {
+                    if (!mlp_wait(wait, full_at + 8 * s, phase, kMlpSiteFull)) { ok = false; break; }
                     tcgen05_after_sync();
-                    const uint32_t at = smem_u32(smem + s * Ring::kBytes);
-                    const uint64_t da = mlp_desc(at, prm.a.mn_major), db = mlp_desc(at + kMlpBM * kMlpBK * 2, prm.b.mn_major);
+                    const uint64_t da = desc_a + s * (uint32_t)(block_bytes / 16), db = desc_b + s * (uint32_t)(block_bytes / 16);
 #pragma unroll
-                    for (int i = 0; i < kMlpBK / 16; ++i) mlp_mma<CG>(d, da + i * step_a, db + i * step_b, idesc, kb > tl.k0 || i > 0);
-                    mlp_commit<CG>(&empty[s]);
+                    for (int i = 0; i < kMlpBK / 16; ++i) {
+                        mlp_mma<CG>(d, da + i * step_a, db + i * step_b, idesc, add);
+                        add = true;
+                    }
+                    mlp_commit<CG>(empty_at + 8 * s);
+                    if (++s == S) { s = 0; phase ^= 1; }
                 }
-                if (ok) mlp_commit<CG>(&acc_full[acc % 2]);
+                if (ok) mlp_commit<CG>(acc_full_at + 8 * acc);
+                if (++acc == 2) { acc = 0; acc_phase ^= 1; }
             }
             if (!ok) *failed = 1;
         }
     } else if (warp >= 4) {
         const int quad = warp % 4, part = (warp - 4) / 4;
-        const MlpStage st{epi + (warp - 4) * 2 * 32 * kMlpPitch, lane}, st2{st.base + 32 * kMlpPitch, lane};
+        const MlpStage st{epi + (warp - 4) * 2 * 32 * 64, lane}, st2{st.base + 32 * 64, lane};
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const int width = MODE == kMlpGated ? prm.BN / 2 : prm.BN, c0 = part * (width / 2), c1 = c0 + width / 2;
         const int row0 = (int)rank * kMlpBM + quad * 32;
@@ -437,20 +464,21 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
                 st.fetch(f2, p + prm.side_half, prm.side_stride, prm.M - m, prm.N - n, true);
             }
         };
-        int acc = 0;
-        for (int t = first; t < tiles; t += step, ++acc) {
+        uint32_t acc = 0, acc_phase = 0;
+        for (int t = first; t < tiles; t += step) {
             const MlpTile tl = mlp_tile<CG>(prm, t);
             const int m = tl.m + row0, rows = prm.M - m;
             fetch(m, tl.n + c0);
             bool ok = true;
-            if (lane == 0) ok = mlp_wait(prm.wait, &acc_full[acc % 2], (acc / 2) & 1, kMlpSiteAccFull);
+            if (lane == 0) ok = mlp_wait(prm.wait, acc_full_at + 8 * acc, acc_phase, kMlpSiteAccFull);
             ok = __shfl_sync(0xffffffffu, ok, 0);
             if (!ok) {
                 if (lane == 0) *failed = 1;
                 break;
             }
             tcgen05_after_sync();
-            const uint32_t d = tmem + acc % 2 * kMlpMaxBN + lanes;
+            const uint32_t d = tmem + acc * kMlpMaxBN + lanes, acc_done = acc_empty_at + 8 * acc;
+            if (++acc == 2) { acc = 0; acc_phase ^= 1; }
             for (int c = c0; c < c1; c += 32) {
                 const int n = tl.n + c, cols = prm.N - n;
                 float v[32], w[32];
@@ -471,7 +499,7 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
                 if (c + 32 >= c1) {
                     tcgen05_before_sync();
                     __syncwarp();
-                    if (lane == 0) mlp_arrive_leader<CG>(&acc_empty[acc % 2]);
+                    if (lane == 0) mlp_arrive_leader<CG>(acc_done);
                 }
                 if (cols <= 0) continue;
                 if (MODE == kMlpPartial) {
@@ -571,10 +599,10 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
     }
     if (bad) {  // a wait ran out: copies and products still under way end, or get as long again, before their memory is given back
         if (warp == 0 && lane == 0 && rank == 0)
-            for (int b = max(0, issued - S); b < issued; ++b) mlp_wait(prm.wait, &full[b % S], (b / S) & 1, kMlpSiteDrain);
+            for (int b = max(0, issued - S); b < issued; ++b) mlp_wait(prm.wait, full_at + 8 * (b % S), (b / S) & 1, kMlpSiteDrain);
         if (warp == 1 && lane == 0 && rank == 0) {
-            mlp_commit<CG>(drain);
-            mlp_wait(prm.wait, drain, 0, kMlpSiteDrain);
+            mlp_commit<CG>(smem_u32(drain));
+            mlp_wait(prm.wait, smem_u32(drain), 0, kMlpSiteDrain);
         }
         __syncwarp();
     }
