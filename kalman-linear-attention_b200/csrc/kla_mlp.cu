@@ -53,7 +53,7 @@ Plan plan(const Product &p, bool may_split, int sms) {
     for (const int cg : {2, 1})
         for (const int bn : {256, 192, 128, 64}) {
             if (p.gated() && bn % 128) continue;
-            const double cost = (bn == 256 ? 1.0 : bn == 192 ? 0.8 : bn == 128 ? 0.62 : 0.5) * (cg == 1 ? 1.6 : 1.0);
+            const double cost = (bn == 256 ? 1.0 : bn == 192 ? 0.78 : bn == 128 ? 0.62 : 0.5) * (cg == 1 ? 1.05 : 1.0);
             const int64_t tm = up(p.M, kMlpBM * cg) * (p.a.halves == kHalvesRows ? 2 : 1);
             const int64_t tn = up(p.N, p.gated() ? bn / 2 : bn), tiles = tm * tn;
             for (int s = 1; s <= (may_split ? 32 : 1) && s <= blocks; ++s) {

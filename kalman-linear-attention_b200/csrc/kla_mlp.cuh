@@ -91,7 +91,8 @@ __device__ __forceinline__ bool mlp_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-__device__ __noinline__ bool mlp_wait_long(const WaitCtl &w, uint32_t bar, uint32_t parity, int site) {
+__device__ __forceinline__ bool mlp_wait(const WaitCtl &w, uint32_t bar, uint32_t parity, int site) {
+    if (mlp_try(bar, parity)) return true;
     const long long begin = clock64(), limit = 2ll * w.limit_ns;
     do {
         for (int i = 0; i < 32; ++i)
@@ -100,8 +101,13 @@ __device__ __noinline__ bool mlp_wait_long(const WaitCtl &w, uint32_t bar, uint3
     atomicCAS(w.status, 0, kStatusWait | site);
     return false;
 }
-__device__ __forceinline__ bool mlp_wait(const WaitCtl &w, uint32_t bar, uint32_t parity, int site) {
-    return mlp_try(bar, parity) || mlp_wait_long(w, bar, parity, site);
+// One lane of a converged warp. The warps that issue loads and products run their loops whole and leave the issuing to this lane by
+// a predicate on the instruction: the operands then stay in the uniform registers those instructions take. With a loop of one lane
+// every product cost its thread 36 ns of moves between register files and a block's hand-over 155 ns.
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r;
 }
 
 // Shared memory descriptor of an operand tile in the 128-byte swizzle: 8 rows of 128 bytes make an atom of 1024.
@@ -118,25 +124,28 @@ __device__ __forceinline__ uint64_t mlp_desc(uint32_t addr, bool mn_major) {
 }
 
 template <int CG>
-__device__ __forceinline__ void mlp_mma(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mlp_mma(uint32_t on, uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
     if constexpr (CG == 2)
         asm volatile(
-            "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(acc), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+            "{\n.reg .pred p, q;\nsetp.ne.u32 p, %4, 0;\nsetp.ne.u32 q, %5, 0;\n"
+            "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(acc), "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(on)
             : "memory");
     else
         asm volatile(
-            "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(acc), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+            "{\n.reg .pred p, q;\nsetp.ne.u32 p, %4, 0;\nsetp.ne.u32 q, %5, 0;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(acc), "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(on)
             : "memory");
 }
 // an arrival at the barrier, in a pair at both CTAs', when the products issued so far are done
 template <int CG>
-__device__ __forceinline__ void mlp_commit(uint32_t bar) {
+__device__ __forceinline__ void mlp_commit(uint32_t on, uint32_t bar) {
     if constexpr (CG == 2)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+        asm volatile(
+            "{\n.reg .pred q;\nsetp.ne.u32 q, %2, 0;\n"
+            "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}\n" ::"r"(bar), "h"((uint16_t)3), "r"(on)
+            : "memory");
     else
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+        asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %1, 0;\n@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar), "r"(on) : "memory");
 }
 // the address that `addr` has in the pair's first CTA
 __device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
@@ -149,20 +158,22 @@ __device__ __forceinline__ void mlp_arrive_leader(uint32_t bar) {
     if constexpr (CG == 2) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_leader(bar)) : "memory");
     else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void mlp_expect(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+__device__ __forceinline__ void mlp_expect(uint32_t on, uint32_t bar, uint32_t bytes) {
+    asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %2, 0;\n@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}\n" ::"r"(bar), "r"(bytes), "r"(on) : "memory");
 }
 template <int CG>
-__device__ __forceinline__ void mlp_load(uint32_t dst, uint64_t tm, int x, int y, int z, uint32_t bar) {  // bar: the leader's
+__device__ __forceinline__ void mlp_load(uint32_t on, uint32_t dst, uint64_t tm, int x, int y, int z, uint32_t bar) {  // bar: the leader's
     if constexpr (CG == 2)
         asm volatile(
-            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-            " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(tm), "r"(x), "r"(y), "r"(z), "r"(bar)
+            "{\n.reg .pred q;\nsetp.ne.u32 q, %6, 0;\n"
+            "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%2, %3, %4}], [%5];\n}\n" ::"r"(dst), "l"(tm), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(on)
             : "memory");
     else
         asm volatile(
-            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-            " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(tm), "r"(x), "r"(y), "r"(z), "r"(bar)
+            "{\n.reg .pred q;\nsetp.ne.u32 q, %6, 0;\n"
+            "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%2, %3, %4}], [%5];\n}\n" ::"r"(dst), "l"(tm), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(on)
             : "memory");
 }
 __device__ __forceinline__ void mlp_cluster_sync() {
@@ -287,23 +298,46 @@ __device__ __forceinline__ float mlp_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// The activation and its derivative.
-template <bool SLOPE>
-__device__ __forceinline__ void mlp_act(float g, int act, float &f, float &df) {
-    if (act == 0) {  // silu
+// The activation and its derivative. Which one is chosen once for 32 columns, not per element: with the choice (and gelu's error
+// function) inside the unrolled loops their code left the instruction cache, and the gated product took 288 us in place of @G@, the
+// one of the gradients 342 in place of @D@ (32768 rows of 768, H = 2048).
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ void mlp_act(float g, float &f, float &df) {
+    if (ACT == 0) {  // silu
         const float s = rcp_approx(1.0f + mlp_ex2(-1.4426950408889634f * g));
         f = g * s;
         if (SLOPE) df = fmaf(f, 1.0f - s, s);
-    } else if (act == 1) {  // gelu
+    } else if (ACT == 1) {  // gelu
         const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
         f = g * cdf;
         if (SLOPE) df = fmaf(g * 0.3989422804014327f, mlp_ex2(-0.72134752044448170f * g * g), cdf);
-    } else if (act == 2) {  // relu; NaN stays
+    } else if (ACT == 2) {  // relu; NaN stays
         f = g < 0.0f ? 0.0f : g;
         if (SLOPE) df = g > 0.0f ? 1.0f : 0.0f;
     } else {
         f = g;
         if (SLOPE) df = 1.0f;
+    }
+}
+// g -> act(g) u
+template <int ACT>
+__device__ __forceinline__ void mlp_gate(float (&g)[32], const float (&u)[32]) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+        float f, df;
+        mlp_act<ACT, false>(g[j], f, df);
+        g[j] = f * u[j];
+    }
+}
+// dh -> the gradients of gate (in its place) and of up, from the kept rows
+template <int ACT>
+__device__ __forceinline__ void mlp_slopes(float (&dh)[32], float (&du)[32], const uint4 (&g)[4], const uint4 (&u)[4]) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+        float f, df;
+        mlp_act<ACT, true>(kept(word_at(g, j), j % 2), f, df);
+        du[j] = dh[j] * f;
+        dh[j] = dh[j] * kept(word_at(u, j), j % 2) * df;
     }
 }
 
@@ -338,7 +372,7 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
     uint64_t *full = reinterpret_cast<uint64_t *>(epi + kMlpEpiBytes), *empty = full + kMlpMaxStages, *acc_full = empty + kMlpMaxStages, *acc_empty = acc_full + 2, *drain = acc_empty + 2;
     uint32_t *tmem_at = reinterpret_cast<uint32_t *>(drain + 1);
     int *failed = reinterpret_cast<int *>(tmem_at + 1);
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;  // (known to be uniform)
     uint32_t rank = 0;
     if (CG == 2) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     const int first = blockIdx.x / CG, step = gridDim.x / CG;
@@ -370,56 +404,55 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
     const uint32_t smem_at = smem_u32(smem), full_at = smem_u32(full), empty_at = smem_u32(empty), acc_full_at = smem_u32(acc_full), acc_empty_at = smem_u32(acc_empty);
 
     if (warp == 0) {
-        if (lane == 0) {
-            const WaitCtl wait = prm.wait;
-            const uint64_t map_a = reinterpret_cast<uint64_t>(&prm.map_a), map_b = reinterpret_cast<uint64_t>(&prm.map_b);
-            const bool a_lines = prm.a.mn_major != 0, b_lines = prm.b.mn_major != 0;
-            // B's rows of this CTA; a gated pair's first CTA has gate's, its second up's, a CTA alone both, one behind the other
-            const bool both = prm.b.halves == kHalvesBoth, a_rows_half = prm.a.halves == kHalvesRows;
-            const int b_rows = prm.BN / CG / (both && CG == 1 ? 2 : 1), b_first = both ? 0 : (int)rank * b_rows, stretch_blocks = prm.blocks_stretch;
-            const uint32_t bytes = CG * block_bytes;
-            const uint32_t leader_full = CG == 2 ? in_leader(full_at) : full_at;
-            int s = 0;
-            uint32_t phase = 1;  // the ring begins empty: a wait for the phase before the first passes
-            bool ok = true;
-            for (int t = first; ok && t < tiles; t += step) {
-                const MlpTile tl = mlp_tile<CG>(prm, t);
-                int stretch = tl.k0 / stretch_blocks, kb = tl.k0 - stretch * stretch_blocks;
-                const int m = tl.m + (int)rank * kMlpBM, n = tl.n + b_first;
-                for (int left = tl.k1 - tl.k0; left > 0; --left) {
-                    if (!mlp_wait(wait, empty_at + 8 * s, phase, kMlpSiteEmpty) || issued == wait.skip_tile) {  // skip_tile: the tests'
-                        ok = false;                                                                            // incomplete hand-over
-                        break;
-                    }
-                    const uint32_t at_a = smem_at + s * block_bytes, at_b = at_a + kMlpBM * kMlpBK * 2, bar = leader_full + 8 * s;
-                    const int k = kb * kMlpBK, za = a_rows_half ? tl.m_half : stretch, zb = both ? (int)rank : stretch;
-                    if (rank == 0) mlp_expect(full_at + 8 * s, bytes);
-                    if (a_lines) {
-                        mlp_load<CG>(at_a, map_a, m, k, za, bar);
-                        mlp_load<CG>(at_a + 64 * 128, map_a, m + 64, k, za, bar);
-                    } else {
-                        mlp_load<CG>(at_a, map_a, k, m, za, bar);
-                    }
-                    if (b_lines) {
-                        for (int r = 0; r < b_rows; r += 64) mlp_load<CG>(at_b + r * 128, map_b, n + r, k, zb, bar);
-                    } else {
-                        mlp_load<CG>(at_b, map_b, k, n, zb, bar);
-                        if (both && CG == 1) mlp_load<CG>(at_b + b_rows * 128, map_b, k, n, 1, bar);
-                    }
-                    ++issued;
-                    if (++s == S) { s = 0; phase ^= 1; }
-                    if (++kb == stretch_blocks) { kb = 0; ++stretch; }
+        const uint32_t on = elect_one();
+        const WaitCtl wait = prm.wait;
+        const uint64_t map_a = reinterpret_cast<uint64_t>(&prm.map_a), map_b = reinterpret_cast<uint64_t>(&prm.map_b);
+        const bool a_lines = prm.a.mn_major != 0, b_lines = prm.b.mn_major != 0;
+        // B's rows of this CTA; a gated pair's first CTA has gate's, its second up's, a CTA alone both, one behind the other
+        const bool both = prm.b.halves == kHalvesBoth, a_rows_half = prm.a.halves == kHalvesRows;
+        const int b_rows = prm.BN / CG / (both && CG == 1 ? 2 : 1), b_first = both ? 0 : (int)rank * b_rows, stretch_blocks = prm.blocks_stretch;
+        const uint32_t bytes = CG * block_bytes, leader_full = CG == 2 ? in_leader(full_at) : full_at;
+        int s = 0;
+        uint32_t phase = 1;  // the ring begins empty: a wait for the phase before the first passes
+        bool ok = true;
+        for (int t = first; ok && t < tiles; t += step) {
+            const MlpTile tl = mlp_tile<CG>(prm, t);
+            int stretch = tl.k0 / stretch_blocks, kb = tl.k0 - stretch * stretch_blocks;
+            const int m = tl.m + (int)rank * kMlpBM, n = tl.n + b_first;
+            for (int left = tl.k1 - tl.k0; left > 0; --left) {
+                if (!mlp_wait(wait, empty_at + 8 * s, phase, kMlpSiteEmpty) || issued == wait.skip_tile) {  // skip_tile: the tests'
+                    ok = false;                                                                            // incomplete hand-over
+                    break;
                 }
+                const uint32_t at_a = smem_at + s * block_bytes, at_b = at_a + kMlpBM * kMlpBK * 2, bar = leader_full + 8 * s;
+                const int k = kb * kMlpBK, za = a_rows_half ? tl.m_half : stretch, zb = both ? (int)rank : stretch;
+                if (rank == 0) mlp_expect(on, full_at + 8 * s, bytes);
+                if (a_lines) {
+                    mlp_load<CG>(on, at_a, map_a, m, k, za, bar);
+                    mlp_load<CG>(on, at_a + 64 * 128, map_a, m + 64, k, za, bar);
+                } else {
+                    mlp_load<CG>(on, at_a, map_a, k, m, za, bar);
+                }
+                if (b_lines) {
+                    for (int r = 0; r < b_rows; r += 64) mlp_load<CG>(on, at_b + r * 128, map_b, n + r, k, zb, bar);
+                } else {
+                    mlp_load<CG>(on, at_b, map_b, k, n, zb, bar);
+                    if (both && CG == 1) mlp_load<CG>(on, at_b + b_rows * 128, map_b, k, n, 1, bar);
+                }
+                ++issued;
+                if (++s == S) { s = 0; phase ^= 1; }
+                if (++kb == stretch_blocks) { kb = 0; ++stretch; }
             }
-            if (!ok) *failed = 1;
         }
+        if (!ok && lane == 0) *failed = 1;
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
+            const uint32_t on = elect_one();
             const WaitCtl wait = prm.wait;
             // float32 accumulators of bfloat16 operands; majors; N / 8; M / 16
             const uint32_t idesc = 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(prm.a.mn_major != 0) << 15 | (uint32_t)(prm.b.mn_major != 0) << 16 |
                                    (uint32_t)(prm.BN / 8) << 17 | (uint32_t)(kMlpBM * CG / 16) << 24;
-            const uint64_t step_a = (prm.a.mn_major ? 2048 : 32) / 16, step_b = (prm.b.mn_major ? 2048 : 32) / 16;
+            const uint32_t step_a = (prm.a.mn_major ? 2048 : 32) / 16, step_b = (prm.b.mn_major ? 2048 : 32) / 16;
             const uint64_t desc_a = mlp_desc(smem_at, prm.a.mn_major), desc_b = mlp_desc(smem_at + kMlpBM * kMlpBK * 2, prm.b.mn_major);
             int s = 0;
             uint32_t phase = 0, acc = 0, acc_phase = 1;
@@ -429,23 +462,23 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
                 if (!mlp_wait(wait, acc_empty_at + 8 * acc, acc_phase, kMlpSiteAccEmpty)) { ok = false; break; }
                 tcgen05_after_sync();
                 const uint32_t d = tmem + acc * kMlpMaxBN;
-                bool add = false;
+                uint32_t add = 0;
                 for (int left = tl.k1 - tl.k0; left > 0; --left) {
                     if (!mlp_wait(wait, full_at + 8 * s, phase, kMlpSiteFull)) { ok = false; break; }
                     tcgen05_after_sync();
-                    const uint64_t da = desc_a + s * (uint32_t)(block_bytes / 16), db = desc_b + s * (uint32_t)(block_bytes / 16);
+                    const uint64_t da = desc_a + (uint32_t)(s * block_bytes / 16), db = desc_b + (uint32_t)(s * block_bytes / 16);
 #pragma unroll
                     for (int i = 0; i < kMlpBK / 16; ++i) {
-                        mlp_mma<CG>(d, da + i * step_a, db + i * step_b, idesc, add);
-                        add = true;
+                        mlp_mma<CG>(on, d, da + i * step_a, db + i * step_b, idesc, add);
+                        add = 1;
                     }
-                    mlp_commit<CG>(empty_at + 8 * s);
+                    mlp_commit<CG>(on, empty_at + 8 * s);
                     if (++s == S) { s = 0; phase ^= 1; }
                 }
-                if (ok) mlp_commit<CG>(acc_full_at + 8 * acc);
+                if (ok) mlp_commit<CG>(on, acc_full_at + 8 * acc);
                 if (++acc == 2) { acc = 0; acc_phase ^= 1; }
             }
-            if (!ok) *failed = 1;
+            if (!ok && lane == 0) *failed = 1;
         }
     } else if (warp >= 4) {
         const int quad = warp % 4, part = (warp - 4) / 4;
@@ -556,24 +589,19 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
                         st2.store(gu + prm.gu_half, prm.gu_stride, rows, cols, true);
                         __syncwarp();
                     }
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        float f, df;
-                        mlp_act<false>(v[j], prm.act, f, df);
-                        v[j] = f * w[j];
-                    }
+                    if (prm.act == 0) mlp_gate<0>(v, w);
+                    else if (prm.act == 1) mlp_gate<1>(v, w);
+                    else if (prm.act == 2) mlp_gate<2>(v, w);
+                    else mlp_gate<3>(v, w);
                     pack_row(r, v);
                     st.put_row(r);
                     __syncwarp();
                     st.store(out, prm.out_stride, rows, cols, prm.out_vec);
                 } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        float f, df;
-                        mlp_act<true>(kept(word_at(r, j), j % 2), prm.act, f, df);
-                        w[j] = v[j] * f;                                      // of up
-                        v[j] = v[j] * kept(word_at(q, j), j % 2) * df;        // of gate
-                    }
+                    if (prm.act == 0) mlp_slopes<0>(v, w, r, q);
+                    else if (prm.act == 1) mlp_slopes<1>(v, w, r, q);
+                    else if (prm.act == 2) mlp_slopes<2>(v, w, r, q);
+                    else mlp_slopes<3>(v, w, r, q);
                     pack_row(r, v);
                     st.put_row(r);
                     pack_row(r, w);
@@ -600,8 +628,8 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
     if (bad) {  // a wait ran out: copies and products still under way end, or get as long again, before their memory is given back
         if (warp == 0 && lane == 0 && rank == 0)
             for (int b = max(0, issued - S); b < issued; ++b) mlp_wait(prm.wait, full_at + 8 * (b % S), (b / S) & 1, kMlpSiteDrain);
-        if (warp == 1 && lane == 0 && rank == 0) {
-            mlp_commit<CG>(smem_u32(drain));
+        if (warp == 1 && rank == 0) {
+            mlp_commit<CG>(elect_one(), smem_u32(drain));
             mlp_wait(prm.wait, smem_u32(drain), 0, kMlpSiteDrain);
         }
         __syncwarp();
