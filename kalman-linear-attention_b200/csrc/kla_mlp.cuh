@@ -153,10 +153,12 @@ __device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
     return r;
 }
+// Without release semantics, which would wait for the warp's stores to memory: what the arrival reports, that the accumulator has
+// been read, is complete (tcgen05.wait::ld) and fenced before it.
 template <int CG>
 __device__ __forceinline__ void mlp_arrive_leader(uint32_t bar) {
-    if constexpr (CG == 2) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_leader(bar)) : "memory");
-    else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+    if constexpr (CG == 2) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_leader(bar)) : "memory");
+    else asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void mlp_expect(uint32_t on, uint32_t bar, uint32_t bytes) {
     asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %2, 0;\n@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}\n" ::"r"(bar), "r"(bytes), "r"(on) : "memory");
@@ -275,14 +277,15 @@ __device__ __forceinline__ void pack_row(uint4 (&v)[4], const float (&x)[32]) {
 // the result alone); nine bits leave the rounding of the gradients that go into the products (0.0025). 2^-31 to 2^33 at full
 // accuracy, steps of 2^-40 below; what is larger, infinite or NaN comes back as NaN.
 constexpr uint32_t kKeptTop = 0x7fffu << 14;
-__device__ __forceinline__ uint32_t keep2(float lo, float hi) {
-    const uint32_t a = __float_as_uint(lo * 0x1p-96f), b = __float_as_uint(hi * 0x1p-96f);
-    const uint32_t ma = min((a & 0x7fffffffu) + 0x2000u, kKeptTop), mb = min((b & 0x7fffffffu) + 0x2000u, kKeptTop);
-    return (ma >> 14 | (a >> 16 & 0x8000u)) | ((mb << 2 & 0x7fff0000u) | (b & 0x80000000u));
+// the code in the upper half; the least of the value and kKeptTop makes NaN the top code, too
+__device__ __forceinline__ uint32_t keep(float x) {
+    const float m = fminf(fabsf(x) * 0x1p-96f, __uint_as_float(kKeptTop));
+    return __float_as_uint(m) * 4u + 0x8000u | __float_as_uint(x) & 0x80000000u;
 }
+__device__ __forceinline__ uint32_t keep2(float lo, float hi) { return __byte_perm(keep(lo), keep(hi), 0x7632); }
 __device__ __forceinline__ float kept(uint32_t w, bool high) {  // one half of a word
-    const uint32_t m = high ? (w >> 2 & kKeptTop) : (w << 14 & kKeptTop), sign = high ? w & 0x80000000u : w << 16 & 0x80000000u;
-    return m == kKeptTop ? __uint_as_float(0x7fffffffu) : __uint_as_float(m | sign) * 0x1p96f;
+    const uint32_t m = (uint32_t)((int32_t)(high ? w : w << 16) >> 2) & 0x9fffc000u;
+    return (m & 0x7fffffffu) == kKeptTop ? __uint_as_float(0x7fffffffu) : __uint_as_float(m) * 0x1p96f;
 }
 __device__ __forceinline__ uint32_t word_at(const uint4 (&v)[4], int j) {  // j a constant after unrolling
     return j / 2 % 4 == 0 ? v[j / 8].x : j / 2 % 4 == 1 ? v[j / 8].y : j / 2 % 4 == 2 ? v[j / 8].z : v[j / 8].w;
@@ -502,6 +505,17 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
             const MlpTile tl = mlp_tile<CG>(prm, t);
             const int m = tl.m + row0, rows = prm.M - m;
             fetch(m, tl.n + c0);
+            if (MODE == kMlpGrad && t + step < tiles) {  // the next tile's gate and up into L2: a chunk ahead covers L2's latency only
+                const MlpTile nx = mlp_tile<CG>(prm, t + step);
+                const int nm = nx.m + row0 + lane, nn = nx.n + c0;
+                if (nm < prm.M) {
+                    const __nv_bfloat16 *p = prm.side + (long long)nm * prm.side_stride + nn;
+                    for (int c = 0; c < c1 - c0 && nn + c < prm.N; c += 64) {
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(p + c));
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(p + prm.side_half + c));
+                    }
+                }
+            }
             bool ok = true;
             if (lane == 0) ok = mlp_wait(prm.wait, acc_full_at + 8 * acc, acc_phase, kMlpSiteAccFull);
             ok = __shfl_sync(0xffffffffu, ok, 0);
