@@ -84,7 +84,7 @@ int fill(MlpParams *prm, const Product &p, const Plan &pl) {
     prm->b = MlpOperand{p.b.adjacent_rows, p.b.halves};
     prm->M = (int)p.M; prm->N = (int)p.N; prm->K = (int)p.K;
     prm->BN = pl.BN; prm->tiles_m = pl.tiles_m; prm->tiles_n = pl.tiles_n; prm->splits = pl.splits;
-    prm->stages = std::min(kMlpMaxStages, kMlpRingBytes / mlp_block_bytes(pl.BN, pl.CG, p.b.adjacent_rows));
+    prm->stages = std::min(kMlpMaxStages, mlp_ring_bytes(p.mode) / mlp_block_bytes(pl.BN, pl.CG, p.b.adjacent_rows));
     prm->blocks_stretch = (int)up(p.K, kMlpBK);
     prm->blocks_k = prm->blocks_stretch * (p.a.halves == kHalvesSummed ? 2 : 1);
     return entry::wait_ctl(&prm->wait);
@@ -104,8 +104,8 @@ int resident_pairs() {
         attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)device_sms() / 2 * 2);
-        cfg.blockDim = dim3(kMlpThreads);
-        cfg.dynamicSmemBytes = kMlpSmem;
+        cfg.blockDim = dim3(mlp_threads(kMlpPlain));
+        cfg.dynamicSmemBytes = mlp_smem(kMlpPlain);
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
         int n = 0;
@@ -120,9 +120,9 @@ int resident_pairs() {
 
 template <int MODE, int CG>
 int launch_as(const MlpParams &prm, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(kla_mlp_kernel<MODE, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMlpSmem);
+    cudaError_t e = cudaFuncSetAttribute(kla_mlp_kernel<MODE, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)mlp_smem(MODE));
     if (e == cudaSuccess && CG == 2)
-        e = cudaFuncSetAttribute(kla_mlp_kernel<kMlpPlain, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMlpSmem);
+        e = cudaFuncSetAttribute(kla_mlp_kernel<kMlpPlain, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)mlp_smem(kMlpPlain));
     if (e != cudaSuccess) return entry::cuda_fail(e);
     const int64_t tiles = (int64_t)prm.tiles_m * prm.tiles_n * prm.splits;
     if (tiles > 0x3fffffffll) return KLA_B200_EUNSUPPORTED;
@@ -133,8 +133,8 @@ int launch_as(const MlpParams &prm, cudaStream_t st) {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(tiles < most ? tiles : most) * CG);
-    cfg.blockDim = dim3(kMlpThreads);
-    cfg.dynamicSmemBytes = kMlpSmem;
+    cfg.blockDim = dim3(mlp_threads(MODE));
+    cfg.dynamicSmemBytes = mlp_smem(MODE);
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = CG == 2 ? 1 : 0;

@@ -23,11 +23,14 @@
 namespace kla {
 
 constexpr int kMlpBM = 128, kMlpBK = 64, kMlpMaxBN = 256;  // rows of a CTA, summed length of a block, columns of a tile
-constexpr int kMlpEpiWarps = 8;
-constexpr int kMlpThreads = (4 + kMlpEpiWarps) * 32;
-constexpr int kMlpEpiBytes = kMlpEpiWarps * 2 * 32 * 64;  // two stages of 32 rows of 64 bytes a warp
-constexpr int kMlpRingBytes = 192 * 1024, kMlpMaxStages = 8;
-constexpr size_t kMlpSmem = 1024 + kMlpRingBytes + kMlpEpiBytes + 256;
+// Warps of the epilogue. The gradients of gate and up take 16: with 8 the four instructions' latencies of a warp's chunk (its loads, the
+// accumulator's, the stage's, the stores) were not covered, 179 us in place of @D@ at 32768 rows of 768, H = 2048.
+constexpr int kMlpStageBytes = 2 * 32 * 64;  // two stages of 32 rows of 64 bytes a warp
+constexpr int kMlpMaxStages = 8;
+__host__ __device__ constexpr int mlp_epi_warps(int mode) { return mode == 2 ? 16 : 8; }
+__host__ __device__ constexpr int mlp_threads(int mode) { return (4 + mlp_epi_warps(mode)) * 32; }
+__host__ __device__ constexpr int mlp_ring_bytes(int mode) { return (224 - mlp_epi_warps(mode) * 4) * 1024; }
+__host__ __device__ constexpr size_t mlp_smem(int mode) { return 1024 + mlp_ring_bytes(mode) + mlp_epi_warps(mode) * kMlpStageBytes + 256; }
 // A block of the ring: A's rows of a CTA and its share of B's, which in a pair of CTAs is half of them. What is in flight is what
 // bounds the loads (a tile's block takes about 1 us from L2): with 5 blocks of 32 KB in place of 6 K=4096 N=1024 ran at 1213 TFLOP/s
 inline __host__ __device__ int mlp_b_rows(int BN, int cg, bool mn_major) { return mn_major ? (BN / cg + 63) / 64 * 64 : BN / cg; }
@@ -193,7 +196,30 @@ __device__ __forceinline__ void tmem_load32(float (&v)[32], uint32_t addr) {
           "=r"(r[31])
         : "r"(addr));
 }
-__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_load8(float (&v)[8], uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "r"(addr));
+}
+// The loads have arrived; the registers pass through, so that nothing is taken from them before.
+__device__ __forceinline__ void tmem_load_wait(float (&v)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7])::"memory");
+}
+__device__ __forceinline__ void tmem_load_wait(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]),
+                   "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]),
+                   "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]),
+                   "+f"(v[31])::"memory");
+}
+// behind a wait already made: the registers pass through
+__device__ __forceinline__ void tmem_loaded(float (&v)[32]) {
+    asm volatile(""
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]),
+                   "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]),
+                   "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]),
+                   "+f"(v[31])::"memory");
+}
 __device__ __forceinline__ void tcgen05_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tcgen05_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
@@ -332,15 +358,37 @@ __device__ __forceinline__ void mlp_gate(float (&g)[32], const float (&u)[32]) {
         g[j] = f * u[j];
     }
 }
-// dh -> the gradients of gate (in its place) and of up, from the kept rows
+// The gradients of gate and up of a row's eight columns, in place of the kept gate and up.
 template <int ACT>
-__device__ __forceinline__ void mlp_slopes(float (&dh)[32], float (&du)[32], const uint4 (&g)[4], const uint4 (&u)[4]) {
+__device__ __forceinline__ void mlp_slopes(const float (&dh)[8], uint4 &gate, uint4 &up) {
+    uint32_t *g = reinterpret_cast<uint32_t *>(&gate), *u = reinterpret_cast<uint32_t *>(&up);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-        float f, df;
-        mlp_act<ACT, true>(kept(word_at(g, j), j % 2), f, df);
-        du[j] = dh[j] * f;
-        dh[j] = dh[j] * kept(word_at(u, j), j % 2) * df;
+    for (int j = 0; j < 4; ++j) {
+        float f[2], df[2];
+        mlp_act<ACT, true>(kept(g[j], false), f[0], df[0]);
+        mlp_act<ACT, true>(kept(g[j], true), f[1], df[1]);
+        g[j] = pack2(dh[2 * j] * kept(u[j], false) * df[0], dh[2 * j + 1] * kept(u[j], true) * df[1]);
+        u[j] = pack2(dh[2 * j] * f[0], dh[2 * j + 1] * f[1]);
+    }
+}
+// ... of a chunk of 32 columns: dh from the accumulator, the kept ones from the warp's two stages, eight columns at a time while the
+// next eight are on their way.
+template <int ACT>
+__device__ __forceinline__ void mlp_slopes_chunk(uint32_t acc, const MlpStage &st, const MlpStage &st2) {
+    float next[8];
+    tmem_load8(next, acc);
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+        float dh[8];
+        tmem_load_wait(next);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dh[j] = next[j];
+        if (i < 3) tmem_load8(next, acc + 8 * (i + 1));
+        uint4 *pg = reinterpret_cast<uint4 *>(st.piece(st.lane, i)), *pu = reinterpret_cast<uint4 *>(st2.piece(st.lane, i));
+        uint4 g = *pg, u = *pu;
+        mlp_slopes<ACT>(dh, g, u);
+        *pg = g;
+        *pu = u;
     }
 }
 
@@ -366,13 +414,14 @@ __device__ __forceinline__ MlpTile mlp_tile(const MlpParams &p, int t) {
 }
 
 template <int MODE, int CG>
-__global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_constant__ MlpParams prm) {
+__global__ void __launch_bounds__(mlp_threads(MODE), 1) kla_mlp_kernel(const __grid_constant__ MlpParams prm) {
     extern __shared__ char raw[];
     char *smem = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    char *epi = smem + kMlpRingBytes;
+    constexpr int W = mlp_epi_warps(MODE), PARTS = W / 4;
+    char *epi = smem + mlp_ring_bytes(MODE);
     const int S = prm.stages, block_bytes = mlp_block_bytes(prm.BN, CG, prm.b.mn_major);
     // full, acc_empty: of the leader (the pair's first CTA); empty, acc_full: of each CTA
-    uint64_t *full = reinterpret_cast<uint64_t *>(epi + kMlpEpiBytes), *empty = full + kMlpMaxStages, *acc_full = empty + kMlpMaxStages, *acc_empty = acc_full + 2, *drain = acc_empty + 2;
+    uint64_t *full = reinterpret_cast<uint64_t *>(epi + W * kMlpStageBytes), *empty = full + kMlpMaxStages, *acc_full = empty + kMlpMaxStages, *acc_empty = acc_full + 2, *drain = acc_empty + 2;
     uint32_t *tmem_at = reinterpret_cast<uint32_t *>(drain + 1);
     int *failed = reinterpret_cast<int *>(tmem_at + 1);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;  // (known to be uniform)
@@ -382,7 +431,7 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], kMlpEpiWarps * CG); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], W * CG); }
         mbar_init(drain, 1);
         *failed = 0;
         mbar_fence_init();
@@ -485,9 +534,10 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
         }
     } else if (warp >= 4) {
         const int quad = warp % 4, part = (warp - 4) / 4;
-        const MlpStage st{epi + (warp - 4) * 2 * 32 * 64, lane}, st2{st.base + 32 * 64, lane};
+        const MlpStage st{epi + (warp - 4) * kMlpStageBytes, lane}, st2{st.base + 32 * 64, lane};
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-        const int width = MODE == kMlpGated ? prm.BN / 2 : prm.BN, c0 = part * (width / 2), c1 = c0 + width / 2;
+        // chunks of 32 columns are dealt to the warps of a quarter of the rows in turn
+        const int width = MODE == kMlpGated ? prm.BN / 2 : prm.BN, c0 = part * 32, cstep = PARTS * 32;
         const int row0 = (int)rank * kMlpBM + quad * 32;
         // what the epilogue reads besides the accumulator is fetched a chunk of 32 columns ahead, the next tile's first during the
         // wait for its accumulator
@@ -504,13 +554,13 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
         for (int t = first; t < tiles; t += step) {
             const MlpTile tl = mlp_tile<CG>(prm, t);
             const int m = tl.m + row0, rows = prm.M - m;
-            fetch(m, tl.n + c0);
+            if (c0 < width) fetch(m, tl.n + c0);
             if (MODE == kMlpGrad && t + step < tiles) {  // the next tile's gate and up into L2: a chunk ahead covers L2's latency only
                 const MlpTile nx = mlp_tile<CG>(prm, t + step);
                 const int nm = nx.m + row0 + lane, nn = nx.n + c0;
                 if (nm < prm.M) {
                     const __nv_bfloat16 *p = prm.side + (long long)nm * prm.side_stride + nn;
-                    for (int c = 0; c < c1 - c0 && nn + c < prm.N; c += 64) {
+                    for (int c = 0; c0 + c < width && nn + c < prm.N; c += cstep) {
                         asm volatile("prefetch.global.L2 [%0];" ::"l"(p + c));
                         asm volatile("prefetch.global.L2 [%0];" ::"l"(p + prm.side_half + c));
                     }
@@ -526,28 +576,51 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
             tcgen05_after_sync();
             const uint32_t d = tmem + acc * kMlpMaxBN + lanes, acc_done = acc_empty_at + 8 * acc;
             if (++acc == 2) { acc = 0; acc_phase ^= 1; }
-            for (int c = c0; c < c1; c += 32) {
+            if (c0 >= width) {
+                __syncwarp();
+                if (lane == 0) mlp_arrive_leader<CG>(acc_done);
+            }
+            for (int c = c0; c < width; c += cstep) {
                 const int n = tl.n + c, cols = prm.N - n;
+                auto done = [&] {  // behind the last read of the accumulator
+                    if (c + cstep >= width) {
+                        tcgen05_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mlp_arrive_leader<CG>(acc_done);
+                    }
+                };
+                __nv_bfloat16 *out = prm.out + tl.m_half * prm.out_half + (long long)m * prm.out_stride + n;
+                if constexpr (MODE == kMlpGrad) {
+                    st.put_fetched(f1);
+                    st2.put_fetched(f2);
+                    __syncwarp();
+                    if (c + cstep < width) fetch(m, n + cstep);
+                    if (prm.act == 0) mlp_slopes_chunk<0>(d + c, st, st2);
+                    else if (prm.act == 1) mlp_slopes_chunk<1>(d + c, st, st2);
+                    else if (prm.act == 2) mlp_slopes_chunk<2>(d + c, st, st2);
+                    else mlp_slopes_chunk<3>(d + c, st, st2);
+                    done();
+                    __syncwarp();
+                    st.store(out, prm.out_stride, rows, cols, true);
+                    st2.store(out + prm.out_half, prm.out_stride, rows, cols, true);
+                    __syncwarp();
+                    continue;
+                }
                 float v[32], w[32];
-                uint4 r[4], q[4];
+                uint4 r[4];
                 tmem_load32(v, d + c);
                 if (MODE == kMlpGated) tmem_load32(w, d + width + c);
-                const bool side = (MODE == kMlpPlain && prm.side != nullptr) || MODE == kMlpGrad;
+                const bool side = MODE == kMlpPlain && prm.side != nullptr;
                 if (side) {
                     st.put_fetched(f1);
-                    if (MODE == kMlpGrad) st2.put_fetched(f2);
                     __syncwarp();
                     st.get_row(r);
-                    if (MODE == kMlpGrad) st2.get_row(q);
                     __syncwarp();
-                    if (c + 32 < c1) fetch(m, n + 32);
+                    if (c + cstep < width) fetch(m, n + cstep);
                 }
-                tmem_load_wait();
-                if (c + 32 >= c1) {
-                    tcgen05_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mlp_arrive_leader<CG>(acc_done);
-                }
+                tmem_load_wait(v);
+                if (MODE == kMlpGated) tmem_loaded(w);
+                done();
                 if (cols <= 0) continue;
                 if (MODE == kMlpPartial) {
                     float *p = prm.partial + (long long)tl.split * prm.partial_rows * prm.partial_stride +
@@ -566,7 +639,6 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
                     __syncwarp();
                     continue;
                 }
-                __nv_bfloat16 *out = prm.out + tl.m_half * prm.out_half + (long long)m * prm.out_stride + n;
                 if (MODE == kMlpPlain) {
                     if (prm.bias != nullptr) {
 #pragma unroll
@@ -583,7 +655,7 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
                     st.put_row(r);
                     __syncwarp();
                     st.store(out, prm.out_stride, rows, cols, prm.out_vec);
-                } else if (MODE == kMlpGated) {
+                } else {
                     if (prm.bias != nullptr) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
@@ -611,18 +683,6 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
                     st.put_row(r);
                     __syncwarp();
                     st.store(out, prm.out_stride, rows, cols, prm.out_vec);
-                } else {
-                    if (prm.act == 0) mlp_slopes<0>(v, w, r, q);
-                    else if (prm.act == 1) mlp_slopes<1>(v, w, r, q);
-                    else if (prm.act == 2) mlp_slopes<2>(v, w, r, q);
-                    else mlp_slopes<3>(v, w, r, q);
-                    pack_row(r, v);
-                    st.put_row(r);
-                    pack_row(r, w);
-                    st2.put_row(r);
-                    __syncwarp();
-                    st.store(out, prm.out_stride, rows, cols, true);
-                    st2.store(out + prm.out_half, prm.out_stride, rows, cols, true);
                 }
                 __syncwarp();
             }
