@@ -1,5 +1,6 @@
 // Entry points of the gated feed-forward block (kla_mlp.cuh): argument checks, tensor maps, tile choice, launches.
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 
 #include "../../include/kla_b200.h"
@@ -56,7 +57,9 @@ Plan plan(const Product &p, bool may_split, int sms) {
             const double cost = (bn == 256 ? 1.0 : bn == 192 ? 0.78 : bn == 128 ? 0.62 : 0.5) * (cg == 1 ? 1.05 : 1.0);
             const int64_t tm = up(p.M, kMlpBM * cg) * (p.a.halves == kHalvesRows ? 2 : 1);
             const int64_t tn = up(p.N, p.gated() ? bn / 2 : bn), tiles = tm * tn;
-            for (int s = 1; s <= (may_split ? 32 : 1) && s <= blocks; ++s) {
+            // shares of the summed axis up to four rounds of CTAs
+            const int64_t most = may_split ? std::min<int64_t>({32, blocks, 1 + 4 * sms / (tiles * cg)}) : 1;
+            for (int s = 1; s <= most; ++s) {
                 // a tile's end (the last epilogue, filling the ring) is about 4 blocks; partial sums are written and read again
                 const double t = (double)up(tiles * s, sms / cg) * (up(blocks, s) * cost + (s > 1 ? 1.0 : 0.0)) + 4.0 + (s > 1 ? 5.0 + 0.3 * s * tiles * cg / sms : 0.0);
                 if (best.BN == 0 || t < least) { best = Plan{bn, cg, (int)tm, (int)tn, s}; least = t; }
@@ -84,7 +87,7 @@ int fill(MlpParams *prm, const Product &p, const Plan &pl) {
     prm->b = MlpOperand{p.b.adjacent_rows, p.b.halves};
     prm->M = (int)p.M; prm->N = (int)p.N; prm->K = (int)p.K;
     prm->BN = pl.BN; prm->tiles_m = pl.tiles_m; prm->tiles_n = pl.tiles_n; prm->splits = pl.splits;
-    prm->stages = std::min(kMlpMaxStages, mlp_ring_bytes(p.mode) / mlp_block_bytes(pl.BN, pl.CG, p.b.adjacent_rows));
+    prm->stages = std::min(kMlpMaxStages, kMlpRingBytes / mlp_block_bytes(pl.BN, pl.CG, p.b.adjacent_rows));
     prm->blocks_stretch = (int)up(p.K, kMlpBK);
     prm->blocks_k = prm->blocks_stretch * (p.a.halves == kHalvesSummed ? 2 : 1);
     return entry::wait_ctl(&prm->wait);
@@ -104,8 +107,8 @@ int resident_pairs() {
         attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)device_sms() / 2 * 2);
-        cfg.blockDim = dim3(mlp_threads(kMlpPlain));
-        cfg.dynamicSmemBytes = mlp_smem(kMlpPlain);
+        cfg.blockDim = dim3(kMlpThreads);
+        cfg.dynamicSmemBytes = kMlpSmem;
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
         int n = 0;
@@ -118,11 +121,22 @@ int resident_pairs() {
     return pairs[dev];
 }
 
+// The kernel may use its shared memory; asked for once per device.
+template <int MODE, int CG>
+cudaError_t allow_smem() {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && done.load() >> dev & 1)) return e;
+    e = cudaFuncSetAttribute(kla_mlp_kernel<MODE, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMlpSmem);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev);
+    return e;
+}
+
 template <int MODE, int CG>
 int launch_as(const MlpParams &prm, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(kla_mlp_kernel<MODE, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)mlp_smem(MODE));
-    if (e == cudaSuccess && CG == 2)
-        e = cudaFuncSetAttribute(kla_mlp_kernel<kMlpPlain, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)mlp_smem(kMlpPlain));
+    cudaError_t e = allow_smem<MODE, CG>();
+    if (e == cudaSuccess && CG == 2) e = allow_smem<kMlpPlain, 2>();  // (resident_pairs asks about that kernel)
     if (e != cudaSuccess) return entry::cuda_fail(e);
     const int64_t tiles = (int64_t)prm.tiles_m * prm.tiles_n * prm.splits;
     if (tiles > 0x3fffffffll) return KLA_B200_EUNSUPPORTED;
@@ -133,8 +147,8 @@ int launch_as(const MlpParams &prm, cudaStream_t st) {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(tiles < most ? tiles : most) * CG);
-    cfg.blockDim = dim3(mlp_threads(MODE));
-    cfg.dynamicSmemBytes = mlp_smem(MODE);
+    cfg.blockDim = dim3(kMlpThreads);
+    cfg.dynamicSmemBytes = kMlpSmem;
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = CG == 2 ? 1 : 0;
@@ -170,7 +184,9 @@ size_t partial_bytes(const Product &p, int sms) {
     const int splits = plan(p, true, sms).splits;
     return splits > 1 ? (size_t)splits * weight_rows(p) * up(p.N, 4) * 4 * sizeof(float) : 0;
 }
-size_t sum_bytes(int64_t rows, int64_t cols) { return (size_t)up(rows, kMlpSumRows) * cols * sizeof(float); }
+// rows of a stretch of the row sums: at least eight a warp, and no more than 1024 stretches
+int64_t sum_rows(int64_t rows) { return std::max<int64_t>(64, up(rows, 1024 * 8) * 8); }
+size_t sum_bytes(int64_t rows, int64_t cols) { return (size_t)up(rows, sum_rows(rows)) * up(cols, 8) * 8 * sizeof(float); }
 
 // The gradient of a weight: in one go, or partial sums of shares of the rows and then their sum.
 int weight_gradient(const Product &p, void *out, float *work, cudaStream_t st) {
@@ -198,12 +214,18 @@ int weight_gradient(const Product &p, void *out, float *work, cudaStream_t st) {
     return KLA_B200_OK;
 }
 
-int row_sums(const void *x, int64_t stride, int64_t rows, int64_t cols, float *work, void *out, cudaStream_t st) {
-    const int64_t stretches = up(rows, kMlpSumRows);
-    MlpSumParams s{static_cast<const __nv_bfloat16 *>(x), stride, (int)rows, (int)cols, work};
-    kla_mlp_rowsum_kernel<<<dim3((unsigned)up(cols, 64), (unsigned)stretches), 256, 0, st>>>(s);
-    MlpSumEndParams e{work, (int)stretches, (int)cols, static_cast<__nv_bfloat16 *>(out)};
-    kla_mlp_rowsum_end_kernel<<<(unsigned)up(cols, 256), 256, 0, st>>>(e);
+// out[c] = sum over rows of x[r][c]; cols of `half` columns each twice (`half_gap` apart) where half > 0
+int row_sums(const void *x, int64_t stride, int64_t rows, int64_t cols, int64_t half_gap, int halves, float *work, void *out, cudaStream_t st) {
+    MlpSumParams s{};
+    s.x = static_cast<const __nv_bfloat16 *>(x);
+    s.stride = stride; s.half_gap = half_gap; s.rows = (int)rows; s.cols = (int)cols;
+    s.blocks = (int)up(cols, kMlpSumCols); s.stretch_rows = (int)sum_rows(rows); s.stretches = (int)up(rows, s.stretch_rows);
+    s.partial = work;
+    s.partial_stride = up(halves * cols, 8) * 8;
+    s.out = static_cast<__nv_bfloat16 *>(out);
+    s.total = (int)(halves * cols);
+    kla_mlp_rowsum_kernel<<<dim3((unsigned)(s.blocks * halves), (unsigned)s.stretches), 256, 0, st>>>(s);
+    kla_mlp_rowsum_end_kernel<<<(unsigned)up(s.total, 32), 256, 0, st>>>(s);
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return entry::cuda_fail(err);
     entry::count_launch();
@@ -214,8 +236,7 @@ int row_sums(const void *x, int64_t stride, int64_t rows, int64_t cols, float *w
 int check_sizes(const kla_b200_mlp_args *a) {
     if (a == nullptr || a->rows < 0 || a->d <= 0 || a->H <= 0 || a->out <= 0) return KLA_B200_EINVAL;
     if (a->activation < KLA_B200_ACT_SILU || a->activation > KLA_B200_ACT_NONE) return KLA_B200_EINVAL;
-    // row sums walk stretches of kMlpSumRows rows as a grid's second axis; coordinates of tensor maps are 32 bits
-    if (a->rows > 65535ll * kMlpSumRows || a->d > (1 << 24) || a->H > (1 << 24) || a->out > (1 << 24)) return KLA_B200_EUNSUPPORTED;
+    if (a->rows > (1 << 30) || a->d > (1 << 24) || a->H > (1 << 24) || a->out > (1 << 24)) return KLA_B200_EUNSUPPORTED;
     return KLA_B200_OK;
 }
 // an operand of the tensor cores: rows of `width` elements, 16 bytes at a time
@@ -299,7 +320,7 @@ int kla_b200_mlp_bwd(const kla_b200_mlp_args *a, void *stream) {
     float *work = static_cast<float *>(a->work);
     MlpParams prm;
     if (a->dw3 != nullptr && (rc = weight_gradient(product_dw3(*a), a->dw3, work, st))) return rc;
-    if (a->db3 != nullptr && (rc = row_sums(a->dy, a->dy_stride, a->rows, a->out, work, a->db3, st))) return rc;
+    if (a->db3 != nullptr && (rc = row_sums(a->dy, a->dy_stride, a->rows, a->out, 0, 1, work, a->db3, st))) return rc;
     if (!inner) return KLA_B200_OK;
     const Product dgu = product_dgu(*a);
     Plan pl = plan(dgu, false, sms);
@@ -316,11 +337,7 @@ int kla_b200_mlp_bwd(const kla_b200_mlp_args *a, void *stream) {
         if ((rc = launch<kMlpPlain>(prm, pl, st))) return rc;
     }
     if (a->dw12 != nullptr && (rc = weight_gradient(product_dw12(*a), a->dw12, work, st))) return rc;
-    if (a->db12 != nullptr) {
-        __nv_bfloat16 *g = static_cast<__nv_bfloat16 *>(a->dgu), *out = static_cast<__nv_bfloat16 *>(a->db12);
-        if ((rc = row_sums(g, a->gu_stride, a->rows, a->H, work, out, st))) return rc;
-        if ((rc = row_sums(g + a->gu_stride / 2, a->gu_stride, a->rows, a->H, work, out + a->H, st))) return rc;
-    }
+    if (a->db12 != nullptr) return row_sums(a->dgu, a->gu_stride, a->rows, a->H, a->gu_stride / 2, 2, work, a->db12, st);
     return KLA_B200_OK;
 }
 

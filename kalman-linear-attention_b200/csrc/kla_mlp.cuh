@@ -23,14 +23,12 @@
 namespace kla {
 
 constexpr int kMlpBM = 128, kMlpBK = 64, kMlpMaxBN = 256;  // rows of a CTA, summed length of a block, columns of a tile
-// Warps of the epilogue. The gradients of gate and up take 16: with 8 the four instructions' latencies of a warp's chunk (its loads, the
-// accumulator's, the stage's, the stores) were not covered, 179 us in place of @D@ at 32768 rows of 768, H = 2048.
+// Sixteen warps empty an accumulator: with eight the latencies of a warp's chunk (of what it fetches, of the accumulator, of its stage,
+// of the stores) were not covered, and the gradients of gate and up took 179 us in place of 157 at 32768 rows of 768, H = 2048.
+constexpr int kMlpEpiWarps = 16, kMlpThreads = (4 + kMlpEpiWarps) * 32;
 constexpr int kMlpStageBytes = 2 * 32 * 64;  // two stages of 32 rows of 64 bytes a warp
-constexpr int kMlpMaxStages = 8;
-__host__ __device__ constexpr int mlp_epi_warps(int mode) { return mode == 2 ? 16 : 8; }
-__host__ __device__ constexpr int mlp_threads(int mode) { return (4 + mlp_epi_warps(mode)) * 32; }
-__host__ __device__ constexpr int mlp_ring_bytes(int mode) { return (224 - mlp_epi_warps(mode) * 4) * 1024; }
-__host__ __device__ constexpr size_t mlp_smem(int mode) { return 1024 + mlp_ring_bytes(mode) + mlp_epi_warps(mode) * kMlpStageBytes + 256; }
+constexpr int kMlpRingBytes = 160 * 1024, kMlpMaxStages = 8;
+constexpr size_t kMlpSmem = 1024 + kMlpRingBytes + kMlpEpiWarps * kMlpStageBytes + 256;
 // A block of the ring: A's rows of a CTA and its share of B's, which in a pair of CTAs is half of them. What is in flight is what
 // bounds the loads (a tile's block takes about 1 us from L2): with 5 blocks of 32 KB in place of 6 K=4096 N=1024 ran at 1213 TFLOP/s
 inline __host__ __device__ int mlp_b_rows(int BN, int cg, bool mn_major) { return mn_major ? (BN / cg + 63) / 64 * 64 : BN / cg; }
@@ -184,41 +182,18 @@ __device__ __forceinline__ void mlp_load(uint32_t on, uint32_t dst, uint64_t tm,
 __device__ __forceinline__ void mlp_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_load32(float (&v)[32], uint32_t addr) {
-    uint32_t *r = reinterpret_cast<uint32_t *>(v);
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-          "=r"(r[31])
-        : "r"(addr));
-}
-__device__ __forceinline__ void tmem_load8(float (&v)[8], uint32_t addr) {
+__device__ __forceinline__ void tmem_load8(float2 (&v)[4], uint32_t addr) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "=f"(v[0].x), "=f"(v[0].y), "=f"(v[1].x), "=f"(v[1].y), "=f"(v[2].x), "=f"(v[2].y), "=f"(v[3].x), "=f"(v[3].y)
                  : "r"(addr));
 }
 // The loads have arrived; the registers pass through, so that nothing is taken from them before.
-__device__ __forceinline__ void tmem_load_wait(float (&v)[8]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7])::"memory");
+__device__ __forceinline__ void tmem_load_wait(float2 (&v)[4]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+f"(v[0].x), "+f"(v[0].y), "+f"(v[1].x), "+f"(v[1].y), "+f"(v[2].x), "+f"(v[2].y), "+f"(v[3].x), "+f"(v[3].y)::"memory");
 }
-__device__ __forceinline__ void tmem_load_wait(float (&v)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]),
-                   "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]),
-                   "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]),
-                   "+f"(v[31])::"memory");
-}
-// behind a wait already made: the registers pass through
-__device__ __forceinline__ void tmem_loaded(float (&v)[32]) {
-    asm volatile(""
-                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]),
-                   "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]),
-                   "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]),
-                   "+f"(v[31])::"memory");
+// behind a wait already made
+__device__ __forceinline__ void tmem_loaded(float2 (&v)[4]) {
+    asm volatile("" : "+f"(v[0].x), "+f"(v[0].y), "+f"(v[1].x), "+f"(v[1].y), "+f"(v[2].x), "+f"(v[2].y), "+f"(v[3].x), "+f"(v[3].y)::"memory");
 }
 __device__ __forceinline__ void tcgen05_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tcgen05_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -233,10 +208,6 @@ struct MlpStage {
     __device__ __forceinline__ void put_row(const uint4 (&v)[4]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(piece(lane, i)) = v[i];
-    }
-    __device__ __forceinline__ void get_row(uint4 (&v)[4]) const {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4 *>(piece(lane, i));
     }
     // E: element type; rows x cols of them are there
     template <typename E>
@@ -292,34 +263,26 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&v);
 }
-__device__ __forceinline__ void pack_row(uint4 (&v)[4], const float (&x)[32]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        v[i] = make_uint4(pack2(x[8 * i], x[8 * i + 1]), pack2(x[8 * i + 2], x[8 * i + 3]), pack2(x[8 * i + 4], x[8 * i + 5]), pack2(x[8 * i + 6], x[8 * i + 7]));
-}
 
 // Gate and up as the backward finds them: 16 bits with a sign, six of exponent and nine of mantissa. Rounded to bfloat16 their
 // two roundings would be half of the error of a gradient (0.0030 of dx and dW12 in the 2-norm, against 0.0017 of rounding
 // the result alone); nine bits leave the rounding of the gradients that go into the products (0.0025). 2^-31 to 2^33 at full
 // accuracy, steps of 2^-40 below; what is larger, infinite or NaN comes back as NaN.
 constexpr uint32_t kKeptTop = 0x7fffu << 14;
-// the code in the upper half; the least of the value and kKeptTop makes NaN the top code, too
-__device__ __forceinline__ uint32_t keep(float x) {
-    const float m = fminf(fabsf(x) * 0x1p-96f, __uint_as_float(kKeptTop));
+// the code in the upper half, s being x 2^-96; the least of its size and kKeptTop makes NaN the top code, too
+__device__ __forceinline__ uint32_t keep(float x, float s) {
+    const float m = fminf(fabsf(s), __uint_as_float(kKeptTop));
     return __float_as_uint(m) * 4u + 0x8000u | __float_as_uint(x) & 0x80000000u;
 }
-__device__ __forceinline__ uint32_t keep2(float lo, float hi) { return __byte_perm(keep(lo), keep(hi), 0x7632); }
-__device__ __forceinline__ float kept(uint32_t w, bool high) {  // one half of a word
-    const uint32_t m = (uint32_t)((int32_t)(high ? w : w << 16) >> 2) & 0x9fffc000u;
-    return (m & 0x7fffffffu) == kKeptTop ? __uint_as_float(0x7fffffffu) : __uint_as_float(m) * 0x1p96f;
+__device__ __forceinline__ uint32_t keep2(float2 x) {
+    const float2 s = mul2(x, dup2(0x1p-96f));
+    return __byte_perm(keep(x.x, s.x), keep(x.y, s.y), 0x7632);
 }
-__device__ __forceinline__ uint32_t word_at(const uint4 (&v)[4], int j) {  // j a constant after unrolling
-    return j / 2 % 4 == 0 ? v[j / 8].x : j / 2 % 4 == 1 ? v[j / 8].y : j / 2 % 4 == 2 ? v[j / 8].z : v[j / 8].w;
-}
-__device__ __forceinline__ void keep_row(uint4 (&v)[4], const float (&x)[32]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        v[i] = make_uint4(keep2(x[8 * i], x[8 * i + 1]), keep2(x[8 * i + 2], x[8 * i + 3]), keep2(x[8 * i + 4], x[8 * i + 5]), keep2(x[8 * i + 6], x[8 * i + 7]));
+__device__ __forceinline__ float2 kept2(uint32_t w) {
+    const uint32_t lo = (uint32_t)((int32_t)(w << 16) >> 2) & 0x9fffc000u, hi = (uint32_t)((int32_t)w >> 2) & 0x9fffc000u;
+    const float2 v = mul2(make_float2(__uint_as_float(lo), __uint_as_float(hi)), dup2(0x1p96f));
+    const float nan = __uint_as_float(0x7fffffffu);
+    return make_float2((lo & 0x7fffffffu) == kKeptTop ? nan : v.x, (hi & 0x7fffffffu) == kKeptTop ? nan : v.y);
 }
 
 __device__ __forceinline__ float mlp_ex2(float x) {
@@ -332,11 +295,7 @@ __device__ __forceinline__ float mlp_ex2(float x) {
 // one of the gradients 342 in place of @D@ (32768 rows of 768, H = 2048).
 template <int ACT, bool SLOPE>
 __device__ __forceinline__ void mlp_act(float g, float &f, float &df) {
-    if (ACT == 0) {  // silu
-        const float s = rcp_approx(1.0f + mlp_ex2(-1.4426950408889634f * g));
-        f = g * s;
-        if (SLOPE) df = fmaf(f, 1.0f - s, s);
-    } else if (ACT == 1) {  // gelu
+    if (ACT == 1) {  // gelu
         const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
         f = g * cdf;
         if (SLOPE) df = fmaf(g * 0.3989422804014327f, mlp_ex2(-0.72134752044448170f * g * g), cdf);
@@ -348,41 +307,97 @@ __device__ __forceinline__ void mlp_act(float g, float &f, float &df) {
         if (SLOPE) df = 1.0f;
     }
 }
-// g -> act(g) u
-template <int ACT>
-__device__ __forceinline__ void mlp_gate(float (&g)[32], const float (&u)[32]) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-        float f, df;
-        mlp_act<ACT, false>(g[j], f, df);
-        g[j] = f * u[j];
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ void mlp_act2(float2 g, float2 &f, float2 &df) {
+    if (ACT == 0) {  // silu, in paired instructions: what bounds these epilogues is instruction issue
+        const float2 e = mul2(g, dup2(-1.4426950408889634f)), d = add2(make_float2(mlp_ex2(e.x), mlp_ex2(e.y)), dup2(1.0f));
+        const float2 s = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+        f = mul2(g, s);
+        if (SLOPE) df = fma2(f, fma2(s, dup2(-1.0f), dup2(1.0f)), s);
+    } else {
+        mlp_act<ACT, SLOPE>(g.x, f.x, df.x);
+        mlp_act<ACT, SLOPE>(g.y, f.y, df.y);
     }
+}
+__device__ __forceinline__ uint4 pack8(const float2 (&x)[4]) { return make_uint4(pack2(x[0].x, x[0].y), pack2(x[1].x, x[1].y), pack2(x[2].x, x[2].y), pack2(x[3].x, x[3].y)); }
+__device__ __forceinline__ uint4 keep8(const float2 (&x)[4]) { return make_uint4(keep2(x[0]), keep2(x[1]), keep2(x[2]), keep2(x[3])); }
+// cols: of the eight that exist
+__device__ __forceinline__ void add_bias(float2 (&x)[4], const __nv_bfloat16 *bias, int cols) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (2 * j < cols) x[j].x += __bfloat162float(bias[2 * j]);
+        if (2 * j + 1 < cols) x[j].y += __bfloat162float(bias[2 * j + 1]);
+    }
+}
+// A chunk of 32 columns of a row: f is called for its four pieces of eight columns, the accumulator's (and, TWO, those of a second
+// place in it) on their way a piece ahead.
+template <bool TWO, typename F>
+__device__ __forceinline__ void mlp_pieces(uint32_t acc, uint32_t acc2, F &&f) {
+    float2 a[4], b[4], x[4], y[4];
+    tmem_load8(a, acc);
+    if (TWO) tmem_load8(b, acc2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        tmem_load_wait(a);
+        if (TWO) tmem_loaded(b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[j] = a[j];
+            if (TWO) y[j] = b[j];
+        }
+        if (i < 3) {
+            tmem_load8(a, acc + 8 * (i + 1));
+            if (TWO) tmem_load8(b, acc2 + 8 * (i + 1));
+        }
+        f(i, x, y);
+    }
+}
+// act(gate) up of a chunk to h; gate and up to the warp's stages where they are kept.
+template <int ACT>
+__device__ __forceinline__ void mlp_gated_chunk(uint32_t gate, uint32_t up, const __nv_bfloat16 *bias, int N, int cols, bool kept, const MlpStage &st, const MlpStage &st2,
+                                                uint4 (&h)[4]) {
+    mlp_pieces<true>(gate, up, [&](int i, float2 (&g)[4], float2 (&u)[4]) {
+        if (bias != nullptr) {
+            add_bias(g, bias + 8 * i, cols - 8 * i);
+            add_bias(u, bias + N + 8 * i, cols - 8 * i);
+        }
+        if (kept) {
+            *reinterpret_cast<uint4 *>(st.piece(st.lane, i)) = keep8(g);
+            *reinterpret_cast<uint4 *>(st2.piece(st.lane, i)) = keep8(u);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float2 f, df;
+            mlp_act2<ACT, false>(g[j], f, df);
+            g[j] = mul2(f, u[j]);
+        }
+        h[i] = pack8(g);
+    });
 }
 // The gradients of gate and up of a row's eight columns, in place of the kept gate and up.
 template <int ACT>
-__device__ __forceinline__ void mlp_slopes(const float (&dh)[8], uint4 &gate, uint4 &up) {
+__device__ __forceinline__ void mlp_slopes(const float2 (&dh)[4], uint4 &gate, uint4 &up) {
     uint32_t *g = reinterpret_cast<uint32_t *>(&gate), *u = reinterpret_cast<uint32_t *>(&up);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        float f[2], df[2];
-        mlp_act<ACT, true>(kept(g[j], false), f[0], df[0]);
-        mlp_act<ACT, true>(kept(g[j], true), f[1], df[1]);
-        g[j] = pack2(dh[2 * j] * kept(u[j], false) * df[0], dh[2 * j + 1] * kept(u[j], true) * df[1]);
-        u[j] = pack2(dh[2 * j] * f[0], dh[2 * j + 1] * f[1]);
+        float2 f, df;
+        mlp_act2<ACT, true>(kept2(g[j]), f, df);
+        const float2 dg = mul2(mul2(dh[j], kept2(u[j])), df), du = mul2(dh[j], f);
+        g[j] = pack2(dg.x, dg.y);
+        u[j] = pack2(du.x, du.y);
     }
 }
-// ... of a chunk of 32 columns: dh from the accumulator, the kept ones from the warp's two stages, eight columns at a time while the
-// next eight are on their way.
+// ... of a chunk: dh from the accumulator, the kept ones from the warp's two stages.
 template <int ACT>
 __device__ __forceinline__ void mlp_slopes_chunk(uint32_t acc, const MlpStage &st, const MlpStage &st2) {
-    float next[8];
+    float2 next[4];
     tmem_load8(next, acc);
 #pragma unroll 1
     for (int i = 0; i < 4; ++i) {
-        float dh[8];
+        float2 dh[4];
         tmem_load_wait(next);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) dh[j] = next[j];
+        for (int j = 0; j < 4; ++j) dh[j] = next[j];
         if (i < 3) tmem_load8(next, acc + 8 * (i + 1));
         uint4 *pg = reinterpret_cast<uint4 *>(st.piece(st.lane, i)), *pu = reinterpret_cast<uint4 *>(st2.piece(st.lane, i));
         uint4 g = *pg, u = *pu;
@@ -414,11 +429,11 @@ __device__ __forceinline__ MlpTile mlp_tile(const MlpParams &p, int t) {
 }
 
 template <int MODE, int CG>
-__global__ void __launch_bounds__(mlp_threads(MODE), 1) kla_mlp_kernel(const __grid_constant__ MlpParams prm) {
+__global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_constant__ MlpParams prm) {
     extern __shared__ char raw[];
     char *smem = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    constexpr int W = mlp_epi_warps(MODE), PARTS = W / 4;
-    char *epi = smem + mlp_ring_bytes(MODE);
+    constexpr int W = kMlpEpiWarps, PARTS = W / 4;
+    char *epi = smem + kMlpRingBytes;
     const int S = prm.stages, block_bytes = mlp_block_bytes(prm.BN, CG, prm.b.mn_major);
     // full, acc_empty: of the leader (the pair's first CTA); empty, acc_full: of each CTA
     uint64_t *full = reinterpret_cast<uint64_t *>(epi + W * kMlpStageBytes), *empty = full + kMlpMaxStages, *acc_full = empty + kMlpMaxStages, *acc_empty = acc_full + 2, *drain = acc_empty + 2;
@@ -606,81 +621,58 @@ __global__ void __launch_bounds__(mlp_threads(MODE), 1) kla_mlp_kernel(const __g
                     __syncwarp();
                     continue;
                 }
-                float v[32], w[32];
-                uint4 r[4];
-                tmem_load32(v, d + c);
-                if (MODE == kMlpGated) tmem_load32(w, d + width + c);
-                const bool side = MODE == kMlpPlain && prm.side != nullptr;
-                if (side) {
-                    st.put_fetched(f1);
-                    __syncwarp();
-                    st.get_row(r);
-                    __syncwarp();
-                    if (c + cstep < width) fetch(m, n + cstep);
-                }
-                tmem_load_wait(v);
-                if (MODE == kMlpGated) tmem_loaded(w);
-                done();
-                if (cols <= 0) continue;
-                if (MODE == kMlpPartial) {
-                    float *p = prm.partial + (long long)tl.split * prm.partial_rows * prm.partial_stride +
-                               ((long long)tl.m_half * prm.M + m) * prm.partial_stride + n;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            r[i] = make_uint4(__float_as_uint(v[16 * h + 4 * i]), __float_as_uint(v[16 * h + 4 * i + 1]),
-                                              __float_as_uint(v[16 * h + 4 * i + 2]), __float_as_uint(v[16 * h + 4 * i + 3]));
-                        (h ? st2 : st).put_row(r);
-                    }
-                    __syncwarp();
-                    st.store(p, prm.partial_stride, rows, cols, true);
-                    st2.store(p + 16, prm.partial_stride, rows, cols - 16, true);
-                    __syncwarp();
-                    continue;
-                }
-                if (MODE == kMlpPlain) {
-                    if (prm.bias != nullptr) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] += j < cols ? __bfloat162float(prm.bias[n + j]) : 0.0f;
-                    }
-                    if (side) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const uint32_t x = word_at(r, j);
-                            v[j] += __uint_as_float(j % 2 ? x & 0xffff0000u : x << 16);
-                        }
-                    }
-                    pack_row(r, v);
-                    st.put_row(r);
-                    __syncwarp();
-                    st.store(out, prm.out_stride, rows, cols, prm.out_vec);
-                } else {
-                    if (prm.bias != nullptr) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (j < cols) {
-                                v[j] += __bfloat162float(prm.bias[n + j]);
-                                w[j] += __bfloat162float(prm.bias[prm.N + n + j]);
-                            }
-                    }
-                    if (prm.gu != nullptr) {
-                        keep_row(r, v);
-                        st.put_row(r);
-                        keep_row(r, w);
-                        st2.put_row(r);
-                        __syncwarp();
+                const __nv_bfloat16 *bias = prm.bias != nullptr ? prm.bias + n : nullptr;
+                if constexpr (MODE == kMlpGated) {
+                    uint4 h[4];
+                    const bool keeps = prm.gu != nullptr;
+                    if (prm.act == 0) mlp_gated_chunk<0>(d + c, d + width + c, bias, prm.N, cols, keeps, st, st2, h);
+                    else if (prm.act == 1) mlp_gated_chunk<1>(d + c, d + width + c, bias, prm.N, cols, keeps, st, st2, h);
+                    else if (prm.act == 2) mlp_gated_chunk<2>(d + c, d + width + c, bias, prm.N, cols, keeps, st, st2, h);
+                    else mlp_gated_chunk<3>(d + c, d + width + c, bias, prm.N, cols, keeps, st, st2, h);
+                    done();
+                    if (keeps) {
                         __nv_bfloat16 *gu = prm.gu + (long long)m * prm.gu_stride + n;
+                        __syncwarp();
                         st.store(gu, prm.gu_stride, rows, cols, true);
                         st2.store(gu + prm.gu_half, prm.gu_stride, rows, cols, true);
                         __syncwarp();
                     }
-                    if (prm.act == 0) mlp_gate<0>(v, w);
-                    else if (prm.act == 1) mlp_gate<1>(v, w);
-                    else if (prm.act == 2) mlp_gate<2>(v, w);
-                    else mlp_gate<3>(v, w);
-                    pack_row(r, v);
-                    st.put_row(r);
+                    st.put_row(h);
+                    __syncwarp();
+                    st.store(out, prm.out_stride, rows, cols, prm.out_vec);
+                } else if constexpr (MODE == kMlpPartial) {
+                    // four of a row's 16-byte pieces in either stage
+                    mlp_pieces<false>(d + c, 0u, [&](int i, float2 (&x)[4], float2 (&)[4]) {
+                        const MlpStage &to = i < 2 ? st : st2;
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            *reinterpret_cast<float4 *>(to.piece(lane, i % 2 * 2 + e)) = make_float4(x[2 * e].x, x[2 * e].y, x[2 * e + 1].x, x[2 * e + 1].y);
+                    });
+                    done();
+                    __syncwarp();
+                    float *p = prm.partial + (long long)tl.split * prm.partial_rows * prm.partial_stride +
+                               ((long long)tl.m_half * prm.M + m) * prm.partial_stride + n;
+                    st.store(p, prm.partial_stride, rows, cols, true);
+                    st2.store(p + 16, prm.partial_stride, rows, cols - 16, true);
+                } else {
+                    const bool side = prm.side != nullptr;
+                    if (side) {
+                        st.put_fetched(f1);
+                        __syncwarp();
+                        if (c + cstep < width) fetch(m, n + cstep);
+                    }
+                    mlp_pieces<false>(d + c, 0u, [&](int i, float2 (&x)[4], float2 (&)[4]) {
+                        uint4 *p = reinterpret_cast<uint4 *>(st.piece(lane, i));
+                        if (bias != nullptr) add_bias(x, bias + 8 * i, cols - 8 * i);
+                        if (side) {
+                            const uint4 r = *p;
+                            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) x[j] = add2(x[j], make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u)));
+                        }
+                        *p = pack8(x);
+                    });
+                    done();
                     __syncwarp();
                     st.store(out, prm.out_stride, rows, cols, prm.out_vec);
                 }
@@ -748,38 +740,68 @@ __global__ void __launch_bounds__(256) kla_mlp_reduce_kernel(const MlpReducePara
     }
 }
 
-// Sums over rows of a bfloat16 matrix (a bias's gradient): a block adds 64 columns of a stretch of rows, the sums of the
-// stretches are added by the same kernel's second launch in their order, as float32 [stretches][cols].
-constexpr int kMlpSumRows = 256;
+// Sums over rows of a bfloat16 matrix (a bias's gradient) whose rows are 16-byte aligned: a block adds 256 columns of a stretch of
+// rows, eight rows side by side and eight columns a thread by one access; the sums of the stretches, float32 [stretches][total], are
+// added by a second kernel in their order. Of gate and up, whose halves lie half_gap apart, in one go.
+constexpr int kMlpSumCols = 256;
 struct MlpSumParams {
     const __nv_bfloat16 *x;
-    long long stride;
-    int rows, cols;
+    long long stride, half_gap;
+    int rows, cols, blocks, stretch_rows, stretches, total;
     float *partial;
-};
-__global__ void __launch_bounds__(256) kla_mlp_rowsum_kernel(const MlpSumParams prm) {
-    __shared__ float part[4][64];
-    const int c = blockIdx.x * 64 + threadIdx.x % 64, g = threadIdx.x / 64;
-    const int r0 = blockIdx.y * kMlpSumRows, r1 = min(prm.rows, r0 + kMlpSumRows);
-    float s = 0.0f;
-    if (c < prm.cols)
-        for (int r = r0 + g; r < r1; r += 4) s += __bfloat162float(prm.x[(long long)r * prm.stride + c]);
-    part[g][threadIdx.x % 64] = s;
-    __syncthreads();
-    if (g == 0 && c < prm.cols)
-        prm.partial[(long long)blockIdx.y * prm.cols + c] = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
-}
-struct MlpSumEndParams {
-    const float *partial;
-    int stretches, cols;
+    long long partial_stride;
     __nv_bfloat16 *out;
 };
-__global__ void __launch_bounds__(256) kla_mlp_rowsum_end_kernel(const MlpSumEndParams prm) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= prm.cols) return;
+__global__ void __launch_bounds__(256) kla_mlp_rowsum_kernel(const MlpSumParams prm) {
+    __shared__ float part[8][kMlpSumCols];
+    const int half = blockIdx.x / prm.blocks, c0 = (blockIdx.x - half * prm.blocks) * kMlpSumCols;
+    const int g = threadIdx.x / 32, c = c0 + threadIdx.x % 32 * 8;
+    const int r0 = blockIdx.y * prm.stretch_rows + g, r1 = min(prm.rows, ((int)blockIdx.y + 1) * prm.stretch_rows);
+    const __nv_bfloat16 *x = prm.x + half * prm.half_gap + c;
+    float s[8] = {};
+    if (c + 8 <= prm.cols) {
+#pragma unroll 8
+        for (int r = r0; r < r1; r += 8) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(x + r * prm.stride));
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[2 * e] += __uint_as_float(w[e] << 16);
+                s[2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u);
+            }
+        }
+    } else {
+        for (int r = r0; r < r1; r += 8)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c + e < prm.cols) s[e] += __bfloat162float(x[r * prm.stride + e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[g][threadIdx.x % 32 * 8 + e] = s[e];
+    __syncthreads();
+    const int col = c0 + threadIdx.x;
+    if (col < prm.cols) {
+        float t = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t += part[i][threadIdx.x];
+        prm.partial[blockIdx.y * prm.partial_stride + half * prm.cols + col] = t;
+    }
+}
+// 32 columns a block, every eighth stretch a warp
+__global__ void __launch_bounds__(256) kla_mlp_rowsum_end_kernel(const MlpSumParams prm) {
+    __shared__ float part[8][32];
+    const int lane = threadIdx.x % 32, g = threadIdx.x / 32, c = blockIdx.x * 32 + lane;
     float s = 0.0f;
-    for (int k = 0; k < prm.stretches; ++k) s += prm.partial[(long long)k * prm.cols + c];
-    prm.out[c] = __float2bfloat16_rn(s);
+    if (c < prm.total)
+#pragma unroll 4
+        for (int k = g; k < prm.stretches; k += 8) s += prm.partial[k * prm.partial_stride + c];
+    part[g][lane] = s;
+    __syncthreads();
+    if (g == 0 && c < prm.total) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) s += part[i][lane];
+        prm.out[c] = __float2bfloat16_rn(s);
+    }
 }
 
 }  // namespace kla

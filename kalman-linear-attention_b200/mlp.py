@@ -44,17 +44,18 @@ def gated_mlp_b200(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, b12: to
     first. Under a bfloat16 autocast other floating types of ``x``, weights and biases are converted as ``F.linear`` does."""
     if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:
         x, w12, w3, b12, b3 = (t.to(torch.bfloat16) if t is not None and t.is_cuda else t for t in (x, w12, w3, b12, b3))
-    if x.dim() == 0:
-        raise ValueError("kla_b200: x is [..., d]")
-    lead = x.shape[:-1]
-    if residual is not None:
-        if residual.dim() == 0 or residual.shape[:-1] != lead:
-            raise ValueError("kla_b200: residual has the output's shape")
-        residual = residual.reshape(lead.numel(), residual.shape[-1])
-    rows = x.reshape(lead.numel(), x.shape[-1])
-    given = (rows, w12, w3, b12, b3, residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given):
-        y = _GatedMlpB200.apply(*given, activation)
+    lead = None
+    if x.dim() != 2:
+        if x.dim() == 0:
+            raise ValueError("kla_b200: x is [..., d]")
+        lead = x.shape[:-1]
+        if residual is not None:
+            if residual.dim() == 0 or residual.shape[:-1] != lead:
+                raise ValueError("kla_b200: residual has the output's shape")
+            residual = residual.reshape(lead.numel(), residual.shape[-1])
+        x = x.reshape(lead.numel(), x.shape[-1])
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w12, w3, b12, b3, residual)):
+        y = _GatedMlpB200.apply(x, w12, w3, b12, b3, residual, activation)
     else:
-        y = _lib.host().mlp_fwd(*given, activation, False)[0]
-    return y.view(*lead, y.shape[-1])
+        y = _lib.host().mlp_fwd(x, w12, w3, b12, b3, residual, activation, False)[0]
+    return y if lead is None else y.view(*lead, y.shape[-1])

@@ -357,7 +357,7 @@ def test_entry_points_reject_bad_arguments_without_cuda():
         assert fn(None, None) == 1
         assert fn(A(rows=-1), None) == 1 and fn(A(d=0), None) == 1
         assert fn(A(activation=4), None) == 1
-        assert fn(A(rows=1 << 25), None) == 2
+        assert fn(A(rows=1 << 31), None) == 2
         assert fn(A(w3=None), None) == 1 and fn(A(w3=72), None) == 4
         assert fn(A(w3_stride=16), None) == 1 and fn(A(w3_stride=28), None) == 4
         assert fn(A(x_stride=20), None) == 4 and fn(A(h=None), None) == 1
