@@ -30,10 +30,12 @@ int pick_ranks(int64_t cells, int64_t steps, int tile) {
 }
 
 template <typename K>
-int launch(K kern, GatedParams &prm, int64_t sequences, int ranks, cudaStream_t st) {
+int launch(K kern, GatedParams &prm, size_t smem, int64_t sequences, int ranks, cudaStream_t st) {
     const int64_t grid = sequences * prm.blocks * ranks;
     if (grid == 0) return KLA_B200_OK;
     if (grid > 0x7fffffffll) return KLA_B200_EUNSUPPORTED;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return entry::cuda_fail(e);
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = ranks;
@@ -41,10 +43,11 @@ int launch(K kern, GatedParams &prm, int64_t sequences, int ranks, cudaStream_t 
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kGatedWarps * 32);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = ranks > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, prm);
+    e = cudaLaunchKernelEx(&cfg, kern, prm);
     if (e != cudaSuccess) return entry::cuda_fail(e);
     entry::count_launch();
     return KLA_B200_OK;
@@ -52,12 +55,20 @@ int launch(K kern, GatedParams &prm, int64_t sequences, int ranks, cudaStream_t 
 
 template <typename T, bool PAIR>
 int run(GatedParams &prm, bool backward, int64_t sequences, int ranks, cudaStream_t st) {
-    constexpr int TS = sizeof(T) == 2 ? 16 : 8;
+    constexpr size_t fwd = GatedFwdShape<T>::kBytes, bwd = GatedBwdShape<T>::kBytes;
     if (backward)
-        return ranks > 1 ? launch(kla_gated_bwd_kernel<T, PAIR, true>, prm, sequences, ranks, st)
-                         : launch(kla_gated_bwd_kernel<T, PAIR, false>, prm, sequences, ranks, st);
-    return ranks > 1 ? launch(kla_gated_fwd_kernel<T, PAIR, true, TS>, prm, sequences, ranks, st)
-                     : launch(kla_gated_fwd_kernel<T, PAIR, false, TS>, prm, sequences, ranks, st);
+        return ranks > 1 ? launch(kla_gated_bwd_kernel<T, PAIR, true>, prm, bwd, sequences, ranks, st)
+                         : launch(kla_gated_bwd_kernel<T, PAIR, false>, prm, bwd, sequences, ranks, st);
+    return ranks > 1 ? launch(kla_gated_fwd_kernel<T, PAIR, true>, prm, fwd, sequences, ranks, st)
+                     : launch(kla_gated_fwd_kernel<T, PAIR, false>, prm, fwd, sequences, ranks, st);
+}
+
+// Bytes an asynchronous copy of the tensor's rows may move: 16 where they are aligned so, else 4; 2 of bfloat16 rows that are not in
+// pairs.
+int width(const kla_b200_tensor3 &t, size_t esz, int64_t D) {
+    const int64_t sb = t.stride_b * (int64_t)esz, st = t.stride_t * (int64_t)esz;
+    if (aligned(t.ptr, 16) && sb % 16 == 0 && st % 16 == 0) return 16;
+    return esz == 4 || (D % 2 == 0 && aligned(t.ptr, 4) && sb % 4 == 0 && st % 4 == 0) ? 4 : 2;
 }
 
 int gated(const kla_b200_gated_args *a, void *stream, bool backward) {
@@ -88,8 +99,9 @@ int gated(const kla_b200_gated_args *a, void *stream, bool backward) {
     prm.cu = a->cu_seqlens; prm.h0 = a->state; prm.end = a->state_out; prm.ckpt = a->ckpt;
     prm.dh = t3(a->dh); prm.dx = t3(a->dx); prm.dg = t3(a->dgate);
     prm.dend = a->dstate_out; prm.dh0 = a->dstate;
+    prm.x_width = width(a->x, esz, a->D); prm.g_width = width(a->gate, esz, a->D); prm.dh_width = width(a->dh, esz, a->D);
     const int64_t sequences = N + packed;
-    const int tile = backward ? kGatedUnit : kGatedWarps * (esz == 2 ? 16 : 8);
+    const int tile = backward ? kGatedUnit : kGatedWarps * (esz == 2 ? GatedFwdShape<__nv_bfloat16>::TS : GatedFwdShape<float>::TS);
     const int ranks = pick_ranks(N * prm.blocks, packed && N > 0 ? (a->L + N - 1) / N : a->L, tile);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (esz == 2) return vec ? run<__nv_bfloat16, true>(prm, backward, sequences, ranks, st) : run<__nv_bfloat16, false>(prm, backward, sequences, ranks, st);

@@ -9,15 +9,17 @@
 // rounded is then small beside 1 - a where a gate holds the state for thousands of steps, which a = 1 - z rounded is not.
 //
 // A CTA owns 64 channels of one sequence and walks it in tiles of kGatedWarps x TS steps. Each warp takes TS consecutive steps
-// of the tile, each lane two channels: it loads its share of x and g straight into registers (one 128-byte row of bfloat16 a
-// warp access) a tile ahead, composes the map of its steps, puts it in shared memory, and after one barrier folds the maps of
-// the warps in front of it to get its own first state; then it walks its steps once more and stores. So every input is read
-// and every output written once. The backward needs the states in front of its steps: the forward leaves one per
+// of the tile, each lane two channels. The warp's rows come in by asynchronous copies into a ring of its own in shared memory,
+// tiles ahead, so that what is in flight (64 KB an SM and more) does not hang on registers or on other warps; it composes the map
+// of its steps, puts it in shared memory, and after one barrier folds the maps of the warps in front of it to get its own first
+// state; then it walks its steps once more and stores. So every input is read and every output written once. The backward needs the states in front of its steps: the forward leaves one per
 // kGatedUnit steps and channel, and the backward, whose tile is one such unit, walks forward from it in registers, which is
 // 4 bytes per 64 steps to read in place of h.
 // With a cluster of CTAs a sequence's tiles go round robin to its CTAs, which exchange their tiles' maps through distributed
 // shared memory once a round: the way to fill the GPU with few sequences or channels.
 #pragma once
+
+#include <type_traits>
 
 #include "kla_common.cuh"
 
@@ -32,6 +34,7 @@ struct GatedParams {
     int N, L, D;        // sequences, rows of a batch entry (packed: of all sequences), channels
     int blocks;         // channel blocks
     Tensor3 x, g, h;
+    int x_width, g_width, dh_width;  // bytes a copy of their rows may move (gated_fetch)
     const int *cu;      // [N + 1] bounds of packed sequences or nullptr: sequences are batch entries
     const float *h0;    // [N, D] or nullptr: zeros
     float *end;         // [N, D]
@@ -41,51 +44,26 @@ struct GatedParams {
     float *dh0;         // [N, D] or nullptr
 };
 
-// Two channels of one row as they lie in memory. PAIR: neighbouring ones by one access (rows allow it); otherwise channels 32
-// apart, one by one, each where it exists.
-template <typename T>
-struct Two;
-template <>
-struct Two<float> {
-    float a, b;
-    __device__ __forceinline__ float2 wide() const { return make_float2(a, b); }
-};
-template <>
-struct Two<__nv_bfloat16> {
-    uint32_t v;  // low half: the first channel
-    __device__ __forceinline__ float2 wide() const { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
-};
-
+// A lane's two channels: neighbours where every row can be written in pairs (PAIR), otherwise 32 apart.
 template <bool PAIR>
 struct Lane {
-    int c0, c1;     // its channels within the tensor
-    bool on0, on1;  // whether they exist
-    __device__ __forceinline__ Lane(int block, int lane, int D) {
+    int lane, c0, c1;  // its channels within the tensor
+    bool on0, on1;     // whether they exist
+    __device__ __forceinline__ Lane(int block, int lane_, int D) : lane(lane_) {
         c0 = block * kGatedChannels + (PAIR ? 2 * lane : lane);
         c1 = PAIR ? c0 + 1 : c0 + 32;
         on0 = c0 < D;
         on1 = c1 < D;
     }
-    __device__ __forceinline__ Two<float> load(const float *row) const {
-        Two<float> r{0.0f, 0.0f};
+    // from a row of the block's 64 channels in shared memory
+    __device__ __forceinline__ float2 take(const float *row) const { return PAIR ? *reinterpret_cast<const float2 *>(row + 2 * lane) : make_float2(row[lane], row[lane + 32]); }
+    __device__ __forceinline__ float2 take(const __nv_bfloat16 *row) const {
         if constexpr (PAIR) {
-            if (on0) asm volatile("ld.global.nc.L1::no_allocate.v2.f32 {%0, %1}, [%2];" : "=f"(r.a), "=f"(r.b) : "l"(row + c0));
+            const uint32_t v = *reinterpret_cast<const uint32_t *>(row + 2 * lane);
+            return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
         } else {
-            if (on0) r.a = __ldg(row + c0);
-            if (on1) r.b = __ldg(row + c1);
+            return make_float2(__bfloat162float(row[lane]), __bfloat162float(row[lane + 32]));
         }
-        return r;
-    }
-    __device__ __forceinline__ Two<__nv_bfloat16> load(const __nv_bfloat16 *row) const {
-        Two<__nv_bfloat16> r{0u};
-        if constexpr (PAIR) {
-            if (on0) asm volatile("ld.global.nc.L1::no_allocate.b32 %0, [%1];" : "=r"(r.v) : "l"(row + c0));
-        } else {
-            const unsigned short *p = reinterpret_cast<const unsigned short *>(row);
-            const uint32_t lo = on0 ? __ldg(p + c0) : 0u, hi = on1 ? __ldg(p + c1) : 0u;
-            r.v = lo | hi << 16;
-        }
-        return r;
     }
     __device__ __forceinline__ void store(float *row, float2 y) const {
         if constexpr (PAIR) {
@@ -110,6 +88,82 @@ struct Lane {
         if (on0) row[c0] = y.x;
         if (on1) row[c1] = y.y;
     }
+};
+
+__device__ __forceinline__ void gated_copy(void *dst, const void *src, int bytes, bool sixteen) {
+    if (sixteen) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+// `rows` (of TS at most) rows of the block's 64 channels into shared memory by one warp. width: bytes a copy moves, as far as
+// the tensor's alignment goes (16 or 4; bfloat16 rows at odd places have 2 and are loaded and stored one by one). Channels past
+// the tensor's are zeros.
+template <typename T, int TS>
+__device__ __forceinline__ void gated_fetch(T *dst, const T *src, long long stride, int rows, int block, int D, int width, int lane) {
+    const int c_block = block * kGatedChannels;
+    src += c_block;
+    if (width >= 4) {
+        const bool sixteen = width == 16;
+        const int per = (sixteen ? 16 : 4) / (int)sizeof(T), pieces = kGatedChannels / per;
+        constexpr int kFirst = 32 / (kGatedChannels * (int)sizeof(T) / 16);  // rows that 32 pieces of 16 bytes are
+        if (sixteen) {
+            const int c = lane % pieces * per;
+            const int bytes = max(0, min(16, (D - c_block - c) * (int)sizeof(T)));
+            const T *from = bytes > 0 ? src + c : src;
+#pragma unroll
+            for (int i = 0; i < TS; i += kFirst) {
+                const int r = i + lane / pieces;
+                if (r < rows) gated_copy(dst + r * kGatedChannels + c, from + r * stride, bytes, true);
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < kGatedChannels * (int)sizeof(T) / 128; ++h) {
+                const int c = (lane + 32 * h) * per;
+                const int bytes = c_block + c < D ? 4 : 0;  // (pairs of bfloat16: D is even)
+                const T *from = bytes > 0 ? src + c : src;
+#pragma unroll
+                for (int r = 0; r < TS; ++r)
+                    if (r < rows) gated_copy(dst + r * kGatedChannels + c, from + r * stride, bytes, false);
+            }
+        }
+    } else {
+        const int n0 = c_block + lane < D, n1 = c_block + lane + 32 < D;
+#pragma unroll
+        for (int r0 = 0; r0 < TS; r0 += 8) {
+            T a[8], b[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                a[r] = b[r] = from_f32<T>(0.0f);
+                if (r0 + r < rows) {
+                    if (n0) a[r] = src[(r0 + r) * stride + lane];
+                    if (n1) b[r] = src[(r0 + r) * stride + lane + 32];
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (r0 + r < rows) {
+                    dst[(r0 + r) * kGatedChannels + lane] = a[r];
+                    dst[(r0 + r) * kGatedChannels + lane + 32] = b[r];
+                }
+        }
+    }
+}
+__device__ __forceinline__ void gated_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void gated_arrived() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+    __syncwarp();
+}
+
+// Steps of a warp and tiles of its ring, so that two CTAs' rings fit an SM.
+template <typename T>
+struct GatedFwdShape {
+    static constexpr int TS = sizeof(T) == 2 ? 16 : 8, S = 3;
+    static constexpr size_t kBytes = (size_t)kGatedWarps * S * 2 * TS * kGatedChannels * sizeof(T);
+};
+template <typename T>
+struct GatedBwdShape {
+    static constexpr int TS = kGatedUnit / kGatedWarps, S = sizeof(T) == 2 ? 3 : 2;
+    static constexpr size_t kBytes = (size_t)kGatedWarps * S * 3 * TS * kGatedChannels * sizeof(T);
 };
 
 // The rows a CTA's sequence covers. Bounds of packed sequences come from the device unseen by the host: clamped, so that no
@@ -232,69 +286,93 @@ __device__ __forceinline__ float2 gated_exchange(GatedShared<CLUSTER> &sh, int b
 
 // Grid: sequences x channel blocks x cluster, the last fastest; with packed sequences one sequence more, which clears the rows
 // that belong to none.
-template <typename T, bool PAIR, bool CLUSTER, int TS>
-__global__ void __launch_bounds__(kGatedWarps * 32) kla_gated_fwd_kernel(const __grid_constant__ GatedParams prm) {
+template <typename T, bool PAIR, bool CLUSTER>
+__global__ void __launch_bounds__(kGatedWarps * 32, 2) kla_gated_fwd_kernel(const __grid_constant__ GatedParams prm) {
+    using Shape = GatedFwdShape<T>;
+    constexpr int TS = Shape::TS, S = Shape::S, TT = kGatedWarps * TS;
     __shared__ GatedShared<CLUSTER> sh;
+    extern __shared__ __align__(16) unsigned char ring_bytes[];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int rank = CLUSTER ? (int)cluster_rank() : 0, ranks = CLUSTER ? (int)cluster_size() : 1;
-    const int cell = blockIdx.x / ranks, n = cell / prm.blocks;
-    const Lane<PAIR> ln(cell % prm.blocks, lane, prm.D);
+    const int cell = blockIdx.x / ranks, n = cell / prm.blocks, block = cell % prm.blocks;
+    const Lane<PAIR> ln(block, lane, prm.D);
     if (n == prm.N) return gated_clear<T, PAIR>(prm, prm.h, ln, warp, rank, ranks);  // the whole cluster returns
     if constexpr (CLUSTER) cluster_sync();  // every CTA has begun: its shared memory may be written
     const GatedSpan span = gated_span(prm, n);
     const T *x = gated_rows<const T>(prm.x, span), *g = gated_rows<const T>(prm.g, span);
     T *h_out = gated_rows<T>(prm.h, span);
-    constexpr int TT = kGatedWarps * TS;
-    const int rounds = (span.len + TT * ranks - 1) / (TT * ranks);
+    T *ring = reinterpret_cast<T *>(ring_bytes) + warp * S * 2 * TS * kGatedChannels;
+    const int rounds = (span.len + TT * ranks - 1) / (TT * ranks), len = span.len;
     float2 carry = prm.h0 ? ln.load_state(prm.h0 + (long long)n * prm.D) : make_float2(0.0f, 0.0f);
 
-    Two<T> xr[TS], gr[TS], xn[TS], gn[TS];
-    auto fetch = [&](int round) {
-        const int t0 = (round * ranks + rank) * TT + warp * TS, cnt = span.len - t0;
-#pragma unroll
-        for (int i = 0; i < TS; ++i)
-            if (i < cnt) {
-                gn[i] = ln.load(g + (long long)(t0 + i) * prm.g.st);
-                xn[i] = ln.load(x + (long long)(t0 + i) * prm.x.st);
-            }
+    int fetched = 0, slot_in = 0;
+    auto fetch = [&] {  // the next round's rows, where there is one; a group of copies either way
+        if (fetched < rounds) {
+            const int t0 = (fetched * ranks + rank) * TT + warp * TS, rows = len - t0;
+            T *to = ring + slot_in * 2 * TS * kGatedChannels;
+            gated_fetch<T, TS>(to, g + (long long)t0 * prm.g.st, prm.g.st, rows, block, prm.D, prm.g_width, lane);
+            gated_fetch<T, TS>(to + TS * kGatedChannels, x + (long long)t0 * prm.x.st, prm.x.st, rows, block, prm.D, prm.x_width, lane);
+        }
+        gated_commit();
+        ++fetched;
+        if (++slot_in == S) slot_in = 0;
     };
-    fetch(0);
-    for (int round = 0; round < rounds; ++round) {
-        const int t0 = (round * ranks + rank) * TT + warp * TS, cnt = span.len - t0;
 #pragma unroll
-        for (int i = 0; i < TS; ++i) { xr[i] = xn[i]; gr[i] = gn[i]; }
-        if (round + 1 < rounds) fetch(round + 1);
+    for (int i = 0; i < S - 1; ++i) fetch();
+    int slot = 0;
+    for (int round = 0; round < rounds; ++round) {
+        const int t0 = (round * ranks + rank) * TT + warp * TS, cnt = len - t0;
+        gated_arrived<S - 2>();
+        fetch();  // over the round before
+        const T *gs = ring + slot * 2 * TS * kGatedChannels, *xs = gs + TS * kGatedChannels;
+        if (++slot == S) slot = 0;
         float2 nz[TS];
         Map2 own{make_float2(1.0f, 1.0f), make_float2(0.0f, 0.0f)};
+        auto compose = [&](int i) {
+            nz[i] = neg_z(ln.take(gs + i * kGatedChannels));
+            own.A = fma2(nz[i], own.A, own.A);
+            own.F = fma2(nz[i], neg2(ln.take(xs + i * kGatedChannels)), fma2(nz[i], own.F, own.F));
+        };
+        if (cnt >= TS) {
 #pragma unroll
-        for (int i = 0; i < TS; ++i)
-            if (i < cnt) {
-                nz[i] = neg_z(gr[i].wide());
-                own.A = fma2(nz[i], own.A, own.A);
-                own.F = fma2(nz[i], neg2(xr[i].wide()), fma2(nz[i], own.F, own.F));
-            }
+            for (int i = 0; i < TS; ++i) compose(i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < TS; ++i)
+                if (i < cnt) compose(i);
+        }
         float2 h = gated_exchange<CLUSTER, false>(sh, round & 1, own, carry, warp, lane, rank, ranks);
         if (prm.ckpt != nullptr && t0 % kGatedUnit == 0 && cnt > 0)
             ln.store_state(prm.ckpt + (long long)(span.unit + t0 / kGatedUnit) * prm.D, h);
+        T *to = h_out + (long long)t0 * prm.h.st;
+        auto walk = [&](int i) {
+            h = fma2(nz[i], neg2(ln.take(xs + i * kGatedChannels)), fma2(nz[i], h, h));
+            ln.store(to, h);
+            to += prm.h.st;
+        };
+        if (cnt >= TS) {
 #pragma unroll
-        for (int i = 0; i < TS; ++i)
-            if (i < cnt) {
-                h = fma2(nz[i], neg2(xr[i].wide()), fma2(nz[i], h, h));
-                ln.store(h_out + (long long)(t0 + i) * prm.h.st, h);
-            }
+            for (int i = 0; i < TS; ++i) walk(i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < TS; ++i)
+                if (i < cnt) walk(i);
+        }
     }
     if (warp == 0 && rank == 0) ln.store_state(prm.end + (long long)n * prm.D, carry);
 }
 
 template <typename T, bool PAIR, bool CLUSTER>
-__global__ void __launch_bounds__(kGatedWarps * 32) kla_gated_bwd_kernel(const __grid_constant__ GatedParams prm) {
-    constexpr int TS = kGatedUnit / kGatedWarps;
+__global__ void __launch_bounds__(kGatedWarps * 32, 2) kla_gated_bwd_kernel(const __grid_constant__ GatedParams prm) {
+    using Shape = GatedBwdShape<T>;
+    constexpr int TS = Shape::TS, S = Shape::S, kTile = TS * kGatedChannels;
     __shared__ GatedShared<CLUSTER> sh;
     __shared__ float4 fw[2][kGatedWarps][32];  // maps of the warps forwards
+    extern __shared__ __align__(16) unsigned char ring_bytes[];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int rank = CLUSTER ? (int)cluster_rank() : 0, ranks = CLUSTER ? (int)cluster_size() : 1;
-    const int cell = blockIdx.x / ranks, n = cell / prm.blocks;
-    const Lane<PAIR> ln(cell % prm.blocks, lane, prm.D);
+    const int cell = blockIdx.x / ranks, n = cell / prm.blocks, block = cell % prm.blocks;
+    const Lane<PAIR> ln(block, lane, prm.D);
     if (n == prm.N) {
         gated_clear<T, PAIR>(prm, prm.dx, ln, warp, rank, ranks);
         return gated_clear<T, PAIR>(prm, prm.dg, ln, warp, rank, ranks);
@@ -303,68 +381,90 @@ __global__ void __launch_bounds__(kGatedWarps * 32) kla_gated_bwd_kernel(const _
     const GatedSpan span = gated_span(prm, n);
     const T *x = gated_rows<const T>(prm.x, span), *g = gated_rows<const T>(prm.g, span), *dh = gated_rows<const T>(prm.dh, span);
     T *dx = gated_rows<T>(prm.dx, span), *dg = gated_rows<T>(prm.dg, span);
-    const int rounds = (span.len + kGatedUnit * ranks - 1) / (kGatedUnit * ranks);
+    T *ring = reinterpret_cast<T *>(ring_bytes) + warp * S * 3 * kTile;
+    const int len = span.len, rounds = (len + kGatedUnit * ranks - 1) / (kGatedUnit * ranks);
     float2 carry = prm.dend ? ln.load_state(prm.dend + (long long)n * prm.D) : make_float2(0.0f, 0.0f);
 
-    Two<T> xr[TS], gr[TS], dr[TS], xn[TS], gn[TS], dn[TS];
-    float2 first, first_next = make_float2(0.0f, 0.0f);
-    auto fetch = [&](int round) {
-        const int unit = round * ranks + rank, t0 = unit * kGatedUnit + warp * TS, cnt = span.len - t0;
-#pragma unroll
-        for (int i = 0; i < TS; ++i)
-            if (i < cnt) {
-                gn[i] = ln.load(g + (long long)(t0 + i) * prm.g.st);
-                dn[i] = ln.load(dh + (long long)(t0 + i) * prm.dh.st);
-                xn[i] = ln.load(x + (long long)(t0 + i) * prm.x.st);
-            }
-        if (unit * kGatedUnit < span.len) first_next = ln.load_state(prm.ckpt + (long long)(span.unit + unit) * prm.D);
+    int fetched = rounds - 1, slot_in = 0;
+    auto fetch = [&] {  // rounds from the last one on
+        if (fetched >= 0) {
+            const int t0 = (fetched * ranks + rank) * kGatedUnit + warp * TS, rows = len - t0;
+            T *to = ring + slot_in * 3 * kTile;
+            gated_fetch<T, TS>(to, g + (long long)t0 * prm.g.st, prm.g.st, rows, block, prm.D, prm.g_width, lane);
+            gated_fetch<T, TS>(to + kTile, x + (long long)t0 * prm.x.st, prm.x.st, rows, block, prm.D, prm.x_width, lane);
+            gated_fetch<T, TS>(to + 2 * kTile, dh + (long long)t0 * prm.dh.st, prm.dh.st, rows, block, prm.D, prm.dh_width, lane);
+        }
+        gated_commit();
+        --fetched;
+        if (++slot_in == S) slot_in = 0;
     };
-    if (rounds > 0) fetch(rounds - 1);
-    for (int round = rounds - 1; round >= 0; --round) {
-        const int t0 = (round * ranks + rank) * kGatedUnit + warp * TS, cnt = span.len - t0, buf = round & 1;
+    // the state in front of a round's unit
+    auto front = [&](int round) {
+        const int unit = round * ranks + rank;
+        return round >= 0 && unit * kGatedUnit < len ? ln.load_state(prm.ckpt + (long long)(span.unit + unit) * prm.D) : make_float2(0.0f, 0.0f);
+    };
 #pragma unroll
-        for (int i = 0; i < TS; ++i) { xr[i] = xn[i]; gr[i] = gn[i]; dr[i] = dn[i]; }
-        first = first_next;
-        if (round > 0) fetch(round - 1);
-        float2 nz[TS], za[TS], c[TS];
+    for (int i = 0; i < S - 1; ++i) fetch();
+    float2 next = front(rounds - 1);
+    int slot = 0;
+    for (int round = rounds - 1; round >= 0; --round) {
+        const int t0 = (round * ranks + rank) * kGatedUnit + warp * TS, cnt = len - t0, buf = round & 1;
+        float2 h = next;
+        next = front(round - 1);
+        gated_arrived<S - 2>();
+        fetch();
+        const T *gs = ring + slot * 3 * kTile, *xs = gs + kTile, *ds = xs + kTile;
+        if (++slot == S) slot = 0;
+        float2 nz[TS], za[TS];
         Map2 back{make_float2(1.0f, 1.0f), make_float2(0.0f, 0.0f)};
         float2 F = make_float2(0.0f, 0.0f);
+        auto compose = [&](auto full) {
+            constexpr bool FULL = decltype(full)::value;
 #pragma unroll
-        for (int i = 0; i < TS; ++i)
-            if (i < cnt) {
-                const float2 gi = gr[i].wide();
-                neg_z_slope(gi.x, nz[i].x, za[i].x);
-                neg_z_slope(gi.y, nz[i].y, za[i].y);
-                back.A = fma2(nz[i], back.A, back.A);
-                F = fma2(nz[i], neg2(xr[i].wide()), fma2(nz[i], F, F));
-            }
+            for (int i = 0; i < TS; ++i)
+                if (FULL || i < cnt) {
+                    const float2 gi = ln.take(gs + i * kGatedChannels);
+                    neg_z_slope(gi.x, nz[i].x, za[i].x);
+                    neg_z_slope(gi.y, nz[i].y, za[i].y);
+                    back.A = fma2(nz[i], back.A, back.A);
+                    F = fma2(nz[i], neg2(ln.take(xs + i * kGatedChannels)), fma2(nz[i], F, F));
+                }
 #pragma unroll
-        for (int i = TS - 1; i >= 0; --i)
-            if (i < cnt) {
-                const float2 ci = add2(dr[i].wide(), back.F);
-                back.F = fma2(nz[i], ci, ci);
-            }
+            for (int i = TS - 1; i >= 0; --i)
+                if (FULL || i < cnt) {
+                    const float2 ci = add2(ln.take(ds + i * kGatedChannels), back.F);
+                    back.F = fma2(nz[i], ci, ci);
+                }
+        };
+        if (cnt >= TS) compose(std::true_type{});
+        else compose(std::false_type{});
         fw[buf][warp][lane] = make_float4(back.A.x, back.A.y, F.x, F.y);
         float2 u = gated_exchange<CLUSTER, true>(sh, buf, back, carry, warp, lane, rank, ranks);
-        float2 h = first;
         for (int w = 0; w < warp; ++w) {
             const float4 m = fw[buf][w][lane];
             h = fma2(make_float2(m.x, m.y), h, make_float2(m.z, m.w));
         }
+        auto walk = [&](auto full) {
+            constexpr bool FULL = decltype(full)::value;
+            float2 c[TS];
 #pragma unroll
-        for (int i = TS - 1; i >= 0; --i)
-            if (i < cnt) {
-                c[i] = add2(dr[i].wide(), u);
-                u = fma2(nz[i], c[i], c[i]);
-            }
+            for (int i = TS - 1; i >= 0; --i)
+                if (FULL || i < cnt) {
+                    c[i] = add2(ln.take(ds + i * kGatedChannels), u);
+                    u = fma2(nz[i], c[i], c[i]);
+                }
+            T *to_x = dx + (long long)t0 * prm.dx.st, *to_g = dg + (long long)t0 * prm.dg.st;
 #pragma unroll
-        for (int i = 0; i < TS; ++i)
-            if (i < cnt) {
-                const float2 xi = xr[i].wide();
-                ln.store(dx + (long long)(t0 + i) * prm.dx.st, mul2(neg2(nz[i]), c[i]));
-                ln.store(dg + (long long)(t0 + i) * prm.dg.st, mul2(mul2(za[i], c[i]), add2(h, neg2(xi))));
-                h = fma2(nz[i], neg2(xi), fma2(nz[i], h, h));
-            }
+            for (int i = 0; i < TS; ++i)
+                if (FULL || i < cnt) {
+                    const float2 nx = neg2(ln.take(xs + i * kGatedChannels));
+                    ln.store(to_x + i * prm.dx.st, mul2(neg2(nz[i]), c[i]));
+                    ln.store(to_g + i * prm.dg.st, mul2(mul2(za[i], c[i]), add2(h, nx)));
+                    h = fma2(nz[i], nx, fma2(nz[i], h, h));
+                }
+        };
+        if (cnt >= TS) walk(std::true_type{});
+        else walk(std::false_type{});
     }
     if (prm.dh0 != nullptr && warp == 0 && rank == 0) ln.store_state(prm.dh0 + (long long)n * prm.D, carry);
 }
