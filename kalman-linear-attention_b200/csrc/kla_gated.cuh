@@ -239,49 +239,48 @@ template <bool CLUSTER>
 struct GatedShared {
     float4 warp[2][kGatedWarps][32];
     float4 cta[2][CLUSTER ? kGatedMaxCluster : 1][32];
+    float2 carry[2][32];
 };
 
-// Called by all threads with the map of the warp's own steps: the value in front of the warp's steps, and `carry` moved past the
-// whole round (a tile of every CTA). REVERSE: values come from behind. One barrier of the CTA, with CLUSTER one of the cluster.
+// Called by all threads with the map of the warp's own steps: the value in front of the warp's steps. The value in front of the round is
+// sh.carry[buf] (for the first round put there by the warp that is last in the fold), the one behind it goes to the other copy.
+// REVERSE: values come from behind. One barrier of the CTA, with CLUSTER one of the cluster.
 template <bool CLUSTER, bool REVERSE>
-__device__ __forceinline__ float2 gated_exchange(GatedShared<CLUSTER> &sh, int buf, Map2 own, float2 &carry, int warp, int lane, int rank, int ranks) {
+__device__ __forceinline__ float2 gated_exchange(GatedShared<CLUSTER> &sh, int buf, Map2 own, int warp, int lane, int rank, int ranks) {
     auto map = [](const float4 &v) { return Map2{make_float2(v.x, v.y), make_float2(v.z, v.w)}; };
-    sh.warp[buf][warp][lane] = make_float4(own.A.x, own.A.y, own.F.x, own.F.y);
+    const int place = REVERSE ? kGatedWarps - 1 - warp : warp;  // in the order of the fold
+    sh.warp[buf][place][lane] = make_float4(own.A.x, own.A.y, own.F.x, own.F.y);
     __syncthreads();
+    float2 mine;
     if constexpr (CLUSTER) {
-        if (warp < ranks) {  // warp r takes the CTA's map to rank r
+        if (warp == 0) {  // the CTA's map to all
             Map2 all{make_float2(1.0f, 1.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
             for (int i = 0; i < kGatedWarps; ++i) {
-                const Map2 m = map(sh.warp[buf][REVERSE ? kGatedWarps - 1 - i : i][lane]);
+                const Map2 m = map(sh.warp[buf][i][lane]);
                 all.F = m(all.F);
                 all.A = mul2(m.A, all.A);
             }
-            cluster_store(&sh.cta[buf][rank][lane], warp, make_float4(all.A.x, all.A.y, all.F.x, all.F.y));
+            const float4 v = make_float4(all.A.x, all.A.y, all.F.x, all.F.y);
+            for (int r = 0; r < ranks; ++r) cluster_store(&sh.cta[buf][rank][lane], r, v);
         }
         cluster_sync();
-        float2 mine = carry;
-        for (int i = 0; i < ranks; ++i) {
-            const int r = REVERSE ? ranks - 1 - i : i;
-            if (r == rank) mine = carry;
-            carry = map(sh.cta[buf][r][lane])(carry);
+        mine = sh.carry[buf][lane];
+        const int before = REVERSE ? ranks - 1 - rank : rank;
+        for (int i = 0; i < before; ++i) mine = map(sh.cta[buf][REVERSE ? ranks - 1 - i : i][lane])(mine);
+        if (place == kGatedWarps - 1) {  // (the warp that folds most anyway)
+            float2 end = mine;
+            for (int i = before; i < ranks; ++i) end = map(sh.cta[buf][REVERSE ? ranks - 1 - i : i][lane])(end);
+            sh.carry[buf ^ 1][lane] = end;
         }
-        for (int i = 0; i < kGatedWarps - 1; ++i) {
-            const int w = REVERSE ? kGatedWarps - 1 - i : i;
-            if (REVERSE ? w <= warp : w >= warp) break;
-            mine = map(sh.warp[buf][w][lane])(mine);
-        }
-        return mine;
     } else {
-        float2 mine = carry;
-#pragma unroll
-        for (int i = 0; i < kGatedWarps; ++i) {
-            const int w = REVERSE ? kGatedWarps - 1 - i : i;
-            if (w == warp) mine = carry;
-            carry = map(sh.warp[buf][w][lane])(carry);
-        }
-        return mine;
+        mine = sh.carry[buf][lane];
     }
+#pragma unroll
+    for (int i = 0; i < kGatedWarps - 1; ++i)
+        if (i < place) mine = map(sh.warp[buf][i][lane])(mine);
+    if (!CLUSTER && place == kGatedWarps - 1) sh.carry[buf ^ 1][lane] = own(mine);
+    return mine;
 }
 
 // Grid: sequences x channel blocks x cluster, the last fastest; with packed sequences one sequence more, which clears the rows
@@ -303,7 +302,7 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) kla_gated_fwd_kernel(cons
     T *h_out = gated_rows<T>(prm.h, span);
     T *ring = reinterpret_cast<T *>(ring_bytes) + warp * S * 2 * TS * kGatedChannels;
     const int rounds = (span.len + TT * ranks - 1) / (TT * ranks), len = span.len;
-    float2 carry = prm.h0 ? ln.load_state(prm.h0 + (long long)n * prm.D) : make_float2(0.0f, 0.0f);
+    if (warp == kGatedWarps - 1) sh.carry[0][lane] = prm.h0 ? ln.load_state(prm.h0 + (long long)n * prm.D) : make_float2(0.0f, 0.0f);
 
     int fetched = 0, slot_in = 0;
     auto fetch = [&] {  // the next round's rows, where there is one; a group of copies either way
@@ -341,7 +340,7 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) kla_gated_fwd_kernel(cons
             for (int i = 0; i < TS; ++i)
                 if (i < cnt) compose(i);
         }
-        float2 h = gated_exchange<CLUSTER, false>(sh, round & 1, own, carry, warp, lane, rank, ranks);
+        float2 h = gated_exchange<CLUSTER, false>(sh, round & 1, own, warp, lane, rank, ranks);
         if (prm.ckpt != nullptr && t0 % kGatedUnit == 0 && cnt > 0)
             ln.store_state(prm.ckpt + (long long)(span.unit + t0 / kGatedUnit) * prm.D, h);
         T *to = h_out + (long long)t0 * prm.h.st;
@@ -359,7 +358,7 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) kla_gated_fwd_kernel(cons
                 if (i < cnt) walk(i);
         }
     }
-    if (warp == 0 && rank == 0) ln.store_state(prm.end + (long long)n * prm.D, carry);
+    if (warp == kGatedWarps - 1 && rank == 0) ln.store_state(prm.end + (long long)n * prm.D, sh.carry[rounds & 1][lane]);  // its own
 }
 
 template <typename T, bool PAIR, bool CLUSTER>
@@ -383,7 +382,8 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) kla_gated_bwd_kernel(cons
     T *dx = gated_rows<T>(prm.dx, span), *dg = gated_rows<T>(prm.dg, span);
     T *ring = reinterpret_cast<T *>(ring_bytes) + warp * S * 3 * kTile;
     const int len = span.len, rounds = (len + kGatedUnit * ranks - 1) / (kGatedUnit * ranks);
-    float2 carry = prm.dend ? ln.load_state(prm.dend + (long long)n * prm.D) : make_float2(0.0f, 0.0f);
+    // copies of the exchange by parity of the rounds done
+    if (warp == 0) sh.carry[0][lane] = prm.dend ? ln.load_state(prm.dend + (long long)n * prm.D) : make_float2(0.0f, 0.0f);
 
     int fetched = rounds - 1, slot_in = 0;
     auto fetch = [&] {  // rounds from the last one on
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) kla_gated_bwd_kernel(cons
     float2 next = front(rounds - 1);
     int slot = 0;
     for (int round = rounds - 1; round >= 0; --round) {
-        const int t0 = (round * ranks + rank) * kGatedUnit + warp * TS, cnt = len - t0, buf = round & 1;
+        const int t0 = (round * ranks + rank) * kGatedUnit + warp * TS, cnt = len - t0, buf = (rounds - 1 - round) & 1;
         float2 h = next;
         next = front(round - 1);
         gated_arrived<S - 2>();
@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) kla_gated_bwd_kernel(cons
         if (cnt >= TS) compose(std::true_type{});
         else compose(std::false_type{});
         fw[buf][warp][lane] = make_float4(back.A.x, back.A.y, F.x, F.y);
-        float2 u = gated_exchange<CLUSTER, true>(sh, buf, back, carry, warp, lane, rank, ranks);
+        float2 u = gated_exchange<CLUSTER, true>(sh, buf, back, warp, lane, rank, ranks);
         for (int w = 0; w < warp; ++w) {
             const float4 m = fw[buf][w][lane];
             h = fma2(make_float2(m.x, m.y), h, make_float2(m.z, m.w));
@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) kla_gated_bwd_kernel(cons
         if (cnt >= TS) walk(std::true_type{});
         else walk(std::false_type{});
     }
-    if (prm.dh0 != nullptr && warp == 0 && rank == 0) ln.store_state(prm.dh0 + (long long)n * prm.D, carry);
+    if (prm.dh0 != nullptr && warp == 0 && rank == 0) ln.store_state(prm.dh0 + (long long)n * prm.D, sh.carry[rounds & 1][lane]);  // its own
 }
 
 // One token: rows [B, D] of x and g, the state read and written as float32 (in place where both are the same).
