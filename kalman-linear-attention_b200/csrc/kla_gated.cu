@@ -1,4 +1,7 @@
 // Entry points of the gated recurrence (kla_gated.cuh): argument checks, kernel and cluster choice, launches.
+#include <algorithm>
+#include <cmath>
+
 #include "../../include/kla_b200.h"
 #include "kla_entry.h"
 #include "kla_gated.cuh"
@@ -17,20 +20,36 @@ int check_rows(const kla_b200_tensor3 &t, size_t esz) {
 bool pairs(const kla_b200_tensor3 &t, size_t esz) { return aligned(t.ptr, 2 * esz) && t.stride_b % 2 == 0 && t.stride_t % 2 == 0; }
 Tensor3 t3(const kla_b200_tensor3 &t) { return Tensor3{t.ptr, t.stride_b, t.stride_t}; }
 
-// Sequences of this many steps in tiles of `tile`: how many CTAs of a cluster share one.
-int pick_ranks(int64_t cells, int64_t steps, int tile) {
-    const int64_t slots = 2 * device_sms(), tiles = (steps + tile - 1) / tile;
+// How many CTAs of a cluster share a sequence: the least time by a model of what was measured on B200 (us). A round, a tile of each
+// CTA of a cluster, takes `round` alone on its SM and by `share` more for the exchange; a second and third CTA on the SM add 35 % each;
+// launching takes `start`; and no choice is faster than 80 % of the memory's rate. Measured, clusters of 1 / 2 / 4 / 8: forward bfloat16
+// B=4 L=8192 D=2048 102 / 85 / 93 / 105, B=16 L=2048 D=1536 60 / 72 / 84 / 107, B=1 L=8192 D=1024 98 / 62 / 33 / 24, B=8 L=512 D=768
+// 8.3 / 8.7 / 11.5 / 17.6; backward 103 / 119 / 129 / 148 (B=16 ...), 192 / 121 / 65 / 45 (B=1 ...), 14.2 / 13.7 / 10.7 / 13.8 (B=8 ...).
+// Of packed sequences the host knows the number and the sum of the lengths; the longest of n random ones is about ln n + 0.6 times
+// their mean, and clusters of 8 were no gain there.
+int pick_ranks(int64_t cells, int64_t rows, int64_t sequences, int64_t L, bool packed, bool backward, size_t esz, int64_t D) {
+    const double sms = device_sms();
+    const int tile = backward ? kGatedUnit : esz == 2 ? GatedFwdShape<__nv_bfloat16>::W * GatedFwdShape<__nv_bfloat16>::TS : GatedFwdShape<float>::W * GatedFwdShape<float>::TS;
+    const int ctas = !backward ? GatedFwdShape<float>::kCtas : esz == 2 ? GatedBwdShape<__nv_bfloat16>::kCtas : GatedBwdShape<float>::kCtas;
+    const double round = backward ? (esz == 2 ? 1.5 : 2.2) : (esz == 2 ? 1.53 : 1.15), shares[4] = {1.0, 1.27, 1.37, 1.6}, starts[4] = {2.0, 3.5, 5.0, 6.0};
+    double steps = (double)L;
+    if (packed && sequences > 0) steps = std::min(steps, (double)L / sequences * (std::log((double)sequences) + 0.6));
+    const double tiles = std::ceil(steps / tile), least_us = (double)rows * D * esz * (backward ? 5 : 3) / 5.2e6;
     int best = 1;
     double least = 0.0;
-    for (int r = 1; r <= kGatedMaxCluster && (r == 1 || r <= tiles); r *= 2) {
-        const double t = (double)((cells * r + slots - 1) / slots) * (double)((tiles + r - 1) / r) * (r == 1 ? 1.0 : 1.15);
+    for (int k = 0; k < (packed ? 3 : 4); ++k) {
+        const int r = 1 << k;
+        if (r > 1 && (r > tiles || r > kGatedMaxCluster)) break;
+        const double n = (double)cells * r, waves = packed ? 1.0 : std::max(1.0, std::ceil(n / (ctas * sms)));
+        const double load = std::min((double)ctas, std::max(1.0, std::ceil(n / waves / sms)));
+        const double t = std::max(waves * (std::ceil(tiles / r) * round * shares[k] * (1.0 + 0.35 * (load - 1.0)) + starts[k]), least_us);
         if (r == 1 || t < least) { best = r; least = t; }
     }
     return best;
 }
 
 template <typename K>
-int launch(K kern, GatedParams &prm, size_t smem, int64_t sequences, int ranks, cudaStream_t st) {
+int launch(K kern, GatedParams &prm, int warps, size_t smem, int64_t sequences, int ranks, cudaStream_t st) {
     const int64_t grid = sequences * prm.blocks * ranks;
     if (grid == 0) return KLA_B200_OK;
     if (grid > 0x7fffffffll) return KLA_B200_EUNSUPPORTED;
@@ -42,7 +61,7 @@ int launch(K kern, GatedParams &prm, size_t smem, int64_t sequences, int ranks, 
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(kGatedWarps * 32);
+    cfg.blockDim = dim3(warps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cfg.attrs = &attr;
@@ -56,11 +75,12 @@ int launch(K kern, GatedParams &prm, size_t smem, int64_t sequences, int ranks, 
 template <typename T, bool PAIR>
 int run(GatedParams &prm, bool backward, int64_t sequences, int ranks, cudaStream_t st) {
     constexpr size_t fwd = GatedFwdShape<T>::kBytes, bwd = GatedBwdShape<T>::kBytes;
+    constexpr int wf = GatedFwdShape<T>::W, wb = GatedBwdShape<T>::W;
     if (backward)
-        return ranks > 1 ? launch(kla_gated_bwd_kernel<T, PAIR, true>, prm, bwd, sequences, ranks, st)
-                         : launch(kla_gated_bwd_kernel<T, PAIR, false>, prm, bwd, sequences, ranks, st);
-    return ranks > 1 ? launch(kla_gated_fwd_kernel<T, PAIR, true>, prm, fwd, sequences, ranks, st)
-                     : launch(kla_gated_fwd_kernel<T, PAIR, false>, prm, fwd, sequences, ranks, st);
+        return ranks > 1 ? launch(kla_gated_bwd_kernel<T, PAIR, true>, prm, wb, bwd, sequences, ranks, st)
+                         : launch(kla_gated_bwd_kernel<T, PAIR, false>, prm, wb, bwd, sequences, ranks, st);
+    return ranks > 1 ? launch(kla_gated_fwd_kernel<T, PAIR, true>, prm, wf, fwd, sequences, ranks, st)
+                     : launch(kla_gated_fwd_kernel<T, PAIR, false>, prm, wf, fwd, sequences, ranks, st);
 }
 
 // Bytes an asynchronous copy of the tensor's rows may move: 16 where they are aligned so, else 4; 2 of bfloat16 rows that are not in
@@ -100,9 +120,9 @@ int gated(const kla_b200_gated_args *a, void *stream, bool backward) {
     prm.dh = t3(a->dh); prm.dx = t3(a->dx); prm.dg = t3(a->dgate);
     prm.dend = a->dstate_out; prm.dh0 = a->dstate;
     prm.x_width = width(a->x, esz, a->D); prm.g_width = width(a->gate, esz, a->D); prm.dh_width = width(a->dh, esz, a->D);
+    if (const int rc = entry::wait_ctl(&prm.wait)) return rc;
     const int64_t sequences = N + packed;
-    const int tile = backward ? kGatedUnit : kGatedWarps * (esz == 2 ? GatedFwdShape<__nv_bfloat16>::TS : GatedFwdShape<float>::TS);
-    const int ranks = pick_ranks(N * prm.blocks, packed && N > 0 ? (a->L + N - 1) / N : a->L, tile);
+    const int ranks = pick_ranks(N * prm.blocks, packed ? a->L : a->B * a->L, N, a->L, packed, backward, esz, a->D);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (esz == 2) return vec ? run<__nv_bfloat16, true>(prm, backward, sequences, ranks, st) : run<__nv_bfloat16, false>(prm, backward, sequences, ranks, st);
     return vec ? run<float, true>(prm, backward, sequences, ranks, st) : run<float, false>(prm, backward, sequences, ranks, st);

@@ -8,7 +8,7 @@
 // same slope A = prod a_t: h -> A h + F and u -> A u + R. A step is taken as h - z h + z x with two fused operations: what is
 // rounded is then small beside 1 - a where a gate holds the state for thousands of steps, which a = 1 - z rounded is not.
 //
-// A CTA owns 64 channels of one sequence and walks it in tiles of kGatedWarps x TS steps. Each warp takes TS consecutive steps
+// A CTA owns 64 channels of one sequence and walks it in tiles of W x TS steps. Each warp takes TS consecutive steps
 // of the tile, each lane two channels. The warp's rows come in by asynchronous copies into a ring of its own in shared memory,
 // tiles ahead, so that what is in flight (64 KB an SM and more) does not hang on registers or on other warps; it composes the map
 // of its steps, puts it in shared memory, and after one barrier folds the maps of the warps in front of it to get its own first
@@ -25,10 +25,10 @@
 
 namespace kla {
 
-constexpr int kGatedWarps = 8;
 constexpr int kGatedChannels = 64;  // of a CTA
 constexpr int kGatedUnit = 64;      // steps between the states the forward leaves for the backward
 constexpr int kGatedMaxCluster = 8;
+constexpr int kGatedSite = 0x50;  // of the status word: the wait for the other CTAs' maps
 
 struct GatedParams {
     int N, L, D;        // sequences, rows of a batch entry (packed: of all sequences), channels
@@ -42,6 +42,7 @@ struct GatedParams {
     Tensor3 dh, dx, dg;
     const float *dend;  // [N, D] or nullptr: zeros
     float *dh0;         // [N, D] or nullptr
+    WaitCtl wait;
 };
 
 // A lane's two channels: neighbours where every row can be written in pairs (PAIR), otherwise 32 apart.
@@ -65,21 +66,24 @@ struct Lane {
             return make_float2(__bfloat162float(row[lane]), __bfloat162float(row[lane + 32]));
         }
     }
-    __device__ __forceinline__ void store(float *row, float2 y) const {
+    // -y to a row; `row` points at c0
+    __device__ __forceinline__ void store_negated(float *row, float2 y) const {
+        y = neg2(y);
         if constexpr (PAIR) {
-            if (on0) *reinterpret_cast<float2 *>(row + c0) = y;
+            if (on0) *reinterpret_cast<float2 *>(row) = y;
         } else {
-            if (on0) row[c0] = y.x;
-            if (on1) row[c1] = y.y;
+            if (on0) row[0] = y.x;
+            if (on1) row[32] = y.y;
         }
     }
-    __device__ __forceinline__ void store(__nv_bfloat16 *row, float2 y) const {
+    __device__ __forceinline__ void store_negated(__nv_bfloat16 *row, float2 y) const {
         const __nv_bfloat162 v = __floats2bfloat162_rn(y.x, y.y);
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(&v) ^ 0x80008000u;  // one operation for both signs
         if constexpr (PAIR) {
-            if (on0) *reinterpret_cast<__nv_bfloat162 *>(row + c0) = v;
+            if (on0) *reinterpret_cast<uint32_t *>(row) = w;
         } else {
-            if (on0) row[c0] = __low2bfloat16(v);
-            if (on1) row[c1] = __high2bfloat16(v);
+            if (on0) reinterpret_cast<unsigned short *>(row)[0] = (unsigned short)w;
+            if (on1) reinterpret_cast<unsigned short *>(row)[32] = (unsigned short)(w >> 16);
         }
     }
     // states are rows of their own alignment: one by one
@@ -96,38 +100,22 @@ __device__ __forceinline__ void gated_copy(void *dst, const void *src, int bytes
 }
 // `rows` (of TS at most) rows of the block's 64 channels into shared memory by one warp. width: bytes a copy moves, as far as
 // the tensor's alignment goes (16 or 4; bfloat16 rows at odd places have 2 and are loaded and stored one by one). Channels past
-// the tensor's are zeros.
+// the tensor's are zeros, rows past the sequence's `fill`. src: at the block's first channel. Any tile; gated_fetch has its own way
+// for whole tiles of aligned rows.
 template <typename T, int TS>
-__device__ __forceinline__ void gated_fetch(T *dst, const T *src, long long stride, int rows, int block, int D, int width, int lane) {
-    const int c_block = block * kGatedChannels;
-    src += c_block;
+__device__ __noinline__ void gated_fetch_any(T *dst, const T *src, long long stride, int rows, int channels, int width, int lane, float fill) {
+    if (rows < TS)
+        for (int i = max(rows, 0) * kGatedChannels + lane; i < TS * kGatedChannels; i += 32) dst[i] = from_f32<T>(fill);
     if (width >= 4) {
-        const bool sixteen = width == 16;
-        const int per = (sixteen ? 16 : 4) / (int)sizeof(T), pieces = kGatedChannels / per;
-        constexpr int kFirst = 32 / (kGatedChannels * (int)sizeof(T) / 16);  // rows that 32 pieces of 16 bytes are
-        if (sixteen) {
-            const int c = lane % pieces * per;
-            const int bytes = max(0, min(16, (D - c_block - c) * (int)sizeof(T)));
-            const T *from = bytes > 0 ? src + c : src;
-#pragma unroll
-            for (int i = 0; i < TS; i += kFirst) {
-                const int r = i + lane / pieces;
-                if (r < rows) gated_copy(dst + r * kGatedChannels + c, from + r * stride, bytes, true);
-            }
-        } else {
-#pragma unroll
-            for (int h = 0; h < kGatedChannels * (int)sizeof(T) / 128; ++h) {
-                const int c = (lane + 32 * h) * per;
-                const int bytes = c_block + c < D ? 4 : 0;  // (pairs of bfloat16: D is even)
-                const T *from = bytes > 0 ? src + c : src;
-#pragma unroll
-                for (int r = 0; r < TS; ++r)
-                    if (r < rows) gated_copy(dst + r * kGatedChannels + c, from + r * stride, bytes, false);
-            }
+        const int per = width / (int)sizeof(T), pieces = kGatedChannels / per;
+#pragma unroll 4
+        for (int i = lane; i < rows * pieces && i < TS * pieces; i += 32) {
+            const int r = i / pieces, c = (i - r * pieces) * per;
+            const int bytes = max(0, min(width, (channels - c) * (int)sizeof(T)));  // (pairs of bfloat16: channels is even)
+            gated_copy(dst + r * kGatedChannels + c, bytes > 0 ? src + r * stride + c : src, bytes, width == 16);
         }
     } else {
-        const int n0 = c_block + lane < D, n1 = c_block + lane + 32 < D;
-#pragma unroll
+        const int n0 = lane < channels, n1 = lane + 32 < channels;
         for (int r0 = 0; r0 < TS; r0 += 8) {
             T a[8], b[8];
 #pragma unroll
@@ -147,6 +135,47 @@ __device__ __forceinline__ void gated_fetch(T *dst, const T *src, long long stri
         }
     }
 }
+// A warp's tiles of one tensor: src moves on from tile to tile.
+template <typename T, int TS>
+struct GatedRows {
+    static constexpr int kPer = 16 / (int)sizeof(T), kPieces = kGatedChannels / kPer, kRows = 32 / kPieces;  // rows a warp's copies of 16 bytes cover
+    const T *src;         // the next tile's first row, at the block's first channel
+    long long stride, tile;  // elements between rows, to the next tile
+    int channels, width, lane, bytes;
+    float fill;
+    __device__ __forceinline__ GatedRows(const T *rows, long long stride_, long long t0, long long tile_rows, int block, int D, int width_, int lane_, float fill_)
+        : src(rows + t0 * stride_ + block * kGatedChannels), stride(stride_), tile(tile_rows * stride_), channels(D - block * kGatedChannels), width(width_),
+          lane(lane_), fill(fill_) {
+        bytes = max(0, min(16, (channels - lane % kPieces * kPer) * (int)sizeof(T)));
+    }
+    __device__ __forceinline__ void fetch(T *dst, int rows) {
+        if (width == 16 && rows >= TS) {
+            const T *from = src + lane / kPieces * stride + (bytes > 0 ? lane % kPieces * kPer : 0);
+            T *to = dst + lane / kPieces * kGatedChannels + lane % kPieces * kPer;
+            const long long next = kRows * stride;
+#pragma unroll
+            for (int i = 0; i < TS; i += kRows) {
+                gated_copy(to + i * kGatedChannels, from, bytes, true);
+                from += next;
+            }
+        } else if (width == 4 && rows >= TS) {
+            constexpr int kWord = 4 / (int)sizeof(T);
+#pragma unroll
+            for (int h = 0; h < kGatedChannels / kWord / 32; ++h) {
+                const int c = (lane + 32 * h) * kWord, there = c < channels ? 4 : 0;  // (pairs of bfloat16: channels is even)
+                const T *from = src + (there ? c : 0);
+#pragma unroll
+                for (int i = 0; i < TS; ++i) {
+                    gated_copy(dst + i * kGatedChannels + c, from, there, false);
+                    from += stride;
+                }
+            }
+        } else {
+            gated_fetch_any<T, TS>(dst, src, stride, rows, channels, width, lane, fill);
+        }
+        src += tile;
+    }
+};
 __device__ __forceinline__ void gated_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void gated_arrived() {
@@ -154,16 +183,16 @@ __device__ __forceinline__ void gated_arrived() {
     __syncwarp();
 }
 
-// Steps of a warp and tiles of its ring, so that two CTAs' rings fit an SM.
+// Warps of a CTA, steps of a warp in a tile, tiles of its ring, CTAs an SM holds.
 template <typename T>
 struct GatedFwdShape {
-    static constexpr int TS = sizeof(T) == 2 ? 16 : 8, S = 3;
-    static constexpr size_t kBytes = (size_t)kGatedWarps * S * 2 * TS * kGatedChannels * sizeof(T);
+    static constexpr int W = 4, TS = 64 / (int)sizeof(T), S = 2, kCtas = 3;
+    static constexpr size_t kBytes = (size_t)W * S * 2 * TS * kGatedChannels * sizeof(T);
 };
 template <typename T>
 struct GatedBwdShape {
-    static constexpr int TS = kGatedUnit / kGatedWarps, S = sizeof(T) == 2 ? 3 : 2;
-    static constexpr size_t kBytes = (size_t)kGatedWarps * S * 3 * TS * kGatedChannels * sizeof(T);
+    static constexpr int W = 4, TS = kGatedUnit / W, S = 2, kCtas = sizeof(T) == 2 ? 3 : 2;
+    static constexpr size_t kBytes = (size_t)W * S * 3 * TS * kGatedChannels * sizeof(T);
 };
 
 // The rows a CTA's sequence covers. Bounds of packed sequences come from the device unseen by the host: clamped, so that no
@@ -183,10 +212,10 @@ __device__ __forceinline__ T *gated_rows(const Tensor3 &t, const GatedSpan &s) {
 
 // Rows in front of the first and behind the last packed sequence belong to none: zeros.
 template <typename T, bool PAIR>
-__device__ __forceinline__ void gated_clear(const GatedParams &p, const Tensor3 &t, const Lane<PAIR> &ln, int warp, int rank, int ranks) {
+__device__ __forceinline__ void gated_clear(const GatedParams &p, const Tensor3 &t, const Lane<PAIR> &ln, int warp, int warps, int rank, int ranks) {
     const int first = min(max(p.cu[0], 0), p.L), last = min(max(p.cu[p.N], 0), p.L);
-    for (int r = rank * kGatedWarps + warp; r < p.L; r += ranks * kGatedWarps)
-        if (r < first || r >= last) ln.store(static_cast<T *>(const_cast<void *>(t.ptr)) + (long long)r * t.st, make_float2(0.0f, 0.0f));
+    for (int r = rank * warps + warp; r < p.L; r += ranks * warps)
+        if (r < first || r >= last) ln.store_negated(static_cast<T *>(const_cast<void *>(t.ptr)) + (long long)r * t.st + ln.c0, make_float2(-0.0f, -0.0f));
 }
 
 __device__ __forceinline__ float ex2_approx(float x) {
@@ -195,22 +224,29 @@ __device__ __forceinline__ float ex2_approx(float x) {
     return y;
 }
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kHold = 1e30f;  // a gate that holds: z is exactly 0
 
-// -z of a gate: a gate of +-inf gives exactly 0 or -1
-__device__ __forceinline__ float2 neg_z(float2 g) {
-    return make_float2(rcp_approx(-1.0f - ex2_approx(g.x * kLog2e)), rcp_approx(-1.0f - ex2_approx(g.y * kLog2e)));
+// -z of gates: a gate of +-inf gives exactly 0 or -1
+__device__ __forceinline__ float2 gate_nz(float2 g) {
+    const float2 t = mul2(g, dup2(kLog2e)), d = fma2(make_float2(ex2_approx(t.x), ex2_approx(t.y)), dup2(-1.0f), dup2(-1.0f));
+    return make_float2(rcp_approx(d.x), rcp_approx(d.y));
 }
 // -z and z a, both with the relative accuracy of the smaller of z and a
-__device__ __forceinline__ void neg_z_slope(float g, float &nz, float &za) {
-    const float e = ex2_approx(-fabsf(g) * kLog2e), r = rcp_approx(1.0f + e), small = e * r;
-    nz = g >= 0.0f ? -small : -r;
-    za = small * r;
+__device__ __forceinline__ void gate_slope(float2 g, float2 &nz, float2 &za) {
+    const float2 e = make_float2(ex2_approx(fabsf(g.x) * -kLog2e), ex2_approx(fabsf(g.y) * -kLog2e)), d = add2(e, dup2(1.0f));
+    const float2 r = make_float2(rcp_approx(d.x), rcp_approx(d.y)), small = mul2(e, r);
+    nz = make_float2(g.x >= 0.0f ? -small.x : -r.x, g.y >= 0.0f ? -small.y : -r.y);
+    za = mul2(small, r);
 }
+// A step for two channels of the negated state, -h_t = -h + z h - z x, and the factor alone. (The state is carried negated because -z
+// comes out of the gate and x out of memory as they are: each negation would be an operation a step.)
+__device__ __forceinline__ float2 decay(float2 nz, float2 v) { return fma2(nz, v, v); }
+__device__ __forceinline__ float2 gate_step(float2 nz, float2 x, float2 nh) { return fma2(nz, x, decay(nz, nh)); }
 
 // h -> A h + F of a stretch, two channels
 struct Map2 {
     float2 A, F;
-    __device__ __forceinline__ float2 operator()(float2 h) const { return fma2(A, h, F); }
+    __device__ __forceinline__ float2 operator()(float2 h) const { return make_float2(fmaf(A.x, h.x, F.x), fmaf(A.y, h.y, F.y)); }
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -226,29 +262,51 @@ __device__ __forceinline__ uint32_t cluster_size() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// a 16-byte store into another CTA of the cluster, at the place `here` has in this one
-__device__ __forceinline__ void cluster_store(const void *here, uint32_t rank, float4 v) {
+__device__ __forceinline__ uint32_t at_rank(uint32_t here, uint32_t rank) {  // the address `here` has in another CTA of the cluster
     uint32_t there;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_u32(here)), "r"(rank));
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(rank));
+    return there;
+}
+// 16 bytes into another CTA's shared memory, counted by a barrier of that CTA
+__device__ __forceinline__ void cluster_send(uint32_t there, float4 v, uint32_t bar) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(there), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(bar)
+                 : "memory");
 }
 
 // Maps of the CTA's warps and (CLUSTER) of the cluster's CTAs, twice: a round writes one copy while the slowest reader of the
 // round before may still be in the other.
-template <bool CLUSTER>
+template <bool CLUSTER, int W>
 struct GatedShared {
-    float4 warp[2][kGatedWarps][32];
+    float4 warp[2][W][32];
     float4 cta[2][CLUSTER ? kGatedMaxCluster : 1][32];
     float2 carry[2][32];
+    uint64_t arrived[2];  // (CLUSTER) of the copies: all CTAs' maps are here
 };
+
+// mbar_wait without sleeps between its polls (which suspend the thread themselves), counted in cycles of at most 2 GHz.
+__device__ __forceinline__ bool gated_wait(const WaitCtl &w, uint64_t *bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long begin = clock64(), limit = 2ll * w.limit_ns;
+    do {
+        for (int i = 0; i < 32; ++i)
+            if (mbar_try_wait(bar, parity)) return true;
+    } while (clock64() - begin < limit);
+    atomicCAS(w.status, 0, kStatusWait | kGatedSite);
+    return false;
+}
 
 // Called by all threads with the map of the warp's own steps: the value in front of the warp's steps. The value in front of the round is
 // sh.carry[buf] (for the first round put there by the warp that is last in the fold), the one behind it goes to the other copy.
-// REVERSE: values come from behind. One barrier of the CTA, with CLUSTER one of the cluster.
-template <bool CLUSTER, bool REVERSE>
-__device__ __forceinline__ float2 gated_exchange(GatedShared<CLUSTER> &sh, int buf, Map2 own, int warp, int lane, int rank, int ranks) {
+// REVERSE: values come from behind. One barrier of the CTA. With CLUSTER the CTAs send one another their maps and wait for those of the
+// others by a barrier that counts bytes: a barrier of the cluster would wait for every warp's stores to memory each round. A copy
+// is written again two rounds later, by a CTA that has this CTA's map of the round between, which is sent behind the barrier that
+// the copy's last reader has passed. ok: false once a bounded wait has run out; the thread then waits no more, but goes on with
+// whatever is there, so that all threads meet in the remaining barriers and the kernel ends.
+template <bool CLUSTER, bool REVERSE, int W>
+__device__ __forceinline__ float2 gated_exchange(GatedShared<CLUSTER, W> &sh, const WaitCtl &wait, int round, Map2 own, int warp, int lane, int rank, int ranks, bool &ok) {
+    const int buf = round & 1;
     auto map = [](const float4 &v) { return Map2{make_float2(v.x, v.y), make_float2(v.z, v.w)}; };
-    const int place = REVERSE ? kGatedWarps - 1 - warp : warp;  // in the order of the fold
+    const int place = REVERSE ? W - 1 - warp : warp;  // in the order of the fold
     sh.warp[buf][place][lane] = make_float4(own.A.x, own.A.y, own.F.x, own.F.y);
     __syncthreads();
     float2 mine;
@@ -256,19 +314,23 @@ __device__ __forceinline__ float2 gated_exchange(GatedShared<CLUSTER> &sh, int b
         if (warp == 0) {  // the CTA's map to all
             Map2 all{make_float2(1.0f, 1.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-            for (int i = 0; i < kGatedWarps; ++i) {
+            for (int i = 0; i < W; ++i) {
                 const Map2 m = map(sh.warp[buf][i][lane]);
                 all.F = m(all.F);
-                all.A = mul2(m.A, all.A);
+                all.A = make_float2(m.A.x * all.A.x, m.A.y * all.A.y);
             }
             const float4 v = make_float4(all.A.x, all.A.y, all.F.x, all.F.y);
-            for (int r = 0; r < ranks; ++r) cluster_store(&sh.cta[buf][rank][lane], r, v);
+            const uint32_t here = smem_u32(&sh.cta[buf][rank][lane]), bar = smem_u32(&sh.arrived[buf]);
+            // (not after a wait that ran out: its barrier's phase is not complete, and a second arrival in one phase is an error)
+            if (ok && lane == 0) mbar_arrive_expect_tx(&sh.arrived[buf], ranks * 512);
+            if (ok && round != wait.skip_tile)  // skip_tile: the tests' incomplete hand-over
+                for (int r = 0; r < ranks; ++r) cluster_send(at_rank(here, r), v, at_rank(bar, r));
         }
-        cluster_sync();
+        ok = ok && gated_wait(wait, &sh.arrived[buf], (round >> 1) & 1);
         mine = sh.carry[buf][lane];
         const int before = REVERSE ? ranks - 1 - rank : rank;
         for (int i = 0; i < before; ++i) mine = map(sh.cta[buf][REVERSE ? ranks - 1 - i : i][lane])(mine);
-        if (place == kGatedWarps - 1) {  // (the warp that folds most anyway)
+        if (place == W - 1) {  // (the warp that folds most anyway)
             float2 end = mine;
             for (int i = before; i < ranks; ++i) end = map(sh.cta[buf][REVERSE ? ranks - 1 - i : i][lane])(end);
             sh.carry[buf ^ 1][lane] = end;
@@ -277,106 +339,121 @@ __device__ __forceinline__ float2 gated_exchange(GatedShared<CLUSTER> &sh, int b
         mine = sh.carry[buf][lane];
     }
 #pragma unroll
-    for (int i = 0; i < kGatedWarps - 1; ++i)
+    for (int i = 0; i < W - 1; ++i)
         if (i < place) mine = map(sh.warp[buf][i][lane])(mine);
-    if (!CLUSTER && place == kGatedWarps - 1) sh.carry[buf ^ 1][lane] = own(mine);
+    if (!CLUSTER && place == W - 1) sh.carry[buf ^ 1][lane] = own(mine);
     return mine;
 }
 
 // Grid: sequences x channel blocks x cluster, the last fastest; with packed sequences one sequence more, which clears the rows
 // that belong to none.
 template <typename T, bool PAIR, bool CLUSTER>
-__global__ void __launch_bounds__(kGatedWarps * 32, 2) kla_gated_fwd_kernel(const __grid_constant__ GatedParams prm) {
+__global__ void __launch_bounds__(GatedFwdShape<T>::W * 32, GatedFwdShape<T>::kCtas) kla_gated_fwd_kernel(const __grid_constant__ GatedParams prm) {
     using Shape = GatedFwdShape<T>;
-    constexpr int TS = Shape::TS, S = Shape::S, TT = kGatedWarps * TS;
-    __shared__ GatedShared<CLUSTER> sh;
+    constexpr int W = Shape::W, TS = Shape::TS, S = Shape::S, TT = W * TS;
+    __shared__ GatedShared<CLUSTER, W> sh;
     extern __shared__ __align__(16) unsigned char ring_bytes[];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int rank = CLUSTER ? (int)cluster_rank() : 0, ranks = CLUSTER ? (int)cluster_size() : 1;
     const int cell = blockIdx.x / ranks, n = cell / prm.blocks, block = cell % prm.blocks;
     const Lane<PAIR> ln(block, lane, prm.D);
-    if (n == prm.N) return gated_clear<T, PAIR>(prm, prm.h, ln, warp, rank, ranks);  // the whole cluster returns
-    if constexpr (CLUSTER) cluster_sync();  // every CTA has begun: its shared memory may be written
+    if (n == prm.N) return gated_clear<T, PAIR>(prm, prm.h, ln, warp, W, rank, ranks);  // the whole cluster returns
+    if constexpr (CLUSTER) {
+        if (threadIdx.x == 0) {
+            mbar_init(&sh.arrived[0], 1);
+            mbar_init(&sh.arrived[1], 1);
+            mbar_fence_init();
+        }
+        cluster_sync();  // every CTA has begun: its shared memory may be written
+    }
+    bool ok = true;
     const GatedSpan span = gated_span(prm, n);
     const T *x = gated_rows<const T>(prm.x, span), *g = gated_rows<const T>(prm.g, span);
     T *h_out = gated_rows<T>(prm.h, span);
     T *ring = reinterpret_cast<T *>(ring_bytes) + warp * S * 2 * TS * kGatedChannels;
     const int rounds = (span.len + TT * ranks - 1) / (TT * ranks), len = span.len;
-    if (warp == kGatedWarps - 1) sh.carry[0][lane] = prm.h0 ? ln.load_state(prm.h0 + (long long)n * prm.D) : make_float2(0.0f, 0.0f);
+    if (warp == W - 1) sh.carry[0][lane] = prm.h0 ? neg2(ln.load_state(prm.h0 + (long long)n * prm.D)) : make_float2(0.0f, 0.0f);
 
+    const int first = rank * TT + warp * TS;
+    GatedRows<T, TS> gates(g, prm.g.st, first, (long long)ranks * TT, block, prm.D, prm.g_width, lane, kHold);
+    GatedRows<T, TS> inputs(x, prm.x.st, first, (long long)ranks * TT, block, prm.D, prm.x_width, lane, 0.0f);
     int fetched = 0, slot_in = 0;
     auto fetch = [&] {  // the next round's rows, where there is one; a group of copies either way
         if (fetched < rounds) {
-            const int t0 = (fetched * ranks + rank) * TT + warp * TS, rows = len - t0;
+            const int rows = len - (fetched * ranks * TT + first);
             T *to = ring + slot_in * 2 * TS * kGatedChannels;
-            gated_fetch<T, TS>(to, g + (long long)t0 * prm.g.st, prm.g.st, rows, block, prm.D, prm.g_width, lane);
-            gated_fetch<T, TS>(to + TS * kGatedChannels, x + (long long)t0 * prm.x.st, prm.x.st, rows, block, prm.D, prm.x_width, lane);
+            gates.fetch(to, rows);
+            inputs.fetch(to + TS * kGatedChannels, rows);
         }
         gated_commit();
         ++fetched;
         if (++slot_in == S) slot_in = 0;
     };
-#pragma unroll
-    for (int i = 0; i < S - 1; ++i) fetch();
     int slot = 0;
-    for (int round = 0; round < rounds; ++round) {
+    for (int round = 1 - S; round < rounds; ++round) {  // (the first S - 1 only fetch: one copy of that code)
         const int t0 = (round * ranks + rank) * TT + warp * TS, cnt = len - t0;
-        gated_arrived<S - 2>();
+        if (round >= 0) gated_arrived<S - 2>();
         fetch();  // over the round before
+        if (round < 0) continue;
         const T *gs = ring + slot * 2 * TS * kGatedChannels, *xs = gs + TS * kGatedChannels;
         if (++slot == S) slot = 0;
         float2 nz[TS];
         Map2 own{make_float2(1.0f, 1.0f), make_float2(0.0f, 0.0f)};
-        auto compose = [&](int i) {
-            nz[i] = neg_z(ln.take(gs + i * kGatedChannels));
-            own.A = fma2(nz[i], own.A, own.A);
-            own.F = fma2(nz[i], neg2(ln.take(xs + i * kGatedChannels)), fma2(nz[i], own.F, own.F));
-        };
-        if (cnt >= TS) {
 #pragma unroll
-            for (int i = 0; i < TS; ++i) compose(i);
-        } else {
-#pragma unroll
-            for (int i = 0; i < TS; ++i)
-                if (i < cnt) compose(i);
+        for (int i = 0; i < TS; ++i) {
+            nz[i] = gate_nz(ln.take(gs + i * kGatedChannels));
+            own.A = decay(nz[i], own.A);
+            own.F = gate_step(nz[i], ln.take(xs + i * kGatedChannels), own.F);
         }
-        float2 h = gated_exchange<CLUSTER, false>(sh, round & 1, own, warp, lane, rank, ranks);
+        float2 h = gated_exchange<CLUSTER, false, W>(sh, prm.wait, round, own, warp, lane, rank, ranks, ok);
         if (prm.ckpt != nullptr && t0 % kGatedUnit == 0 && cnt > 0)
-            ln.store_state(prm.ckpt + (long long)(span.unit + t0 / kGatedUnit) * prm.D, h);
-        T *to = h_out + (long long)t0 * prm.h.st;
-        auto walk = [&](int i) {
-            h = fma2(nz[i], neg2(ln.take(xs + i * kGatedChannels)), fma2(nz[i], h, h));
-            ln.store(to, h);
-            to += prm.h.st;
-        };
+            ln.store_state(prm.ckpt + (long long)(span.unit + t0 / kGatedUnit) * prm.D, neg2(h));
+        T *to = h_out + (long long)t0 * prm.h.st + ln.c0;
         if (cnt >= TS) {
 #pragma unroll
-            for (int i = 0; i < TS; ++i) walk(i);
+            for (int i = 0; i < TS; ++i) {
+                h = gate_step(nz[i], ln.take(xs + i * kGatedChannels), h);
+                ln.store_negated(to, h);
+                to += prm.h.st;
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < TS; ++i)
-                if (i < cnt) walk(i);
+                if (i < cnt) {
+                    h = gate_step(nz[i], ln.take(xs + i * kGatedChannels), h);
+                    ln.store_negated(to, h);
+                    to += prm.h.st;
+                }
         }
     }
-    if (warp == kGatedWarps - 1 && rank == 0) ln.store_state(prm.end + (long long)n * prm.D, sh.carry[rounds & 1][lane]);  // its own
+    if constexpr (CLUSTER) cluster_sync();  // no CTA leaves while another may send to it (all has arrived, unless a wait ran out)
+    if (warp == W - 1 && rank == 0) ln.store_state(prm.end + (long long)n * prm.D, neg2(sh.carry[rounds & 1][lane]));  // its own
 }
 
 template <typename T, bool PAIR, bool CLUSTER>
-__global__ void __launch_bounds__(kGatedWarps * 32, 2) kla_gated_bwd_kernel(const __grid_constant__ GatedParams prm) {
+__global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kCtas) kla_gated_bwd_kernel(const __grid_constant__ GatedParams prm) {
     using Shape = GatedBwdShape<T>;
-    constexpr int TS = Shape::TS, S = Shape::S, kTile = TS * kGatedChannels;
-    __shared__ GatedShared<CLUSTER> sh;
-    __shared__ float4 fw[2][kGatedWarps][32];  // maps of the warps forwards
+    constexpr int W = Shape::W, TS = Shape::TS, S = Shape::S, kTile = TS * kGatedChannels;
+    __shared__ GatedShared<CLUSTER, W> sh;
+    __shared__ float4 fw[2][W][32];  // maps of the warps forwards
     extern __shared__ __align__(16) unsigned char ring_bytes[];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int rank = CLUSTER ? (int)cluster_rank() : 0, ranks = CLUSTER ? (int)cluster_size() : 1;
     const int cell = blockIdx.x / ranks, n = cell / prm.blocks, block = cell % prm.blocks;
     const Lane<PAIR> ln(block, lane, prm.D);
     if (n == prm.N) {
-        gated_clear<T, PAIR>(prm, prm.dx, ln, warp, rank, ranks);
-        return gated_clear<T, PAIR>(prm, prm.dg, ln, warp, rank, ranks);
+        gated_clear<T, PAIR>(prm, prm.dx, ln, warp, W, rank, ranks);
+        return gated_clear<T, PAIR>(prm, prm.dg, ln, warp, W, rank, ranks);
     }
-    if constexpr (CLUSTER) cluster_sync();
+    if constexpr (CLUSTER) {
+        if (threadIdx.x == 0) {
+            mbar_init(&sh.arrived[0], 1);
+            mbar_init(&sh.arrived[1], 1);
+            mbar_fence_init();
+        }
+        cluster_sync();
+    }
+    bool ok = true;
     const GatedSpan span = gated_span(prm, n);
     const T *x = gated_rows<const T>(prm.x, span), *g = gated_rows<const T>(prm.g, span), *dh = gated_rows<const T>(prm.dh, span);
     T *dx = gated_rows<T>(prm.dx, span), *dg = gated_rows<T>(prm.dg, span);
@@ -385,14 +462,19 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) kla_gated_bwd_kernel(cons
     // copies of the exchange by parity of the rounds done
     if (warp == 0) sh.carry[0][lane] = prm.dend ? ln.load_state(prm.dend + (long long)n * prm.D) : make_float2(0.0f, 0.0f);
 
+    const int first = ((rounds - 1) * ranks + rank) * kGatedUnit + warp * TS;  // the last round's
+    const long long tile = -(long long)ranks * kGatedUnit;
+    GatedRows<T, TS> gates(g, prm.g.st, first, tile, block, prm.D, prm.g_width, lane, kHold);
+    GatedRows<T, TS> inputs(x, prm.x.st, first, tile, block, prm.D, prm.x_width, lane, 0.0f);
+    GatedRows<T, TS> grads(dh, prm.dh.st, first, tile, block, prm.D, prm.dh_width, lane, 0.0f);
     int fetched = rounds - 1, slot_in = 0;
     auto fetch = [&] {  // rounds from the last one on
         if (fetched >= 0) {
-            const int t0 = (fetched * ranks + rank) * kGatedUnit + warp * TS, rows = len - t0;
+            const int rows = len - ((fetched * ranks + rank) * kGatedUnit + warp * TS);
             T *to = ring + slot_in * 3 * kTile;
-            gated_fetch<T, TS>(to, g + (long long)t0 * prm.g.st, prm.g.st, rows, block, prm.D, prm.g_width, lane);
-            gated_fetch<T, TS>(to + kTile, x + (long long)t0 * prm.x.st, prm.x.st, rows, block, prm.D, prm.x_width, lane);
-            gated_fetch<T, TS>(to + 2 * kTile, dh + (long long)t0 * prm.dh.st, prm.dh.st, rows, block, prm.D, prm.dh_width, lane);
+            gates.fetch(to, rows);
+            inputs.fetch(to + kTile, rows);
+            grads.fetch(to + 2 * kTile, rows);
         }
         gated_commit();
         --fetched;
@@ -401,71 +483,66 @@ __global__ void __launch_bounds__(kGatedWarps * 32, 2) kla_gated_bwd_kernel(cons
     // the state in front of a round's unit
     auto front = [&](int round) {
         const int unit = round * ranks + rank;
-        return round >= 0 && unit * kGatedUnit < len ? ln.load_state(prm.ckpt + (long long)(span.unit + unit) * prm.D) : make_float2(0.0f, 0.0f);
+        return round >= 0 && unit * kGatedUnit < len ? neg2(ln.load_state(prm.ckpt + (long long)(span.unit + unit) * prm.D)) : make_float2(0.0f, 0.0f);
     };
-#pragma unroll
-    for (int i = 0; i < S - 1; ++i) fetch();
     float2 next = front(rounds - 1);
     int slot = 0;
-    for (int round = rounds - 1; round >= 0; --round) {
+    for (int round = rounds - 2 + S; round >= 0; --round) {  // (the first S - 1 only fetch)
         const int t0 = (round * ranks + rank) * kGatedUnit + warp * TS, cnt = len - t0, buf = (rounds - 1 - round) & 1;
+        if (round < rounds) gated_arrived<S - 2>();
+        fetch();
+        if (round >= rounds) continue;
         float2 h = next;
         next = front(round - 1);
-        gated_arrived<S - 2>();
-        fetch();
         const T *gs = ring + slot * 3 * kTile, *xs = gs + kTile, *ds = xs + kTile;
         if (++slot == S) slot = 0;
-        float2 nz[TS], za[TS];
+        float2 nz[TS], za[TS], c[TS];
         Map2 back{make_float2(1.0f, 1.0f), make_float2(0.0f, 0.0f)};
         float2 F = make_float2(0.0f, 0.0f);
-        auto compose = [&](auto full) {
-            constexpr bool FULL = decltype(full)::value;
 #pragma unroll
-            for (int i = 0; i < TS; ++i)
-                if (FULL || i < cnt) {
-                    const float2 gi = ln.take(gs + i * kGatedChannels);
-                    neg_z_slope(gi.x, nz[i].x, za[i].x);
-                    neg_z_slope(gi.y, nz[i].y, za[i].y);
-                    back.A = fma2(nz[i], back.A, back.A);
-                    F = fma2(nz[i], neg2(ln.take(xs + i * kGatedChannels)), fma2(nz[i], F, F));
-                }
-#pragma unroll
-            for (int i = TS - 1; i >= 0; --i)
-                if (FULL || i < cnt) {
-                    const float2 ci = add2(ln.take(ds + i * kGatedChannels), back.F);
-                    back.F = fma2(nz[i], ci, ci);
-                }
-        };
-        if (cnt >= TS) compose(std::true_type{});
-        else compose(std::false_type{});
-        fw[buf][warp][lane] = make_float4(back.A.x, back.A.y, F.x, F.y);
-        float2 u = gated_exchange<CLUSTER, true>(sh, buf, back, warp, lane, rank, ranks);
-        for (int w = 0; w < warp; ++w) {
-            const float4 m = fw[buf][w][lane];
-            h = fma2(make_float2(m.x, m.y), h, make_float2(m.z, m.w));
+        for (int i = 0; i < TS; ++i) {
+            gate_slope(ln.take(gs + i * kGatedChannels), nz[i], za[i]);
+            back.A = decay(nz[i], back.A);
+            F = gate_step(nz[i], ln.take(xs + i * kGatedChannels), F);
         }
-        auto walk = [&](auto full) {
-            constexpr bool FULL = decltype(full)::value;
-            float2 c[TS];
+        auto behind = [&](int i, float2 u) {  // the gradient that reaches step i
+            const float2 d = ln.take(ds + i * kGatedChannels);
+            return add2(d, u);
+        };
 #pragma unroll
-            for (int i = TS - 1; i >= 0; --i)
-                if (FULL || i < cnt) {
-                    c[i] = add2(ln.take(ds + i * kGatedChannels), u);
-                    u = fma2(nz[i], c[i], c[i]);
-                }
-            T *to_x = dx + (long long)t0 * prm.dx.st, *to_g = dg + (long long)t0 * prm.dg.st;
+        for (int i = TS - 1; i >= 0; --i) back.F = decay(nz[i], behind(i, back.F));
+        fw[buf][warp][lane] = make_float4(back.A.x, back.A.y, F.x, F.y);
+        float2 u = gated_exchange<CLUSTER, true, W>(sh, prm.wait, rounds - 1 - round, back, warp, lane, rank, ranks, ok);
+#pragma unroll
+        for (int w = 0; w < W - 1; ++w)
+            if (w < warp) {
+                const float4 m = fw[buf][w][lane];
+                h = Map2{make_float2(m.x, m.y), make_float2(m.z, m.w)}(h);
+            }
+#pragma unroll
+        for (int i = TS - 1; i >= 0; --i) {
+            c[i] = behind(i, u);
+            u = decay(nz[i], c[i]);
+        }
+        T *to_x = dx + (long long)t0 * prm.dx.st + ln.c0, *to_g = dg + (long long)t0 * prm.dg.st + ln.c0;
+        auto out = [&](int i) {  // h: negated
+            const float2 xi = ln.take(xs + i * kGatedChannels);
+            ln.store_negated(to_x, mul2(nz[i], c[i]));
+            ln.store_negated(to_g, mul2(mul2(za[i], c[i]), add2(h, xi)));
+            to_x += prm.dx.st;
+            to_g += prm.dg.st;
+            h = gate_step(nz[i], xi, h);
+        };
+        if (cnt >= TS) {
+#pragma unroll
+            for (int i = 0; i < TS; ++i) out(i);
+        } else {
 #pragma unroll
             for (int i = 0; i < TS; ++i)
-                if (FULL || i < cnt) {
-                    const float2 nx = neg2(ln.take(xs + i * kGatedChannels));
-                    ln.store(to_x + i * prm.dx.st, mul2(neg2(nz[i]), c[i]));
-                    ln.store(to_g + i * prm.dg.st, mul2(mul2(za[i], c[i]), add2(h, nx)));
-                    h = fma2(nz[i], nx, fma2(nz[i], h, h));
-                }
-        };
-        if (cnt >= TS) walk(std::true_type{});
-        else walk(std::false_type{});
+                if (i < cnt) out(i);
+        }
     }
+    if constexpr (CLUSTER) cluster_sync();
     if (prm.dh0 != nullptr && warp == 0 && rank == 0) ln.store_state(prm.dh0 + (long long)n * prm.D, sh.carry[rounds & 1][lane]);  // its own
 }
 
@@ -486,7 +563,7 @@ __global__ void __launch_bounds__(256) kla_gated_step_kernel(const GatedStepPara
     const long long b = i / prm.D;
     const int d = (int)(i - b * prm.D);
     const float x = to_f32<T>(static_cast<const T *>(prm.x)[b * prm.x_sb + d]);
-    const float nz = rcp_approx(-1.0f - ex2_approx(to_f32<T>(static_cast<const T *>(prm.g)[b * prm.g_sb + d]) * kLog2e));
+    const float nz = gate_nz(make_float2(to_f32<T>(static_cast<const T *>(prm.g)[b * prm.g_sb + d]), 0.0f)).x;
     const float s = prm.state[i], h = fmaf(nz, -x, fmaf(nz, s, s));
     prm.state_out[i] = h;
     static_cast<T *>(prm.h)[i] = from_f32<T>(h);

@@ -268,6 +268,34 @@ def test_captured_and_on_another_stream():
     assert all(torch.equal(a, b) for a, b in zip(got, again)) and not torch.equal(again[0], want[0])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_waits_that_run_out_are_reported_and_the_next_call_is_right(dtype):
+    """One sequence of few channels is shared by a cluster of CTAs, which wait for one another's maps."""
+    L = lib.load()
+    both, _, dh, _ = (t.cuda() for t in inputs(1, 2000, 64, 1, dtype))
+    x, g = (t.requires_grad_() for t in (both[..., :64], both[..., 64:]))
+
+    def step():
+        h, _ = kla_b200.gated_scan_b200(x, g)
+        return h, lambda: torch.autograd.grad(h, (x, g), dh, retain_graph=True)
+
+    h0, grads0 = step()
+    grads0 = grads0()
+    assert lib.device_status() == 0
+    for where in ("forward", "backward"):
+        h, grads = step()
+        try:
+            assert L.kla_b200_test_hooks(3_000_000, 1) == 0  # 3 ms; the second round's maps are not sent
+            step() if where == "forward" else grads()
+            st = lib.device_status()
+        finally:
+            assert L.kla_b200_test_hooks(0, -1) == 0
+        assert st == 0x150, hex(st)
+        h, grads = step()
+        assert torch.equal(h, h0) and all(torch.equal(a, b) for a, b in zip(grads(), grads0)) and lib.device_status() == 0
+
+
 def gated_refusals(dev):
     x = torch.zeros(2, 3, 4, device=dev)
     s = torch.zeros(2, 4, device=dev)
