@@ -1,6 +1,7 @@
 // Entry points of the gated recurrence (kla_gated.cuh): argument checks, kernel and cluster choice, launches.
 #include <algorithm>
 #include <cmath>
+#include <mutex>
 
 #include "../../include/kla_b200.h"
 #include "kla_entry.h"
@@ -20,67 +21,121 @@ int check_rows(const kla_b200_tensor3 &t, size_t esz) {
 bool pairs(const kla_b200_tensor3 &t, size_t esz) { return aligned(t.ptr, 2 * esz) && t.stride_b % 2 == 0 && t.stride_t % 2 == 0; }
 Tensor3 t3(const kla_b200_tensor3 &t) { return Tensor3{t.ptr, t.stride_b, t.stride_t}; }
 
+constexpr int kRanks[] = {1, 2, 3, 4, 5, 6, 8};  // sizes of clusters
+constexpr int kRankCount = 7;
+
+// One of the two kernels for a type, alone or in clusters.
+struct Kernel {
+    void (*kern)(GatedParams);
+    int warps, tile;
+    size_t smem;  // without the maps of a cluster's CTAs
+};
+template <typename T, bool PAIR>
+Kernel kernel_of(bool backward, bool cluster) {
+    using F = GatedFwdShape<T>;
+    using B = GatedBwdShape<T>;
+    if (backward) return Kernel{cluster ? kla_gated_bwd_kernel<T, PAIR, true> : kla_gated_bwd_kernel<T, PAIR, false>, B::W, kGatedUnit, B::kBytes};
+    return Kernel{cluster ? kla_gated_fwd_kernel<T, PAIR, true> : kla_gated_fwd_kernel<T, PAIR, false>, F::W, F::W * F::TS, F::kBytes};
+}
+Kernel kernel_of(bool bf16, bool pairs, bool backward, bool cluster) {
+    if (bf16) return pairs ? kernel_of<__nv_bfloat16, true>(backward, cluster) : kernel_of<__nv_bfloat16, false>(backward, cluster);
+    return pairs ? kernel_of<float, true>(backward, cluster) : kernel_of<float, false>(backward, cluster);
+}
+size_t smem_of(const Kernel &k, int ranks) { return k.smem + (ranks > 1 ? ranks * kGatedCtaMap : 0); }
+
+void fill(cudaLaunchConfig_t *cfg, cudaLaunchAttribute *attr, const Kernel &k, int64_t grid, int ranks, cudaStream_t st) {
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = ranks;
+    attr->val.clusterDim.y = attr->val.clusterDim.z = 1;
+    *cfg = cudaLaunchConfig_t{};
+    cfg->gridDim = dim3((unsigned)grid);
+    cfg->blockDim = dim3(k.warps * 32);
+    cfg->dynamicSmemBytes = smem_of(k, ranks);
+    cfg->stream = st;
+    cfg->attrs = attr;
+    cfg->numAttrs = ranks > 1 ? 1 : 0;
+}
+
+// CTAs that are resident at once by size of cluster; looked up once per device and kernel, which also lets the kernel use its shared
+// memory.
+struct Slots {
+    bool known;
+    int ctas[kRankCount];
+};
+int slots_of(bool bf16, bool pairs, bool backward, Slots *out) {
+    static std::mutex mu;
+    static Slots table[64][2][2][2];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return entry::cuda_fail(e);
+    if (dev < 0 || dev >= 64) return KLA_B200_EUNSUPPORTED;
+    std::lock_guard<std::mutex> lock(mu);
+    Slots &s = table[dev][bf16][pairs][backward];
+    if (!s.known) {
+        for (const bool cluster : {false, true}) {
+            const Kernel k = kernel_of(bf16, pairs, backward, cluster);
+            if ((e = cudaFuncSetAttribute(k.kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(k, kGatedMaxCluster))) != cudaSuccess) return entry::cuda_fail(e);
+        }
+        for (int i = 0; i < kRankCount; ++i) {
+            const Kernel k = kernel_of(bf16, pairs, backward, i > 0);
+            int n = 0;
+            if (i == 0) {
+                e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k.kern, k.warps * 32, k.smem);
+                n *= device_sms();
+            } else {
+                cudaLaunchAttribute attr;
+                cudaLaunchConfig_t cfg;
+                fill(&cfg, &attr, k, 1024 * kRanks[i], kRanks[i], nullptr);
+                e = cudaOccupancyMaxActiveClusters(&n, k.kern, &cfg);
+                n *= kRanks[i];
+            }
+            if (e != cudaSuccess) return entry::cuda_fail(e);
+            s.ctas[i] = n;
+        }
+        s.known = true;
+    }
+    *out = s;
+    return KLA_B200_OK;
+}
+
 // How many CTAs of a cluster share a sequence: the least time by a model of what was measured on B200 (us). A round, a tile of each
 // CTA of a cluster, takes `round` alone on its SM and by `share` more for the exchange; a second and third CTA on the SM add 35 % each;
 // launching takes `start`; and no choice is faster than 80 % of the memory's rate. Measured, clusters of 1 / 2 / 4 / 8: forward bfloat16
 // B=4 L=8192 D=2048 102 / 85 / 93 / 105, B=16 L=2048 D=1536 60 / 72 / 84 / 107, B=1 L=8192 D=1024 98 / 62 / 33 / 24, B=8 L=512 D=768
 // 8.3 / 8.7 / 11.5 / 17.6; backward 103 / 119 / 129 / 148 (B=16 ...), 192 / 121 / 65 / 45 (B=1 ...), 14.2 / 13.7 / 10.7 / 13.8 (B=8 ...).
 // Of packed sequences the host knows the number and the sum of the lengths; the longest of n random ones is about ln n + 0.6 times
-// their mean, and clusters of 8 were no gain there.
-int pick_ranks(int64_t cells, int64_t rows, int64_t sequences, int64_t L, bool packed, bool backward, size_t esz, int64_t D) {
+// their mean, and clusters of more than four were no gain there.
+int pick_ranks(const Slots &slots, const Kernel &k, int64_t cells, int64_t rows, int64_t sequences, int64_t L, bool packed, bool backward, size_t esz, int64_t D) {
     const double sms = device_sms();
-    const int tile = backward ? kGatedUnit : esz == 2 ? GatedFwdShape<__nv_bfloat16>::W * GatedFwdShape<__nv_bfloat16>::TS : GatedFwdShape<float>::W * GatedFwdShape<float>::TS;
-    const int ctas = !backward ? GatedFwdShape<float>::kCtas : esz == 2 ? GatedBwdShape<__nv_bfloat16>::kCtas : GatedBwdShape<float>::kCtas;
-    const double round = backward ? (esz == 2 ? 1.5 : 2.2) : (esz == 2 ? 1.53 : 1.15), shares[4] = {1.0, 1.27, 1.37, 1.6}, starts[4] = {2.0, 3.5, 5.0, 6.0};
+    const double round = backward ? (esz == 2 ? 1.5 : 2.2) : (esz == 2 ? 1.53 : 1.15);
+    constexpr double shares[kRankCount] = {1.0, 1.27, 1.32, 1.37, 1.42, 1.47, 1.6}, starts[kRankCount] = {2.0, 3.5, 4.3, 5.0, 5.3, 5.6, 6.0};
     double steps = (double)L;
     if (packed && sequences > 0) steps = std::min(steps, (double)L / sequences * (std::log((double)sequences) + 0.6));
-    const double tiles = std::ceil(steps / tile), least_us = (double)rows * D * esz * (backward ? 5 : 3) / 5.2e6;
+    const double tiles = std::ceil(steps / k.tile), least_us = (double)rows * D * esz * (backward ? 5 : 3) / 5.2e6;
     int best = 1;
     double least = 0.0;
-    for (int k = 0; k < (packed ? 3 : 4); ++k) {
-        const int r = 1 << k;
-        if (r > 1 && (r > tiles || r > kGatedMaxCluster)) break;
-        const double n = (double)cells * r, waves = packed ? 1.0 : std::max(1.0, std::ceil(n / (ctas * sms)));
-        const double load = std::min((double)ctas, std::max(1.0, std::ceil(n / waves / sms)));
-        const double t = std::max(waves * (std::ceil(tiles / r) * round * shares[k] * (1.0 + 0.35 * (load - 1.0)) + starts[k]), least_us);
+    for (int i = 0; i < kRankCount; ++i) {
+        const int r = kRanks[i];
+        if (r > 1 && (r > tiles || slots.ctas[i] < r || (packed && r > 4))) continue;
+        const double n = (double)cells * r, waves = packed ? 1.0 : std::max(1.0, std::ceil(n / slots.ctas[i]));
+        const double load = std::min(3.0, std::max(1.0, std::ceil(n / waves / sms)));
+        const double t = std::max(waves * (std::ceil(tiles / r) * round * shares[i] * (1.0 + 0.35 * (load - 1.0)) + starts[i]), least_us);
         if (r == 1 || t < least) { best = r; least = t; }
     }
     return best;
 }
 
-template <typename K>
-int launch(K kern, GatedParams &prm, int warps, size_t smem, int64_t sequences, int ranks, cudaStream_t st) {
+int launch(const Kernel &k, const GatedParams &prm, int64_t sequences, int ranks, cudaStream_t st) {
     const int64_t grid = sequences * prm.blocks * ranks;
     if (grid == 0) return KLA_B200_OK;
     if (grid > 0x7fffffffll) return KLA_B200_EUNSUPPORTED;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return entry::cuda_fail(e);
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = ranks;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(warps * 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = ranks > 1 ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kern, prm);
+    cudaLaunchAttribute attr;
+    cudaLaunchConfig_t cfg;
+    fill(&cfg, &attr, k, grid, ranks, st);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k.kern, prm);
     if (e != cudaSuccess) return entry::cuda_fail(e);
     entry::count_launch();
     return KLA_B200_OK;
-}
-
-template <typename T, bool PAIR>
-int run(GatedParams &prm, bool backward, int64_t sequences, int ranks, cudaStream_t st) {
-    constexpr size_t fwd = GatedFwdShape<T>::kBytes, bwd = GatedBwdShape<T>::kBytes;
-    constexpr int wf = GatedFwdShape<T>::W, wb = GatedBwdShape<T>::W;
-    if (backward)
-        return ranks > 1 ? launch(kla_gated_bwd_kernel<T, PAIR, true>, prm, wb, bwd, sequences, ranks, st)
-                         : launch(kla_gated_bwd_kernel<T, PAIR, false>, prm, wb, bwd, sequences, ranks, st);
-    return ranks > 1 ? launch(kla_gated_fwd_kernel<T, PAIR, true>, prm, wf, fwd, sequences, ranks, st)
-                     : launch(kla_gated_fwd_kernel<T, PAIR, false>, prm, wf, fwd, sequences, ranks, st);
 }
 
 // Bytes an asynchronous copy of the tensor's rows may move: 16 where they are aligned so, else 4; 2 of bfloat16 rows that are not in
@@ -122,10 +177,10 @@ int gated(const kla_b200_gated_args *a, void *stream, bool backward) {
     prm.x_width = width(a->x, esz, a->D); prm.g_width = width(a->gate, esz, a->D); prm.dh_width = width(a->dh, esz, a->D);
     if (const int rc = entry::wait_ctl(&prm.wait)) return rc;
     const int64_t sequences = N + packed;
-    const int ranks = pick_ranks(N * prm.blocks, packed ? a->L : a->B * a->L, N, a->L, packed, backward, esz, a->D);
-    const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (esz == 2) return vec ? run<__nv_bfloat16, true>(prm, backward, sequences, ranks, st) : run<__nv_bfloat16, false>(prm, backward, sequences, ranks, st);
-    return vec ? run<float, true>(prm, backward, sequences, ranks, st) : run<float, false>(prm, backward, sequences, ranks, st);
+    Slots slots;
+    if (const int rc = slots_of(esz == 2, vec, backward, &slots)) return rc;
+    const int ranks = pick_ranks(slots, kernel_of(esz == 2, vec, backward, false), N * prm.blocks, packed ? a->L : a->B * a->L, N, a->L, packed, backward, esz, a->D);
+    return launch(kernel_of(esz == 2, vec, backward, ranks > 1), prm, sequences, ranks, static_cast<cudaStream_t>(stream));
 }
 
 }  // namespace

@@ -275,10 +275,12 @@ __device__ __forceinline__ void cluster_send(uint32_t there, float4 v, uint32_t 
 
 // Maps of the CTA's warps and (CLUSTER) of the cluster's CTAs, twice: a round writes one copy while the slowest reader of the
 // round before may still be in the other.
+// The CTAs' maps, [2][ranks][32] of 16 bytes, lie behind the ring: as many as there are, so that three CTAs of a cluster of up to six
+// fit an SM.
+constexpr size_t kGatedCtaMap = 2 * 32 * sizeof(float4);
 template <bool CLUSTER, int W>
 struct GatedShared {
     float4 warp[2][W][32];
-    float4 cta[2][CLUSTER ? kGatedMaxCluster : 1][32];
     float2 carry[2][32];
     uint64_t arrived[2];  // (CLUSTER) of the copies: all CTAs' maps are here
 };
@@ -303,8 +305,9 @@ __device__ __forceinline__ bool gated_wait(const WaitCtl &w, uint64_t *bar, uint
 // the copy's last reader has passed. ok: false once a bounded wait has run out; the thread then waits no more, but goes on with
 // whatever is there, so that all threads meet in the remaining barriers and the kernel ends.
 template <bool CLUSTER, bool REVERSE, int W>
-__device__ __forceinline__ float2 gated_exchange(GatedShared<CLUSTER, W> &sh, const WaitCtl &wait, int round, Map2 own, int warp, int lane, int rank, int ranks, bool &ok) {
+__device__ __forceinline__ float2 gated_exchange(GatedShared<CLUSTER, W> &sh, float4 *ctas, const WaitCtl &wait, int round, Map2 own, int warp, int lane, int rank, int ranks, bool &ok) {
     const int buf = round & 1;
+    ctas += buf * ranks * 32 + lane;  // of this copy
     auto map = [](const float4 &v) { return Map2{make_float2(v.x, v.y), make_float2(v.z, v.w)}; };
     const int place = REVERSE ? W - 1 - warp : warp;  // in the order of the fold
     sh.warp[buf][place][lane] = make_float4(own.A.x, own.A.y, own.F.x, own.F.y);
@@ -320,7 +323,7 @@ __device__ __forceinline__ float2 gated_exchange(GatedShared<CLUSTER, W> &sh, co
                 all.A = make_float2(m.A.x * all.A.x, m.A.y * all.A.y);
             }
             const float4 v = make_float4(all.A.x, all.A.y, all.F.x, all.F.y);
-            const uint32_t here = smem_u32(&sh.cta[buf][rank][lane]), bar = smem_u32(&sh.arrived[buf]);
+            const uint32_t here = smem_u32(ctas + rank * 32), bar = smem_u32(&sh.arrived[buf]);
             // (not after a wait that ran out: its barrier's phase is not complete, and a second arrival in one phase is an error)
             if (ok && lane == 0) mbar_arrive_expect_tx(&sh.arrived[buf], ranks * 512);
             if (ok && round != wait.skip_tile)  // skip_tile: the tests' incomplete hand-over
@@ -329,10 +332,10 @@ __device__ __forceinline__ float2 gated_exchange(GatedShared<CLUSTER, W> &sh, co
         ok = ok && gated_wait(wait, &sh.arrived[buf], (round >> 1) & 1);
         mine = sh.carry[buf][lane];
         const int before = REVERSE ? ranks - 1 - rank : rank;
-        for (int i = 0; i < before; ++i) mine = map(sh.cta[buf][REVERSE ? ranks - 1 - i : i][lane])(mine);
+        for (int i = 0; i < before; ++i) mine = map(ctas[(REVERSE ? ranks - 1 - i : i) * 32])(mine);
         if (place == W - 1) {  // (the warp that folds most anyway)
             float2 end = mine;
-            for (int i = before; i < ranks; ++i) end = map(sh.cta[buf][REVERSE ? ranks - 1 - i : i][lane])(end);
+            for (int i = before; i < ranks; ++i) end = map(ctas[(REVERSE ? ranks - 1 - i : i) * 32])(end);
             sh.carry[buf ^ 1][lane] = end;
         }
     } else {
@@ -371,6 +374,7 @@ __global__ void __launch_bounds__(GatedFwdShape<T>::W * 32, GatedFwdShape<T>::kC
     const T *x = gated_rows<const T>(prm.x, span), *g = gated_rows<const T>(prm.g, span);
     T *h_out = gated_rows<T>(prm.h, span);
     T *ring = reinterpret_cast<T *>(ring_bytes) + warp * S * 2 * TS * kGatedChannels;
+    float4 *ctas = reinterpret_cast<float4 *>(ring_bytes + Shape::kBytes);
     const int rounds = (span.len + TT * ranks - 1) / (TT * ranks), len = span.len;
     if (warp == W - 1) sh.carry[0][lane] = prm.h0 ? neg2(ln.load_state(prm.h0 + (long long)n * prm.D)) : make_float2(0.0f, 0.0f);
 
@@ -405,7 +409,7 @@ __global__ void __launch_bounds__(GatedFwdShape<T>::W * 32, GatedFwdShape<T>::kC
             own.A = decay(nz[i], own.A);
             own.F = gate_step(nz[i], ln.take(xs + i * kGatedChannels), own.F);
         }
-        float2 h = gated_exchange<CLUSTER, false, W>(sh, prm.wait, round, own, warp, lane, rank, ranks, ok);
+        float2 h = gated_exchange<CLUSTER, false, W>(sh, ctas, prm.wait, round, own, warp, lane, rank, ranks, ok);
         if (prm.ckpt != nullptr && t0 % kGatedUnit == 0 && cnt > 0)
             ln.store_state(prm.ckpt + (long long)(span.unit + t0 / kGatedUnit) * prm.D, neg2(h));
         T *to = h_out + (long long)t0 * prm.h.st + ln.c0;
@@ -458,6 +462,7 @@ __global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kC
     const T *x = gated_rows<const T>(prm.x, span), *g = gated_rows<const T>(prm.g, span), *dh = gated_rows<const T>(prm.dh, span);
     T *dx = gated_rows<T>(prm.dx, span), *dg = gated_rows<T>(prm.dg, span);
     T *ring = reinterpret_cast<T *>(ring_bytes) + warp * S * 3 * kTile;
+    float4 *ctas = reinterpret_cast<float4 *>(ring_bytes + Shape::kBytes);
     const int len = span.len, rounds = (len + kGatedUnit * ranks - 1) / (kGatedUnit * ranks);
     // copies of the exchange by parity of the rounds done
     if (warp == 0) sh.carry[0][lane] = prm.dend ? ln.load_state(prm.dend + (long long)n * prm.D) : make_float2(0.0f, 0.0f);
@@ -512,7 +517,7 @@ __global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kC
 #pragma unroll
         for (int i = TS - 1; i >= 0; --i) back.F = decay(nz[i], behind(i, back.F));
         fw[buf][warp][lane] = make_float4(back.A.x, back.A.y, F.x, F.y);
-        float2 u = gated_exchange<CLUSTER, true, W>(sh, prm.wait, rounds - 1 - round, back, warp, lane, rank, ranks, ok);
+        float2 u = gated_exchange<CLUSTER, true, W>(sh, ctas, prm.wait, rounds - 1 - round, back, warp, lane, rank, ranks, ok);
 #pragma unroll
         for (int w = 0; w < W - 1; ++w)
             if (w < warp) {
