@@ -14,9 +14,12 @@
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
+#include <array>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -695,6 +698,23 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, OptTensor, OptTensor> gated_fwd(const
     return {h, end, x, gate, cu, ckpt};
 }
 
+// The status of a call on an autograd thread, which does not hold the interpreter: no Python error may be set there.
+void check_native(int rc) {
+    if (rc == KLA_B200_OK) return;
+    const std::string msg = std::string("kla_b200: ") + lib.strerror(rc);
+    TORCH_CHECK_NOT_IMPLEMENTED(rc != KLA_B200_EUNSUPPORTED, msg);
+    TORCH_CHECK_VALUE(rc == KLA_B200_ECUDA, msg);
+    TORCH_CHECK(false, msg);
+}
+// What a backward that has no derivative of its own returns for the gradients it got: where a graph of it is made, using them raises.
+torch::autograd::variable_list once(const torch::autograd::variable_list &got, torch::autograd::variable_list grads) {
+    if (!c10::GradMode::is_enabled() || std::none_of(got.begin(), got.end(), [](const Tensor &t) { return t.defined() && t.requires_grad(); })) return grads;
+    auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", (int64_t)grads.size());
+    for (Tensor &g : grads)
+        if (g.defined()) g = g.detach().requires_grad_();
+    return (*error)(std::move(grads));
+}
+
 // kla_b200_gated_scan_bwd -> dx, dgate, and (where wanted) the gradient of the states sequences start from
 std::tuple<Tensor, Tensor, OptTensor> gated_bwd(const Tensor &x, const Tensor &gate, const OptTensor &cu, const Tensor &ckpt, const Tensor &dh_,
                                                 const OptTensor &dend_, bool want_state) {
@@ -707,8 +727,46 @@ std::tuple<Tensor, Tensor, OptTensor> gated_bwd(const Tensor &x, const Tensor &g
     if (want_state) dstate = f32(x, {a.sequences, a.D});
     a.dh = t3(dh); a.dx = t3(dx); a.dgate = t3(dgate); a.ckpt = fp(ckpt);
     a.dstate_out = fp(dend); a.dstate = fp(dstate);
-    check(lib.gated_bwd(&a, stream_of(x)));
+    check_native(lib.gated_bwd(&a, stream_of(x)));
     return {dx, dgate, dstate};
+}
+
+struct GatedScan : torch::autograd::Function<GatedScan> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &gate, const OptTensor &state,
+                                                  const OptTensor &cu) {
+        auto [h, end, xk, gk, cuk, ckpt] = gated_fwd(x, gate, state, cu, true);
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["state"] = state.has_value();
+        torch::autograd::variable_list kept{xk, gk, *ckpt};
+        if (cuk) {
+            kept.push_back(*cuk);
+        }
+        ctx->save_for_backward(std::move(kept));
+        return {h, end};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, const torch::autograd::variable_list &grads) {
+        const auto kept = ctx->get_saved_variables();
+        if (!grads[0].defined() && !grads[1].defined()) return torch::autograd::variable_list(4);
+        torch::autograd::variable_list out(4);
+        {
+            const c10::AutoGradMode off(false);
+            const Tensor &x = kept[0], dh = grads[0].defined() ? grads[0] : at::zeros({}, x.options()).expand(x.sizes());
+            const OptTensor cu = kept.size() > 3 ? OptTensor(kept[3]) : OptTensor(), dend = grads[1].defined() ? OptTensor(grads[1]) : OptTensor();
+            auto [dx, dgate, dstate] = gated_bwd(x, kept[1], cu, kept[2], dh, dend, ctx->saved_data["state"].toBool() && ctx->needs_input_grad(2));
+            out[0] = dx;
+            out[1] = dgate;
+            out[2] = dstate.value_or(Tensor());
+        }
+        return once(grads, std::move(out));
+    }
+};
+std::tuple<Tensor, Tensor> gated_scan(const Tensor &x, const Tensor &gate, const OptTensor &state, const OptTensor &cu) {
+    if (wants_grad({&x, &gate, state ? &*state : &x})) {
+        auto out = GatedScan::apply(x, gate, state, cu);
+        return {out[0], out[1]};
+    }
+    const auto out = gated_fwd(x, gate, state, cu, false);
+    return {std::get<0>(out), std::get<1>(out)};
 }
 
 // kla_b200_gated_step -> h, the new state (state_out where given)
@@ -761,15 +819,8 @@ kla_b200_mlp_args mlp_args(const Tensor &x, const Tensor &w12, const Tensor &w3,
 
 // x [rows, d] -> y [rows, out]; with `train` also what the backward takes: x, w12 and w3 as they were read, h, gate and up
 std::tuple<Tensor, OptTensor, OptTensor, OptTensor, OptTensor, OptTensor> mlp_fwd(
-    const Tensor &x_, const Tensor &w12_, const Tensor &w3_, const OptTensor &b12_, const OptTensor &b3_, const OptTensor &residual_,
-    const py::object &activation, bool train) {
+    const Tensor &x_, const Tensor &w12_, const Tensor &w3_, const OptTensor &b12_, const OptTensor &b3_, const OptTensor &residual_, int act, bool train) {
     if (!x_.is_cuda()) unsupported("The b200 gated feed-forward block needs CUDA tensors; x is on " + x_.device().str() + ".");
-    int act = 0;
-    try {
-        act = act_code(activation);
-    } catch (const std::exception &) {
-        throw py::value_error("kla_b200: activation is 'silu', 'gelu', 'relu' or None");
-    }
     require(x_.dim() == 2 && w12_.dim() == 2 && w3_.dim() == 2, "w12 and w3 are matrices, x has rows");
     const int64_t rows_n = x_.size(0), d = x_.size(1), H = w3_.size(1), out = w3_.size(0);
     require(w12_.size(0) == 2 * H && w12_.size(1) == d, "w12 is [2 H, d] for x [..., d] and w3 [out, H]");
@@ -812,11 +863,11 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor, OptTensor, OptTensor> mlp_fw
 
 // -> dx, dw12, dw3, db12, db3, each where wanted
 std::tuple<OptTensor, OptTensor, OptTensor, OptTensor, OptTensor> mlp_bwd(
-    const Tensor &dy_, const Tensor &x, const Tensor &w12, const Tensor &w3, const Tensor &h, const Tensor &gu, int64_t d, const py::object &activation,
-    const std::vector<bool> &want) {
+    const Tensor &dy_, const Tensor &x, const Tensor &w12, const Tensor &w3, const Tensor &h, const Tensor &gu, int64_t d, int act,
+    const std::array<bool, 5> &want) {
     const c10::cuda::CUDAGuard guard(x.device());
     const Tensor dy = tile_rows(dy_.scalar_type() == at::kBFloat16 ? dy_ : dy_.to(at::kBFloat16));
-    kla_b200_mlp_args a = mlp_args(x, w12, w3, act_code(activation));
+    kla_b200_mlp_args a = mlp_args(x, w12, w3, act);
     a.dy = dy.data_ptr(); a.dy_stride = row_stride(dy);
     a.h = h.data_ptr(); a.h_stride = h.size(1);
     a.gu = gu.data_ptr(); a.gu_stride = gu.size(1);
@@ -829,8 +880,53 @@ std::tuple<OptTensor, OptTensor, OptTensor, OptTensor, OptTensor> mlp_bwd(
     const Tensor work = fresh(x, {want[1] || want[2] || want[3] || want[4] ? (int64_t)lib.mlp_work_bytes(&a) : 0}, at::kByte);
     a.dgu = dgu.data_ptr();
     a.work = work.data_ptr();
-    check(lib.mlp_bwd(&a, stream_of(x)));
+    check_native(lib.mlp_bwd(&a, stream_of(x)));
     return {dx, dw12, dw3, db12, db3};
+}
+
+struct GatedMlp : torch::autograd::Function<GatedMlp> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &w12, const Tensor &w3, const OptTensor &b12, const OptTensor &b3,
+                          const OptTensor &residual, int64_t act) {
+        auto [y, xk, w12k, w3k, h, gu] = mlp_fwd(x, w12, w3, b12, b3, residual, (int)act, true);
+        ctx->save_for_backward({*xk, *w12k, *w3k, *h, *gu});
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["given"] = (int64_t)(b12.has_value() | b3.has_value() << 1 | residual.has_value() << 2);
+        return y;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, const torch::autograd::variable_list &grads) {
+        const auto kept = ctx->get_saved_variables();
+        const int64_t given = ctx->saved_data["given"].toInt();
+        // tensors that were not given have no place among the edges
+        std::array<bool, 6> want{ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2), false, false, false};
+        for (int i = 0, edge = 3; i < 3; ++i)
+            if (given >> i & 1) want[3 + i] = ctx->needs_input_grad(edge++);
+        torch::autograd::variable_list out(7);
+        const Tensor &dy = grads[0];
+        if (want[0] || want[1] || want[2] || want[3] || want[4]) {
+            const c10::AutoGradMode off(false);
+            auto got = mlp_bwd(dy, kept[0], kept[1], kept[2], kept[3], kept[4], kept[0].size(1), (int)ctx->saved_data["act"].toInt(),
+                               {want[0], want[1], want[2], want[3], want[4]});
+            out[0] = std::get<0>(got).value_or(Tensor());
+            out[1] = std::get<1>(got).value_or(Tensor());
+            out[2] = std::get<2>(got).value_or(Tensor());
+            out[3] = std::get<3>(got).value_or(Tensor());
+            out[4] = std::get<4>(got).value_or(Tensor());
+        }
+        out = once(grads, std::move(out));
+        if (want[5]) out[5] = dy;
+        return out;
+    }
+};
+// x [rows, d] -> y [rows, out]
+Tensor gated_mlp(const Tensor &x, const Tensor &w12, const Tensor &w3, const OptTensor &b12, const OptTensor &b3, const OptTensor &residual, const py::object &activation) {
+    int act = 0;
+    try {
+        act = act_code(activation);
+    } catch (const std::exception &) {
+        throw py::value_error("kla_b200: activation is 'silu', 'gelu', 'relu' or None");
+    }
+    if (wants_grad({&x, &w12, &w3, b12 ? &*b12 : &x, b3 ? &*b3 : &x, residual ? &*residual : &x})) return GatedMlp::apply(x, w12, w3, b12, b3, residual, (int64_t)act);
+    return std::get<0>(mlp_fwd(x, w12, w3, b12, b3, residual, act, false));
 }
 
 // ------------------------------------------------------------------------------------------ a token as one kernel
@@ -1195,10 +1291,8 @@ PYBIND11_MODULE(_kla_host, m) {
     m.def("conv_seq", &conv_seq);
     m.def("conv_seq_bwd", &conv_seq_bwd);
     m.def("rawscan", &rawscan);
-    m.def("mlp_fwd", &mlp_fwd);
-    m.def("mlp_bwd", &mlp_bwd);
-    m.def("gated_fwd", &gated_fwd);
-    m.def("gated_bwd", &gated_bwd);
+    m.def("gated_mlp", &gated_mlp);
+    m.def("gated_scan", &gated_scan);
     m.def("gated_step", &gated_step);
     m.def("step", &step);
     m.def("layer_step", &layer_step);

@@ -16,28 +16,6 @@ import torch
 from . import _lib
 
 
-class _GatedScanB200(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, gate, initial_state, cu_seqlens):
-        h, end, x, gate, cu, ckpt = _lib.host().gated_fwd(x, gate, initial_state, cu_seqlens, True)
-        ctx.set_materialize_grads(False)
-        ctx.packed, ctx.carried = cu is not None, initial_state is not None
-        ctx.save_for_backward(x, gate, ckpt, *((cu,) if cu is not None else ()))
-        return h, end
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dh, dend):
-        x, gate, ckpt, *rest = ctx.saved_tensors
-        if dh is None:
-            if dend is None:
-                return None, None, None, None
-            dh = torch.zeros((), device=x.device, dtype=x.dtype).expand(x.shape)
-        want_state = ctx.carried and ctx.needs_input_grad[2]
-        dx, dgate, dstate = _lib.host().gated_bwd(x, gate, rest[0] if ctx.packed else None, ckpt, dh, dend, want_state)
-        return dx, dgate, dstate, None
-
-
 def gated_scan_b200(x: torch.Tensor, gate: torch.Tensor, initial_state: torch.Tensor | None = None,
                     cu_seqlens: torch.Tensor | None = None):
     """``(h, state)``: ``h`` like ``x``, ``state`` float32 ``[sequences, D]``, the value behind every sequence's last step.
@@ -48,9 +26,7 @@ def gated_scan_b200(x: torch.Tensor, gate: torch.Tensor, initial_state: torch.Te
     ``cu_seqlens[n]`` to ``cu_seqlens[n + 1]``; the bounds must not decrease, which is not checked (values outside ``[0, L]``
     are clamped). A sequence without rows leaves the state it started from; rows that belong to no sequence get zeros, in
     ``h`` and in the gradients. Once a state is infinite the values after it are NaN."""
-    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (initial_state is not None and initial_state.requires_grad)):
-        return _GatedScanB200.apply(x, gate, initial_state, cu_seqlens)
-    return _lib.host().gated_fwd(x, gate, initial_state, cu_seqlens, False)[:2]
+    return _lib.host().gated_scan(x, gate, initial_state, cu_seqlens)
 
 
 def gated_step_b200(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, state_out: torch.Tensor | None = None):

@@ -17,25 +17,6 @@ import torch
 from . import _lib
 
 
-class _GatedMlpB200(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w12, w3, b12, b3, residual, activation):
-        y, *kept = _lib.host().mlp_fwd(x, w12, w3, b12, b3, residual, activation, True)
-        ctx.save_for_backward(*kept)
-        ctx.activation = activation
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, w12, w3, h, gu = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        grads = (None,) * 5
-        if any(need[:5]):
-            grads = _lib.host().mlp_bwd(dy, x, w12, w3, h, gu, x.shape[1], ctx.activation, list(need[:5]))
-        return (*grads, dy if need[5] else None, None)
-
-
 def gated_mlp_b200(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, b12: torch.Tensor | None = None, b3: torch.Tensor | None = None,
                    residual: torch.Tensor | None = None, activation: str | None = "silu") -> torch.Tensor:
     """``x`` ``[..., d]``, ``w12`` ``[2 H, d]`` (gate's rows, then up's), ``w3`` ``[out, H]``, ``b12`` ``[2 H]``, ``b3`` ``[out]``,
@@ -54,8 +35,5 @@ def gated_mlp_b200(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, b12: to
                 raise ValueError("kla_b200: residual has the output's shape")
             residual = residual.reshape(lead.numel(), residual.shape[-1])
         x = x.reshape(lead.numel(), x.shape[-1])
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w12, w3, b12, b3, residual)):
-        y = _GatedMlpB200.apply(x, w12, w3, b12, b3, residual, activation)
-    else:
-        y = _lib.host().mlp_fwd(x, w12, w3, b12, b3, residual, activation, False)[0]
+    y = _lib.host().gated_mlp(x, w12, w3, b12, b3, residual, activation)
     return y if lead is None else y.view(*lead, y.shape[-1])

@@ -215,6 +215,28 @@ def test_gradients_of_one_output_alone_and_of_broadcast_gradients():
 
 
 @pytest.mark.gpu
+def test_a_second_derivative_raises():
+    x = torch.randn(1, 20, 8, device="cuda").requires_grad_()
+    h, _ = kla_b200.gated_scan_b200(x, x * 2)
+    dx, = torch.autograd.grad(h.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
+
+
+@pytest.mark.gpu
+def test_only_the_gradients_that_are_wanted():
+    both, h0, dh, _ = (t.cuda() for t in inputs(2, 90, 64, 2, torch.float32))
+    x, g = both[..., :64], both[..., 64:]
+    full = None
+    for wanted in ((0, 1, 2), (0,), (1,), (2,)):
+        args = [t.detach().requires_grad_(i in wanted) for i, t in enumerate((x, g, h0))]
+        h, end = kla_b200.gated_scan_b200(*args)
+        got = dict(zip(wanted, torch.autograd.grad(h, [args[i] for i in wanted], dh)))
+        full = full or got
+        assert all(torch.equal(got[i], full[i]) for i in wanted)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("B,D", [(1, 1), (3, 65), (32, 2048)])
 def test_tokens_continue_a_prompt(B, D, dtype):

@@ -197,6 +197,16 @@ def test_only_the_gradients_that_are_wanted():
 
 
 @pytest.mark.gpu
+def test_a_second_derivative_raises():
+    t, _ = inputs(20, 16, 24, 16, residual=True)
+    x = t["x"].requires_grad_()
+    y = kla_b200.gated_mlp_b200(**t)
+    dx, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
+
+
+@pytest.mark.gpu
 def test_no_rows():
     t, dy = inputs(0, 16, 24, 16, bias=True)
     leaves = {n: v.detach().requires_grad_() for n, v in t.items() if v is not None}
@@ -366,4 +376,4 @@ def test_entry_points_reject_bad_arguments_without_cuda():
     assert L.kla_b200_mlp_fwd(A(y_stride=8), None) == 1 and L.kla_b200_mlp_fwd(A(residual=65, residual_stride=16), None) == 4
     assert L.kla_b200_mlp_bwd(A(work=None), None) == 1 and L.kla_b200_mlp_bwd(A(dw3=72), None) == 4 and L.kla_b200_mlp_bwd(A(dx_stride=8), None) == 1
     assert L.kla_b200_mlp_work_bytes(A(rows=0)) == 0 and L.kla_b200_mlp_work_bytes(None) == 0
-    assert L.kla_b200_mlp_work_bytes(A()) >= 4 * 2 * 24 * 16
+    assert L.kla_b200_mlp_work_bytes(A()) >= 4 * 2 * 24  # the row sums of gate's and up's gradients
