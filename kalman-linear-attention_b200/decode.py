@@ -23,6 +23,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
+from .mlp import gated_mlp_b200
 from .ops import kla_scan_b200
 
 CONFIG_KEYS = (
@@ -320,6 +321,9 @@ class ModelDecoder:
     off a reference model. The reference package is not needed at run time."""
 
     whole_gpu = None  # or True, False
+    # True: a prompt's swiglu MLP runs as ``gated_mlp_b200`` where it is bfloat16 (two kernels, gate and up never in memory), in place
+    # of two library GEMMs and a kernel between them; rounded in fewer places, so its results are other bits. @FIG@
+    fused_mlp = False
 
     def __init__(self, weights: dict, layer_configs, model_config: dict):
         missing = [k for k in MODEL_KEYS if k not in model_config]
@@ -368,6 +372,8 @@ class ModelDecoder:
     def _mlp(self, i, x):  # src/kla/layers/common.py:99-122
         pre = f"blocks.{i}.mlp."
         if self.cfg["mlp"] == "swiglu":
+            if self.fused_mlp and x.dtype == torch.bfloat16:
+                return gated_mlp_b200(x, self.w[pre + "w12.weight"], self.w[pre + "w3.weight"], self.w.get(pre + "w12.bias"), self.w.get(pre + "w3.bias"))
             h = _lib.host().swiglu(F.linear(x, self.w[pre + "w12.weight"], self.w.get(pre + "w12.bias")))
             return F.linear(h, self.w[pre + "w3.weight"], self.w.get(pre + "w3.bias"))
         return F.linear(F.gelu(F.linear(x, self.w[pre + "w1.weight"], self.w.get(pre + "w1.bias"))),
