@@ -45,23 +45,28 @@ struct Plan {
     int BN, CG, tiles_m, tiles_n, splits;
 };
 
-// Columns of a tile, CTAs sharing it and shares of the summed axis: the least time of the busiest CTA, counted in blocks of 128 x 256 x
-// 64 a CTA. A block of fewer columns costs more than its share, A being read all the same, and a CTA alone reads twice as much of B.
+// Columns of a tile, CTAs sharing it and shares of the summed axis: the least time (us) by what was measured on B200. A CTA spends
+// `block` on a 64-wide block of its tile with the GPU full (two CTAs with 256 columns 0.40, one 0.42; K=4096 N=1024 of 18944 rows) and
+// `fixed` on a launch, its first loads and its last epilogue (one block of 64 rows: pairs of CTAs 8.3, one CTA 6.2 to 7.7). Partial
+// sums are written, and read again by a kernel more.
 Plan plan(const Product &p, bool may_split, int sms) {
     const int64_t blocks = up(p.K, kMlpBK) * (p.a.halves == kHalvesSummed ? 2 : 1);
+    constexpr struct { int bn; double block[2], fixed[2]; } kinds[] = {
+        {256, {0.42, 0.40}, {7.5, 8.3}}, {192, {0.34, 0.32}, {6.7, 8.3}}, {128, {0.24, 0.25}, {6.2, 8.3}}, {64, {0.20, 0.215}, {6.2, 8.3}}};
     Plan best{};
     double least = 0.0;
     for (const int cg : {2, 1})
-        for (const int bn : {256, 192, 128, 64}) {
+        for (const auto &kind : kinds) {
+            const int bn = kind.bn;
             if (p.gated() && bn % 128) continue;
-            const double cost = (bn == 256 ? 1.0 : bn == 192 ? 0.78 : bn == 128 ? 0.62 : 0.5) * (cg == 1 ? 1.05 : 1.0);
             const int64_t tm = up(p.M, kMlpBM * cg) * (p.a.halves == kHalvesRows ? 2 : 1);
             const int64_t tn = up(p.N, p.gated() ? bn / 2 : bn), tiles = tm * tn;
             // shares of the summed axis up to four rounds of CTAs
             const int64_t most = may_split ? std::min<int64_t>({32, blocks, 1 + 4 * sms / (tiles * cg)}) : 1;
             for (int s = 1; s <= most; ++s) {
-                // a tile's end (the last epilogue, filling the ring) is about 4 blocks; partial sums are written and read again
-                const double t = (double)up(tiles * s, sms / cg) * (up(blocks, s) * cost + (s > 1 ? 1.0 : 0.0)) + 4.0 + (s > 1 ? 5.0 + 0.3 * s * tiles * cg / sms : 0.0);
+                const double sums = s > 1 ? 3.5 + 8e-6 * s * (double)tm * tn * kMlpBM * cg * bn / 4.0 : 0.0;
+                const double thin = p.gated() && bn == 128 ? 1.2 : 1.0;  // 64 columns of h leave half of the epilogue's warps idle
+                const double t = (double)up(tiles * s, sms / cg) * up(blocks, s) * kind.block[cg - 1] * thin + kind.fixed[cg - 1] + sums;
                 if (best.BN == 0 || t < least) { best = Plan{bn, cg, (int)tm, (int)tn, s}; least = t; }
             }
         }
@@ -91,6 +96,28 @@ int fill(MlpParams *prm, const Product &p, const Plan &pl) {
     prm->blocks_stretch = (int)up(p.K, kMlpBK);
     prm->blocks_k = prm->blocks_stretch * (p.a.halves == kHalvesSummed ? 2 : 1);
     return entry::wait_ctl(&prm->wait);
+}
+
+// A launch that may begin before the kernel in front of it has ended: the kernels wait (grid_dep_wait) before they touch memory.
+template <typename Params>
+int launch_behind(void (*kern)(Params), dim3 grid, unsigned threads, size_t smem, int cluster, cudaStream_t st, const Params &prm) {
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, prm);
+    if (e != cudaSuccess) return entry::cuda_fail(e);
+    entry::count_launch();
+    return KLA_B200_OK;
 }
 
 // CTA pairs that can be resident at once: SMs without a partner in their cluster of SMs take none.
@@ -141,21 +168,7 @@ int launch_as(const MlpParams &prm, cudaStream_t st) {
     const int64_t tiles = (int64_t)prm.tiles_m * prm.tiles_n * prm.splits;
     if (tiles > 0x3fffffffll) return KLA_B200_EUNSUPPORTED;
     const int64_t most = CG == 2 ? resident_pairs() : device_sms();
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = CG;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(tiles < most ? tiles : most) * CG);
-    cfg.blockDim = dim3(kMlpThreads);
-    cfg.dynamicSmemBytes = kMlpSmem;
-    cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = CG == 2 ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kla_mlp_kernel<MODE, CG>, prm);
-    if (e != cudaSuccess) return entry::cuda_fail(e);
-    entry::count_launch();
-    return KLA_B200_OK;
+    return launch_behind(kla_mlp_kernel<MODE, CG>, dim3((unsigned)(tiles < most ? tiles : most) * CG), kMlpThreads, kMlpSmem, CG, st, prm);
 }
 template <int MODE>
 int launch(const MlpParams &prm, const Plan &pl, cudaStream_t st) {
@@ -207,11 +220,7 @@ int weight_gradient(const Product &p, void *out, float *work, cudaStream_t st) {
     MlpReduceParams r{work, prm.partial_rows * prm.partial_stride, prm.partial_stride, pl.splits, (int)prm.partial_rows, (int)p.N,
                       static_cast<__nv_bfloat16 *>(out)};
     const int64_t grid = up(prm.partial_rows * up(p.N, 4), 256);
-    kla_mlp_reduce_kernel<<<(unsigned)grid, 256, 0, st>>>(r);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return entry::cuda_fail(e);
-    entry::count_launch();
-    return KLA_B200_OK;
+    return launch_behind(kla_mlp_reduce_kernel, dim3((unsigned)grid), 256, 0, 1, st, r);
 }
 
 // out[c] = sum over rows of x[r][c]; cols of `half` columns each twice (`half_gap` apart) where half > 0
@@ -224,13 +233,8 @@ int row_sums(const void *x, int64_t stride, int64_t rows, int64_t cols, int64_t 
     s.partial_stride = up(halves * cols, 8) * 8;
     s.out = static_cast<__nv_bfloat16 *>(out);
     s.total = (int)(halves * cols);
-    kla_mlp_rowsum_kernel<<<dim3((unsigned)(s.blocks * halves), (unsigned)s.stretches), 256, 0, st>>>(s);
-    kla_mlp_rowsum_end_kernel<<<(unsigned)up(s.total, 32), 256, 0, st>>>(s);
-    const cudaError_t err = cudaGetLastError();
-    if (err != cudaSuccess) return entry::cuda_fail(err);
-    entry::count_launch();
-    entry::count_launch();
-    return KLA_B200_OK;
+    if (const int rc = launch_behind(kla_mlp_rowsum_kernel, dim3((unsigned)(s.blocks * halves), (unsigned)s.stretches), 256, 0, 1, st, s)) return rc;
+    return launch_behind(kla_mlp_rowsum_end_kernel, dim3((unsigned)up(s.total, 32)), 256, 0, 1, st, s);
 }
 
 int check_sizes(const kla_b200_mlp_args *a) {

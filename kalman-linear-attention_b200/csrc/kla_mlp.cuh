@@ -450,6 +450,8 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
         mbar_init(drain, 1);
         *failed = 0;
         mbar_fence_init();
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&prm.map_a)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&prm.map_b)) : "memory");
     }
     if (warp == 2) {
         if constexpr (CG == 2) {
@@ -465,6 +467,9 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
     else __syncthreads();
     tcgen05_after_sync();
     const uint32_t tmem = *tmem_at;
+    // what stands above runs beside the end of the kernel in front (programmatic dependent launch); memory is touched from here on
+    grid_dep_launch();
+    grid_dep_wait();
     const int tiles = prm.tiles_m * prm.tiles_n * prm.splits;
     int issued = 0;  // producer: blocks whose loads were issued
 
@@ -717,7 +722,9 @@ struct MlpReduceParams {
     int splits, rows, cols;
     __nv_bfloat16 *out;              // [rows, cols] contiguous
 };
-__global__ void __launch_bounds__(256) kla_mlp_reduce_kernel(const MlpReduceParams prm) {
+__global__ void __launch_bounds__(256) kla_mlp_reduce_kernel(const __grid_constant__ MlpReduceParams prm) {
+    grid_dep_launch();
+    grid_dep_wait();
     const int quads = (prm.cols + 3) / 4;
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= (long long)prm.rows * quads) return;
@@ -752,8 +759,10 @@ struct MlpSumParams {
     long long partial_stride;
     __nv_bfloat16 *out;
 };
-__global__ void __launch_bounds__(256) kla_mlp_rowsum_kernel(const MlpSumParams prm) {
+__global__ void __launch_bounds__(256) kla_mlp_rowsum_kernel(const __grid_constant__ MlpSumParams prm) {
     __shared__ float part[8][kMlpSumCols];
+    grid_dep_launch();
+    grid_dep_wait();
     const int half = blockIdx.x / prm.blocks, c0 = (blockIdx.x - half * prm.blocks) * kMlpSumCols;
     const int g = threadIdx.x / 32, c = c0 + threadIdx.x % 32 * 8;
     const int r0 = blockIdx.y * prm.stretch_rows + g, r1 = min(prm.rows, ((int)blockIdx.y + 1) * prm.stretch_rows);
@@ -788,8 +797,10 @@ __global__ void __launch_bounds__(256) kla_mlp_rowsum_kernel(const MlpSumParams 
     }
 }
 // 32 columns a block, every eighth stretch a warp
-__global__ void __launch_bounds__(256) kla_mlp_rowsum_end_kernel(const MlpSumParams prm) {
+__global__ void __launch_bounds__(256) kla_mlp_rowsum_end_kernel(const __grid_constant__ MlpSumParams prm) {
     __shared__ float part[8][32];
+    grid_dep_launch();
+    grid_dep_wait();
     const int lane = threadIdx.x % 32, g = threadIdx.x / 32, c = blockIdx.x * 32 + lane;
     float s = 0.0f;
     if (c < prm.total)
