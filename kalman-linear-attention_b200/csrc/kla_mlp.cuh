@@ -407,6 +407,7 @@ __device__ __forceinline__ void mlp_slopes_chunk(uint32_t acc, const MlpStage &s
     }
 }
 
+constexpr int kMlpGroup = 8;
 struct MlpTile {
     int m, n, split;    // first row (of its half), first column (gated: of gate), share of the summed axis
     int m_half;
@@ -418,7 +419,10 @@ __device__ __forceinline__ MlpTile mlp_tile(const MlpParams &p, int t) {
     const int per = p.tiles_m * p.tiles_n;
     r.split = t / per;
     t -= r.split * per;
-    const int tm = t / p.tiles_n, tn = t - tm * p.tiles_n;
+    // tiles side by side in time are a block of tiles, so that their operands meet in L2: kMlpGroup rows of tiles, column after column
+    const int first = t / (kMlpGroup * p.tiles_n) * kMlpGroup, high = min(kMlpGroup, p.tiles_m - first);
+    t -= first * p.tiles_n;
+    const int tn = t / high, tm = first + t - tn * high;
     const int per_half = p.a.halves == kHalvesRows ? p.tiles_m / 2 : p.tiles_m;
     r.m_half = tm / per_half;
     r.m = (tm - r.m_half * per_half) * kMlpBM * CG;
