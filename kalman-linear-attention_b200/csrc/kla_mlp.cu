@@ -16,15 +16,16 @@ bool aligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % 
 bool rows_of_16(const void *p, int64_t stride) { return aligned(p, 16) && stride % 8 == 0; }
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
 
-// A [halves][outer][inner] bfloat16 tensor of boxes box_inner x box_outer in the 128-byte swizzle.
-int make_map(CUtensorMap *tm, const void *p, int64_t inner, int64_t outer, int64_t stride, int64_t halves, int64_t half_stride, int box_outer) {
+// A [halves][outer][inner] bfloat16 tensor of boxes box_inner (64, or 32 of a warp's stage) x box_outer, swizzled by a row of the box.
+int make_map(CUtensorMap *tm, const void *p, int64_t inner, int64_t outer, int64_t stride, int64_t halves, int64_t half_stride, int box_outer,
+             int box_inner = 64) {
     entry::EncodeTiledFn enc = entry::encode_tiled_fn();
     if (enc == nullptr) return KLA_B200_EUNSUPPORTED;
     const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)halves};
     const cuuint64_t strides[2] = {(cuuint64_t)stride * 2, (cuuint64_t)(halves > 1 ? half_stride : stride * outer) * 2};
-    const cuuint32_t box[3] = {64, (cuuint32_t)box_outer, 1}, ones[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer, 1}, ones[3] = {1, 1, 1};
     const CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                           box_inner == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? KLA_B200_OK : KLA_B200_EINVAL;
 }
 
@@ -275,8 +276,9 @@ int kla_b200_mlp_fwd(const kla_b200_mlp_args *a, void *stream) {
     if ((rc = fill(&prm, first, pl))) return rc;
     prm.act = a->activation;
     prm.bias = static_cast<const __nv_bfloat16 *>(a->b12);
-    prm.out = static_cast<__nv_bfloat16 *>(a->h); prm.out_stride = a->h_stride; prm.out_vec = 1;
-    prm.gu = static_cast<__nv_bfloat16 *>(a->gu); prm.gu_stride = a->gu_stride; prm.gu_half = a->gu_stride / 2;
+    if ((rc = make_map(&prm.map_out, a->h, a->H, a->rows, a->h_stride, 1, 0, 32, 32))) return rc;
+    prm.keeps = a->gu != nullptr;
+    if (prm.keeps && (rc = make_map(&prm.map_kept, a->gu, a->H, a->rows, a->gu_stride, 2, a->gu_stride / 2, 32, 32))) return rc;
     if ((rc = launch<kMlpGated>(prm, pl, st))) return rc;
     pl = plan(second, false, sms);
     if ((rc = fill(&prm, second, pl))) return rc;
@@ -331,7 +333,7 @@ int kla_b200_mlp_bwd(const kla_b200_mlp_args *a, void *stream) {
     if ((rc = fill(&prm, dgu, pl))) return rc;
     prm.act = a->activation;
     prm.side = static_cast<const __nv_bfloat16 *>(a->gu); prm.side_stride = a->gu_stride; prm.side_half = a->gu_stride / 2; prm.side_vec = 1;
-    prm.out = static_cast<__nv_bfloat16 *>(a->dgu); prm.out_stride = a->gu_stride; prm.out_half = a->gu_stride / 2; prm.out_vec = 1;
+    if ((rc = make_map(&prm.map_out, a->dgu, a->H, a->rows, a->gu_stride, 2, a->gu_stride / 2, 32, 32))) return rc;
     if ((rc = launch<kMlpGrad>(prm, pl, st))) return rc;
     if (a->dx != nullptr) {
         const Product dx = product_dx(*a);

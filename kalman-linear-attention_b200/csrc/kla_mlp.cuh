@@ -58,6 +58,7 @@ struct MlpOperand {
 
 struct MlpParams {
     CUtensorMap map_a, map_b;
+    CUtensorMap map_out, map_kept;  // gated: h, gate and up; grad: their gradients (map_out). Chunks of 32 columns by 32 rows
     MlpOperand a, b;
     int M, N, K;       // rows, columns (of one half where halves are rows), summed length (of one stretch)
     int BN;            // columns of a tile (gated: of gate and up together)
@@ -73,8 +74,7 @@ struct MlpParams {
     const __nv_bfloat16 *side;       // residual [M, N], grad: gate and up
     long long side_stride, side_half;
     int side_vec;
-    __nv_bfloat16 *gu;               // gated, training: gate and up, rows of gu_stride, up gu_half behind
-    long long gu_stride, gu_half;
+    int keeps;                       // gated, training: gate and up are kept (map_kept)
     float *partial;                  // [splits][M (both halves)][partial_stride]
     long long partial_stride, partial_rows;
     WaitCtl wait;
@@ -178,6 +178,19 @@ __device__ __forceinline__ void mlp_load(uint32_t on, uint32_t dst, uint64_t tm,
             "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
             " [%0], [%1, {%2, %3, %4}], [%5];\n}\n" ::"r"(dst), "l"(tm), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(on)
             : "memory");
+}
+// A warp's stage (32 rows of 32 columns, 64-byte swizzle) to memory by one lane's copy, which clips what lies outside; all lanes have
+// written their rows. The stage may be written again after mlp_stored.
+__device__ __forceinline__ void mlp_store(const CUtensorMap *tm, const void *stage, int x, int y, int z, int lane) {
+    if (lane == 0)
+        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z),
+                     "r"(smem_u32(stage))
+                     : "memory");
+}
+__device__ __forceinline__ void mlp_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void mlp_stored() {  // (lanes that issued nothing pass)
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
 }
 __device__ __forceinline__ void mlp_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -291,8 +304,8 @@ __device__ __forceinline__ float mlp_ex2(float x) {
     return y;
 }
 // The activation and its derivative. Which one is chosen once for 32 columns, not per element: with the choice (and gelu's error
-// function) inside the unrolled loops their code left the instruction cache, and the gated product took 288 us in place of @G@, the
-// one of the gradients 342 in place of @D@ (32768 rows of 768, H = 2048).
+// function) inside the unrolled loops their code left the instruction cache, and the gated product took 288 us in place of 193, the
+// one of the gradients 342 in place of 197 (32768 rows of 768, H = 2048).
 template <int ACT, bool SLOPE>
 __device__ __forceinline__ void mlp_act(float g, float &f, float &df) {
     if (ACT == 1) {  // gelu
@@ -615,6 +628,7 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
                 };
                 __nv_bfloat16 *out = prm.out + tl.m_half * prm.out_half + (long long)m * prm.out_stride + n;
                 if constexpr (MODE == kMlpGrad) {
+                    mlp_stored();  // of the chunk before
                     st.put_fetched(f1);
                     st2.put_fetched(f2);
                     __syncwarp();
@@ -624,31 +638,42 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
                     else if (prm.act == 2) mlp_slopes_chunk<2>(d + c, st, st2);
                     else mlp_slopes_chunk<3>(d + c, st, st2);
                     done();
+                    fence_proxy_async();
                     __syncwarp();
-                    st.store(out, prm.out_stride, rows, cols, true);
-                    st2.store(out + prm.out_half, prm.out_stride, rows, cols, true);
-                    __syncwarp();
+                    if (cols > 0 && rows > 0) {
+                        mlp_store(&prm.map_out, st.base, n, m, 0, lane);
+                        mlp_store(&prm.map_out, st2.base, n, m, 1, lane);
+                    }
+                    mlp_store_commit();
                     continue;
                 }
                 const __nv_bfloat16 *bias = prm.bias != nullptr ? prm.bias + n : nullptr;
                 if constexpr (MODE == kMlpGated) {
                     uint4 h[4];
-                    const bool keeps = prm.gu != nullptr;
+                    const bool keeps = prm.keeps != 0;
+                    mlp_stored();
                     if (prm.act == 0) mlp_gated_chunk<0>(d + c, d + width + c, bias, prm.N, cols, keeps, st, st2, h);
                     else if (prm.act == 1) mlp_gated_chunk<1>(d + c, d + width + c, bias, prm.N, cols, keeps, st, st2, h);
                     else if (prm.act == 2) mlp_gated_chunk<2>(d + c, d + width + c, bias, prm.N, cols, keeps, st, st2, h);
                     else mlp_gated_chunk<3>(d + c, d + width + c, bias, prm.N, cols, keeps, st, st2, h);
                     done();
+                    const bool some = rows > 0;
                     if (keeps) {
-                        __nv_bfloat16 *gu = prm.gu + (long long)m * prm.gu_stride + n;
+                        fence_proxy_async();
                         __syncwarp();
-                        st.store(gu, prm.gu_stride, rows, cols, true);
-                        st2.store(gu + prm.gu_half, prm.gu_stride, rows, cols, true);
-                        __syncwarp();
+                        if (some) {
+                            mlp_store(&prm.map_kept, st.base, n, m, 0, lane);
+                            mlp_store(&prm.map_kept, st2.base, n, m, 1, lane);
+                        }
+                        mlp_store_commit();
+                        mlp_stored();
                     }
                     st.put_row(h);
+                    fence_proxy_async();
                     __syncwarp();
-                    st.store(out, prm.out_stride, rows, cols, prm.out_vec);
+                    if (some) mlp_store(&prm.map_out, st.base, n, m, 0, lane);
+                    mlp_store_commit();
+                    continue;
                 } else if constexpr (MODE == kMlpPartial) {
                     // four of a row's 16-byte pieces in either stage
                     mlp_pieces<false>(d + c, 0u, [&](int i, float2 (&x)[4], float2 (&)[4]) {
@@ -689,6 +714,7 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
             }
         }
     }
+    if (MODE == kMlpGated || MODE == kMlpGrad) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // own stores are done
     __syncwarp();
     if constexpr (CG == 2) mlp_cluster_sync();
     else __syncthreads();
