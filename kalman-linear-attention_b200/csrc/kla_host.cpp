@@ -649,6 +649,11 @@ void unsupported(const std::string &what) {
     PyErr_SetString(PyExc_NotImplementedError, what.c_str());
     throw py::error_already_set();
 }
+// Forward-mode tangents would be dropped.
+void no_tangents(std::initializer_list<const Tensor *> ts) {
+    for (const Tensor *t : ts)
+        if (t->_fw_grad(0).defined()) unsupported("The b200 kernels have no forward-mode derivative; use torch operations for it.");
+}
 // x and gate of the gated recurrence: one shape, type and device the kernels take.
 void check_gated(const Tensor &x, const Tensor &gate, int64_t dims) {
     if (!x.is_cuda() || !gate.is_cuda()) unsupported("The b200 gated recurrence needs CUDA tensors; x is on " + x.device().str() + ", gate on " + gate.device().str() + ".");
@@ -761,6 +766,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
     }
 };
 std::tuple<Tensor, Tensor> gated_scan(const Tensor &x, const Tensor &gate, const OptTensor &state, const OptTensor &cu) {
+    no_tangents({&x, &gate, state ? &*state : &x});
     if (wants_grad({&x, &gate, state ? &*state : &x})) {
         auto out = GatedScan::apply(x, gate, state, cu);
         return {out[0], out[1]};
@@ -772,6 +778,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor &x, const Tensor &gate, const
 // kla_b200_gated_step -> h, the new state (state_out where given)
 std::tuple<Tensor, Tensor> gated_step(const Tensor &x_, const Tensor &gate_, const Tensor &state_, const OptTensor &out) {
     check_gated(x_, gate_, 2);
+    no_tangents({&x_, &gate_, &state_});
     const c10::cuda::CUDAGuard guard(x_.device());
     const Tensor x = rows(x_), gate = rows(gate_);
     const int64_t B = x.size(0), D = x.size(1);
@@ -836,7 +843,8 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor, OptTensor, OptTensor> mlp_fw
     if (!sm100(x_.device())) unsupported("The b200 kernels need an sm_100 device.");
     const c10::cuda::CUDAGuard guard(x_.device());
     const OptTensor b12 = b12_ ? OptTensor(b12_->contiguous()) : b12_, b3 = b3_ ? OptTensor(b3_->contiguous()) : b3_;
-    const OptTensor residual = residual_ ? OptTensor(rows(*residual_)) : residual_;
+    OptTensor residual = residual_ ? OptTensor(rows(*residual_)) : residual_;
+    if (residual && rows_n > 1 && residual->stride(0) < out) residual = residual->contiguous();  // rows that share memory
     if (!train && act == KLA_B200_ACT_SILU && few_rows(x_, w12_, b12, {}) && kernel_pays(rows_n, 2 * H, d) && out < kWidePlain && kernel_pays(rows_n, out, H) && H % 8 == 0) {
         // a token: the projections of the decode kernels, which read the weights once with all SMs
         const OptTensor none;
@@ -925,6 +933,7 @@ Tensor gated_mlp(const Tensor &x, const Tensor &w12, const Tensor &w3, const Opt
     } catch (const std::exception &) {
         throw py::value_error("kla_b200: activation is 'silu', 'gelu', 'relu' or None");
     }
+    no_tangents({&x, &w12, &w3, b12 ? &*b12 : &x, b3 ? &*b3 : &x, residual ? &*residual : &x});
     if (wants_grad({&x, &w12, &w3, b12 ? &*b12 : &x, b3 ? &*b3 : &x, residual ? &*residual : &x})) return GatedMlp::apply(x, w12, w3, b12, b3, residual, (int64_t)act);
     return std::get<0>(mlp_fwd(x, w12, w3, b12, b3, residual, act, false));
 }

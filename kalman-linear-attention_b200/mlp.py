@@ -22,9 +22,13 @@ def gated_mlp_b200(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, b12: to
     """``x`` ``[..., d]``, ``w12`` ``[2 H, d]`` (gate's rows, then up's), ``w3`` ``[out, H]``, ``b12`` ``[2 H]``, ``b3`` ``[out]``,
     ``residual`` ``[..., out]`` added to the result in float32 before it is rounded. ``activation``: ``"silu"``, ``"gelu"`` (the exact
     one), ``"relu"`` or None. Any sizes and strides: rows that are not 16-byte aligned (a width that is no multiple of 8) are copied
-    first. Under a bfloat16 autocast other floating types of ``x``, weights and biases are converted as ``F.linear`` does."""
+    first. Under a bfloat16 autocast float32 and float16 ``x``, weights and biases are converted as ``F.linear`` does.
+
+    A call that is to be differentiated keeps ``x``, the weights and three ``[rows, H]`` tensors of 16 bits for the backward: the
+    product, and gate and up with nine bits of mantissa over 2^-31 to 2^33 (beyond, their gradients are NaN)."""
     if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:
-        x, w12, w3, b12, b3 = (t.to(torch.bfloat16) if t is not None and t.is_cuda else t for t in (x, w12, w3, b12, b3))
+        x, w12, w3, b12, b3 = (t.to(torch.bfloat16) if t is not None and t.is_cuda and t.dtype in (torch.float32, torch.float16) else t
+                               for t in (x, w12, w3, b12, b3))
     lead = None
     if x.dim() != 2:
         if x.dim() == 0:

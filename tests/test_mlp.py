@@ -207,6 +207,35 @@ def test_a_second_derivative_raises():
 
 
 @pytest.mark.gpu
+def test_a_broadcast_residual():
+    t, dy = inputs(40, 64, 72, 64)
+    row = torch.randn(64, device="cuda").bfloat16().requires_grad_()
+    t["residual"] = row.expand(40, 64)
+    want = oracle(*(t[n] for n in NAMES), "silu", dy)
+    y = kla_b200.gated_mlp_b200(**t)
+    held(y, want["y"], "y")
+    got, = torch.autograd.grad(y, row, dy)
+    assert torch.equal(got, torch.autograd.grad(row.expand(40, 64), row, dy)[0])
+
+
+@pytest.mark.gpu
+def test_forward_mode_tangents_are_refused_not_dropped():
+    from torch.autograd import forward_ad
+
+    t, _ = inputs(8, 16, 24, 16)
+    x = torch.randn(1, 8, 16, device="cuda")
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(t["w3"], torch.ones_like(t["w3"]))
+        with pytest.raises(NotImplementedError):
+            kla_b200.gated_mlp_b200(**{**t, "w3": dual})
+        gate = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError):
+            kla_b200.gated_scan_b200(x, gate)
+        with pytest.raises(NotImplementedError):
+            kla_b200.gated_step_b200(x[0], gate[0], x[0].clone())
+
+
+@pytest.mark.gpu
 def test_no_rows():
     t, dy = inputs(0, 16, 24, 16, bias=True)
     leaves = {n: v.detach().requires_grad_() for n, v in t.items() if v is not None}
