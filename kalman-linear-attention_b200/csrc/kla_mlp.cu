@@ -194,16 +194,29 @@ Product product_dw12(const kla_b200_mlp_args &a) {
 }
 
 int64_t weight_rows(const Product &p) { return p.M * (p.a.halves == kHalvesRows ? 2 : 1); }
-size_t partial_bytes(const Product &p, int sms) {
+int64_t partial_words(const Product &p, int sms) {
     const int splits = plan(p, true, sms).splits;
-    return splits > 1 ? (size_t)splits * weight_rows(p) * up(p.N, 4) * 4 * sizeof(float) : 0;
+    return splits > 1 ? splits * weight_rows(p) * up(p.N, 4) * 4 : 0;
 }
 // rows of a stretch of the row sums: at least eight a warp, and no more than 1024 stretches
 int64_t sum_rows(int64_t rows) { return std::max<int64_t>(64, up(rows, 1024 * 8) * 8); }
-size_t sum_bytes(int64_t rows, int64_t cols) { return (size_t)up(rows, sum_rows(rows)) * up(cols, 8) * 8 * sizeof(float); }
 
-// The gradient of a weight: in one go, or partial sums of shares of the rows and then their sum.
-int weight_gradient(const Product &p, void *out, float *work, cudaStream_t st) {
+// The working memory of a backward, in words: partial sums of dW3 and dW12, of db3 and db12.
+struct Work {
+    int64_t w12, b3, b12, all;  // where they begin (dW3's at 0)
+};
+Work work_of(const kla_b200_mlp_args &a, int sms) {
+    const int64_t stretches = up(a.rows, sum_rows(a.rows));
+    Work w;
+    w.w12 = partial_words(product_dw3(a), sms);
+    w.b3 = w.w12 + partial_words(product_dw12(a), sms);
+    w.b12 = w.b3 + stretches * a.out;
+    w.all = w.b12 + stretches * 2 * a.H;
+    return w;
+}
+
+// The gradient of a weight: in one go, or partial sums of shares of the rows, to be added by the end's kernel.
+int weight_gradient(const Product &p, void *out, float *work, MlpReduce *end, cudaStream_t st) {
     const Plan pl = plan(p, true, device_sms());
     MlpParams prm;
     if (const int rc = fill(&prm, p, pl)) return rc;
@@ -217,25 +230,15 @@ int weight_gradient(const Product &p, void *out, float *work, cudaStream_t st) {
     prm.partial = work;
     prm.partial_stride = up(p.N, 4) * 4;
     prm.partial_rows = weight_rows(p);
-    if (const int rc = launch<kMlpPartial>(prm, pl, st)) return rc;
-    MlpReduceParams r{work, prm.partial_rows * prm.partial_stride, prm.partial_stride, pl.splits, (int)prm.partial_rows, (int)p.N,
-                      static_cast<__nv_bfloat16 *>(out)};
-    const int64_t grid = up(prm.partial_rows * up(p.N, 4), 256);
-    return launch_behind(kla_mlp_reduce_kernel, dim3((unsigned)grid), 256, 0, 1, st, r);
+    *end = MlpReduce{work, prm.partial_rows * prm.partial_stride, prm.partial_stride, pl.splits, (int)prm.partial_rows, (int)p.N,
+                     (int)up(prm.partial_rows * up(p.N, 4), 256), static_cast<__nv_bfloat16 *>(out)};
+    return launch<kMlpPartial>(prm, pl, st);
 }
 
-// out[c] = sum over rows of x[r][c]; cols of `half` columns each twice (`half_gap` apart) where half > 0
-int row_sums(const void *x, int64_t stride, int64_t rows, int64_t cols, int64_t half_gap, int halves, float *work, void *out, cudaStream_t st) {
-    MlpSumParams s{};
-    s.x = static_cast<const __nv_bfloat16 *>(x);
-    s.stride = stride; s.half_gap = half_gap; s.rows = (int)rows; s.cols = (int)cols;
-    s.blocks = (int)up(cols, kMlpSumCols); s.stretch_rows = (int)sum_rows(rows); s.stretches = (int)up(rows, s.stretch_rows);
-    s.partial = work;
-    s.partial_stride = up(halves * cols, 8) * 8;
-    s.out = static_cast<__nv_bfloat16 *>(out);
-    s.total = (int)(halves * cols);
-    if (const int rc = launch_behind(kla_mlp_rowsum_kernel, dim3((unsigned)(s.blocks * halves), (unsigned)s.stretches), 256, 0, 1, st, s)) return rc;
-    return launch_behind(kla_mlp_rowsum_end_kernel, dim3((unsigned)up(s.total, 32)), 256, 0, 1, st, s);
+MlpSum sum_of(const void *x, int64_t stride, int64_t cols, int64_t half_gap, int halves, float *work, void *out) {
+    const int half_blocks = (int)up(cols, kMlpSumCols);
+    return MlpSum{static_cast<const __nv_bfloat16 *>(x), stride, half_gap, (int)cols, half_blocks, halves * half_blocks, (int)(halves * cols), work,
+                  static_cast<__nv_bfloat16 *>(out)};
 }
 
 int check_sizes(const kla_b200_mlp_args *a) {
@@ -291,10 +294,7 @@ int kla_b200_mlp_fwd(const kla_b200_mlp_args *a, void *stream) {
 
 size_t kla_b200_mlp_work_bytes(const kla_b200_mlp_args *a) {
     if (check_sizes(a) || a->rows == 0) return 0;
-    const int sms = device_sms();
-    size_t n = partial_bytes(product_dw3(*a), sms);
-    for (const size_t m : {partial_bytes(product_dw12(*a), sms), sum_bytes(a->rows, 2 * a->H), sum_bytes(a->rows, a->out)}) n = m > n ? m : n;
-    return n;
+    return (size_t)work_of(*a, device_sms()).all * sizeof(float);
 }
 
 int kla_b200_mlp_bwd(const kla_b200_mlp_args *a, void *stream) {
@@ -324,27 +324,43 @@ int kla_b200_mlp_bwd(const kla_b200_mlp_args *a, void *stream) {
     if ((a->dw12 || a->dw3 || a->db12 || a->db3) && a->work == nullptr) return KLA_B200_EINVAL;
     const int sms = device_sms();
     float *work = static_cast<float *>(a->work);
+    const Work at = work_of(*a, sms);
     MlpParams prm;
-    if (a->dw3 != nullptr && (rc = weight_gradient(product_dw3(*a), a->dw3, work, st))) return rc;
-    if (a->db3 != nullptr && (rc = row_sums(a->dy, a->dy_stride, a->rows, a->out, 0, 1, work, a->db3, st))) return rc;
-    if (!inner) return KLA_B200_OK;
-    const Product dgu = product_dgu(*a);
-    Plan pl = plan(dgu, false, sms);
-    if ((rc = fill(&prm, dgu, pl))) return rc;
-    prm.act = a->activation;
-    prm.side = static_cast<const __nv_bfloat16 *>(a->gu); prm.side_stride = a->gu_stride; prm.side_half = a->gu_stride / 2; prm.side_vec = 1;
-    if ((rc = make_map(&prm.map_out, a->dgu, a->H, a->rows, a->gu_stride, 2, a->gu_stride / 2, 32, 32))) return rc;
-    if ((rc = launch<kMlpGrad>(prm, pl, st))) return rc;
-    if (a->dx != nullptr) {
-        const Product dx = product_dx(*a);
-        pl = plan(dx, false, sms);
-        if ((rc = fill(&prm, dx, pl))) return rc;
-        prm.out = static_cast<__nv_bfloat16 *>(a->dx); prm.out_stride = a->dx_stride; prm.out_vec = rows_of_16(a->dx, a->dx_stride);
-        if ((rc = launch<kMlpPlain>(prm, pl, st))) return rc;
+    MlpEndParams end{};
+    MlpSumParams sums{};
+    if (a->dw3 != nullptr && (rc = weight_gradient(product_dw3(*a), a->dw3, work, &end.weight[0], st))) return rc;
+    if (inner) {
+        const Product dgu = product_dgu(*a);
+        Plan pl = plan(dgu, false, sms);
+        if ((rc = fill(&prm, dgu, pl))) return rc;
+        prm.act = a->activation;
+        prm.side = static_cast<const __nv_bfloat16 *>(a->gu); prm.side_stride = a->gu_stride; prm.side_half = a->gu_stride / 2; prm.side_vec = 1;
+        if ((rc = make_map(&prm.map_out, a->dgu, a->H, a->rows, a->gu_stride, 2, a->gu_stride / 2, 32, 32))) return rc;
+        if ((rc = launch<kMlpGrad>(prm, pl, st))) return rc;
+        if (a->dx != nullptr) {
+            const Product dx = product_dx(*a);
+            pl = plan(dx, false, sms);
+            if ((rc = fill(&prm, dx, pl))) return rc;
+            prm.out = static_cast<__nv_bfloat16 *>(a->dx); prm.out_stride = a->dx_stride; prm.out_vec = rows_of_16(a->dx, a->dx_stride);
+            if ((rc = launch<kMlpPlain>(prm, pl, st))) return rc;
+        }
+        if (a->dw12 != nullptr && (rc = weight_gradient(product_dw12(*a), a->dw12, work + at.w12, &end.weight[1], st))) return rc;
     }
-    if (a->dw12 != nullptr && (rc = weight_gradient(product_dw12(*a), a->dw12, work, st))) return rc;
-    if (a->db12 != nullptr) return row_sums(a->dgu, a->gu_stride, a->rows, a->H, a->gu_stride / 2, 2, work, a->db12, st);
-    return KLA_B200_OK;
+    if (a->db3 != nullptr) sums.of[0] = sum_of(a->dy, a->dy_stride, a->out, 0, 1, work + at.b3, a->db3);
+    if (a->db12 != nullptr) sums.of[1] = sum_of(a->dgu, a->gu_stride, a->H, a->gu_stride / 2, 2, work + at.b12, a->db12);
+    const int sum_blocks = sums.of[0].blocks + sums.of[1].blocks;
+    if (sum_blocks > 0) {
+        sums.rows = (int)a->rows;
+        sums.stretch_rows = (int)sum_rows(a->rows);
+        end.stretches = (int)up(a->rows, sums.stretch_rows);
+        if ((rc = launch_behind(kla_mlp_rowsum_kernel, dim3((unsigned)sum_blocks, (unsigned)end.stretches), 256, 0, 1, st, sums))) return rc;
+    }
+    end.bias[0] = sums.of[0];
+    end.bias[1] = sums.of[1];
+    end.weight[1].blocks += end.weight[0].blocks;
+    end.bias_blocks = end.weight[1].blocks + (int)up(end.bias[0].total, 32);
+    const int64_t blocks = end.bias_blocks + up(end.bias[1].total, 32);
+    return blocks > 0 ? launch_behind(kla_mlp_end_kernel, dim3((unsigned)blocks), 256, 0, 1, st, end) : KLA_B200_OK;
 }
 
 }  // extern "C"

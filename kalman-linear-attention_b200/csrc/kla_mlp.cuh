@@ -745,63 +745,36 @@ __global__ void __launch_bounds__(kMlpThreads, 1) kla_mlp_kernel(const __grid_co
     }
 }
 
-// out[r][c] = sum over splits, in their order, of partial[split][r][c]; four columns a thread.
-struct MlpReduceParams {
-    const float *partial;
-    long long split_stride, stride;  // elements; stride a multiple of 4
-    int splits, rows, cols;
-    __nv_bfloat16 *out;              // [rows, cols] contiguous
-};
-__global__ void __launch_bounds__(256) kla_mlp_reduce_kernel(const __grid_constant__ MlpReduceParams prm) {
-    grid_dep_launch();
-    grid_dep_wait();
-    const int quads = (prm.cols + 3) / 4;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (long long)prm.rows * quads) return;
-    const long long r = i / quads;
-    const int c = (int)(i - r * quads) * 4;
-    const float *p = prm.partial + r * prm.stride + c;
-    float4 s = *reinterpret_cast<const float4 *>(p);
-    for (int k = 1; k < prm.splits; ++k) {
-        const float4 v = *reinterpret_cast<const float4 *>(p + k * prm.split_stride);
-        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-    }
-    __nv_bfloat16 *out = prm.out + r * prm.cols + c;
-    const float v[4] = {s.x, s.y, s.z, s.w};
-    if (prm.cols % 4 == 0) {
-        *reinterpret_cast<uint2 *>(out) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c + e < prm.cols) out[e] = __float2bfloat16_rn(v[e]);
-    }
-}
-
-// Sums over rows of a bfloat16 matrix (a bias's gradient) whose rows are 16-byte aligned: a block adds 256 columns of a stretch of
-// rows, eight rows side by side and eight columns a thread by one access; the sums of the stretches, float32 [stretches][total], are
-// added by a second kernel in their order. Of gate and up, whose halves lie half_gap apart, in one go.
+// Sums over rows of bfloat16 matrices (the biases' gradients) whose rows are 16-byte aligned: a block adds 256 columns of a stretch of
+// rows, eight rows side by side and eight columns a thread by one access, into float32 [stretches][total]. `blocks` blocks of columns
+// are of the first matrix, the others of the second (gate's and up's gradients are one matrix of two halves half_gap apart).
 constexpr int kMlpSumCols = 256;
-struct MlpSumParams {
+struct MlpSum {
     const __nv_bfloat16 *x;
     long long stride, half_gap;
-    int rows, cols, blocks, stretch_rows, stretches, total;
+    int cols, half_blocks, blocks, total;  // cols, half_blocks: of one half; blocks, total: of all
     float *partial;
-    long long partial_stride;
     __nv_bfloat16 *out;
+};
+struct MlpSumParams {
+    MlpSum of[2];
+    int rows, stretch_rows;
 };
 __global__ void __launch_bounds__(256) kla_mlp_rowsum_kernel(const __grid_constant__ MlpSumParams prm) {
     __shared__ float part[8][kMlpSumCols];
     grid_dep_launch();
     grid_dep_wait();
-    const int half = blockIdx.x / prm.blocks, c0 = (blockIdx.x - half * prm.blocks) * kMlpSumCols;
+    const bool second = (int)blockIdx.x >= prm.of[0].blocks;
+    const MlpSum &m = prm.of[second];
+    const int bx = blockIdx.x - (second ? prm.of[0].blocks : 0), half = bx / m.half_blocks, c0 = (bx - half * m.half_blocks) * kMlpSumCols;
     const int g = threadIdx.x / 32, c = c0 + threadIdx.x % 32 * 8;
     const int r0 = blockIdx.y * prm.stretch_rows + g, r1 = min(prm.rows, ((int)blockIdx.y + 1) * prm.stretch_rows);
-    const __nv_bfloat16 *x = prm.x + half * prm.half_gap + c;
+    const __nv_bfloat16 *x = m.x + half * m.half_gap + c;
     float s[8] = {};
-    if (c + 8 <= prm.cols) {
+    if (c + 8 <= m.cols) {
 #pragma unroll 8
         for (int r = r0; r < r1; r += 8) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(x + r * prm.stride));
+            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(x + r * m.stride));
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -813,35 +786,76 @@ __global__ void __launch_bounds__(256) kla_mlp_rowsum_kernel(const __grid_consta
         for (int r = r0; r < r1; r += 8)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (c + e < prm.cols) s[e] += __bfloat162float(x[r * prm.stride + e]);
+                if (c + e < m.cols) s[e] += __bfloat162float(x[r * m.stride + e]);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) part[g][threadIdx.x % 32 * 8 + e] = s[e];
     __syncthreads();
     const int col = c0 + threadIdx.x;
-    if (col < prm.cols) {
+    if (col < m.cols) {
         float t = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) t += part[i][threadIdx.x];
-        prm.partial[blockIdx.y * prm.partial_stride + half * prm.cols + col] = t;
+        m.partial[(long long)blockIdx.y * m.total + half * m.cols + col] = t;
     }
 }
-// 32 columns a block, every eighth stretch a warp
-__global__ void __launch_bounds__(256) kla_mlp_rowsum_end_kernel(const __grid_constant__ MlpSumParams prm) {
-    __shared__ float part[8][32];
+
+// The end of a backward, one launch for all: the partial sums of the weights' gradients, four columns a thread, and those of the
+// biases', 32 columns a block and every eighth stretch a warp; each in a fixed order.
+struct MlpReduce {
+    const float *partial;
+    long long split_stride, stride;  // elements; stride a multiple of 4
+    int splits, rows, cols, blocks;  // blocks: of the grid, up to this one's last
+    __nv_bfloat16 *out;              // [rows, cols] contiguous
+};
+struct MlpEndParams {
+    MlpReduce weight[2];
+    MlpSum bias[2];
+    int bias_blocks, stretches;      // bias_blocks: of the grid, up to the first bias's last
+};
+__global__ void __launch_bounds__(256) kla_mlp_end_kernel(const __grid_constant__ MlpEndParams prm) {
     grid_dep_launch();
     grid_dep_wait();
-    const int lane = threadIdx.x % 32, g = threadIdx.x / 32, c = blockIdx.x * 32 + lane;
+    const int block = blockIdx.x;
+    if (block < prm.weight[1].blocks) {
+        const bool second = block >= prm.weight[0].blocks;
+        const MlpReduce &w = prm.weight[second];
+        const int quads = (w.cols + 3) / 4;
+        const long long i = (long long)(block - (second ? prm.weight[0].blocks : 0)) * 256 + threadIdx.x;
+        if (i >= (long long)w.rows * quads) return;
+        const long long r = i / quads;
+        const int c = (int)(i - r * quads) * 4;
+        const float *p = w.partial + r * w.stride + c;
+        float4 s = *reinterpret_cast<const float4 *>(p);
+        for (int k = 1; k < w.splits; ++k) {
+            const float4 v = *reinterpret_cast<const float4 *>(p + k * w.split_stride);
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+        __nv_bfloat16 *out = w.out + r * w.cols + c;
+        const float v[4] = {s.x, s.y, s.z, s.w};
+        if (w.cols % 4 == 0) {
+            *reinterpret_cast<uint2 *>(out) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < w.cols) out[e] = __float2bfloat16_rn(v[e]);
+        }
+        return;
+    }
+    __shared__ float part[8][32];
+    const bool second = block >= prm.bias_blocks;
+    const MlpSum &b = prm.bias[second];
+    const int lane = threadIdx.x % 32, g = threadIdx.x / 32, c = (block - (second ? prm.bias_blocks : prm.weight[1].blocks)) * 32 + lane;
     float s = 0.0f;
-    if (c < prm.total)
+    if (c < b.total)
 #pragma unroll 4
-        for (int k = g; k < prm.stretches; k += 8) s += prm.partial[k * prm.partial_stride + c];
+        for (int k = g; k < prm.stretches; k += 8) s += b.partial[(long long)k * b.total + c];
     part[g][lane] = s;
     __syncthreads();
-    if (g == 0 && c < prm.total) {
+    if (g == 0 && c < b.total) {
 #pragma unroll
         for (int i = 1; i < 8; ++i) s += part[i][lane];
-        prm.out[c] = __float2bfloat16_rn(s);
+        b.out[c] = __float2bfloat16_rn(s);
     }
 }
 
