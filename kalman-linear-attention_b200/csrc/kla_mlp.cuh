@@ -12,10 +12,18 @@
 // An operand whose summed axis is not the adjacent one in memory (W3, W12, and both of a weight's gradient) is read as it is, as
 // an MN-major operand of the tensor core; nothing is transposed in memory.
 //
-// A CTA per SM walks output tiles of 128 x BN. One warp issues TMA loads of 64-wide blocks of the summed axis into a ring of
-// blocks, one thread issues tcgen05.mma from them into one of two accumulators in tensor memory, eight warps empty the
-// other accumulator meanwhile, through a stage of shared memory that turns a thread's row into coalesced 64-byte pieces.
-// Rows and columns past the ends are zeros of the TMA loads; widths that are no multiple of a tile cost only the padding.
+// A CTA (or a pair of them, which share a tile of 256 rows and each hold half of B's) walks output tiles of 128 x BN. One warp
+// issues TMA loads of 64-wide blocks of the summed axis into a ring of blocks, one issues tcgen05.mma from them into one of two
+// accumulators in tensor memory, sixteen warps empty the other accumulator meanwhile, through stages of shared memory that TMA
+// stores empty. Rows and columns past the ends are zeros of the TMA loads and left out by its stores; widths that are no multiple
+// of a tile cost only the padding.
+//
+// What bounds it: 18 M D H operations forward and backward together for M rows, and for few rows the weights, once from memory. Measured
+// at 32768 rows of 768 with H = 2048, forward and backward together 922 us of 556 at the rate of a library product in a burst of its
+// own (1668 TFLOP/s) and 670 at the rate such products hold for seconds under the power limit (1384); by product gate and up
+// 141 us (1459 TFLOP/s, with gate and up kept 175), down 70, dh and with it dg and du 157, dx 137, dW12 127, dW3 68. The products
+// whose epilogue moves more than an accumulator's worth of data (gate and up kept, dg and du) are bound by that epilogue: at 768
+// or 2048 summed elements a tile's products take no longer than its 16 warps take to bring in, work out and send out its data.
 #pragma once
 
 #include "kla_common.cuh"
@@ -29,8 +37,8 @@ constexpr int kMlpEpiWarps = 16, kMlpThreads = (4 + kMlpEpiWarps) * 32;
 constexpr int kMlpStageBytes = 2 * 32 * 64;  // two stages of 32 rows of 64 bytes a warp
 constexpr int kMlpRingBytes = 160 * 1024, kMlpMaxStages = 8;
 constexpr size_t kMlpSmem = 1024 + kMlpRingBytes + kMlpEpiWarps * kMlpStageBytes + 256;
-// A block of the ring: A's rows of a CTA and its share of B's, which in a pair of CTAs is half of them. What is in flight is what
-// bounds the loads (a tile's block takes about 1 us from L2): with 5 blocks of 32 KB in place of 6 K=4096 N=1024 ran at 1213 TFLOP/s
+// A block of the ring: A's rows of a CTA and its share of B's, which in a pair of CTAs is half of them. Rings of 4, 5 and 6 blocks
+// of 32 KB measured alike (16384 x 768 x 2048), so that the ring gives way to the sixteen warps' stages.
 inline __host__ __device__ int mlp_b_rows(int BN, int cg, bool mn_major) { return mn_major ? (BN / cg + 63) / 64 * 64 : BN / cg; }
 inline __host__ __device__ int mlp_block_bytes(int BN, int cg, bool mn_major) { return (kMlpBM + mlp_b_rows(BN, cg, mn_major)) * kMlpBK * 2; }
 
