@@ -611,7 +611,9 @@ int kla_b200_gated_step(const kla_b200_gated_step_args *args, void *stream);
  * (elements) that is at least the width; y, residual and dx: any stride; gradients of weights and biases contiguous, the
  * weights' 16-byte aligned.
  * h is an output of the forward and an input of the backward; so is gu (rows [g, u], gu_stride a multiple of 16, u half a row
- * behind g), which is NULL in inference. dgu is scratch like gu, work scratch of kla_b200_mlp_work_bytes. In the backward every
+ * behind g), which is NULL in inference. dgu is scratch like gu. work is 16-byte aligned scratch, in the forward of
+ * kla_b200_mlp_fwd_work_bytes and in the backward of kla_b200_mlp_work_bytes; NULL: y and dx of few rows are not split along their
+ * summed axis (which takes longer, and rounds otherwise), and no gradient of a weight or bias can be had. In the backward every
  * gradient may be NULL: not wanted. Sums over rows are added in a fixed order: results do not change from run to run.
  */
 typedef struct kla_b200_mlp_args {
@@ -627,6 +629,7 @@ typedef struct kla_b200_mlp_args {
     int64_t dx_stride;
 } kla_b200_mlp_args;
 
+size_t kla_b200_mlp_fwd_work_bytes(const kla_b200_mlp_args *args); /* 0: none */
 size_t kla_b200_mlp_work_bytes(const kla_b200_mlp_args *args);
 int kla_b200_mlp_fwd(const kla_b200_mlp_args *args, void *stream);
 int kla_b200_mlp_bwd(const kla_b200_mlp_args *args, void *stream);

@@ -46,6 +46,7 @@ SYMBOLS = (
     "kla_b200_gated_scan_fwd",
     "kla_b200_gated_scan_bwd",
     "kla_b200_gated_step",
+    "kla_b200_mlp_fwd_work_bytes",
     "kla_b200_mlp_work_bytes",
     "kla_b200_mlp_fwd",
     "kla_b200_mlp_bwd",
@@ -297,8 +298,10 @@ def load() -> ctypes.CDLL:
     lib.kla_b200_gated_scan_bwd.argtypes = [POINTER(GatedArgs), c_void_p]
     lib.kla_b200_gated_step.restype = c_int
     lib.kla_b200_gated_step.argtypes = [POINTER(GatedStepArgs), c_void_p]
-    lib.kla_b200_mlp_work_bytes.restype = c_size_t
-    lib.kla_b200_mlp_work_bytes.argtypes = [POINTER(MlpArgs)]
+    for name in ("mlp_work_bytes", "mlp_fwd_work_bytes"):
+        fn = getattr(lib, "kla_b200_" + name)
+        fn.restype = c_size_t
+        fn.argtypes = [POINTER(MlpArgs)]
     for name in ("mlp_fwd", "mlp_bwd"):
         fn = getattr(lib, "kla_b200_" + name)
         fn.restype = c_int
@@ -341,7 +344,7 @@ _host = None
 _HOST_ENTRIES = (
     "scan_fwd", "scan_bwd", "slab_aggregate", "chunk_fold", "epilogue_bwd", "step", "conv_step", "step_layer",
     "linear", "token_work_bytes", "token", "add_norm", "swiglu", "argmax", "qk_norm", "conv_seq", "conv_seq_bwd", "mobius_scan_fwd", "mobius_scan_bwd", "affine_scan_fwd", "affine_scan_bwd",
-    "mlp_work_bytes", "mlp_fwd", "mlp_bwd", "gated_ckpt_bytes", "gated_scan_fwd", "gated_scan_bwd", "gated_step", "ckpt_bytes", "segment_scratch_bytes", "strerror",
+    "mlp_work_bytes", "mlp_fwd_work_bytes", "mlp_fwd", "mlp_bwd", "gated_ckpt_bytes", "gated_scan_fwd", "gated_scan_bwd", "gated_step", "ckpt_bytes", "segment_scratch_bytes", "strerror",
 )
 
 

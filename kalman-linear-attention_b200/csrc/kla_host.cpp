@@ -56,6 +56,7 @@ struct Entry {
     int (*gated_bwd)(const kla_b200_gated_args *, void *) = nullptr;
     int (*gated_step)(const kla_b200_gated_step_args *, void *) = nullptr;
     size_t (*mlp_work_bytes)(const kla_b200_mlp_args *) = nullptr;
+    size_t (*mlp_fwd_work_bytes)(const kla_b200_mlp_args *) = nullptr;
     int (*mlp_fwd)(const kla_b200_mlp_args *, void *) = nullptr;
     int (*mlp_bwd)(const kla_b200_mlp_args *, void *) = nullptr;
     int (*rawscan[4])(const kla_b200_rawscan_args *, void *) = {};  // Moebius forward, backward, affine forward, backward
@@ -96,6 +97,7 @@ void bind(const py::dict &d) {
     take(lib.gated_bwd, d, "kla_b200_gated_scan_bwd");
     take(lib.gated_step, d, "kla_b200_gated_step");
     take(lib.mlp_work_bytes, d, "kla_b200_mlp_work_bytes");
+    take(lib.mlp_fwd_work_bytes, d, "kla_b200_mlp_fwd_work_bytes");
     take(lib.mlp_fwd, d, "kla_b200_mlp_fwd");
     take(lib.mlp_bwd, d, "kla_b200_mlp_bwd");
     take(lib.ckpt_bytes, d, "kla_b200_ckpt_bytes");
@@ -864,6 +866,11 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor, OptTensor, OptTensor> mlp_fw
     a.h = h.data_ptr(); a.h_stride = Hp;
     if (gu) { a.gu = gu->data_ptr(); a.gu_stride = 2 * Hp; }
     a.y = y.data_ptr(); a.y_stride = out;
+    Tensor work;
+    if (const size_t bytes = lib.mlp_fwd_work_bytes(&a)) {
+        work = fresh(x, {(int64_t)bytes}, at::kByte);
+        a.work = work.data_ptr();
+    }
     check(lib.mlp_fwd(&a, stream_of(x)));
     if (!train) return {y, {}, {}, {}, {}, {}};
     return {y, x, w12, w3, h, gu};
@@ -885,7 +892,7 @@ std::tuple<OptTensor, OptTensor, OptTensor, OptTensor, OptTensor> mlp_bwd(
     auto ptr = [](const OptTensor &t) { return t ? t->data_ptr() : nullptr; };
     a.dx = ptr(dx); a.dx_stride = d; a.dw12 = ptr(dw12); a.dw3 = ptr(dw3); a.db12 = ptr(db12); a.db3 = ptr(db3);
     const Tensor dgu = fresh(x, {want[0] || want[1] || want[3] ? a.rows : 0, gu.size(1)});
-    const Tensor work = fresh(x, {want[1] || want[2] || want[3] || want[4] ? (int64_t)lib.mlp_work_bytes(&a) : 0}, at::kByte);
+    const Tensor work = fresh(x, {(int64_t)lib.mlp_work_bytes(&a)}, at::kByte);
     a.dgu = dgu.data_ptr();
     a.work = work.data_ptr();
     check_native(lib.mlp_bwd(&a, stream_of(x)));

@@ -49,8 +49,9 @@ struct Plan {
 // Columns of a tile, CTAs sharing it and shares of the summed axis: the least time (us) by what was measured on B200. A CTA spends
 // `block` on a 64-wide block of its tile with the GPU full (two CTAs with 256 columns 0.40, one 0.42; K=4096 N=1024 of 18944 rows) and
 // `fixed` on a launch, its first loads and its last epilogue (one block of 64 rows: pairs of CTAs 8.3, one CTA 6.2 to 7.7). Partial
-// sums are written, and read again by a kernel more.
-Plan plan(const Product &p, bool may_split, int sms) {
+// sums are written, and read again by a kernel whose launch takes `split_us`: less in a backward, which ends in one anyway.
+constexpr double kNoSplit = -1.0, kSplitForward = 5.0, kSplitBackward = 3.5;
+Plan plan(const Product &p, double split_us, int sms) {
     const int64_t blocks = up(p.K, kMlpBK) * (p.a.halves == kHalvesSummed ? 2 : 1);
     constexpr struct { int bn; double block[2], fixed[2]; } kinds[] = {
         {256, {0.42, 0.40}, {7.5, 8.3}}, {192, {0.34, 0.32}, {6.7, 8.3}}, {128, {0.24, 0.25}, {6.2, 8.3}}, {64, {0.20, 0.215}, {6.2, 8.3}}};
@@ -63,9 +64,9 @@ Plan plan(const Product &p, bool may_split, int sms) {
             const int64_t tm = up(p.M, kMlpBM * cg) * (p.a.halves == kHalvesRows ? 2 : 1);
             const int64_t tn = up(p.N, p.gated() ? bn / 2 : bn), tiles = tm * tn;
             // shares of the summed axis up to four rounds of CTAs
-            const int64_t most = may_split ? std::min<int64_t>({32, blocks, 1 + 4 * sms / (tiles * cg)}) : 1;
+            const int64_t most = split_us >= 0.0 ? std::min<int64_t>({32, blocks, 1 + 4 * sms / (tiles * cg)}) : 1;
             for (int s = 1; s <= most; ++s) {
-                const double sums = s > 1 ? 3.5 + 8e-6 * s * (double)tm * tn * kMlpBM * cg * bn / 4.0 : 0.0;
+                const double sums = s > 1 ? split_us + 8e-6 * s * (double)tm * tn * kMlpBM * cg * bn / 4.0 : 0.0;
                 const double thin = p.gated() && bn == 128 ? 1.2 : 1.0;  // 64 columns of h leave half of the epilogue's warps idle
                 const double t = (double)up(tiles * s, sms / cg) * up(blocks, s) * kind.block[cg - 1] * thin + kind.fixed[cg - 1] + sums;
                 if (best.BN == 0 || t < least) { best = Plan{bn, cg, (int)tm, (int)tn, s}; least = t; }
@@ -193,46 +194,63 @@ Product product_dw12(const kla_b200_mlp_args &a) {
     return product(Operand{a.dgu, a.gu_stride, a.gu_stride / 2, true, kHalvesRows}, plain(a.x, a.x_stride, true), a.H, a.d, a.rows, kMlpPartial);
 }
 
-int64_t weight_rows(const Product &p) { return p.M * (p.a.halves == kHalvesRows ? 2 : 1); }
-int64_t partial_words(const Product &p, int sms) {
-    const int splits = plan(p, true, sms).splits;
-    return splits > 1 ? splits * weight_rows(p) * up(p.N, 4) * 4 : 0;
+int64_t product_rows(const Product &p) { return p.M * (p.a.halves == kHalvesRows ? 2 : 1); }
+int64_t partial_words(const Product &p, double split_us, int sms) {
+    const int splits = plan(p, split_us, sms).splits;
+    return splits > 1 ? splits * product_rows(p) * up(p.N, 4) * 4 : 0;
 }
 // rows of a stretch of the row sums: at least eight a warp, and no more than 1024 stretches
 int64_t sum_rows(int64_t rows) { return std::max<int64_t>(64, up(rows, 1024 * 8) * 8); }
 
-// The working memory of a backward, in words: partial sums of dW3 and dW12, of db3 and db12.
+// The working memory of a backward, in words: partial sums of dW3, dW12 and dx, of db3 and db12.
 struct Work {
-    int64_t w12, b3, b12, all;  // where they begin (dW3's at 0)
+    int64_t w12, dx, b3, b12, all;  // where they begin (dW3's at 0)
 };
 Work work_of(const kla_b200_mlp_args &a, int sms) {
     const int64_t stretches = up(a.rows, sum_rows(a.rows));
     Work w;
-    w.w12 = partial_words(product_dw3(a), sms);
-    w.b3 = w.w12 + partial_words(product_dw12(a), sms);
+    w.w12 = partial_words(product_dw3(a), kSplitBackward, sms);
+    w.dx = w.w12 + partial_words(product_dw12(a), kSplitBackward, sms);
+    w.b3 = w.dx + partial_words(product_dx(a), kSplitBackward, sms);
     w.b12 = w.b3 + stretches * a.out;
     w.all = w.b12 + stretches * 2 * a.H;
     return w;
 }
 
-// The gradient of a weight: in one go, or partial sums of shares of the rows, to be added by the end's kernel.
-int weight_gradient(const Product &p, void *out, float *work, MlpReduce *end, cudaStream_t st) {
-    const Plan pl = plan(p, true, device_sms());
+// What a product without activation is stored to, with what is added to it. half: elements to the second half of the rows
+struct Result {
+    void *out;
+    int64_t stride, half;
+    const void *bias, *side;
+    int64_t side_stride;
+};
+// In one go, or (split_us) partial sums of shares of the summed axis, to be added by the end's kernel.
+int launch_plain(const Product &p, const Result &r, double split_us, float *work, MlpReduce *end, cudaStream_t st) {
+    const Plan pl = plan(p, split_us, device_sms());
     MlpParams prm;
     if (const int rc = fill(&prm, p, pl)) return rc;
     if (pl.splits == 1) {
-        prm.out = static_cast<__nv_bfloat16 *>(out);
-        prm.out_stride = p.N;
-        prm.out_half = p.M * p.N;
-        prm.out_vec = rows_of_16(out, p.N);
+        prm.out = static_cast<__nv_bfloat16 *>(r.out); prm.out_stride = r.stride; prm.out_half = r.half; prm.out_vec = rows_of_16(r.out, r.stride);
+        prm.bias = static_cast<const __nv_bfloat16 *>(r.bias);
+        prm.side = static_cast<const __nv_bfloat16 *>(r.side); prm.side_stride = r.side_stride; prm.side_vec = rows_of_16(r.side, r.side_stride);
         return launch<kMlpPlain>(prm, pl, st);
     }
     prm.partial = work;
     prm.partial_stride = up(p.N, 4) * 4;
-    prm.partial_rows = weight_rows(p);
+    prm.partial_rows = product_rows(p);  // (halves of rows: the second's follow the first's in `out` too)
     *end = MlpReduce{work, prm.partial_rows * prm.partial_stride, prm.partial_stride, pl.splits, (int)prm.partial_rows, (int)p.N,
-                     (int)up(prm.partial_rows * up(p.N, 4), 256), static_cast<__nv_bfloat16 *>(out)};
+                     (int)up(prm.partial_rows * up(p.N, 4), 256), static_cast<__nv_bfloat16 *>(r.out), r.stride, aligned(r.out, 8) && r.stride % 4 == 0,
+                     static_cast<const __nv_bfloat16 *>(r.bias), static_cast<const __nv_bfloat16 *>(r.side), r.side_stride};
     return launch<kMlpPartial>(prm, pl, st);
+}
+Result weight(void *out, const Product &p) { return Result{out, p.N, p.M * p.N, nullptr, nullptr, 0}; }
+
+// The kernel that adds what is left to be added; of[].blocks: of each alone.
+int launch_end(MlpEndParams *end, cudaStream_t st) {
+    for (int i = 1; i < kMlpSums; ++i) end->of[i].blocks += end->of[i - 1].blocks;
+    end->bias_blocks = end->of[kMlpSums - 1].blocks + (int)up(end->bias[0].total, 32);
+    const int64_t blocks = end->bias_blocks + up(end->bias[1].total, 32);
+    return blocks > 0 ? launch_behind(kla_mlp_end_kernel, dim3((unsigned)blocks), 256, 0, 1, st, *end) : KLA_B200_OK;
 }
 
 MlpSum sum_of(const void *x, int64_t stride, int64_t cols, int64_t half_gap, int halves, float *work, void *out) {
@@ -270,12 +288,12 @@ int kla_b200_mlp_fwd(const kla_b200_mlp_args *a, void *stream) {
         return rc;
     if (a->gu != nullptr && (a->gu_stride % 16 || (rc = check_operand(a->gu, a->gu_stride, 2 * a->H)))) return rc ? rc : KLA_B200_EALIGN;
     if (a->residual != nullptr && (rc = check_plain(a->residual, a->residual_stride, a->out))) return rc;
-    if (!aligned(a->b12, 2) || !aligned(a->b3, 2)) return KLA_B200_EALIGN;
+    if (!aligned(a->b12, 2) || !aligned(a->b3, 2) || !aligned(a->work, 16)) return KLA_B200_EALIGN;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int sms = device_sms();
     MlpParams prm;
     const Product first = product_gate_up(*a), second = product_down(*a);
-    Plan pl = plan(first, false, sms);
+    const Plan pl = plan(first, kNoSplit, sms);
     if ((rc = fill(&prm, first, pl))) return rc;
     prm.act = a->activation;
     prm.bias = static_cast<const __nv_bfloat16 *>(a->b12);
@@ -283,13 +301,15 @@ int kla_b200_mlp_fwd(const kla_b200_mlp_args *a, void *stream) {
     prm.keeps = a->gu != nullptr;
     if (prm.keeps && (rc = make_map(&prm.map_kept, a->gu, a->H, a->rows, a->gu_stride, 2, a->gu_stride / 2, 32, 32))) return rc;
     if ((rc = launch<kMlpGated>(prm, pl, st))) return rc;
-    pl = plan(second, false, sms);
-    if ((rc = fill(&prm, second, pl))) return rc;
-    prm.bias = static_cast<const __nv_bfloat16 *>(a->b3);
-    prm.out = static_cast<__nv_bfloat16 *>(a->y); prm.out_stride = a->y_stride; prm.out_vec = rows_of_16(a->y, a->y_stride);
-    prm.side = static_cast<const __nv_bfloat16 *>(a->residual); prm.side_stride = a->residual_stride;
-    prm.side_vec = rows_of_16(a->residual, a->residual_stride);
-    return launch<kMlpPlain>(prm, pl, st);
+    MlpEndParams end{};
+    const Result y{a->y, a->y_stride, 0, a->b3, a->residual, a->residual_stride};
+    if ((rc = launch_plain(second, y, a->work != nullptr ? kSplitForward : kNoSplit, static_cast<float *>(a->work), &end.of[0], st))) return rc;
+    return launch_end(&end, st);
+}
+
+size_t kla_b200_mlp_fwd_work_bytes(const kla_b200_mlp_args *a) {
+    if (check_sizes(a) || a->rows == 0) return 0;
+    return (size_t)partial_words(product_down(*a), kSplitForward, device_sms()) * sizeof(float);
 }
 
 size_t kla_b200_mlp_work_bytes(const kla_b200_mlp_args *a) {
@@ -328,23 +348,20 @@ int kla_b200_mlp_bwd(const kla_b200_mlp_args *a, void *stream) {
     MlpParams prm;
     MlpEndParams end{};
     MlpSumParams sums{};
-    if (a->dw3 != nullptr && (rc = weight_gradient(product_dw3(*a), a->dw3, work, &end.weight[0], st))) return rc;
+    if (a->dw3 != nullptr && (rc = launch_plain(product_dw3(*a), weight(a->dw3, product_dw3(*a)), kSplitBackward, work, &end.of[0], st))) return rc;
     if (inner) {
         const Product dgu = product_dgu(*a);
-        Plan pl = plan(dgu, false, sms);
+        const Plan pl = plan(dgu, kNoSplit, sms);
         if ((rc = fill(&prm, dgu, pl))) return rc;
         prm.act = a->activation;
         prm.side = static_cast<const __nv_bfloat16 *>(a->gu); prm.side_stride = a->gu_stride; prm.side_half = a->gu_stride / 2; prm.side_vec = 1;
         if ((rc = make_map(&prm.map_out, a->dgu, a->H, a->rows, a->gu_stride, 2, a->gu_stride / 2, 32, 32))) return rc;
         if ((rc = launch<kMlpGrad>(prm, pl, st))) return rc;
         if (a->dx != nullptr) {
-            const Product dx = product_dx(*a);
-            pl = plan(dx, false, sms);
-            if ((rc = fill(&prm, dx, pl))) return rc;
-            prm.out = static_cast<__nv_bfloat16 *>(a->dx); prm.out_stride = a->dx_stride; prm.out_vec = rows_of_16(a->dx, a->dx_stride);
-            if ((rc = launch<kMlpPlain>(prm, pl, st))) return rc;
+            const Result dx{a->dx, a->dx_stride, 0, nullptr, nullptr, 0};
+            if ((rc = launch_plain(product_dx(*a), dx, work != nullptr ? kSplitBackward : kNoSplit, work + at.dx, &end.of[2], st))) return rc;
         }
-        if (a->dw12 != nullptr && (rc = weight_gradient(product_dw12(*a), a->dw12, work + at.w12, &end.weight[1], st))) return rc;
+        if (a->dw12 != nullptr && (rc = launch_plain(product_dw12(*a), weight(a->dw12, product_dw12(*a)), kSplitBackward, work + at.w12, &end.of[1], st))) return rc;
     }
     if (a->db3 != nullptr) sums.of[0] = sum_of(a->dy, a->dy_stride, a->out, 0, 1, work + at.b3, a->db3);
     if (a->db12 != nullptr) sums.of[1] = sum_of(a->dgu, a->gu_stride, a->H, a->gu_stride / 2, 2, work + at.b12, a->db12);
@@ -357,10 +374,7 @@ int kla_b200_mlp_bwd(const kla_b200_mlp_args *a, void *stream) {
     }
     end.bias[0] = sums.of[0];
     end.bias[1] = sums.of[1];
-    end.weight[1].blocks += end.weight[0].blocks;
-    end.bias_blocks = end.weight[1].blocks + (int)up(end.bias[0].total, 32);
-    const int64_t blocks = end.bias_blocks + up(end.bias[1].total, 32);
-    return blocks > 0 ? launch_behind(kla_mlp_end_kernel, dim3((unsigned)blocks), 256, 0, 1, st, end) : KLA_B200_OK;
+    return launch_end(&end, st);
 }
 
 }  // extern "C"

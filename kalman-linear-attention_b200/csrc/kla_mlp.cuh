@@ -7,8 +7,8 @@
 //   * x Wg^T and x Wu^T are one product whose B tile is rows of Wg beside the same rows of Wu, so that the accumulator holds
 //     gate and up of the same columns: the epilogue adds the biases and writes act(g) u (in training g and u, too);
 //   * dy W3 turns into dg and du in its epilogue, from the stored g and u;
-//   * sums over the rows (the weights' gradients) have few output tiles and a long axis: it is split over CTAs, whose float32
-//     partial sums a second kernel adds in a fixed order.
+//   * sums over the rows (the weights' gradients) have few output tiles and a long axis, and so do y and dx of few rows: it is split
+//     over CTAs, whose float32 partial sums a second kernel adds in a fixed order (64 rows of 2048 with H = 5456, forward: @ us).
 // An operand whose summed axis is not the adjacent one in memory (W3, W12, and both of a weight's gradient) is read as it is, as
 // an MN-major operand of the tensor core; nothing is transposed in memory.
 //
@@ -808,52 +808,66 @@ __global__ void __launch_bounds__(256) kla_mlp_rowsum_kernel(const __grid_consta
     }
 }
 
-// The end of a backward, one launch for all: the partial sums of the weights' gradients, four columns a thread, and those of the
-// biases', 32 columns a block and every eighth stretch a warp; each in a fixed order.
+// The end of split products, one launch for all of a backward: the partial sums of up to three products, four columns a thread, and those
+// of the biases' gradients, 32 columns a block and every eighth stretch a warp; each in a fixed order. A product's bias and residual
+// are added here in float32, in the order of the unsplit product's epilogue.
 struct MlpReduce {
     const float *partial;
     long long split_stride, stride;  // elements; stride a multiple of 4
     int splits, rows, cols, blocks;  // blocks: of the grid, up to this one's last
-    __nv_bfloat16 *out;              // [rows, cols] contiguous
+    __nv_bfloat16 *out;
+    long long out_stride;
+    int vec;                         // four columns of a row of `out` can be written at once
+    const __nv_bfloat16 *bias, *side;  // or nullptr
+    long long side_stride;
 };
+constexpr int kMlpSums = 3;
 struct MlpEndParams {
-    MlpReduce weight[2];
+    MlpReduce of[kMlpSums];
     MlpSum bias[2];
     int bias_blocks, stretches;      // bias_blocks: of the grid, up to the first bias's last
 };
 __global__ void __launch_bounds__(256) kla_mlp_end_kernel(const __grid_constant__ MlpEndParams prm) {
     grid_dep_launch();
     grid_dep_wait();
-    const int block = blockIdx.x;
-    if (block < prm.weight[1].blocks) {
-        const bool second = block >= prm.weight[0].blocks;
-        const MlpReduce &w = prm.weight[second];
+    const int block = blockIdx.x, sums = prm.of[kMlpSums - 1].blocks;
+    if (block < sums) {
+        const int which = (block >= prm.of[0].blocks) + (block >= prm.of[1].blocks);
+        const MlpReduce &w = prm.of[which];
         const int quads = (w.cols + 3) / 4;
-        const long long i = (long long)(block - (second ? prm.weight[0].blocks : 0)) * 256 + threadIdx.x;
+        const long long i = (long long)(block - (which ? prm.of[which - 1].blocks : 0)) * 256 + threadIdx.x;
         if (i >= (long long)w.rows * quads) return;
         const long long r = i / quads;
-        const int c = (int)(i - r * quads) * 4;
+        const int c = (int)(i - r * quads) * 4, n = min(4, w.cols - c);
         const float *p = w.partial + r * w.stride + c;
         float4 s = *reinterpret_cast<const float4 *>(p);
         for (int k = 1; k < w.splits; ++k) {
             const float4 v = *reinterpret_cast<const float4 *>(p + k * w.split_stride);
             s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
         }
-        __nv_bfloat16 *out = w.out + r * w.cols + c;
-        const float v[4] = {s.x, s.y, s.z, s.w};
-        if (w.cols % 4 == 0) {
+        float v[4] = {s.x, s.y, s.z, s.w};
+        if (w.bias != nullptr)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < n) v[e] += __bfloat162float(w.bias[c + e]);
+        if (w.side != nullptr)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < n) v[e] += __bfloat162float(w.side[r * w.side_stride + c + e]);
+        __nv_bfloat16 *out = w.out + r * w.out_stride + c;
+        if (w.vec && n == 4) {
             *reinterpret_cast<uint2 *>(out) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (c + e < w.cols) out[e] = __float2bfloat16_rn(v[e]);
+                if (e < n) out[e] = __float2bfloat16_rn(v[e]);
         }
         return;
     }
     __shared__ float part[8][32];
     const bool second = block >= prm.bias_blocks;
     const MlpSum &b = prm.bias[second];
-    const int lane = threadIdx.x % 32, g = threadIdx.x / 32, c = (block - (second ? prm.bias_blocks : prm.weight[1].blocks)) * 32 + lane;
+    const int lane = threadIdx.x % 32, g = threadIdx.x / 32, c = (block - (second ? prm.bias_blocks : sums)) * 32 + lane;
     float s = 0.0f;
     if (c < b.total)
 #pragma unroll 4

@@ -166,6 +166,14 @@ def test_few_rows(rows, bias):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("rows,d,H,out", [(33, 64, 5456, 200), (64, 512, 2731, 511), (1, 100, 4000, 36), (257, 330, 6001, 67), (130, 1024, 5456, 1024)])
+def test_few_rows_of_long_sums_are_split(rows, d, H, out, bias):
+    assert lib.load().kla_b200_mlp_fwd_work_bytes(ctypes.byref(lib.MlpArgs(rows=rows, d=d, H=H, out=out))) >= 2 * 4 * rows * out
+    check(*inputs(rows, d, H, out, bias=bias, residual=bias), act="gelu" if bias else "silu")
+
+
+@pytest.mark.gpu
 def test_leading_dimensions_strides_and_broadcast_gradients():
     t, _ = inputs(6 * 50, 64, 96, 40, residual=True)
     want = oracle(*(t[n] for n in NAMES), "silu", torch.ones(300, 40))
