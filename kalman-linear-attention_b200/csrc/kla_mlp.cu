@@ -60,14 +60,14 @@ Plan plan(const Product &p, double split_us, int sms) {
     for (const int cg : {2, 1})
         for (const auto &kind : kinds) {
             const int bn = kind.bn;
-            if (p.gated() && bn % 128) continue;
+            if (p.gated() && bn == 64) continue;
             const int64_t tm = up(p.M, kMlpBM * cg) * (p.a.halves == kHalvesRows ? 2 : 1);
             const int64_t tn = up(p.N, p.gated() ? bn / 2 : bn), tiles = tm * tn;
             // shares of the summed axis up to four rounds of CTAs
             const int64_t most = split_us >= 0.0 ? std::min<int64_t>({32, blocks, 1 + 4 * sms / (tiles * cg)}) : 1;
             for (int s = 1; s <= most; ++s) {
                 const double sums = s > 1 ? split_us + 8e-6 * s * (double)tm * tn * kMlpBM * cg * bn / 4.0 : 0.0;
-                const double thin = p.gated() && bn == 128 ? 1.2 : 1.0;  // 64 columns of h leave half of the epilogue's warps idle
+                const double thin = p.gated() ? (bn == 128 ? 1.2 : bn == 192 ? 1.1 : 1.0) : 1.0;  // fewer than 128 columns of h leave warps of the epilogue idle
                 const double t = (double)up(tiles * s, sms / cg) * up(blocks, s) * kind.block[cg - 1] * thin + kind.fixed[cg - 1] + sums;
                 if (best.BN == 0 || t < least) { best = Plan{bn, cg, (int)tm, (int)tn, s}; least = t; }
             }

@@ -8,7 +8,7 @@
 //     gate and up of the same columns: the epilogue adds the biases and writes act(g) u (in training g and u, too);
 //   * dy W3 turns into dg and du in its epilogue, from the stored g and u;
 //   * sums over the rows (the weights' gradients) have few output tiles and a long axis, and so do y and dx of few rows: it is split
-//     over CTAs, whose float32 partial sums a second kernel adds in a fixed order (64 rows of 2048 with H = 5456, forward: @ us).
+//     over CTAs, whose float32 partial sums a second kernel adds in a fixed order (64 rows of 2048 with H = 5456, forward: 35 -> 25 us).
 // An operand whose summed axis is not the adjacent one in memory (W3, W12, and both of a weight's gradient) is read as it is, as
 // an MN-major operand of the tensor core; nothing is transposed in memory.
 //

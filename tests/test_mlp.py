@@ -166,6 +166,13 @@ def test_few_rows(rows, bias):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,d,H,out", [(1000, 328, 2721, 72), (1000, 2400, 2721, 64)])
+def test_tiles_of_96_columns_of_gate_and_up(rows, d, H, out):
+    """Sizes that tiles of 128 columns would leave in a second round of CTAs."""
+    check(*inputs(rows, d, H, out, bias=True))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bias", [False, True])
 @pytest.mark.parametrize("rows,d,H,out", [(33, 64, 5456, 200), (64, 512, 2731, 511), (1, 100, 4000, 36), (257, 330, 6001, 67), (130, 1024, 5456, 1024)])
 def test_few_rows_of_long_sums_are_split(rows, d, H, out, bias):
