@@ -49,9 +49,9 @@ struct Plan {
 // Columns of a tile, CTAs sharing it and shares of the summed axis: the least time (us) by what was measured on B200. A CTA spends
 // `block` on a 64-wide block of its tile with the GPU full (two CTAs with 256 columns 0.40, one 0.42; K=4096 N=1024 of 18944 rows) and
 // `fixed` on a launch, its first loads and its last epilogue (one block of 64 rows: pairs of CTAs 8.3, one CTA 6.2 to 7.7). Partial
-// sums are written, and read again by a kernel whose launch takes `split_us`: less in a backward, which ends in one anyway.
-constexpr double kNoSplit = -1.0, kSplitForward = 5.0, kSplitBackward = 3.5;
-Plan plan(const Product &p, double split_us, int sms) {
+// sums are written, and read again by a kernel more, 2.5 us: 64 rows of 768 with H = 2048 forward 20.5 us whole, 16.4 split, 512 rows
+// 20.6 and 20.7, 300 rows of 1000 with H = 3000 30.8 and 25.1.
+Plan plan(const Product &p, bool may_split, int sms) {
     const int64_t blocks = up(p.K, kMlpBK) * (p.a.halves == kHalvesSummed ? 2 : 1);
     constexpr struct { int bn; double block[2], fixed[2]; } kinds[] = {
         {256, {0.42, 0.40}, {7.5, 8.3}}, {192, {0.34, 0.32}, {6.7, 8.3}}, {128, {0.24, 0.25}, {6.2, 8.3}}, {64, {0.20, 0.215}, {6.2, 8.3}}};
@@ -64,9 +64,9 @@ Plan plan(const Product &p, double split_us, int sms) {
             const int64_t tm = up(p.M, kMlpBM * cg) * (p.a.halves == kHalvesRows ? 2 : 1);
             const int64_t tn = up(p.N, p.gated() ? bn / 2 : bn), tiles = tm * tn;
             // shares of the summed axis up to four rounds of CTAs
-            const int64_t most = split_us >= 0.0 ? std::min<int64_t>({32, blocks, 1 + 4 * sms / (tiles * cg)}) : 1;
+            const int64_t most = may_split ? std::min<int64_t>({32, blocks, 1 + 4 * sms / (tiles * cg)}) : 1;
             for (int s = 1; s <= most; ++s) {
-                const double sums = s > 1 ? split_us + 8e-6 * s * (double)tm * tn * kMlpBM * cg * bn / 4.0 : 0.0;
+                const double sums = s > 1 ? 2.5 + 8e-6 * s * (double)tm * tn * kMlpBM * cg * bn / 4.0 : 0.0;
                 const double thin = p.gated() ? (bn == 128 ? 1.2 : bn == 192 ? 1.1 : 1.0) : 1.0;  // fewer than 128 columns of h leave warps of the epilogue idle
                 const double t = (double)up(tiles * s, sms / cg) * up(blocks, s) * kind.block[cg - 1] * thin + kind.fixed[cg - 1] + sums;
                 if (best.BN == 0 || t < least) { best = Plan{bn, cg, (int)tm, (int)tn, s}; least = t; }
@@ -195,8 +195,8 @@ Product product_dw12(const kla_b200_mlp_args &a) {
 }
 
 int64_t product_rows(const Product &p) { return p.M * (p.a.halves == kHalvesRows ? 2 : 1); }
-int64_t partial_words(const Product &p, double split_us, int sms) {
-    const int splits = plan(p, split_us, sms).splits;
+int64_t partial_words(const Product &p, int sms) {
+    const int splits = plan(p, true, sms).splits;
     return splits > 1 ? splits * product_rows(p) * up(p.N, 4) * 4 : 0;
 }
 // rows of a stretch of the row sums: at least eight a warp, and no more than 1024 stretches
@@ -209,9 +209,9 @@ struct Work {
 Work work_of(const kla_b200_mlp_args &a, int sms) {
     const int64_t stretches = up(a.rows, sum_rows(a.rows));
     Work w;
-    w.w12 = partial_words(product_dw3(a), kSplitBackward, sms);
-    w.dx = w.w12 + partial_words(product_dw12(a), kSplitBackward, sms);
-    w.b3 = w.dx + partial_words(product_dx(a), kSplitBackward, sms);
+    w.w12 = partial_words(product_dw3(a), sms);
+    w.dx = w.w12 + partial_words(product_dw12(a), sms);
+    w.b3 = w.dx + partial_words(product_dx(a), sms);
     w.b12 = w.b3 + stretches * a.out;
     w.all = w.b12 + stretches * 2 * a.H;
     return w;
@@ -224,9 +224,9 @@ struct Result {
     const void *bias, *side;
     int64_t side_stride;
 };
-// In one go, or (split_us) partial sums of shares of the summed axis, to be added by the end's kernel.
-int launch_plain(const Product &p, const Result &r, double split_us, float *work, MlpReduce *end, cudaStream_t st) {
-    const Plan pl = plan(p, split_us, device_sms());
+// In one go, or (may_split) partial sums of shares of the summed axis, to be added by the end's kernel.
+int launch_plain(const Product &p, const Result &r, bool may_split, float *work, MlpReduce *end, cudaStream_t st) {
+    const Plan pl = plan(p, may_split, device_sms());
     MlpParams prm;
     if (const int rc = fill(&prm, p, pl)) return rc;
     if (pl.splits == 1) {
@@ -293,7 +293,7 @@ int kla_b200_mlp_fwd(const kla_b200_mlp_args *a, void *stream) {
     const int sms = device_sms();
     MlpParams prm;
     const Product first = product_gate_up(*a), second = product_down(*a);
-    const Plan pl = plan(first, kNoSplit, sms);
+    const Plan pl = plan(first, false, sms);
     if ((rc = fill(&prm, first, pl))) return rc;
     prm.act = a->activation;
     prm.bias = static_cast<const __nv_bfloat16 *>(a->b12);
@@ -303,13 +303,13 @@ int kla_b200_mlp_fwd(const kla_b200_mlp_args *a, void *stream) {
     if ((rc = launch<kMlpGated>(prm, pl, st))) return rc;
     MlpEndParams end{};
     const Result y{a->y, a->y_stride, 0, a->b3, a->residual, a->residual_stride};
-    if ((rc = launch_plain(second, y, a->work != nullptr ? kSplitForward : kNoSplit, static_cast<float *>(a->work), &end.of[0], st))) return rc;
+    if ((rc = launch_plain(second, y, a->work != nullptr, static_cast<float *>(a->work), &end.of[0], st))) return rc;
     return launch_end(&end, st);
 }
 
 size_t kla_b200_mlp_fwd_work_bytes(const kla_b200_mlp_args *a) {
     if (check_sizes(a) || a->rows == 0) return 0;
-    return (size_t)partial_words(product_down(*a), kSplitForward, device_sms()) * sizeof(float);
+    return (size_t)partial_words(product_down(*a), device_sms()) * sizeof(float);
 }
 
 size_t kla_b200_mlp_work_bytes(const kla_b200_mlp_args *a) {
@@ -348,10 +348,10 @@ int kla_b200_mlp_bwd(const kla_b200_mlp_args *a, void *stream) {
     MlpParams prm;
     MlpEndParams end{};
     MlpSumParams sums{};
-    if (a->dw3 != nullptr && (rc = launch_plain(product_dw3(*a), weight(a->dw3, product_dw3(*a)), kSplitBackward, work, &end.of[0], st))) return rc;
+    if (a->dw3 != nullptr && (rc = launch_plain(product_dw3(*a), weight(a->dw3, product_dw3(*a)), true, work, &end.of[0], st))) return rc;
     if (inner) {
         const Product dgu = product_dgu(*a);
-        const Plan pl = plan(dgu, kNoSplit, sms);
+        const Plan pl = plan(dgu, false, sms);
         if ((rc = fill(&prm, dgu, pl))) return rc;
         prm.act = a->activation;
         prm.side = static_cast<const __nv_bfloat16 *>(a->gu); prm.side_stride = a->gu_stride; prm.side_half = a->gu_stride / 2; prm.side_vec = 1;
@@ -359,9 +359,9 @@ int kla_b200_mlp_bwd(const kla_b200_mlp_args *a, void *stream) {
         if ((rc = launch<kMlpGrad>(prm, pl, st))) return rc;
         if (a->dx != nullptr) {
             const Result dx{a->dx, a->dx_stride, 0, nullptr, nullptr, 0};
-            if ((rc = launch_plain(product_dx(*a), dx, work != nullptr ? kSplitBackward : kNoSplit, work + at.dx, &end.of[2], st))) return rc;
+            if ((rc = launch_plain(product_dx(*a), dx, work != nullptr, work + at.dx, &end.of[2], st))) return rc;
         }
-        if (a->dw12 != nullptr && (rc = launch_plain(product_dw12(*a), weight(a->dw12, product_dw12(*a)), kSplitBackward, work + at.w12, &end.of[1], st))) return rc;
+        if (a->dw12 != nullptr && (rc = launch_plain(product_dw12(*a), weight(a->dw12, product_dw12(*a)), true, work + at.w12, &end.of[1], st))) return rc;
     }
     if (a->db3 != nullptr) sums.of[0] = sum_of(a->dy, a->dy_stride, a->out, 0, 1, work + at.b3, a->db3);
     if (a->db12 != nullptr) sums.of[1] = sum_of(a->dgu, a->gu_stride, a->H, a->gu_stride / 2, 2, work + at.b12, a->db12);
