@@ -21,7 +21,7 @@
 // What bounds it: memory as long as the exponential and the two passes over a step's maps keep up. Forward a pair of steps costs 33
 // instructions of a warp, backward 71, with half of the schedulers' slots used (a chain of 4 to 8 warps a scheduler). Measured in
 // bfloat16: 4 x 8192 x 2048 forward 84 us (4.8 TB/s of x, g and h, of 6.55 that a copy reaches); 16 x 2048 x 1536 forward 60 us,
-// backward 102 (4.9 TB/s); 1 x 65536 x 4096 forward 310 us (5.2 TB/s), backward 630 (4.3). Not kept, as they were slower: eight
+// backward 92 (5.5 TB/s); 1 x 65536 x 4096 forward 310 us (5.2 TB/s), backward 546 (4.9). Not kept, as they were slower: eight
 // steps a warp with three or four CTAs an SM, two chains a warp, z kept in shared memory, rings of more tiles.
 #pragma once
 
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kC
     // the state in front of a round's unit
     auto front = [&](int round) {
         const int unit = round * ranks + rank;
-        return round >= 0 && unit * kGatedUnit < len ? neg2(ln.load_state(prm.ckpt + (long long)(span.unit + unit) * prm.D)) : make_float2(0.0f, 0.0f);
+        return round >= 0 && unit * kGatedUnit < len ? ln.load_state(prm.ckpt + (long long)(span.unit + unit) * prm.D) : make_float2(0.0f, 0.0f);
     };
     float2 next = front(rounds - 1);
     int slot = 0;
@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kC
         if (round < rounds) gated_arrived<S - 2>();
         fetch();
         if (round >= rounds) continue;
-        float2 h = next;
+        float2 h = neg2(next);  // (here, not where it is loaded: that would wait for it)
         next = front(round - 1);
         const T *gs = ring + slot * 3 * kTile, *xs = gs + kTile, *ds = xs + kTile;
         if (++slot == S) slot = 0;
