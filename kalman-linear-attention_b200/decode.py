@@ -323,7 +323,7 @@ class ModelDecoder:
     whole_gpu = None  # or True, False
     # True: a prompt's swiglu MLP runs as ``gated_mlp_b200`` where it is bfloat16 (two kernels, gate and up never in memory), in place
     # of two library GEMMs and a kernel between them; rounded in fewer places, so its results are other bits. us, two GEMMs and a kernel / fused:
-    # 512 rows of 768 14 / 22, 4096 45 / 39, 32768 289 / 229; 16384 of 4096 3151 / 2864.
+    # 512 rows of 768 14 / 21, 4096 45 / 39, 32768 289 / 229; 16384 of 4096 3151 / 2864.
     fused_mlp = False
 
     def __init__(self, weights: dict, layer_configs, model_config: dict):
