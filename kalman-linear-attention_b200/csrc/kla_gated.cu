@@ -104,9 +104,13 @@ int slots_of(bool bf16, bool pairs, bool backward, Slots *out) {
 // B=4 L=8192 D=2048 102 / 85 / 93 / 105, B=16 L=2048 D=1536 60 / 72 / 84 / 107, B=1 L=8192 D=1024 98 / 62 / 33 / 24, B=8 L=512 D=768
 // 8.3 / 8.7 / 11.5 / 17.6; backward 103 / 119 / 129 / 148 (B=16 ...), 192 / 121 / 65 / 45 (B=1 ...), 14.2 / 13.7 / 10.7 / 13.8 (B=8 ...).
 // Of packed sequences the host knows the number and the sum of the lengths; the longest of n random ones is about ln n + 0.6 times
-// their mean, and clusters of more than four were no gain there.
-int pick_ranks(const Slots &slots, const Kernel &k, int64_t cells, int64_t rows, int64_t sequences, int64_t L, bool packed, bool backward, size_t esz, int64_t D) {
+// their mean. They take as long as the longest does or as all their rounds do with full SMs (half a round of a CTA is left over at each
+// end), and a start per wave. Clusters of 1 / 2 / 4 / 6 / 8: 40 in 32768 rows of 1536, bfloat16, forward 84 / 86 / 115 / 139 / 240,
+// 12 in 32768 of 768 103 / 78 / 51 / 55 / 65, 3 in 65536 of 256 420 / 253 / 134 / 94 / 73, 60 in 2000 of 300, float32, 7 / 12 / 18 / 27 /
+// 48, 9 in 6001 of 1024 44 / 34 / 25 / 23 / 36 (nine of one length 18 / 18 / 25 / 26 / 42).
+int pick_ranks(const Slots &slots, const Kernel &k, int64_t blocks, int64_t rows, int64_t sequences, int64_t L, bool packed, bool backward, size_t esz, int64_t D) {
     const double sms = device_sms();
+    const int64_t cells = sequences * blocks;
     const double round = backward ? (esz == 2 ? 1.5 : 2.2) : (esz == 2 ? 1.53 : 1.15);
     constexpr double shares[kRankCount] = {1.0, 1.27, 1.32, 1.37, 1.42, 1.47, 1.6}, starts[kRankCount] = {2.0, 3.5, 4.3, 5.0, 5.3, 5.6, 6.0};
     double steps = (double)L;
@@ -116,10 +120,11 @@ int pick_ranks(const Slots &slots, const Kernel &k, int64_t cells, int64_t rows,
     double least = 0.0;
     for (int i = 0; i < kRankCount; ++i) {
         const int r = kRanks[i];
-        if (r > 1 && (r > tiles || slots.ctas[i] < r || (packed && r > 4))) continue;
-        const double n = (double)cells * r, waves = packed ? 1.0 : std::max(1.0, std::ceil(n / slots.ctas[i]));
-        const double load = std::min(3.0, std::max(1.0, std::ceil(n / waves / sms)));
-        const double t = std::max(waves * (std::ceil(tiles / r) * round * shares[i] * (1.0 + 0.35 * (load - 1.0)) + starts[i]), least_us);
+        if (r > 1 && (r > tiles || slots.ctas[i] < r)) continue;
+        const double n = (double)cells * r, waves = std::max(1.0, std::ceil(n / slots.ctas[i]));
+        const double load = std::min(3.0, std::max(1.0, packed ? n / sms : std::ceil(n / waves / sms))), one = round * shares[i] * (1.0 + 0.35 * (load - 1.0));
+        const double own = std::ceil(tiles / r) * one, all = ((double)L * blocks / k.tile + 0.5 * n) * one / (load * sms);
+        const double t = packed ? std::max({own, all, least_us}) + waves * starts[i] : std::max(waves * (own + starts[i]), least_us);
         if (r == 1 || t < least) { best = r; least = t; }
     }
     return best;
@@ -176,10 +181,11 @@ int gated(const kla_b200_gated_args *a, void *stream, bool backward) {
     prm.dend = a->dstate_out; prm.dh0 = a->dstate;
     prm.x_width = width(a->x, esz, a->D); prm.g_width = width(a->gate, esz, a->D); prm.dh_width = width(a->dh, esz, a->D);
     if (const int rc = entry::wait_ctl(&prm.wait)) return rc;
-    const int64_t sequences = N + packed;
+    prm.clears = packed ? (int)std::clamp<int64_t>(a->L / 4096, 1, 16) : 0;
+    const int64_t sequences = N + prm.clears;
     Slots slots;
     if (const int rc = slots_of(esz == 2, vec, backward, &slots)) return rc;
-    const int ranks = pick_ranks(slots, kernel_of(esz == 2, vec, backward, false), N * prm.blocks, packed ? a->L : a->B * a->L, N, a->L, packed, backward, esz, a->D);
+    const int ranks = pick_ranks(slots, kernel_of(esz == 2, vec, backward, false), prm.blocks, packed ? a->L : a->B * a->L, N, a->L, packed, backward, esz, a->D);
     return launch(kernel_of(esz == 2, vec, backward, ranks > 1), prm, sequences, ranks, static_cast<cudaStream_t>(stream));
 }
 

@@ -154,6 +154,13 @@ def test_packed_sequences(bounds, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_packed_sequences_share_clusters(dtype):
+    """Few sequences, one of them most of the rows, others of one row and none; thousands of rows that belong to no sequence."""
+    check(1, 18000, 40, dtype, bounds=[300, 11001, 11002, 11002, 13500])
+
+
+@pytest.mark.gpu
 def test_bounds_outside_the_rows_are_clamped():
     check_against = lambda b: kla_b200.gated_scan_b200(  # noqa: E731
         *torch.randn(1, 100, 128, generator=torch.Generator("cuda").manual_seed(0), device="cuda").chunk(2, -1),
