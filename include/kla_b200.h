@@ -662,6 +662,8 @@ int kla_b200_device_status(int *status);
  * skip_tile: the scan kernels' loader leaves the hand-over of this tile
  *   incomplete, so that the wait for it runs out after wait_limit_ns, the kernel
  *   returns and kla_b200_device_status reports 0x100 | site; -1 switches it off.
+ *   The gated recurrence's clusters leave out the exchange of that round, the
+ *   gated block the load of that block of its ring.
  * The settings are process-wide and are read when a scan is launched. A tile that
  * is skipped is loaded all the same: nothing is left in flight and nothing faults.
  */
