@@ -340,6 +340,24 @@ __device__ __forceinline__ void mlp_act2(float2 g, float2 &f, float2 &df) {
         mlp_act<ACT, SLOPE>(g.y, f.y, df.y);
     }
 }
+// A gate as it is kept: where the activation closes (silu, gelu and relu of large negative gates) its size says nothing, the value and the
+// slope are 0 whatever it is. It is kept as a gate that closes and has a code, so that a hidden unit masked by a bias of the
+// type's lowest value gets its gradients of 0. NaN and what is NaN forward (silu and gelu of -inf) stay NaN.
+constexpr float kClosedGate = -0x1p20f;
+template <int ACT>
+__device__ __forceinline__ float2 gate_to_keep(float2 g) {
+    if (ACT == 2) {
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(g.x) : "f"(kClosedGate));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(g.y) : "f"(kClosedGate));
+        return g;
+    }
+    if (ACT == 3) return g;
+    return fma2(g, dup2(0.0f), make_float2(fmaxf(g.x, kClosedGate), fmaxf(g.y, kClosedGate)));
+}
+template <int ACT>
+__device__ __forceinline__ uint4 keep8_gates(const float2 (&g)[4]) {
+    return make_uint4(keep2(gate_to_keep<ACT>(g[0])), keep2(gate_to_keep<ACT>(g[1])), keep2(gate_to_keep<ACT>(g[2])), keep2(gate_to_keep<ACT>(g[3])));
+}
 __device__ __forceinline__ uint4 pack8(const float2 (&x)[4]) { return make_uint4(pack2(x[0].x, x[0].y), pack2(x[1].x, x[1].y), pack2(x[2].x, x[2].y), pack2(x[3].x, x[3].y)); }
 __device__ __forceinline__ uint4 keep8(const float2 (&x)[4]) { return make_uint4(keep2(x[0]), keep2(x[1]), keep2(x[2]), keep2(x[3])); }
 // cols: of the eight that exist
@@ -383,7 +401,7 @@ __device__ __forceinline__ void mlp_gated_chunk(uint32_t gate, uint32_t up, cons
             add_bias(u, bias + N + 8 * i, cols - 8 * i);
         }
         if (kept) {
-            *reinterpret_cast<uint4 *>(st.piece(st.lane, i)) = keep8(g);
+            *reinterpret_cast<uint4 *>(st.piece(st.lane, i)) = keep8_gates<ACT>(g);
             *reinterpret_cast<uint4 *>(st2.piece(st.lane, i)) = keep8(u);
         }
 #pragma unroll
