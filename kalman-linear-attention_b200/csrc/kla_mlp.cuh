@@ -287,21 +287,22 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 
 // Gate and up as the backward finds them: 16 bits with a sign, six of exponent and nine of mantissa. Rounded to bfloat16 their
 // two roundings would be half of the error of a gradient (0.0030 of dx and dW12 in the 2-norm, against 0.0017 of rounding
-// the result alone); nine bits leave the rounding of the gradients that go into the products (0.0025). 2^-31 to 2^33 at full
-// accuracy, steps of 2^-40 below; what is larger, infinite or NaN comes back as NaN.
+// the result alone); nine bits leave the rounding of the gradients that go into the products (0.0025). 2^-31 to 2^32 at full
+// accuracy, steps of 2^-40 below; what is larger, infinite or NaN comes back as NaN. (A value times 2^-95 has its 2^-31 at the least
+// normal number, 2^-126, and 14 bits dropped of 2^-149 below are steps of 2^-135.)
 constexpr uint32_t kKeptTop = 0x7fffu << 14;
-// the code in the upper half, s being x 2^-96; the least of its size and kKeptTop makes NaN the top code, too
+// the code in the upper half, s being x 2^-95; the least of its size and kKeptTop makes NaN the top code, too
 __device__ __forceinline__ uint32_t keep(float x, float s) {
     const float m = fminf(fabsf(s), __uint_as_float(kKeptTop));
     return __float_as_uint(m) * 4u + 0x8000u | __float_as_uint(x) & 0x80000000u;
 }
 __device__ __forceinline__ uint32_t keep2(float2 x) {
-    const float2 s = mul2(x, dup2(0x1p-96f));
+    const float2 s = mul2(x, dup2(0x1p-95f));
     return __byte_perm(keep(x.x, s.x), keep(x.y, s.y), 0x7632);
 }
 __device__ __forceinline__ float2 kept2(uint32_t w) {
     const uint32_t lo = (uint32_t)((int32_t)(w << 16) >> 2) & 0x9fffc000u, hi = (uint32_t)((int32_t)w >> 2) & 0x9fffc000u;
-    const float2 v = mul2(make_float2(__uint_as_float(lo), __uint_as_float(hi)), dup2(0x1p96f));
+    const float2 v = mul2(make_float2(__uint_as_float(lo), __uint_as_float(hi)), dup2(0x1p95f));
     const float nan = __uint_as_float(0x7fffffffu);
     return make_float2((lo & 0x7fffffffu) == kKeptTop ? nan : v.x, (hi & 0x7fffffffu) == kKeptTop ? nan : v.y);
 }

@@ -25,7 +25,7 @@ def gated_mlp_b200(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, b12: to
     first. Under a bfloat16 autocast float32 and float16 ``x``, weights and biases are converted as ``F.linear`` does.
 
     A call that is to be differentiated keeps ``x``, the weights and three ``[rows, H]`` tensors of 16 bits for the backward: the
-    product, and gate and up with nine bits of mantissa over 2^-31 to 2^33 (beyond, their gradients are NaN; but a gate that large
+    product, and gate and up with nine bits of mantissa over 2^-31 to 2^32 (beyond, their gradients are NaN; but a gate that large
     and negative under silu, gelu or relu takes no part, whatever its size: a hidden unit may be masked by its bias)."""
     if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:
         x, w12, w3, b12, b3 = (t.to(torch.bfloat16) if t is not None and t.is_cuda and t.dtype in (torch.float32, torch.float16) else t

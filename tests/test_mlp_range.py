@@ -67,3 +67,20 @@ def test_a_gate_of_minus_infinity_is_nan_as_torchs_is(act):
     t["b12"][3] = -float("inf")
     y, grads = gradients(t, dy, act)
     assert torch.isnan(y).all() and torch.isnan(grads["x"]).all() and torch.isnan(grads["w12"][3]).all()
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -40, 2.0 ** -33, 2.0 ** -32, 2.0 ** -31, 2.0 ** -30, 1.0, 2.0 ** 31])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_the_kept_range_and_its_steps(scale, sign):
+    """One row whose gates lie just short of half a step, from where du's rounding goes the same way: nine bits of mantissa down to
+    2^-31, steps of 2^-40 below. Gates are a weight and a bias, which adds bits that bfloat16 does not have."""
+    H = 8
+    fine = sign * scale * torch.tensor([2.0 ** -8 - 2.0 ** -11, 2.0 ** -9 - 2.0 ** -12, 2.0 ** -10 - 2.0 ** -13, 2.0 ** -10, 0.0, 2.0 ** -12, 2.0 ** -7, 2.0 ** -8])
+    t = dict(x=torch.eye(1, 8), w12=torch.zeros(2 * H, 8), w3=torch.full((1, H), 1 - 2.0 ** -8), b12=torch.cat((fine, torch.zeros(H))), b3=None, residual=None)
+    t["w12"][:H, 0], t["w12"][H:, 0] = sign * scale, 1.0
+    t = {n: None if v is None else v.bfloat16().cuda() for n, v in t.items()}
+    dy = torch.full((1, 1), 1 + 2.0 ** -7).bfloat16().cuda()  # dh = 1 + 2^-8 - 2^-15
+    want = oracle(*(t[n] for n in NAMES), None, dy)
+    _, grads = gradients(t, dy, None)
+    held(grads["w12"], want["dw12"], "dw12")
+    held(grads["b12"], want["db12"], "db12")
