@@ -22,12 +22,18 @@ def gated_mlp_b200(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, b12: to
     """``x`` ``[..., d]``, ``w12`` ``[2 H, d]`` (gate's rows, then up's), ``w3`` ``[out, H]``, ``b12`` ``[2 H]``, ``b3`` ``[out]``,
     ``residual`` ``[..., out]`` added to the result in float32 before it is rounded. ``activation``: ``"silu"``, ``"gelu"`` (the exact
     one), ``"relu"`` or None. Any sizes and strides: rows that are not 16-byte aligned (a width that is no multiple of 8) are copied
-    first. Under a bfloat16 autocast float32 and float16 ``x``, weights and biases are converted as ``F.linear`` does.
+    first. Under a bfloat16 autocast float32 and float16 ``x``, weights and biases are converted as ``F.linear`` does; a ``residual`` of
+    those types is not, but added to the rounded bfloat16 result as ``residual + F.linear(...)`` would be, and the sum is float32.
 
     A call that is to be differentiated keeps ``x``, the weights and three ``[rows, H]`` tensors of 16 bits for the backward: the
     product, and gate and up with nine bits of mantissa over 2^-31 to 2^32 (beyond, their gradients are NaN; but a gate that large
     and negative under silu, gelu or relu takes no part, whatever its size: a hidden unit may be masked by its bias)."""
+    wide = None  # a residual the sum with which is float32
     if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:
+        if residual is not None and residual.dtype in (torch.float32, torch.float16) and residual.device == x.device and x.dim() > 0:
+            if residual.shape != (*x.shape[:-1], w3.shape[0] if w3.dim() == 2 else -1):
+                raise ValueError("kla_b200: residual has the output's shape")
+            wide, residual = residual, None
         x, w12, w3, b12, b3 = (t.to(torch.bfloat16) if t is not None and t.is_cuda and t.dtype in (torch.float32, torch.float16) else t
                                for t in (x, w12, w3, b12, b3))
     lead = None
@@ -41,4 +47,6 @@ def gated_mlp_b200(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, b12: to
             residual = residual.reshape(lead.numel(), residual.shape[-1])
         x = x.reshape(lead.numel(), x.shape[-1])
     y = _lib.host().gated_mlp(x, w12, w3, b12, b3, residual, activation)
-    return y if lead is None else y.view(*lead, y.shape[-1])
+    if lead is not None:
+        y = y.view(*lead, y.shape[-1])
+    return y if wide is None else wide.float() + y
