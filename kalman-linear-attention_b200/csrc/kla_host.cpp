@@ -691,7 +691,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, OptTensor, OptTensor> gated_fwd(const
         require(cu_->device() == x_.device() && cu_->dim() == 1 && cu_->size(0) >= 1, "cu_seqlens is a vector of at least one bound on x's device");
         require(cu_->scalar_type() == at::kInt || cu_->scalar_type() == at::kLong, "cu_seqlens holds int32 or int64");
         require(x_.size(0) == 1, "packed sequences are one batch entry: x is [1, L, D]");
-        cu = cu_->to(at::kInt).contiguous();
+        // (clamped as the kernels do, before bits are dropped that a bound past 2^31 has)
+        cu = (cu_->scalar_type() == at::kLong ? cu_->clamp(0, x_.size(1)) : *cu_).to(at::kInt).contiguous();
     }
     const Tensor x = rows(x_), gate = rows(gate_);
     kla_b200_gated_args a = gated_args(x, gate, cu);
