@@ -802,6 +802,7 @@ std::tuple<Tensor, Tensor> gated_step(const Tensor &x_, const Tensor &gate_, con
     a.x = x.data_ptr(); a.gate = gate.data_ptr(); a.x_stride_b = x.stride(0); a.gate_stride_b = gate.stride(0);
     a.state = fp(state); a.state_out = fp(next); a.h = h.data_ptr();
     check(lib.gated_step(&a, stream_of(x)));
+    if (out && !out->is_inference()) out->unsafeGetTensorImpl()->bump_version();  // (what was saved of it for a backward is gone)
     return {h, next};
 }
 

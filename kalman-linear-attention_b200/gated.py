@@ -31,5 +31,6 @@ def gated_scan_b200(x: torch.Tensor, gate: torch.Tensor, initial_state: torch.Te
 
 def gated_step_b200(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, state_out: torch.Tensor | None = None):
     """One token: ``(h, new_state)`` for ``x``, ``gate`` ``[B, D]`` and ``state`` float32 ``[B, D]``. ``state_out`` receives the
-    new state where it is given, and may be ``state`` itself (a captured token then advances it with every replay). No backward."""
+    new state where it is given, and may be ``state`` itself (a captured token then advances it with every replay): an
+    in-place operation like torch's own. No backward."""
     return _lib.host().gated_step(x, gate, state, state_out)

@@ -16,3 +16,33 @@ def test_bounds_past_32_bits_are_clamped(given, same):
     x, g = torch.randn(1, 100, 128, generator=torch.Generator("cuda").manual_seed(0), device="cuda").chunk(2, -1)
     got, want = (kla_b200.gated_scan_b200(x, g, cu_seqlens=torch.tensor(b, device="cuda")) for b in (given, same))
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_a_state_written_in_place_is_known_to_autograd():
+    x, g, state = torch.randn(3, 4, 64, device="cuda")
+    weight = torch.randn(4, 64, device="cuda").requires_grad_()
+    for written in (state, torch.empty_like(state)):
+        before = written._version
+        loss = (weight * written).sum()  # keeps `written` for weight's gradient
+        with torch.no_grad():
+            h, new = kla_b200.gated_step_b200(x, g, state, state_out=written)
+        assert new.data_ptr() == written.data_ptr() and written._version == before + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    before = state._version
+    kla_b200.gated_step_b200(x, g, state)
+    assert state._version == before
+
+
+def test_a_state_written_in_inference_mode():
+    x, g, want = torch.randn(3, 4, 64, device="cuda")
+    with torch.inference_mode():
+        state = want.clone()
+        _, new = kla_b200.gated_step_b200(x, g, want)
+        for _ in range(2):
+            state.copy_(want)
+            kla_b200.gated_step_b200(x, g, state, state_out=state)
+            assert torch.equal(state, new)
+    with torch.no_grad():  # a tensor made there, written outside
+        kla_b200.gated_step_b200(x, g, want, state_out=state)
+    assert torch.equal(state, new)
