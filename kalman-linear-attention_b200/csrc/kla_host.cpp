@@ -794,7 +794,7 @@ std::tuple<Tensor, Tensor> gated_step(const Tensor &x_, const Tensor &gate_, con
         at::assert_no_overlap(*out, x_);
         at::assert_no_overlap(*out, gate_);
     }
-    if (wants_grad({&x_, &gate_, &state_})) unsupported("gated_step_b200 has no backward: use gated_scan_b200, or call it under torch.no_grad().");
+    if (wants_grad({&x_, &gate_, &state_, out ? &*out : &x_})) unsupported("gated_step_b200 has no backward: use gated_scan_b200, or call it under torch.no_grad().");
     const Tensor state = state_.contiguous();
     Tensor h = fresh(x, {B, D}), next = out ? *out : f32(x, {B, D});
     kla_b200_gated_step_args a{};

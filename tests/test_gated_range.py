@@ -46,3 +46,14 @@ def test_a_state_written_in_inference_mode():
     with torch.no_grad():  # a tensor made there, written outside
         kla_b200.gated_step_b200(x, g, want, state_out=state)
     assert torch.equal(state, new)
+
+
+def test_a_state_that_requires_a_gradient_is_not_written():
+    x, g, state = torch.randn(3, 4, 64, device="cuda")
+    leaf = torch.zeros(4, 64, device="cuda").requires_grad_()
+    with pytest.raises(NotImplementedError):
+        kla_b200.gated_step_b200(x, g, state, state_out=leaf)
+    assert not leaf.any()
+    with torch.no_grad():
+        kla_b200.gated_step_b200(x, g, state, state_out=leaf)
+    assert leaf.any()
