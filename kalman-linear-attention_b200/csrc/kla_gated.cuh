@@ -6,7 +6,8 @@
 //
 // Every channel of every sequence is a chain of its own, and over a stretch of steps both recurrences are affine maps with the
 // same slope A = prod a_t: h -> A h + F and u -> A u + R. A step is taken as h - z h + z x with two fused operations: what is
-// rounded is then small beside 1 - a where a gate holds the state for thousands of steps, which a = 1 - z rounded is not.
+// rounded is then small beside 1 - a where a gate holds the state for thousands of steps, which a = 1 - z rounded is not. Where a gate
+// forgets it is taken as (x - a x) + a h (kForgetGate).
 //
 // A CTA owns 64 channels of one sequence and walks it in tiles of W x TS steps. Each warp takes TS consecutive steps
 // of the tile, each lane two channels. The warp's rows come in by asynchronous copies into a ring of its own in shared memory,
@@ -71,6 +72,14 @@ struct Lane {
             return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
         } else {
             return make_float2(__bfloat162float(row[lane]), __bfloat162float(row[lane + 32]));
+        }
+    }
+    __device__ __forceinline__ void put(float *row, float2 y) const {
+        if constexpr (PAIR) {
+            *reinterpret_cast<float2 *>(row + 2 * lane) = y;
+        } else {
+            row[lane] = y.x;
+            row[lane + 32] = y.y;
         }
     }
     // -y to a row; `row` points at c0
@@ -242,17 +251,49 @@ __device__ __forceinline__ float2 gate_nz(float2 g) {
     const float2 t = mul2(g, dup2(kLog2e)), d = fma2(make_float2(ex2_approx(t.x), ex2_approx(t.y)), dup2(-1.0f), dup2(-1.0f));
     return make_float2(rcp_approx(d.x), rcp_approx(d.y));
 }
-// -z and z a, both with the relative accuracy of the smaller of z and a
-__device__ __forceinline__ void gate_slope(float2 g, float2 &nz, float2 &za) {
+// -z and z a, both with the relative accuracy of the smaller of z and a, and that smaller one
+__device__ __forceinline__ void gate_slope(float2 g, float2 &nz, float2 &za, float2 &small) {
     const float2 e = make_float2(ex2_approx(fabsf(g.x) * -kLog2e), ex2_approx(fabsf(g.y) * -kLog2e)), d = add2(e, dup2(1.0f));
-    const float2 r = make_float2(rcp_approx(d.x), rcp_approx(d.y)), small = mul2(e, r);
+    const float2 r = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+    small = mul2(e, r);
     nz = make_float2(g.x >= 0.0f ? -small.x : -r.x, g.y >= 0.0f ? -small.y : -r.y);
     za = mul2(small, r);
 }
+// Where a gate forgets, v - z v is all cancellation: off by 2^-24 of v and more, it has few digits of a v left, or none. So a gate
+// below kForgetGate is taken by a itself, which has full relative accuracy, and a step as (x - a x) + a h. Its factor w is a, with a
+// positive sign (+0 too), in place of -z, whose sign is negative (-0 too). Above it a is at least 0.0067 in float32 and 0.00034 in
+// bfloat16, so that 2^-23 of z are at most 2^-15 and 2^-11 of a. The choice costs instructions, and a warp makes it only in tiles
+// that have such a gate, in loops that are not unrolled and a second time over the steps: unrolled beside the others, they took
+// the backward without any such gate from 91 to 117 us (16 x 2048 x 1536, bfloat16; 94 as it is). Gates from kForgetGate on get the
+// same bits either way. Measured at that shape, gates of mean 2 / of mean 0 and deviation 1.5 / of mean -6, us: float32 forward 111 /
+// 117 / 120, backward 171 / 260 / 302; bfloat16 59 / 60 / 123, 94 / 94 / 243.
+template <typename T>
+constexpr float kForgetGate = sizeof(T) == 2 ? -8.0f : -5.0f;
+__device__ __forceinline__ bool forgets(float w) { return __float_as_int(w) >= 0; }
+template <typename T>
+__device__ __forceinline__ float2 chosen_factor(float2 g, float2 a, float2 nz) { return make_float2(g.x < kForgetGate<T> ? a.x : nz.x, g.y < kForgetGate<T> ? a.y : nz.y); }
+// of the forward (its -z are gate_nz's)
+template <typename T>
+__device__ __forceinline__ float2 gate_factor(float2 g) {
+    const float2 t = mul2(g, dup2(kLog2e)), e = make_float2(ex2_approx(t.x), ex2_approx(t.y)), d = fma2(e, dup2(-1.0f), dup2(-1.0f));
+    const float2 nz = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+    return chosen_factor<T>(g, neg2(mul2(e, nz)), nz);
+}
+__device__ __forceinline__ float lowest(float low, float2 g) { return fminf(low, fminf(g.x, g.y)); }
 // A step for two channels of the negated state, -h_t = -h + z h - z x, and the factor alone. (The state is carried negated because -z
 // comes out of the gate and x out of memory as they are: each negation would be an operation a step.)
-__device__ __forceinline__ float2 decay(float2 nz, float2 v) { return fma2(nz, v, v); }
-__device__ __forceinline__ float2 gate_step(float2 nz, float2 x, float2 nh) { return fma2(nz, x, decay(nz, nh)); }
+template <bool FORGETS>
+__device__ __forceinline__ float2 decay(float2 w, float2 v) {
+    return fma2(w, v, FORGETS ? make_float2(forgets(w.x) ? 0.0f : v.x, forgets(w.y) ? 0.0f : v.y) : v);
+}
+template <bool FORGETS>
+__device__ __forceinline__ float2 gate_step(float2 w, float2 x, float2 nh) {
+    if (!FORGETS) return fma2(w, x, fma2(w, nh, nh));
+    // the larger term first: it alone cannot overflow
+    const bool f0 = forgets(w.x), f1 = forgets(w.y);
+    const float2 near = fma2(w, make_float2(f0 ? x.x : nh.x, f1 ? x.y : nh.y), make_float2(f0 ? -x.x : nh.x, f1 ? -x.y : nh.y));
+    return fma2(w, make_float2(f0 ? nh.x : x.x, f1 ? nh.y : x.y), near);
+}
 
 // h -> A h + F of a stretch, two channels
 struct Map2 {
@@ -410,24 +451,47 @@ __global__ void __launch_bounds__(GatedFwdShape<T>::W * 32, GatedFwdShape<T>::kC
         if (round >= 0) gated_arrived<S - 2>();
         fetch();  // over the round before
         if (round < 0) continue;
-        const T *gs = ring + slot * 2 * TS * kGatedChannels, *xs = gs + TS * kGatedChannels;
+        T *gs = ring + slot * 2 * TS * kGatedChannels, *xs = gs + TS * kGatedChannels;
         if (++slot == S) slot = 0;
         float2 nz[TS];
         Map2 own{make_float2(1.0f, 1.0f), make_float2(0.0f, 0.0f)};
+        float low = 0.0f;
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-            nz[i] = gate_nz(ln.take(gs + i * kGatedChannels));
-            own.A = decay(nz[i], own.A);
-            own.F = gate_step(nz[i], ln.take(xs + i * kGatedChannels), own.F);
+            const float2 gate = ln.take(gs + i * kGatedChannels);
+            low = lowest(low, gate);
+            nz[i] = gate_nz(gate);
+            own.A = decay<false>(nz[i], own.A);
+            own.F = gate_step<false>(nz[i], ln.take(xs + i * kGatedChannels), own.F);
+        }
+        const bool some = __any_sync(0xffffffffu, low < kForgetGate<T>);
+        auto factor = [&](int i) { return gate_factor<T>(ln.take(gs + i * kGatedChannels)); };
+        if (some) {  // float32 factors take the gates' place, bfloat16 has no room for them and forms them again
+            own = Map2{make_float2(1.0f, 1.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll 4
+            for (int i = 0; i < TS; ++i) {
+                const float2 w = factor(i);
+                if constexpr (sizeof(T) == 4) ln.put(gs + i * kGatedChannels, w);
+                own.A = decay<true>(w, own.A);
+                own.F = gate_step<true>(w, ln.take(xs + i * kGatedChannels), own.F);
+            }
         }
         float2 h = gated_exchange<CLUSTER, false, W>(sh, ctas, prm.wait, round, own, warp, lane, rank, ranks, ok);
         if (prm.ckpt != nullptr && t0 % kGatedUnit == 0 && cnt > 0)
             ln.store_state(prm.ckpt + (long long)(span.unit + t0 / kGatedUnit) * prm.D, neg2(h));
         T *to = h_out + (long long)t0 * prm.h.st + ln.c0;
-        if (cnt >= TS) {
+        if (some) {
+#pragma unroll 4
+            for (int i = 0; i < min(cnt, TS); ++i) {
+                const float2 w = sizeof(T) == 4 ? ln.take(gs + i * kGatedChannels) : factor(i);
+                h = gate_step<true>(w, ln.take(xs + i * kGatedChannels), h);
+                ln.store_negated(to, h);
+                to += prm.h.st;
+            }
+        } else if (cnt >= TS) {
 #pragma unroll
             for (int i = 0; i < TS; ++i) {
-                h = gate_step(nz[i], ln.take(xs + i * kGatedChannels), h);
+                h = gate_step<false>(nz[i], ln.take(xs + i * kGatedChannels), h);
                 ln.store_negated(to, h);
                 to += prm.h.st;
             }
@@ -435,7 +499,7 @@ __global__ void __launch_bounds__(GatedFwdShape<T>::W * 32, GatedFwdShape<T>::kC
 #pragma unroll
             for (int i = 0; i < TS; ++i)
                 if (i < cnt) {
-                    h = gate_step(nz[i], ln.take(xs + i * kGatedChannels), h);
+                    h = gate_step<false>(nz[i], ln.take(xs + i * kGatedChannels), h);
                     ln.store_negated(to, h);
                     to += prm.h.st;
                 }
@@ -510,23 +574,54 @@ __global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kC
         if (round >= rounds) continue;
         float2 h = neg2(next);  // (here, not where it is loaded: that would wait for it)
         next = front(round - 1);
-        const T *gs = ring + slot * 3 * kTile, *xs = gs + kTile, *ds = xs + kTile;
+        T *gs = ring + slot * 3 * kTile, *xs = gs + kTile, *ds = xs + kTile;
         if (++slot == S) slot = 0;
         float2 nz[TS], za[TS], c[TS];
         Map2 back{make_float2(1.0f, 1.0f), make_float2(0.0f, 0.0f)};
         float2 F = make_float2(0.0f, 0.0f);
+        float low = 0.0f;
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-            gate_slope(ln.take(gs + i * kGatedChannels), nz[i], za[i]);
-            back.A = decay(nz[i], back.A);
-            F = gate_step(nz[i], ln.take(xs + i * kGatedChannels), F);
+            const float2 gate = ln.take(gs + i * kGatedChannels);
+            low = lowest(low, gate);
+            float2 small;
+            gate_slope(gate, nz[i], za[i], small);
+            back.A = decay<false>(nz[i], back.A);
+            F = gate_step<false>(nz[i], ln.take(xs + i * kGatedChannels), F);
         }
         auto behind = [&](int i, float2 u) {  // the gradient that reaches step i
             const float2 d = ln.take(ds + i * kGatedChannels);
             return add2(d, u);
         };
 #pragma unroll
-        for (int i = TS - 1; i >= 0; --i) back.F = decay(nz[i], behind(i, back.F));
+        for (int i = TS - 1; i >= 0; --i) back.F = decay<false>(nz[i], behind(i, back.F));
+        const bool some = __any_sync(0xffffffffu, low < kForgetGate<T>);
+        // Tiles with gates that forget: what does not fit in shared memory (float32: the factors; bfloat16: c, and factors are formed
+        // again) goes through local memory.
+        float2 local[TS];
+        auto slopes = [&](int i, float2 &n, float2 &s) {
+            const float2 gate = ln.take(gs + i * kGatedChannels);
+            float2 small;
+            gate_slope(gate, n, s, small);
+            return chosen_factor<T>(gate, small, n);
+        };
+        auto factor = [&](int i) {
+            float2 n, s;
+            return slopes(i, n, s);
+        };
+        if (some) {
+            back = Map2{make_float2(1.0f, 1.0f), make_float2(0.0f, 0.0f)};
+            F = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+            for (int i = 0; i < TS; ++i) {
+                const float2 w = factor(i);
+                if constexpr (sizeof(T) == 4) local[i] = w;
+                back.A = decay<true>(w, back.A);
+                F = gate_step<true>(w, ln.take(xs + i * kGatedChannels), F);
+            }
+#pragma unroll 4
+            for (int i = TS - 1; i >= 0; --i) back.F = decay<true>(sizeof(T) == 4 ? local[i] : factor(i), behind(i, back.F));
+        }
         fw[buf][warp][lane] = make_float4(back.A.x, back.A.y, F.x, F.y);
         float2 u = gated_exchange<CLUSTER, true, W>(sh, ctas, prm.wait, rounds - 1 - round, back, warp, lane, rank, ranks, ok);
 #pragma unroll
@@ -535,19 +630,47 @@ __global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kC
                 const float4 m = fw[buf][w][lane];
                 h = Map2{make_float2(m.x, m.y), make_float2(m.z, m.w)}(h);
             }
+        T *to_x = dx + (long long)t0 * prm.dx.st + ln.c0, *to_g = dg + (long long)t0 * prm.dg.st + ln.c0;
+        if (some) {
+#pragma unroll 4
+            for (int i = TS - 1; i >= 0; --i) {
+                const float2 ci = behind(i, u);
+                float2 w;
+                if constexpr (sizeof(T) == 4) {
+                    w = local[i];
+                    ln.put(ds + i * kGatedChannels, ci);
+                } else {
+                    w = factor(i);
+                    local[i] = ci;
+                }
+                u = decay<true>(w, ci);
+            }
+#pragma unroll 4
+            for (int i = 0; i < min(cnt, TS); ++i) {
+                float2 n, s, ci;
+                if constexpr (sizeof(T) == 4) ci = ln.take(ds + i * kGatedChannels);
+                else ci = local[i];
+                const float2 xi = ln.take(xs + i * kGatedChannels), w = slopes(i, n, s);
+                ln.store_negated(to_x, mul2(n, ci));
+                ln.store_negated(to_g, mul2(mul2(s, ci), add2(h, xi)));
+                to_x += prm.dx.st;
+                to_g += prm.dg.st;
+                h = gate_step<true>(w, xi, h);
+            }
+            continue;
+        }
 #pragma unroll
         for (int i = TS - 1; i >= 0; --i) {
             c[i] = behind(i, u);
-            u = decay(nz[i], c[i]);
+            u = decay<false>(nz[i], c[i]);
         }
-        T *to_x = dx + (long long)t0 * prm.dx.st + ln.c0, *to_g = dg + (long long)t0 * prm.dg.st + ln.c0;
         auto out = [&](int i) {  // h: negated
             const float2 xi = ln.take(xs + i * kGatedChannels);
             ln.store_negated(to_x, mul2(nz[i], c[i]));
             ln.store_negated(to_g, mul2(mul2(za[i], c[i]), add2(h, xi)));
             to_x += prm.dx.st;
             to_g += prm.dg.st;
-            h = gate_step(nz[i], xi, h);
+            h = gate_step<false>(nz[i], xi, h);
         };
         if (cnt >= TS) {
 #pragma unroll
@@ -579,8 +702,9 @@ __global__ void __launch_bounds__(256) kla_gated_step_kernel(const GatedStepPara
     const long long b = i / prm.D;
     const int d = (int)(i - b * prm.D);
     const float x = to_f32<T>(static_cast<const T *>(prm.x)[b * prm.x_sb + d]);
-    const float nz = gate_nz(make_float2(to_f32<T>(static_cast<const T *>(prm.g)[b * prm.g_sb + d]), 0.0f)).x;
-    const float s = prm.state[i], h = fmaf(nz, -x, fmaf(nz, s, s));
+    const float2 g = make_float2(to_f32<T>(static_cast<const T *>(prm.g)[b * prm.g_sb + d]), 0.0f);
+    const float2 w = gate_factor<float>(g);
+    const float h = -gate_step<true>(w, make_float2(x, 0.0f), make_float2(-prm.state[i], 0.0f)).x;
     prm.state_out[i] = h;
     static_cast<T *>(prm.h)[i] = from_f32<T>(h);
 }

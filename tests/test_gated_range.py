@@ -57,3 +57,83 @@ def test_a_state_that_requires_a_gradient_is_not_written():
     with torch.no_grad():
         kla_b200.gated_step_b200(x, g, state, state_out=leaf)
     assert leaf.any()
+
+
+U = 2.0 ** -24
+FORGET = {torch.float32: -5.0, torch.bfloat16: -8.0}  # below, a step is taken by a itself
+
+
+def relative_oracle(x, g, h0, dh, dend, forget):
+    """As ``test_gated.oracle`` for a batch, with bounds relative to what a step leaves: where a gate forgets, a is off by 2^-21 + 2^-24 |g| of
+    itself (its exponential, a reciprocal, the argument's rounding), z by that share of a, and up to eight roundings are of
+    a |h| and |x|; where it holds they are of |h| and |x|, and z's error is z's share of either. hm, um: the recurrences of absolute
+    values, which no composed map exceeds."""
+    B, L, D = x.shape
+    z, a = 1 / (1 + np.exp(g)), 1 / (1 + np.exp(-g))
+    dz = 2.0 ** -21 + U * np.minimum(np.abs(g), 104.0)
+    f = g < forget
+
+    def step(t, e, hm, xa):
+        return a[:, t] * e + np.where(f[:, t], a[:, t] * (dz[:, t] + 8 * U) * hm + (a[:, t] * dz[:, t] + 8 * U) * xa,
+                                      z[:, t] * dz[:, t] * (hm + xa) + 8 * U * (hm + xa))
+
+    h, hm, e = h0.copy(), np.abs(h0), np.zeros_like(h0)
+    hs, es = [], []
+    for t in range(L):
+        e = step(t, e, hm, np.abs(x[:, t]))
+        h, hm = a[:, t] * h + z[:, t] * x[:, t], a[:, t] * hm + z[:, t] * np.abs(x[:, t])
+        hs.append(h), es.append(e)
+    u, um, ue = dend.copy(), np.abs(dend), np.zeros_like(dend)
+    for t in reversed(range(L)):
+        c, cm = dh[:, t] + u, np.abs(dh[:, t]) + um
+        ue = step(t, ue + U * cm, cm, 0.0)
+        u, um = a[:, t] * c, a[:, t] * cm
+    return (np.stack(hs, 1), np.stack(es, 1)), (hs[-1], es[-1]), (u, ue)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("spread,keep", [(0.5, -16.0), (3.0, -6.0), (0.5, -30.0), (20.0, -20.0), (2.0, 2.0)])
+@pytest.mark.parametrize("B,L,D", [(2, 1, 64), (1, 2, 5), (3, 3, 66), (2, 70, 8), (1, 700, 64)])
+def test_what_gates_leave_when_they_forget(B, L, D, spread, keep, dtype):
+    """Without input a state, and without gradients of h the gradient of the state a sequence starts from, is a product of a's."""
+    both, h0, dh, dend = inputs(B, L, D, B, dtype, spread=spread, keep=keep)
+    gen = torch.Generator().manual_seed(1)
+    silent = torch.rand(B, L, D, generator=gen) < 0.9
+    silent[:, :, ::2] = True
+    x = both[..., :D].clone()
+    x[silent], dh[silent.flip(1)] = 0.0, 0.0
+    g = both[..., D:]
+    leaves = [t.cuda().requires_grad_() for t in (x, g, h0)]
+    h, end = kla_b200.gated_scan_b200(*leaves)
+    _, _, dstate = torch.autograd.grad((h, end), leaves, (dh.cuda(), dend.cuda()))
+    want = relative_oracle(*(t.double().numpy() for t in (x, g, h0, dh, dend)), FORGET[dtype])
+    for got, (value, bound), what in zip((h, end, dstate), want, ("h", "end", "dstate")):
+        held(got, value, bound, what)
+    one, state = kla_b200.gated_step_b200(x[:, 0].cuda(), g[:, 0].cuda(), h0.cuda())
+    held(one, want[0][0][:, 0], want[0][1][:, 0], "token")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("spread,keep", [(0.5, 9.0), (0.5, -9.0), (4.0, -4.0), (30.0, 0.0)])
+@pytest.mark.parametrize("layout", ["halves", "dense"])
+def test_gates_that_hold_and_forget_of_either_type(spread, keep, dtype, layout):
+    check(2, 700, 48, dtype, spread=spread, keep=keep, layout=layout)
+    check(1, 900, 67, dtype, spread=spread, keep=keep, layout=layout, bounds=[0, 3, 3, 400, 401, 890])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_neighbours_do_not_change_a_channels_bits(dtype):
+    """The choice between the two ways of taking a tile is a warp's; a channel whose gates hold gets the same either way."""
+    both, h0, dh, dend = (t.cuda() for t in inputs(2, 200, 64, 2, dtype))
+    got = []
+    for shut in (False, True):
+        g = both[..., 64:].clone()
+        g[..., :64] = g[..., :64].clamp_min(-2.5)
+        if shut:
+            g[:, ::7, 5] = -12.0
+        leaves = [t.detach().requires_grad_() for t in (both[..., :64], g, h0)]
+        h, end = kla_b200.gated_scan_b200(*leaves)
+        got.append((h, end, *torch.autograd.grad((h, end), leaves, (dh, dend))))
+    others = torch.arange(64, device="cuda") != 5
+    for name, a, b in zip(("h", "end", "dx", "dgate", "dstate"), *got):
+        assert torch.equal(a[..., others], b[..., others]), name
