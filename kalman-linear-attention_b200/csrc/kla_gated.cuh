@@ -7,7 +7,7 @@
 // Every channel of every sequence is a chain of its own, and over a stretch of steps both recurrences are affine maps with the
 // same slope A = prod a_t: h -> A h + F and u -> A u + R. A step is taken as h - z h + z x with two fused operations: what is
 // rounded is then small beside 1 - a where a gate holds the state for thousands of steps, which a = 1 - z rounded is not. Where a gate
-// forgets it is taken as (x - a x) + a h (kForgetGate).
+// forgets it is taken as (x - a x) + a h (kForgetGate), and where a value is infinite as kCareInfinite says.
 //
 // A CTA owns 64 channels of one sequence and walks it in tiles of W x TS steps. Each warp takes TS consecutive steps
 // of the tile, each lane two channels. The warp's rows come in by asynchronous copies into a ring of its own in shared memory,
@@ -266,7 +266,8 @@ __device__ __forceinline__ void gate_slope(float2 g, float2 &nz, float2 &za, flo
 // that have such a gate, in loops that are not unrolled and a second time over the steps: unrolled beside the others, they took
 // the backward without any such gate from 91 to 117 us (16 x 2048 x 1536, bfloat16; 94 as it is). Gates from kForgetGate on get the
 // same bits either way. Measured at that shape, gates of mean 2 / of mean 0 and deviation 1.5 / of mean -6, us: float32 forward 111 /
-// 117 / 120, backward 171 / 260 / 302; bfloat16 59 / 60 / 123, 94 / 94 / 243.
+// 115 / 127, backward 171 / 268 / 321; bfloat16 58 / 58 / 132, 95 / 95 / 254. What infinite values need is a third way (kCareInfinite), for
+// tiles whose map turned out NaN or whose first state is infinite: within the second it would cost as much again.
 template <typename T>
 constexpr float kForgetGate = sizeof(T) == 2 ? -8.0f : -5.0f;
 __device__ __forceinline__ bool forgets(float w) { return __float_as_int(w) >= 0; }
@@ -282,18 +283,39 @@ __device__ __forceinline__ float2 gate_factor(float2 g) {
 __device__ __forceinline__ float lowest(float low, float2 g) { return fminf(low, fminf(g.x, g.y)); }
 // A step for two channels of the negated state, -h_t = -h + z h - z x, and the factor alone. (The state is carried negated because -z
 // comes out of the gate and x out of memory as they are: each negation would be an operation a step.)
-template <bool FORGETS>
-__device__ __forceinline__ float2 decay(float2 w, float2 v) {
-    return fma2(w, v, FORGETS ? make_float2(forgets(w.x) ? 0.0f : v.x, forgets(w.y) ? 0.0f : v.y) : v);
+enum GatedCare {
+    kCareNone = 0,      // no gate below kForgetGate
+    kCareForgets = 1,
+    kCareInfinite = 2   // also infinite values as the formula takes them: a inf is inf as long as a is not 0, where inf - z inf is NaN
+};
+__device__ __forceinline__ bool infinite(float v) { return fabsf(v) == __int_as_float(0x7f800000); }
+__device__ __forceinline__ bool infinite(float2 v) { return infinite(v.x) || infinite(v.y); }
+__device__ __forceinline__ bool nan(float2 v) { return v.x != v.x || v.y != v.y; }
+template <int CARE>
+__device__ __forceinline__ float2 factor_of(float2 v) {  // what a factor multiplies beside v itself
+    return CARE == kCareInfinite ? make_float2(infinite(v.x) ? 0.0f : v.x, infinite(v.y) ? 0.0f : v.y) : v;
 }
-template <bool FORGETS>
+template <int CARE>
+__device__ __forceinline__ float2 decay(float2 w, float2 v) {
+    if (CARE == kCareNone) return fma2(w, v, v);
+    const bool f0 = forgets(w.x), f1 = forgets(w.y);
+    const float2 u = factor_of<CARE>(v);
+    return fma2(w, make_float2(f0 ? v.x : u.x, f1 ? v.y : u.y), make_float2(f0 ? 0.0f : v.x, f1 ? 0.0f : v.y));
+}
+template <int CARE>
 __device__ __forceinline__ float2 gate_step(float2 w, float2 x, float2 nh) {
-    if (!FORGETS) return fma2(w, x, fma2(w, nh, nh));
+    if (CARE == kCareNone) return fma2(w, x, fma2(w, nh, nh));
     // the larger term first: it alone cannot overflow
     const bool f0 = forgets(w.x), f1 = forgets(w.y);
-    const float2 near = fma2(w, make_float2(f0 ? x.x : nh.x, f1 ? x.y : nh.y), make_float2(f0 ? -x.x : nh.x, f1 ? -x.y : nh.y));
+    const float2 near = fma2(w, factor_of<CARE>(make_float2(f0 ? x.x : nh.x, f1 ? x.y : nh.y)), make_float2(f0 ? -x.x : nh.x, f1 ? -x.y : nh.y));
     return fma2(w, make_float2(f0 ? nh.x : x.x, f1 ? nh.y : x.y), near);
 }
+
+// A slope that fell below float32's range is its least number, not 0: an infinite state goes through it, as it does step by step.
+// Only a factor of 0, a gate that leaves nothing, makes 0 (and NaN of an infinite state).
+constexpr float kLeastSlope = 1.401298464e-45f;
+__device__ __forceinline__ bool resets(float w) { return __float_as_uint(w) == 0u; }
+__device__ __forceinline__ float slope_product(float a, float b) { return fmaxf(a * b, fminf(fminf(a, b), kLeastSlope)); }
 
 // h -> A h + F of a stretch, two channels
 struct Map2 {
@@ -372,7 +394,7 @@ __device__ __forceinline__ float2 gated_exchange(GatedShared<CLUSTER, W> &sh, fl
             for (int i = 0; i < W; ++i) {
                 const Map2 m = map(sh.warp[buf][i][lane]);
                 all.F = m(all.F);
-                all.A = make_float2(m.A.x * all.A.x, m.A.y * all.A.y);
+                all.A = make_float2(slope_product(m.A.x, all.A.x), slope_product(m.A.y, all.A.y));
             }
             const float4 v = make_float4(all.A.x, all.A.y, all.F.x, all.F.y);
             const uint32_t here = smem_u32(ctas + rank * 32), bar = smem_u32(&sh.arrived[buf]);
@@ -461,37 +483,67 @@ __global__ void __launch_bounds__(GatedFwdShape<T>::W * 32, GatedFwdShape<T>::kC
             const float2 gate = ln.take(gs + i * kGatedChannels);
             low = lowest(low, gate);
             nz[i] = gate_nz(gate);
-            own.A = decay<false>(nz[i], own.A);
-            own.F = gate_step<false>(nz[i], ln.take(xs + i * kGatedChannels), own.F);
+            own.A = decay<kCareNone>(nz[i], own.A);
+            own.F = gate_step<kCareNone>(nz[i], ln.take(xs + i * kGatedChannels), own.F);
         }
-        const bool some = __any_sync(0xffffffffu, low < kForgetGate<T>);
         auto factor = [&](int i) { return gate_factor<T>(ln.take(gs + i * kGatedChannels)); };
-        if (some) {  // float32 factors take the gates' place, bfloat16 has no room for them and forms them again
+        // The map with care, and the least its slope may be. float32 factors take the gates' place, bfloat16 has no room for them and forms
+        // them again.
+        bool made = false;
+        auto careful = [&](auto care_) {
+            constexpr int CARE = decltype(care_)::value;
             own = Map2{make_float2(1.0f, 1.0f), make_float2(0.0f, 0.0f)};
+            bool r0 = false, r1 = false;
 #pragma unroll 4
             for (int i = 0; i < TS; ++i) {
-                const float2 w = factor(i);
+                float2 w;
+                if (sizeof(T) == 4 && made) w = ln.take(gs + i * kGatedChannels);
+                else w = factor(i);
                 if constexpr (sizeof(T) == 4) ln.put(gs + i * kGatedChannels, w);
-                own.A = decay<true>(w, own.A);
-                own.F = gate_step<true>(w, ln.take(xs + i * kGatedChannels), own.F);
+                r0 |= resets(w.x);
+                r1 |= resets(w.y);
+                own.A = decay<CARE>(w, own.A);
+                own.F = gate_step<CARE>(w, ln.take(xs + i * kGatedChannels), own.F);
+            }
+            made = true;
+            return make_float2(r0 ? 0.0f : kLeastSlope, r1 ? 0.0f : kLeastSlope);
+        };
+        float2 least = dup2(kLeastSlope);
+        int care = kCareNone;
+        if (__any_sync(0xffffffffu, low < kForgetGate<T> || nan(own.F))) {
+            care = kCareForgets;
+            least = careful(std::integral_constant<int, kCareForgets>{});
+            if (__any_sync(0xffffffffu, nan(own.F))) {  // of an infinite value, or of the inputs
+                care = kCareInfinite;
+                careful(std::integral_constant<int, kCareInfinite>{});
             }
         }
+        own.A = make_float2(fmaxf(own.A.x, least.x), fmaxf(own.A.y, least.y));
         float2 h = gated_exchange<CLUSTER, false, W>(sh, ctas, prm.wait, round, own, warp, lane, rank, ranks, ok);
         if (prm.ckpt != nullptr && t0 % kGatedUnit == 0 && cnt > 0)
             ln.store_state(prm.ckpt + (long long)(span.unit + t0 / kGatedUnit) * prm.D, neg2(h));
+        if (__any_sync(0xffffffffu, infinite(h))) {
+            care = kCareInfinite;
+            if (sizeof(T) == 4 && !made) careful(std::integral_constant<int, kCareInfinite>{});
+        }
         T *to = h_out + (long long)t0 * prm.h.st + ln.c0;
-        if (some) {
+        auto walk = [&](auto care_) {
 #pragma unroll 4
             for (int i = 0; i < min(cnt, TS); ++i) {
                 const float2 w = sizeof(T) == 4 ? ln.take(gs + i * kGatedChannels) : factor(i);
-                h = gate_step<true>(w, ln.take(xs + i * kGatedChannels), h);
+                h = gate_step<decltype(care_)::value>(w, ln.take(xs + i * kGatedChannels), h);
                 ln.store_negated(to, h);
                 to += prm.h.st;
             }
+        };
+        if (care == kCareInfinite) {
+            walk(std::integral_constant<int, kCareInfinite>{});
+        } else if (care == kCareForgets) {
+            walk(std::integral_constant<int, kCareForgets>{});
         } else if (cnt >= TS) {
 #pragma unroll
             for (int i = 0; i < TS; ++i) {
-                h = gate_step<false>(nz[i], ln.take(xs + i * kGatedChannels), h);
+                h = gate_step<kCareNone>(nz[i], ln.take(xs + i * kGatedChannels), h);
                 ln.store_negated(to, h);
                 to += prm.h.st;
             }
@@ -499,7 +551,7 @@ __global__ void __launch_bounds__(GatedFwdShape<T>::W * 32, GatedFwdShape<T>::kC
 #pragma unroll
             for (int i = 0; i < TS; ++i)
                 if (i < cnt) {
-                    h = gate_step<false>(nz[i], ln.take(xs + i * kGatedChannels), h);
+                    h = gate_step<kCareNone>(nz[i], ln.take(xs + i * kGatedChannels), h);
                     ln.store_negated(to, h);
                     to += prm.h.st;
                 }
@@ -586,16 +638,15 @@ __global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kC
             low = lowest(low, gate);
             float2 small;
             gate_slope(gate, nz[i], za[i], small);
-            back.A = decay<false>(nz[i], back.A);
-            F = gate_step<false>(nz[i], ln.take(xs + i * kGatedChannels), F);
+            back.A = decay<kCareNone>(nz[i], back.A);
+            F = gate_step<kCareNone>(nz[i], ln.take(xs + i * kGatedChannels), F);
         }
         auto behind = [&](int i, float2 u) {  // the gradient that reaches step i
             const float2 d = ln.take(ds + i * kGatedChannels);
             return add2(d, u);
         };
 #pragma unroll
-        for (int i = TS - 1; i >= 0; --i) back.F = decay<false>(nz[i], behind(i, back.F));
-        const bool some = __any_sync(0xffffffffu, low < kForgetGate<T>);
+        for (int i = TS - 1; i >= 0; --i) back.F = decay<kCareNone>(nz[i], behind(i, back.F));
         // Tiles with gates that forget: what does not fit in shared memory (float32: the factors; bfloat16: c, and factors are formed
         // again) goes through local memory.
         float2 local[TS];
@@ -609,19 +660,37 @@ __global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kC
             float2 n, s;
             return slopes(i, n, s);
         };
-        if (some) {
+        bool made = false;
+        auto careful = [&](auto care_) {
+            constexpr int CARE = decltype(care_)::value;
             back = Map2{make_float2(1.0f, 1.0f), make_float2(0.0f, 0.0f)};
             F = make_float2(0.0f, 0.0f);
+            bool r0 = false, r1 = false;
 #pragma unroll 4
             for (int i = 0; i < TS; ++i) {
                 const float2 w = factor(i);
                 if constexpr (sizeof(T) == 4) local[i] = w;
-                back.A = decay<true>(w, back.A);
-                F = gate_step<true>(w, ln.take(xs + i * kGatedChannels), F);
+                r0 |= resets(w.x);
+                r1 |= resets(w.y);
+                back.A = decay<CARE>(w, back.A);
+                F = gate_step<CARE>(w, ln.take(xs + i * kGatedChannels), F);
             }
 #pragma unroll 4
-            for (int i = TS - 1; i >= 0; --i) back.F = decay<true>(sizeof(T) == 4 ? local[i] : factor(i), behind(i, back.F));
+            for (int i = TS - 1; i >= 0; --i) back.F = decay<CARE>(sizeof(T) == 4 ? local[i] : factor(i), behind(i, back.F));
+            made = true;
+            return make_float2(r0 ? 0.0f : kLeastSlope, r1 ? 0.0f : kLeastSlope);
+        };
+        float2 least = dup2(kLeastSlope);
+        int care = kCareNone;
+        if (__any_sync(0xffffffffu, low < kForgetGate<T> || nan(F) || nan(back.F))) {
+            care = kCareForgets;
+            least = careful(std::integral_constant<int, kCareForgets>{});
+            if (__any_sync(0xffffffffu, nan(F) || nan(back.F))) {
+                care = kCareInfinite;
+                careful(std::integral_constant<int, kCareInfinite>{});
+            }
         }
+        back.A = make_float2(fmaxf(back.A.x, least.x), fmaxf(back.A.y, least.y));
         fw[buf][warp][lane] = make_float4(back.A.x, back.A.y, F.x, F.y);
         float2 u = gated_exchange<CLUSTER, true, W>(sh, ctas, prm.wait, rounds - 1 - round, back, warp, lane, rank, ranks, ok);
 #pragma unroll
@@ -630,8 +699,13 @@ __global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kC
                 const float4 m = fw[buf][w][lane];
                 h = Map2{make_float2(m.x, m.y), make_float2(m.z, m.w)}(h);
             }
+        if (__any_sync(0xffffffffu, infinite(u) || infinite(h))) {
+            care = kCareInfinite;
+            if (sizeof(T) == 4 && !made) careful(std::integral_constant<int, kCareInfinite>{});
+        }
         T *to_x = dx + (long long)t0 * prm.dx.st + ln.c0, *to_g = dg + (long long)t0 * prm.dg.st + ln.c0;
-        if (some) {
+        auto walk = [&](auto care_) {
+            constexpr int CARE = decltype(care_)::value;
 #pragma unroll 4
             for (int i = TS - 1; i >= 0; --i) {
                 const float2 ci = behind(i, u);
@@ -643,7 +717,7 @@ __global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kC
                     w = factor(i);
                     local[i] = ci;
                 }
-                u = decay<true>(w, ci);
+                u = decay<CARE>(w, ci);
             }
 #pragma unroll 4
             for (int i = 0; i < min(cnt, TS); ++i) {
@@ -655,14 +729,18 @@ __global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kC
                 ln.store_negated(to_g, mul2(mul2(s, ci), add2(h, xi)));
                 to_x += prm.dx.st;
                 to_g += prm.dg.st;
-                h = gate_step<true>(w, xi, h);
+                h = gate_step<CARE>(w, xi, h);
             }
+        };
+        if (care != kCareNone) {
+            if (care == kCareInfinite) walk(std::integral_constant<int, kCareInfinite>{});
+            else walk(std::integral_constant<int, kCareForgets>{});
             continue;
         }
 #pragma unroll
         for (int i = TS - 1; i >= 0; --i) {
             c[i] = behind(i, u);
-            u = decay<false>(nz[i], c[i]);
+            u = decay<kCareNone>(nz[i], c[i]);
         }
         auto out = [&](int i) {  // h: negated
             const float2 xi = ln.take(xs + i * kGatedChannels);
@@ -670,7 +748,7 @@ __global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kC
             ln.store_negated(to_g, mul2(mul2(za[i], c[i]), add2(h, xi)));
             to_x += prm.dx.st;
             to_g += prm.dg.st;
-            h = gate_step<false>(nz[i], xi, h);
+            h = gate_step<kCareNone>(nz[i], xi, h);
         };
         if (cnt >= TS) {
 #pragma unroll
@@ -704,7 +782,7 @@ __global__ void __launch_bounds__(256) kla_gated_step_kernel(const GatedStepPara
     const float x = to_f32<T>(static_cast<const T *>(prm.x)[b * prm.x_sb + d]);
     const float2 g = make_float2(to_f32<T>(static_cast<const T *>(prm.g)[b * prm.g_sb + d]), 0.0f);
     const float2 w = gate_factor<float>(g);
-    const float h = -gate_step<true>(w, make_float2(x, 0.0f), make_float2(-prm.state[i], 0.0f)).x;
+    const float h = -gate_step<kCareInfinite>(w, make_float2(x, 0.0f), make_float2(-prm.state[i], 0.0f)).x;
     prm.state_out[i] = h;
     static_cast<T *>(prm.h)[i] = from_f32<T>(h);
 }

@@ -137,3 +137,49 @@ def test_neighbours_do_not_change_a_channels_bits(dtype):
     others = torch.arange(64, device="cuda") != 5
     for name, a, b in zip(("h", "end", "dx", "dgate", "dstate"), *got):
         assert torch.equal(a[..., others], b[..., others]), name
+
+
+def same_kinds(got, want, what):
+    got = got.detach().double().cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(want)), f"{what}: NaN"
+    assert np.array_equal(np.where(np.isinf(got), got, 0.0), np.where(np.isinf(want), want, 0.0)), f"{what}: infinities"
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("spread,keep", [(1.0, 2.0), (1.5, -1.0), (1.0, -6.0)])
+@pytest.mark.parametrize("B,L,D,bounds", [(2, 300, 24, None), (1, 2500, 24, None), (3, 70, 65, None), (1, 900, 24, [0, 40, 41, 41, 700, 880]), (2, 1, 24, None)])
+def test_infinite_values_are_taken_as_the_formula_takes_them(B, L, D, bounds, spread, keep, dtype):
+    """a inf is inf while a is not 0: inputs, states and gradients that are infinite leave infinite values behind, of their sign; NaN
+    comes of infinities that meet with opposite signs and of a gate that leaves nothing. Other channels keep their bits."""
+    n = B if bounds is None else len(bounds) - 1
+    both, h0, dh, dend = inputs(B, L, D, n, dtype, spread=spread, keep=keep)
+    cu = None if bounds is None else torch.tensor(bounds, dtype=torch.int32, device="cuda")
+    inf, i, j = float("inf"), L // 3, 2 * L // 3
+    runs = []
+    for broken in (False, True):
+        x, g, s, d, e = both[..., :D].clone(), both[..., D:].clone(), h0.clone(), dh.clone(), dend.clone()
+        if broken:
+            x[:, i, 0] = inf
+            x[:, L - 1, 1] = -inf
+            s[:, 2] = inf
+            x[:, i, 3], x[:, j, 3] = inf, -inf
+            d[:, j, 4] = inf
+            e[:, 5] = -inf
+            x[:, i, 6], g[:, j, 6] = inf, -inf
+            x[:, i, 7], g[:, i, 7] = -inf, -inf
+            d[:, j, 8], d[:, i, 8] = inf, -inf
+            s[:, 9], d[:, j, 9] = -inf, inf
+            x[:, i, 10], g[:, j, 10] = inf, inf
+        leaves = [t.cuda().requires_grad_() for t in (x, g, s)]
+        h, end = kla_b200.gated_scan_b200(*leaves, cu_seqlens=cu)
+        runs.append((h, end, *torch.autograd.grad((h, end), leaves, (d.cuda(), e.cuda()))))
+    with np.errstate(all="ignore"):
+        want, _ = oracle(*(t.double().numpy() for t in (x, g, s)), bounds, d.double().numpy(), e.double().numpy())
+    for name, clean, got in zip(("h", "end", "dx", "dgate", "dstate"), *runs):
+        same_kinds(got, want[name], name)
+        assert torch.equal(got[..., 11:], clean[..., 11:]), name
+    with np.errstate(all="ignore"):
+        first, _ = oracle(*(t.double().numpy() for t in (x[:, :1], g[:, :1], s[:B])))
+    token, state = kla_b200.gated_step_b200(leaves[0].detach()[:, 0], leaves[1].detach()[:, 0], leaves[2].detach()[:B].contiguous())
+    same_kinds(token, first["h"][:, 0], "token")
+    same_kinds(state, first["end"], "state")
