@@ -103,18 +103,19 @@ int slots_of(bool bf16, bool pairs, bool backward, Slots *out) {
 // launching takes `start`; and no choice is faster than 80 % of the memory's rate. Measured, clusters of 1 / 2 / 4 / 8: forward bfloat16
 // B=4 L=8192 D=2048 102 / 85 / 93 / 105, B=16 L=2048 D=1536 60 / 72 / 84 / 107, B=1 L=8192 D=1024 98 / 62 / 33 / 24, B=8 L=512 D=768
 // 8.3 / 8.7 / 11.5 / 17.6; backward 103 / 119 / 129 / 148 (B=16 ...), 192 / 121 / 65 / 45 (B=1 ...), 14.2 / 13.7 / 10.7 / 13.8 (B=8 ...).
-// Of packed sequences the host knows the number and the sum of the lengths; the longest of n random ones is about ln n + 0.6 times
-// their mean. They take as long as the longest does or as all their rounds do with full SMs (half a round of a CTA is left over at each
+// Of packed sequences the host knows the number and the sum of the lengths (a lone one is a batch of one); the longest of n random
+// ones is about ln n + 0.6 times their mean. They take as long as the longest does or as all their rounds do with full SMs (half a round of a CTA is left over at each
 // end), and a start per wave. Clusters of 1 / 2 / 4 / 6 / 8: 40 in 32768 rows of 1536, bfloat16, forward 84 / 86 / 115 / 139 / 240,
 // 12 in 32768 of 768 103 / 78 / 51 / 55 / 65, 3 in 65536 of 256 420 / 253 / 134 / 94 / 73, 60 in 2000 of 300, float32, 7 / 12 / 18 / 27 /
 // 48, 9 in 6001 of 1024 44 / 34 / 25 / 23 / 36 (nine of one length 18 / 18 / 25 / 26 / 42).
 int pick_ranks(const Slots &slots, const Kernel &k, int64_t blocks, int64_t rows, int64_t sequences, int64_t L, bool packed, bool backward, size_t esz, int64_t D) {
+    packed = packed && sequences > 1;
     const double sms = device_sms();
     const int64_t cells = sequences * blocks;
     const double round = backward ? (esz == 2 ? 1.5 : 2.2) : (esz == 2 ? 1.53 : 1.15);
     constexpr double shares[kRankCount] = {1.0, 1.27, 1.32, 1.37, 1.42, 1.47, 1.6}, starts[kRankCount] = {2.0, 3.5, 4.3, 5.0, 5.3, 5.6, 6.0};
     double steps = (double)L;
-    if (packed && sequences > 0) steps = std::min(steps, (double)L / sequences * (std::log((double)sequences) + 0.6));
+    if (packed) steps = std::min(steps, (double)L / sequences * (std::log((double)sequences) + 0.6));
     const double tiles = std::ceil(steps / k.tile), least_us = (double)rows * D * esz * (backward ? 5 : 3) / 5.2e6;
     int best = 1;
     double least = 0.0;

@@ -183,3 +183,17 @@ def test_infinite_values_are_taken_as_the_formula_takes_them(B, L, D, bounds, sp
     token, state = kla_b200.gated_step_b200(leaves[0].detach()[:, 0], leaves[1].detach()[:, 0], leaves[2].detach()[:B].contiguous())
     same_kinds(token, first["h"][:, 0], "token")
     same_kinds(state, first["end"], "state")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("L,D", [(300, 64), (400, 1024), (700, 256), (1000, 1536), (2000, 64), (2500, 2048)])
+def test_a_lone_packed_sequence_is_taken_as_a_batch_of_one(L, D, dtype):
+    """The same CTAs share it: the same bits."""
+    both, h0, dh, dend = (t.cuda() for t in inputs(1, L, D, 1, dtype))
+    got = []
+    for cu in (None, torch.tensor([0, L], dtype=torch.int32, device="cuda")):
+        leaves = [t.detach().requires_grad_() for t in (both[..., :D], both[..., D:], h0)]
+        h, end = kla_b200.gated_scan_b200(*leaves, cu_seqlens=cu)
+        got.append((h, end, *torch.autograd.grad((h, end), leaves, (dh, dend))))
+    for name, a, b in zip(("h", "end", "dx", "dgate", "dstate"), *got):
+        assert torch.equal(a, b), name
