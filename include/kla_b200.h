@@ -633,6 +633,9 @@ size_t kla_b200_mlp_fwd_work_bytes(const kla_b200_mlp_args *args); /* 0: none */
 size_t kla_b200_mlp_work_bytes(const kla_b200_mlp_args *args);
 int kla_b200_mlp_fwd(const kla_b200_mlp_args *args, void *stream);
 int kla_b200_mlp_bwd(const kla_b200_mlp_args *args, void *stream);
+/* How a call with working memory takes one of its products on the current device: columns of a tile, CTAs that share it (1 or 2) and
+ * shares of the summed axis, by the sizes in args alone. product: 0 gate and up, 1 y, 2 gradients of gate and up, 3 dx, 4 dw3, 5 dw12. */
+int kla_b200_mlp_plan(const kla_b200_mlp_args *args, int product, int *columns, int *ctas, int *splits);
 
 /* Human-readable text for a return code; for KLA_B200_ECUDA it includes the
  * CUDA error string of the failing call on this thread. */

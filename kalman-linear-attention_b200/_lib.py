@@ -50,6 +50,7 @@ SYMBOLS = (
     "kla_b200_mlp_work_bytes",
     "kla_b200_mlp_fwd",
     "kla_b200_mlp_bwd",
+    "kla_b200_mlp_plan",
     "kla_b200_strerror",
     "kla_b200_version",
     "kla_b200_launch_count",
@@ -306,6 +307,8 @@ def load() -> ctypes.CDLL:
         fn = getattr(lib, "kla_b200_" + name)
         fn.restype = c_int
         fn.argtypes = [POINTER(MlpArgs), c_void_p]
+    lib.kla_b200_mlp_plan.restype = c_int
+    lib.kla_b200_mlp_plan.argtypes = [POINTER(MlpArgs), c_int, *[POINTER(c_int)] * 3]
     lib.kla_b200_conv_step.restype = c_int
     lib.kla_b200_conv_step.argtypes = [POINTER(ConvStepArgs), c_void_p]
     lib.kla_b200_conv_seq.restype = c_int

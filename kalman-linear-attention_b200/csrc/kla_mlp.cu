@@ -317,6 +317,16 @@ size_t kla_b200_mlp_work_bytes(const kla_b200_mlp_args *a) {
     return (size_t)work_of(*a, device_sms()).all * sizeof(float);
 }
 
+int kla_b200_mlp_plan(const kla_b200_mlp_args *a, int which, int *columns, int *ctas, int *splits) {
+    if (const int rc = check_sizes(a)) return rc;
+    if (a->rows == 0 || which < 0 || which > 5 || columns == nullptr || ctas == nullptr || splits == nullptr) return KLA_B200_EINVAL;
+    constexpr Product (*products[6])(const kla_b200_mlp_args &) = {product_gate_up, product_down, product_dgu, product_dx, product_dw3, product_dw12};
+    const Product p = products[which](*a);
+    const Plan pl = plan(p, p.mode != kMlpGated && p.mode != kMlpGrad, device_sms());
+    *columns = pl.BN; *ctas = pl.CG; *splits = pl.splits;
+    return KLA_B200_OK;
+}
+
 int kla_b200_mlp_bwd(const kla_b200_mlp_args *a, void *stream) {
     int rc = check_sizes(a);
     if (rc) return rc;
