@@ -197,3 +197,29 @@ def test_a_lone_packed_sequence_is_taken_as_a_batch_of_one(L, D, dtype):
         got.append((h, end, *torch.autograd.grad((h, end), leaves, (dh, dend))))
     for name, a, b in zip(("h", "end", "dx", "dgate", "dstate"), *got):
         assert torch.equal(a, b), name
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("L,bounds", [(300, None), (2500, None), (900, [0, 40, 41, 41, 700, 880]), (1, None)])
+def test_nan_reaches_what_the_formula_takes_it_to(L, bounds, dtype):
+    D, i = 24, L // 3
+    n = 1 if bounds is None else len(bounds) - 1
+    both, h0, dh, dend = inputs(1, L, D, n, dtype)
+    cu = None if bounds is None else torch.tensor(bounds, dtype=torch.int32, device="cuda")
+    runs, nan = [], float("nan")
+    for broken in (False, True):
+        x, g, s, d, e = both[..., :D].clone(), both[..., D:].clone(), h0.clone(), dh.clone(), dend.clone()
+        if broken:
+            x[:, i, 0] = nan
+            g[:, i, 1] = nan
+            s[:, 2] = nan
+            d[:, i, 3] = nan
+            e[:, 4] = nan
+        leaves = [t.cuda().requires_grad_() for t in (x, g, s)]
+        h, end = kla_b200.gated_scan_b200(*leaves, cu_seqlens=cu)
+        runs.append((h, end, *torch.autograd.grad((h, end), leaves, (d.cuda(), e.cuda()))))
+    with np.errstate(all="ignore"):
+        want, _ = oracle(*(t.double().numpy() for t in (x, g, s)), bounds, d.double().numpy(), e.double().numpy())
+    for name, clean, got in zip(("h", "end", "dx", "dgate", "dstate"), *runs):
+        same_kinds(got, want[name], name)
+        assert torch.equal(got[..., 5:], clean[..., 5:]), name

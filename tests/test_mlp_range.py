@@ -84,3 +84,26 @@ def test_the_kept_range_and_its_steps(scale, sign):
     _, grads = gradients(t, dy, None)
     held(grads["w12"], want["dw12"], "dw12")
     held(grads["b12"], want["db12"], "db12")
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu", None])
+def test_the_oracle_itself_is_differences(act):
+    """``test_mlp.oracle``'s own values, for every activation, with biases and residual."""
+    gen = torch.Generator().manual_seed(2)
+    rows, d, H, out, step = 3, 4, 5, 2, 1e-5
+    sizes = dict(x=(rows, d), w12=(2 * H, d), w3=(out, H), b12=(2 * H,), b3=(out,), residual=(rows, out))
+    t = {n: torch.randn(*sizes[n], generator=gen, dtype=torch.float64) for n in NAMES}
+    dy = torch.randn(rows, out, generator=gen, dtype=torch.float64)
+    want = oracle(*t.values(), act, dy)
+    gu = t["x"] @ t["w12"].T + t["b12"]
+    assert act != "relu" or gu[:, :H].abs().min() > 100 * step  # no difference crosses the kink
+    loss = lambda given: (oracle(*given.values(), act, None)["y"].x.cpu() * dy).sum().item()  # noqa: E731
+    for n in NAMES:
+        for i in range(t[n].numel()):
+            v = []
+            for sign in (step, -step):
+                moved = {k: a.clone() for k, a in t.items()}
+                moved[n].view(-1)[i] += sign
+                v.append(loss(moved))
+            # third derivatives of order 10 times step^2, and 2^-53 / step of sums of order 10
+            assert abs((v[0] - v[1]) / (2 * step) - want["d" + n].x.reshape(-1)[i].item()) < 1e-8, (n, i)
