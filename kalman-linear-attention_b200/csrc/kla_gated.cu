@@ -98,21 +98,22 @@ int slots_of(bool bf16, bool pairs, bool backward, Slots *out) {
     return KLA_B200_OK;
 }
 
-// How many CTAs of a cluster share a sequence: the least time by a model of what was measured on B200 (us). A round, a tile of each
-// CTA of a cluster, takes `round` alone on its SM and by `share` more for the exchange; a second and third CTA on the SM add 35 % each;
-// launching takes `start`; and no choice is faster than 80 % of the memory's rate. Measured, clusters of 1 / 2 / 4 / 8: forward bfloat16
-// B=4 L=8192 D=2048 102 / 85 / 93 / 105, B=16 L=2048 D=1536 60 / 72 / 84 / 107, B=1 L=8192 D=1024 98 / 62 / 33 / 24, B=8 L=512 D=768
-// 8.3 / 8.7 / 11.5 / 17.6; backward 103 / 119 / 129 / 148 (B=16 ...), 192 / 121 / 65 / 45 (B=1 ...), 14.2 / 13.7 / 10.7 / 13.8 (B=8 ...).
-// Of packed sequences the host knows the number and the sum of the lengths (a lone one is a batch of one); the longest of n random
-// ones is about ln n + 0.6 times their mean. They take as long as the longest does or as all their rounds do with full SMs (half a round of a CTA is left over at each
-// end), and a start per wave. Clusters of 1 / 2 / 4 / 6 / 8: 40 in 32768 rows of 1536, bfloat16, forward 84 / 86 / 115 / 139 / 240,
-// 12 in 32768 of 768 103 / 78 / 51 / 55 / 65, 3 in 65536 of 256 420 / 253 / 134 / 94 / 73, 60 in 2000 of 300, float32, 7 / 12 / 18 / 27 /
-// 48, 9 in 6001 of 1024 44 / 34 / 25 / 23 / 36 (nine of one length 18 / 18 / 25 / 26 / 42).
+// How many CTAs of a cluster share a sequence: the least time (us) by a model. A round, a tile of each CTA of a cluster, takes `round`
+// alone on its SM and by `share` more for the exchange; a second and third CTA on the SM add 35 % each; launching takes `start`; and no
+// choice is faster than 80 % of the memory's rate. Of packed sequences the host knows the number and the sum of the lengths (a lone one
+// is a batch of one); the longest of n random ones is about ln n + 0.6 times their mean. They take as long as the longest does or as
+// all their rounds do with full SMs (half a round of a CTA is left over at each end), and a start per wave. `round` is what makes the
+// choice best over 19 shapes, both types and directions, each measured with every size of cluster on B200: 1.7 % slower than the
+// best one's kernel on average, 17 % at most. Measured with clusters of 1 / 2 / 4 / 8: forward bfloat16 B=4 L=8192 D=2048 106 / 87 / 103 / 110,
+// B=16 L=2048 D=1536 60 / 64 / 71 / 111, B=1 L=8192 D=1024 103 / 67 / 36 / 26, B=8 L=512 D=768 8.7 / 9.1 / 7.9 / 18.3; backward 183 / 155 / 159 / 165,
+// 95 / 108 / 115 / 139, 177 / 115 / 61 / 43, 13.8 / 13.6 / 10.6 / 13.4. Packed, clusters of 1 / 2 / 4 / 6 / 8: 40 in 32768 rows of 1536, bfloat16, forward
+// 83 / 93 / 113 / 142 / 242, 12 in 32768 of 768 122 / 89 / 65 / 67 / 74, 3 in 65536 of 256 416 / 259 / 138 / 96 / 76, 60 in 2000 of 300, float32, 7 / 13 /
+// 19 / 28 / 50, 9 in 6001 of 1024 48 / 36 / 26 / 24 / 36.
 int pick_ranks(const Slots &slots, const Kernel &k, int64_t blocks, int64_t rows, int64_t sequences, int64_t L, bool packed, bool backward, size_t esz, int64_t D) {
     packed = packed && sequences > 1;
     const double sms = device_sms();
     const int64_t cells = sequences * blocks;
-    const double round = backward ? (esz == 2 ? 1.5 : 2.2) : (esz == 2 ? 1.53 : 1.15);
+    const double round = backward ? (esz == 2 ? 1.43 : 2.5) : (esz == 2 ? 1.37 : 1.38);
     constexpr double shares[kRankCount] = {1.0, 1.27, 1.32, 1.37, 1.42, 1.47, 1.6}, starts[kRankCount] = {2.0, 3.5, 4.3, 5.0, 5.3, 5.6, 6.0};
     double steps = (double)L;
     if (packed) steps = std::min(steps, (double)L / sequences * (std::log((double)sequences) + 0.6));
