@@ -19,11 +19,12 @@
 // With a cluster of CTAs a sequence's tiles go round robin to its CTAs, which exchange their tiles' maps through distributed
 // shared memory once a round: the way to fill the GPU with few sequences or channels.
 //
-// What bounds it: memory as long as the exponential and the two passes over a step's maps keep up. Forward a pair of steps costs 33
-// instructions of a warp, backward 71, with half of the schedulers' slots used (a chain of 4 to 8 warps a scheduler). Measured in
-// bfloat16: 4 x 8192 x 2048 forward 84 us (4.8 TB/s of x, g and h, of 6.55 that a copy reaches); 16 x 2048 x 1536 forward 60 us,
-// backward 92 (5.5 TB/s); 1 x 65536 x 4096 forward 310 us (5.2 TB/s), backward 546 (4.9). Not kept, as they were slower: eight
-// steps a warp with three or four CTAs an SM, two chains a warp, z kept in shared memory, rings of more tiles.
+// What bounds it: memory as long as the exponential and the two passes over a step's maps keep up. Forward a pair of steps costs 35
+// instructions of a warp, backward 74, with half of the schedulers' slots used (a chain of 4 to 8 warps a scheduler). Measured in
+// bfloat16: 4 x 8192 x 2048 forward 84 us (4.8 TB/s of x, g and h, of 6.55 that a copy reaches); 16 x 2048 x 1536 forward 59 us,
+// backward 95 (5.3 TB/s); 1 x 65536 x 4096 forward 320 us (5.0 TB/s), backward 566 (4.7); float32, 16 x 2048 x 1536, forward 111 (5.4 TB/s),
+// backward 171 (5.9). Not kept, as they were slower: eight steps a warp with three or four CTAs an SM, two chains a warp, z kept in
+// shared memory, rings of more tiles.
 #pragma once
 
 #include <type_traits>

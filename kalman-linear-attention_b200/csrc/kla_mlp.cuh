@@ -19,9 +19,11 @@
 // of a tile cost only the padding.
 //
 // What bounds it: 18 M D H operations forward and backward together for M rows, and for few rows the weights, once from memory. Measured
-// at 32768 rows of 768 with H = 2048, forward and backward together 922 us of 556 at the rate of a library product in a burst of its
-// own (1668 TFLOP/s) and 670 at the rate such products hold for seconds under the power limit (1384); by product gate and up
-// 141 us (1459 TFLOP/s, with gate and up kept 175), down 70, dh and with it dg and du 157, dx 137, dW12 127, dW3 68. The products
+// at 32768 rows of 768 with H = 2048, forward and backward together: 810 to 840 us a pass in the first twenty of 556 at the rate of a
+// library product in a burst of its own (1668 TFLOP/s); 965 to 985 in a loop of a second, at the power limit with the clock at 1.3 to
+// 1.4 of 1.97 GHz, of 670 at the rate such products hold there (1384). Each kernel alone, launched one by one: gate and up 126 us
+// (1640 TFLOP/s), with gate and up kept 164, down 78, dW3 65, dh and with it dg and du 150, dx 150, dW12 132, the sums' end 11: 750 in all,
+// the rest of a pass is the clock's fall. The products
 // whose epilogue moves more than an accumulator's worth of data (gate and up kept, dg and du) are bound by that epilogue: at 768
 // or 2048 summed elements a tile's products take no longer than its 16 warps take to bring in, work out and send out its data.
 #pragma once
