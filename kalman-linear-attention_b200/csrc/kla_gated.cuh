@@ -262,15 +262,15 @@ __device__ __forceinline__ void gate_slope(float2 g, float2 &nz, float2 &za, flo
 }
 // Where a gate forgets, v - z v is all cancellation: off by 2^-24 of v and more, it has few digits of a v left, or none. So a gate
 // below kForgetGate is taken by a itself, which has full relative accuracy, and a step as (x - a x) + a h. Its factor w is a, with a
-// positive sign (+0 too), in place of -z, whose sign is negative (-0 too). Above it a is at least 0.0067 in float32 and 0.00034 in
-// bfloat16, so that 2^-23 of z are at most 2^-15 and 2^-11 of a. The choice costs instructions, and a warp makes it only in tiles
+// positive sign (+0 too), in place of -z, whose sign is negative (-0 too). Above it a is at least 0.0025 in float32 and 0.00034 in
+// bfloat16, so that 2^-23 of z are at most 2^-14 and 2^-11 of a. The choice costs instructions, and a warp makes it only in tiles
 // that have such a gate, in loops that are not unrolled and a second time over the steps: unrolled beside the others, they took
 // the backward without any such gate from 91 to 117 us (16 x 2048 x 1536, bfloat16; 94 as it is). Gates from kForgetGate on get the
 // same bits either way. Measured at that shape, gates of mean 2 / of mean 0 and deviation 1.5 / of mean -6, us: float32 forward 111 /
-// 115 / 127, backward 171 / 268 / 321; bfloat16 58 / 58 / 132, 95 / 95 / 254. What infinite values need is a third way (kCareInfinite), for
+// 112 / 128, backward 171 / 195 / 318; bfloat16 59 / 59 / 124, 95 / 95 / 230. What infinite values need is a third way (kCareInfinite), for
 // tiles whose map turned out NaN or whose first state is infinite: within the second it would cost as much again.
 template <typename T>
-constexpr float kForgetGate = sizeof(T) == 2 ? -8.0f : -5.0f;
+constexpr float kForgetGate = sizeof(T) == 2 ? -8.0f : -6.0f;
 __device__ __forceinline__ bool forgets(float w) { return __float_as_int(w) >= 0; }
 template <typename T>
 __device__ __forceinline__ float2 chosen_factor(float2 g, float2 a, float2 nz) { return make_float2(g.x < kForgetGate<T> ? a.x : nz.x, g.y < kForgetGate<T> ? a.y : nz.y); }
@@ -487,20 +487,23 @@ __global__ void __launch_bounds__(GatedFwdShape<T>::W * 32, GatedFwdShape<T>::kC
             own.A = decay<kCareNone>(nz[i], own.A);
             own.F = gate_step<kCareNone>(nz[i], ln.take(xs + i * kGatedChannels), own.F);
         }
-        auto factor = [&](int i) { return gate_factor<T>(ln.take(gs + i * kGatedChannels)); };
-        // The map with care, and the least its slope may be. float32 factors take the gates' place, bfloat16 has no room for them and forms
-        // them again.
+        // The map with care, and the least its slope may be. float32 factors take the gates' place in shared memory, bfloat16 has no room for
+        // them there and keeps them in local memory (which in float32 took 149 us in place of 127 at 16 x 2048 x 1536).
+        float2 local[sizeof(T) == 2 ? TS : 1];
         bool made = false;
+        auto factor = [&](int i) {
+            if constexpr (sizeof(T) == 4) return ln.take(gs + i * kGatedChannels);
+            else return local[i];
+        };
         auto careful = [&](auto care_) {
             constexpr int CARE = decltype(care_)::value;
             own = Map2{make_float2(1.0f, 1.0f), make_float2(0.0f, 0.0f)};
             bool r0 = false, r1 = false;
 #pragma unroll 4
             for (int i = 0; i < TS; ++i) {
-                float2 w;
-                if (sizeof(T) == 4 && made) w = ln.take(gs + i * kGatedChannels);
-                else w = factor(i);
+                const float2 w = made ? factor(i) : gate_factor<T>(ln.take(gs + i * kGatedChannels));
                 if constexpr (sizeof(T) == 4) ln.put(gs + i * kGatedChannels, w);
+                else local[i] = w;
                 r0 |= resets(w.x);
                 r1 |= resets(w.y);
                 own.A = decay<CARE>(w, own.A);
@@ -525,14 +528,13 @@ __global__ void __launch_bounds__(GatedFwdShape<T>::W * 32, GatedFwdShape<T>::kC
             ln.store_state(prm.ckpt + (long long)(span.unit + t0 / kGatedUnit) * prm.D, neg2(h));
         if (__any_sync(0xffffffffu, infinite(h))) {
             care = kCareInfinite;
-            if (sizeof(T) == 4 && !made) careful(std::integral_constant<int, kCareInfinite>{});
+            if (!made) careful(std::integral_constant<int, kCareInfinite>{});
         }
         T *to = h_out + (long long)t0 * prm.h.st + ln.c0;
         auto walk = [&](auto care_) {
 #pragma unroll 4
             for (int i = 0; i < min(cnt, TS); ++i) {
-                const float2 w = sizeof(T) == 4 ? ln.take(gs + i * kGatedChannels) : factor(i);
-                h = gate_step<decltype(care_)::value>(w, ln.take(xs + i * kGatedChannels), h);
+                h = gate_step<decltype(care_)::value>(factor(i), ln.take(xs + i * kGatedChannels), h);
                 ln.store_negated(to, h);
                 to += prm.h.st;
             }
@@ -648,18 +650,13 @@ __global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kC
         };
 #pragma unroll
         for (int i = TS - 1; i >= 0; --i) back.F = decay<kCareNone>(nz[i], behind(i, back.F));
-        // Tiles with gates that forget: what does not fit in shared memory (float32: the factors; bfloat16: c, and factors are formed
-        // again) goes through local memory.
-        float2 local[TS];
+        // With care the factors go through local memory, and c, which in float32 takes the place of dh.
+        float2 factors[TS], local_c[sizeof(T) == 2 ? TS : 1];
         auto slopes = [&](int i, float2 &n, float2 &s) {
             const float2 gate = ln.take(gs + i * kGatedChannels);
             float2 small;
             gate_slope(gate, n, s, small);
             return chosen_factor<T>(gate, small, n);
-        };
-        auto factor = [&](int i) {
-            float2 n, s;
-            return slopes(i, n, s);
         };
         bool made = false;
         auto careful = [&](auto care_) {
@@ -669,15 +666,16 @@ __global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kC
             bool r0 = false, r1 = false;
 #pragma unroll 4
             for (int i = 0; i < TS; ++i) {
-                const float2 w = factor(i);
-                if constexpr (sizeof(T) == 4) local[i] = w;
+                float2 n, s;
+                const float2 w = slopes(i, n, s);
+                factors[i] = w;
                 r0 |= resets(w.x);
                 r1 |= resets(w.y);
                 back.A = decay<CARE>(w, back.A);
                 F = gate_step<CARE>(w, ln.take(xs + i * kGatedChannels), F);
             }
 #pragma unroll 4
-            for (int i = TS - 1; i >= 0; --i) back.F = decay<CARE>(sizeof(T) == 4 ? local[i] : factor(i), behind(i, back.F));
+            for (int i = TS - 1; i >= 0; --i) back.F = decay<CARE>(factors[i], behind(i, back.F));
             made = true;
             return make_float2(r0 ? 0.0f : kLeastSlope, r1 ? 0.0f : kLeastSlope);
         };
@@ -702,7 +700,7 @@ __global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kC
             }
         if (__any_sync(0xffffffffu, infinite(u) || infinite(h))) {
             care = kCareInfinite;
-            if (sizeof(T) == 4 && !made) careful(std::integral_constant<int, kCareInfinite>{});
+            if (!made) careful(std::integral_constant<int, kCareInfinite>{});
         }
         T *to_x = dx + (long long)t0 * prm.dx.st + ln.c0, *to_g = dg + (long long)t0 * prm.dg.st + ln.c0;
         auto walk = [&](auto care_) {
@@ -710,21 +708,15 @@ __global__ void __launch_bounds__(GatedBwdShape<T>::W * 32, GatedBwdShape<T>::kC
 #pragma unroll 4
             for (int i = TS - 1; i >= 0; --i) {
                 const float2 ci = behind(i, u);
-                float2 w;
-                if constexpr (sizeof(T) == 4) {
-                    w = local[i];
-                    ln.put(ds + i * kGatedChannels, ci);
-                } else {
-                    w = factor(i);
-                    local[i] = ci;
-                }
-                u = decay<CARE>(w, ci);
+                if constexpr (sizeof(T) == 4) ln.put(ds + i * kGatedChannels, ci);
+                else local_c[i] = ci;
+                u = decay<CARE>(factors[i], ci);
             }
 #pragma unroll 4
             for (int i = 0; i < min(cnt, TS); ++i) {
                 float2 n, s, ci;
                 if constexpr (sizeof(T) == 4) ci = ln.take(ds + i * kGatedChannels);
-                else ci = local[i];
+                else ci = local_c[i];
                 const float2 xi = ln.take(xs + i * kGatedChannels), w = slopes(i, n, s);
                 ln.store_negated(to_x, mul2(n, ci));
                 ln.store_negated(to_g, mul2(mul2(s, ci), add2(h, xi)));

@@ -26,7 +26,7 @@ def gated_scan_b200(x: torch.Tensor, gate: torch.Tensor, initial_state: torch.Te
     ``cu_seqlens[n]`` to ``cu_seqlens[n + 1]``; the bounds must not decrease, which is not checked (values outside ``[0, L]``
     are clamped). A sequence without rows leaves the state it started from; rows that belong to no sequence get zeros, in
     ``h`` and in the gradients. Where gates forget, what they leave of a state (and of its gradient) has the relative accuracy of
-    ``sigmoid(gate)``: 2^-15 in float32 and 2^-11 in bfloat16 at least. An infinite state stays infinite, unless an infinity of
+    ``sigmoid(gate)``: 2^-14 in float32 and 2^-11 in bfloat16 at least. An infinite state stays infinite, unless an infinity of
     the other sign or a gate whose ``sigmoid`` is 0 in float32 (below -87) makes it NaN; so does an infinite gradient of it."""
     return _lib.host().gated_scan(x, gate, initial_state, cu_seqlens)
 
